@@ -247,7 +247,7 @@ def _plain_adjust(s):
         x = x - frequency * counts - torch.where(counts > 0, presence, 0)
     if "class_bias" in s:
         x = x + s["class_bias"].to(acc)
-    if "bias_classes" in s:
+    if "bias_classes" in s and s["bias_classes"].numel():
         entry = torch.arange(s["bias_classes"].numel(), device=DEVICE)
         row = torch.searchsorted(s["bias_offsets"], entry, right=True) - 1
         last = torch.full((rows * classes,), -1, dtype=torch.int64, device=DEVICE)

@@ -16,6 +16,7 @@ LIB_PATH = os.path.join(_HERE, "lib", "libcatboostmodel.so")
 
 APT_RAW_FORMULA_VAL, APT_EXPONENT, APT_RMSE_WITH_UNCERTAINTY, APT_PROBABILITY, APT_CLASS, APT_MULTI_PROBABILITY = range(6)
 LAYOUT_FLAT_ROWS, LAYOUT_FLAT_COLUMNS, LAYOUT_SPLIT_ROWS = range(3)
+FLOAT64, FLOAT32, FLOAT16, BFLOAT16 = range(4)
 
 _lib = None
 
@@ -70,6 +71,29 @@ class DeviceFeatures(ctypes.Structure):
         ("Stride", ctypes.c_size_t),
         ("Cats", ctypes.c_void_p),
         ("CatStride", ctypes.c_size_t),
+    ]
+
+
+class ScoreAdjustment(ctypes.Structure):
+    """CbHipScoreAdjustment of include/cb_hip_evaluator.h."""
+    _fields_ = [
+        ("HistoryOffsets", ctypes.c_void_p),
+        ("History", ctypes.c_void_p),
+        ("HistoryCount", ctypes.c_size_t),
+        ("PromptLengths", ctypes.c_void_p),
+        ("Repetition", ctypes.c_void_p),
+        ("Frequency", ctypes.c_void_p),
+        ("Presence", ctypes.c_void_p),
+        ("ClassBias", ctypes.c_void_p),
+        ("ClassBiasStride", ctypes.c_size_t),
+        ("BiasOffsets", ctypes.c_void_p),
+        ("BiasClasses", ctypes.c_void_p),
+        ("BiasValues", ctypes.c_void_p),
+        ("BiasCount", ctypes.c_size_t),
+        ("Allowed", ctypes.c_void_p),
+        ("AllowedStride", ctypes.c_size_t),
+        ("AllowedCount", ctypes.c_size_t),
+        ("AllowedRows", ctypes.c_void_p),
     ]
 
 
@@ -148,6 +172,14 @@ def load_library():
         "CbHipLeafIndexesQuantized": (ctypes.c_bool, [vp, vp, sz, sz, sz, vp, vp]),
         "CbHipExportQuantized": (ctypes.c_bool, [vp, vp, sz, vp, vp]),
         "CbHipApplyPredictionTypeDevice": (ctypes.c_bool, [vp, ctypes.c_int, sz, vp, vp, vp]),
+        "CbHipAdjustScores": (ctypes.c_bool, [ctypes.c_int, sz, sz, vp, sz, ctypes.POINTER(ScoreAdjustment), vp, sz, vp]),
+        "CbHipSelectTop": (ctypes.c_bool, [ctypes.c_int, sz, sz, vp, sz, ctypes.c_int32, ctypes.c_bool, vp, vp, vp]),
+        "CbHipSelectTopBackward": (ctypes.c_bool, [ctypes.c_int, sz, sz, vp, sz, ctypes.c_int32, ctypes.c_bool, vp, vp, vp, vp, sz, vp]),
+        "CbHipSortByExpertBytes": (sz, [sz, ctypes.c_int32]),
+        "CbHipSortByExpert": (ctypes.c_bool, [sz, ctypes.c_int32, vp, vp, vp, vp, sz, vp]),
+        "CbHipDispatchRows": (ctypes.c_bool, [ctypes.c_int, sz, sz, ctypes.c_int32, vp, sz, vp, vp, sz, sz, vp]),
+        "CbHipCombineRows": (ctypes.c_bool, [ctypes.c_int, sz, sz, ctypes.c_int32, vp, sz, sz, vp, vp, vp, sz, vp]),
+        "CbHipCombineRowsBackward": (ctypes.c_bool, [ctypes.c_int, sz, sz, ctypes.c_int32, vp, sz, vp, sz, sz, vp, vp, vp, sz, vp, vp]),
         "CbHipSynchronize": (ctypes.c_bool, [vp, vp]),
         "CbHipLastKernelTimes": (ctypes.c_bool, [vp, ctypes.POINTER(ctypes.c_float), ctypes.POINTER(ctypes.c_float)]),
         "CbHipDescribeKernels": (ctypes.c_bool, [vp, ctypes.c_int, sz, ctypes.c_char_p, sz]),
@@ -341,6 +373,68 @@ def make_splits(splits):
         else:
             out[i] = (2, s[1], 0.0, s[2])
     return out
+
+
+# ---- operators on scores and on routed rows (include/cb_hip_evaluator.h says what each does): device pointers in,
+# device pointers out, `value_type` one of FLOAT64, FLOAT32, FLOAT16 and BFLOAT16, strides in values
+
+def score_adjustment(history_offsets_ptr=0, history_ptr=0, history_count=0, prompt_lengths_ptr=0, repetition_ptr=0, frequency_ptr=0,
+                     presence_ptr=0, class_bias_ptr=0, class_bias_stride=0, bias_offsets_ptr=0, bias_classes_ptr=0, bias_values_ptr=0,
+                     bias_count=0, allowed_ptr=0, allowed_stride=0, allowed_count=0, allowed_rows_ptr=0):
+    """What adjust_scores does (CbHipScoreAdjustment); parts that are left out are not done."""
+    return ScoreAdjustment(history_offsets_ptr, history_ptr, history_count, prompt_lengths_ptr, repetition_ptr, frequency_ptr, presence_ptr,
+                           class_bias_ptr, class_bias_stride, bias_offsets_ptr, bias_classes_ptr, bias_values_ptr, bias_count, allowed_ptr,
+                           allowed_stride, allowed_count, allowed_rows_ptr)
+
+
+def adjust_scores(value_type, rows, classes, scores_ptr, score_stride, adjustment, result_ptr, result_stride, stream=None):
+    """Scores with penalties for classes shown already, biases and masks (CbHipAdjustScores)."""
+    _check(load_library().CbHipAdjustScores(value_type, rows, classes, scores_ptr, score_stride, ctypes.byref(adjustment), result_ptr,
+                                            result_stride, stream))
+
+
+def select_top(value_type, rows, classes, scores_ptr, score_stride, count, among_selected, indexes_ptr, weights_ptr, stream=None):
+    """The best classes of every row and their softmax weights (CbHipSelectTop)."""
+    _check(load_library().CbHipSelectTop(value_type, rows, classes, scores_ptr, score_stride, count, among_selected, indexes_ptr, weights_ptr,
+                                         stream))
+
+
+def select_top_backward(value_type, rows, classes, scores_ptr, score_stride, count, among_selected, indexes_ptr, weights_ptr,
+                        weight_gradients_ptr, score_gradients_ptr, gradient_stride, stream=None):
+    """The scores' gradient of select_top (CbHipSelectTopBackward)."""
+    _check(load_library().CbHipSelectTopBackward(value_type, rows, classes, scores_ptr, score_stride, count, among_selected, indexes_ptr,
+                                                 weights_ptr, weight_gradients_ptr, score_gradients_ptr, gradient_stride, stream))
+
+
+def sort_by_expert_bytes(slots, experts):
+    """Bytes of workspace that sort_by_expert needs."""
+    return load_library().CbHipSortByExpertBytes(slots, experts)
+
+
+def sort_by_expert(slots, experts, ids_ptr, places_ptr, offsets_ptr, workspace_ptr, workspace_bytes, stream=None):
+    """Places of the slots, sorted by expert, and the experts' offsets (CbHipSortByExpert)."""
+    _check(load_library().CbHipSortByExpert(slots, experts, ids_ptr, places_ptr, offsets_ptr, workspace_ptr, workspace_bytes, stream))
+
+
+def dispatch_rows(value_type, rows, width, per_row, source_ptr, source_stride, places_ptr, sorted_ptr, sorted_rows, sorted_stride, stream=None):
+    """Every row to the places of its slots (CbHipDispatchRows)."""
+    _check(load_library().CbHipDispatchRows(value_type, rows, width, per_row, source_ptr, source_stride, places_ptr, sorted_ptr, sorted_rows,
+                                            sorted_stride, stream))
+
+
+def combine_rows(value_type, rows, width, per_row, sorted_ptr, sorted_rows, sorted_stride, places_ptr, weights_ptr, result_ptr, result_stride,
+                 stream=None):
+    """The weighted sum of the rows at a row's places; without weights (0) the gradient of dispatch_rows (CbHipCombineRows)."""
+    _check(load_library().CbHipCombineRows(value_type, rows, width, per_row, sorted_ptr, sorted_rows, sorted_stride, places_ptr, weights_ptr,
+                                           result_ptr, result_stride, stream))
+
+
+def combine_rows_backward(value_type, rows, width, per_row, gradients_ptr, gradient_stride, sorted_ptr, sorted_rows, sorted_stride, places_ptr,
+                          weights_ptr, sorted_gradients_ptr, sorted_gradient_stride, weight_gradients_ptr, stream=None):
+    """The gradients of combine_rows (CbHipCombineRowsBackward)."""
+    _check(load_library().CbHipCombineRowsBackward(value_type, rows, width, per_row, gradients_ptr, gradient_stride, sorted_ptr, sorted_rows,
+                                                   sorted_stride, places_ptr, weights_ptr, sorted_gradients_ptr, sorted_gradient_stride,
+                                                   weight_gradients_ptr, stream))
 
 
 class DeviceEvaluator:

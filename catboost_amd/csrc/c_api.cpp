@@ -10,6 +10,7 @@
 #include "hip_evaluator.h"
 #include "model.h"
 #include "model_builder.h"
+#include "operators.h"
 
 #include <algorithm>
 #include <cmath>
@@ -865,6 +866,65 @@ bool CbHipApplyPredictionTypeDevice(CbHipEvaluatorHandle* evaluator, int predict
                                     const double* deviceRaw, double* deviceResult, void* hipStream) {
     return Guard([&] {
         E(evaluator)->ApplyPredictionTypeDevice(predictionType, 0, docCount, docCount, deviceRaw, deviceResult, hipStream);
+    });
+}
+
+bool CbHipAdjustScores(int valueType, size_t rows, size_t classes, const void* scores, size_t scoreStride,
+                       const CbHipScoreAdjustment* adjustment, void* result, size_t resultStride, void* hipStream) {
+    return Guard([&] {
+        CBAMD_ENSURE(adjustment != nullptr, "score adjustment is null");
+        AdjustScores(valueType, rows, classes, scores, scoreStride, *adjustment, result, resultStride, hipStream);
+    });
+}
+
+bool CbHipSelectTop(int valueType, size_t rows, size_t classes, const void* scores, size_t scoreStride, int32_t count,
+                    bool amongSelected, int32_t* indexes, void* weights, void* hipStream) {
+    return Guard([&] {
+        SelectTop(valueType, rows, classes, scores, scoreStride, count, amongSelected, indexes, weights, hipStream);
+    });
+}
+
+bool CbHipSelectTopBackward(int valueType, size_t rows, size_t classes, const void* scores, size_t scoreStride, int32_t count,
+                            bool amongSelected, const int32_t* indexes, const void* weights, const void* weightGradients,
+                            void* scoreGradients, size_t gradientStride, void* hipStream) {
+    return Guard([&] {
+        SelectTopBackward(valueType, rows, classes, scores, scoreStride, count, amongSelected, indexes, weights,
+                          weightGradients, scoreGradients, gradientStride, hipStream);
+    });
+}
+
+size_t CbHipSortByExpertBytes(size_t slots, int32_t experts) {
+    return SortByExpertBytes(slots, experts);
+}
+
+bool CbHipSortByExpert(size_t slots, int32_t experts, const int32_t* ids, int32_t* places, int32_t* offsets,
+                       void* workspace, size_t workspaceBytes, void* hipStream) {
+    return Guard([&] { SortByExpert(slots, experts, ids, places, offsets, workspace, workspaceBytes, hipStream); });
+}
+
+bool CbHipDispatchRows(int valueType, size_t rows, size_t width, int32_t perRow, const void* source, size_t sourceStride,
+                       const int32_t* places, void* sorted, size_t sortedRows, size_t sortedStride, void* hipStream) {
+    return Guard([&] {
+        DispatchRows(valueType, rows, width, perRow, source, sourceStride, places, sorted, sortedRows, sortedStride, hipStream);
+    });
+}
+
+bool CbHipCombineRows(int valueType, size_t rows, size_t width, int32_t perRow, const void* sorted, size_t sortedRows,
+                      size_t sortedStride, const int32_t* places, const void* weights, void* result, size_t resultStride,
+                      void* hipStream) {
+    return Guard([&] {
+        CombineRows(valueType, rows, width, perRow, sorted, sortedRows, sortedStride, places, weights, result, resultStride,
+                    hipStream);
+    });
+}
+
+bool CbHipCombineRowsBackward(int valueType, size_t rows, size_t width, int32_t perRow, const void* resultGradients,
+                              size_t gradientStride, const void* sorted, size_t sortedRows, size_t sortedStride,
+                              const int32_t* places, const void* weights, void* sortedGradients,
+                              size_t sortedGradientStride, void* weightGradients, void* hipStream) {
+    return Guard([&] {
+        CombineRowsBackward(valueType, rows, width, perRow, resultGradients, gradientStride, sorted, sortedRows, sortedStride,
+                            places, weights, sortedGradients, sortedGradientStride, weightGradients, hipStream);
     });
 }
 

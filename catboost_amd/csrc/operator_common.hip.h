@@ -1,0 +1,127 @@
+// What the operators on scores and rows share: value types, the device and stream of a call, launches.
+#pragma once
+
+#include "operators.h"
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+#include <string>
+#include <tuple>
+#include <utility>
+
+namespace cbamd {
+namespace op {
+
+inline void Check(hipError_t e, const char* what) {
+    if (e != hipSuccess) {
+        throw TModelError(std::string("HIP error in ") + what + ": " + hipGetErrorString(e));
+    }
+}
+#define OP_HIP_CHECK(expr) ::cbamd::op::Check((expr), #expr)
+
+// The device that a call's output is on is the thread's current one for as long as this lives. The operators have no
+// handle that knows a device, so the output's address tells it; a stream of another device is refused.
+class TCallDevice {
+public:
+    TCallDevice(const void* output, void* stream)
+        : Stream(static_cast<hipStream_t>(stream))
+    {
+        hipPointerAttribute_t attributes;
+        if (hipPointerGetAttributes(&attributes, output) != hipSuccess || attributes.type == hipMemoryTypeUnregistered) {
+            (void)hipGetLastError();  // what this call left is no later one's
+            throw TModelError("the output is not in memory that a GPU can write");
+        }
+        if (Stream != nullptr) {
+            hipDevice_t device = 0;
+            OP_HIP_CHECK(hipStreamGetDevice(Stream, &device));
+            CBAMD_ENSURE(device == attributes.device, "the stream and the output are on different devices");
+        }
+        OP_HIP_CHECK(hipGetDevice(&Previous));
+        if (Previous != attributes.device) {
+            OP_HIP_CHECK(hipSetDevice(attributes.device));
+            Changed = true;
+        }
+    }
+    ~TCallDevice() {
+        if (Changed) {
+            (void)hipSetDevice(Previous);
+        }
+    }
+    TCallDevice(const TCallDevice&) = delete;
+    TCallDevice& operator=(const TCallDevice&) = delete;
+
+    // (the launch's own status: hipGetLastError would also hand over what another library's call left behind)
+    template <typename... TParams, typename... TArgs>
+    void Launch(void (*kernel)(TParams...), size_t groups, uint32_t threads, size_t ldsBytes, TArgs&&... args) const {
+        std::pair<int, std::tuple<TParams...>> held(0, std::tuple<TParams...>(std::forward<TArgs>(args)...));
+        LaunchHeld(reinterpret_cast<const void*>(kernel), groups, threads, ldsBytes, held.second,
+                   std::index_sequence_for<TParams...>());
+    }
+
+private:
+    template <typename TTuple, size_t... I>
+    void LaunchHeld(const void* kernel, size_t groups, uint32_t threads, size_t ldsBytes, TTuple& held,
+                    std::index_sequence<I...>) const {
+        void* args[] = {static_cast<void*>(&std::get<I>(held))...};
+        OP_HIP_CHECK(hipLaunchKernel(kernel, dim3(static_cast<uint32_t>(groups)), dim3(threads), args, ldsBytes, Stream));
+    }
+
+    hipStream_t Stream = nullptr;
+    int Previous = 0;
+    bool Changed = false;
+};
+
+// Sums, softmax statistics and everything between a load and a store are in 32 bits, in 64 for 64-bit values
+template <typename T>
+struct TAccumulator {
+    using Type = float;
+};
+template <>
+struct TAccumulator<double> {
+    using Type = double;
+};
+template <typename T>
+using TAcc = typename TAccumulator<T>::Type;
+
+// f(T()) for the C++ type of a value type
+template <typename F>
+void WithType(int valueType, F&& f) {
+    switch (valueType) {
+        case CBHIP_FLOAT64: return f(double());
+        case CBHIP_FLOAT32: return f(float());
+        case CBHIP_FLOAT16: return f(_Float16());
+        case CBHIP_BFLOAT16: return f(__bf16());
+    }
+    CBAMD_ENSURE(false, "unknown value type " + std::to_string(valueType));
+}
+
+inline size_t ValueSize(int valueType) {
+    CBAMD_ENSURE(valueType >= CBHIP_FLOAT64 && valueType <= CBHIP_BFLOAT16, "unknown value type " + std::to_string(valueType));
+    return valueType == CBHIP_FLOAT64 ? 8 : valueType == CBHIP_FLOAT32 ? 4 : 2;
+}
+
+// A matrix of `rows` rows of `width` values, `stride` values from row to row: what every operand is asked
+inline void CheckMatrix(const char* name, const void* data, size_t rows, size_t width, size_t stride, size_t valueSize) {
+    CBAMD_ENSURE(data != nullptr, std::string(name) + " pointer is null");
+    CBAMD_ENSURE(rows <= 1 || stride >= width, std::string(name) + ": a stride of " + std::to_string(stride) +
+                                                   " values is shorter than a row of " + std::to_string(width));
+    CBAMD_ENSURE(reinterpret_cast<uintptr_t>(data) % valueSize == 0, std::string(name) + " pointer is not a multiple of the value size");
+    CBAMD_ENSURE(rows <= 1 || stride <= (size_t(1) << 60) / valueSize / rows, std::string(name) + " is too large");
+}
+
+// N values in a row, at any alignment of a value: one wide load or store where N values make one (the hardware's
+// unaligned mode takes any address)
+template <typename T, int N>
+struct TValues {
+    T V[N];
+    __device__ __forceinline__ static TValues Load(const T* at) {
+        TValues r;
+        __builtin_memcpy(&r, at, sizeof(r));
+        return r;
+    }
+    __device__ __forceinline__ void Store(T* at) const { __builtin_memcpy(at, this, sizeof(*this)); }
+};
+
+}  // namespace op
+}  // namespace cbamd

@@ -205,6 +205,105 @@ bool CbHipDescribeKernels(CbHipEvaluatorHandle* evaluator, int layout, size_t do
 bool CbHipEvaluatorSetSmallBatchSlicing(CbHipEvaluatorHandle* evaluator, bool enabled);
 bool CbHipSetSmallBatchSlicing(void* modelHandle, bool enabled);
 
+/* ---- operators on scores and on routed rows -----------------------------------------------------------------
+ * What stands before, between and behind models: scores (raw values, a gate's, a language model's) with penalties,
+ * biases and masks; the best classes with their weights; rows sorted by the model or expert that each goes to, and
+ * brought back. None has a counterpart in the reference. All take DEVICE memory, are asynchronous on `hipStream` (a
+ * hipStream_t, NULL: the default stream of the device that the output is on) and, but for CbHipEvalRouted, only launch
+ * kernels, so they may be captured into HIP graphs; memory that they work in comes from the caller. All operands of a
+ * call are on one device, which need not be the current one. Results are the same for every call on the same inputs.
+ * Rows are `stride` values apart (at least a row's width), at any alignment of a value. Outputs overlap no other
+ * operand of the call, unless said otherwise. Zero rows are fine: nothing is done then. */
+
+enum ECbHipValueType {
+    CBHIP_FLOAT64 = 0,
+    CBHIP_FLOAT32 = 1,
+    CBHIP_FLOAT16 = 2,
+    CBHIP_BFLOAT16 = 3,
+};
+
+/* What CbHipAdjustScores does to the scores. A part whose pointer is NULL is left out. */
+typedef struct CbHipScoreAdjustment {
+    /* Classes that a row has shown already: row r's are History[HistoryOffsets[r]] to History[HistoryOffsets[r + 1] - 1],
+     * rows + 1 offsets, the first PromptLengths[r] of them (NULL: none) given and the others generated. Entries outside
+     * [0, classes) are passed over; less than 2^31 entries a row. HistoryCount: entries that History holds, none
+     * behind them is read. */
+    const int64_t* HistoryOffsets;
+    const int32_t* History;
+    size_t HistoryCount;
+    const int32_t* PromptLengths;
+    /* One value per row. A class of the row's history: score > 0 ? score / Repetition : score * Repetition. */
+    const float* Repetition;
+    /* A class generated n > 0 times: score - Frequency * n - Presence. */
+    const float* Frequency;
+    const float* Presence;
+    /* score + ClassBias[c], or ClassBias[r * ClassBiasStride + c] with a stride other than 0 */
+    const float* ClassBias;
+    size_t ClassBiasStride;
+    /* score + BiasValues[i] for the last of row r's entries i with BiasClasses[i] == c (entries as in History);
+     * less than 2^31 entries in all */
+    const int64_t* BiasOffsets;
+    const int32_t* BiasClasses;
+    const float* BiasValues;
+    size_t BiasCount;
+    /* Masks of (classes + 31) / 32 words, AllowedStride words apart, AllowedCount of them. A class whose bit
+     * (c & 31 of word c >> 5) is clear gets minus infinity, whatever its score. Row r has mask AllowedRows[r], no mask
+     * where that is outside [0, AllowedCount); NULL: mask r. */
+    const uint32_t* Allowed;
+    size_t AllowedStride;
+    size_t AllowedCount;
+    const int32_t* AllowedRows;
+} CbHipScoreAdjustment;
+
+/* result[r * resultStride + c] = scores[r * scoreStride + c], adjusted in the order of the struct's members, computed in
+ * 32 bits (64 for CBHIP_FLOAT64) and rounded once. `result` may be `scores` with the same stride. */
+bool CbHipAdjustScores(int valueType, size_t rows, size_t classes, const void* scores, size_t scoreStride,
+                       const CbHipScoreAdjustment* adjustment, void* result, size_t resultStride, void* hipStream);
+
+/* The `count` (1 to 32) largest scores of every row of at most 1024 classes, largest first, of equal ones the lowest
+ * class first: indexes[r * count + k] and their softmax weights[r * count + k] (float, double for CBHIP_FLOAT64), over
+ * the row's classes or, with amongSelected, over the selected ones. Minus infinity and NaN are never selected and weigh
+ * nothing; where they leave less than `count` classes the rest has index -1 and weight 0. Classes of plus
+ * infinity share the whole weight. */
+bool CbHipSelectTop(int valueType, size_t rows, size_t classes, const void* scores, size_t scoreStride, int32_t count,
+                    bool amongSelected, int32_t* indexes, void* weights, void* hipStream);
+
+/* Its gradient: weightGradients[r * count + k] -> scoreGradients[r * gradientStride + c], every class of it, from what
+ * CbHipSelectTop was given and gave. With amongSelected `scores` is not read and may be NULL. */
+bool CbHipSelectTopBackward(int valueType, size_t rows, size_t classes, const void* scores, size_t scoreStride, int32_t count,
+                            bool amongSelected, const int32_t* indexes, const void* weights, const void* weightGradients,
+                            void* scoreGradients, size_t gradientStride, void* hipStream);
+
+/* Bytes of workspace (at any address that is a multiple of 4) that CbHipSortByExpert needs. */
+size_t CbHipSortByExpertBytes(size_t slots, int32_t experts);
+
+/* Sorts less than 2^31 slots by their expert ids[slot], of equal ones the first first: places[slot] is where the slot
+ * goes, -1 where its id is outside [0, experts), at most 1024 experts; expert e's places are offsets[e] to
+ * offsets[e + 1] - 1 (experts + 1 offsets, written for no slots too). */
+bool CbHipSortByExpert(size_t slots, int32_t experts, const int32_t* ids, int32_t* places, int32_t* offsets,
+                       void* workspace, size_t workspaceBytes, void* hipStream);
+
+/* sorted[places[r * perRow + k]] = source[r] for every row's perRow (1 to 64) slots, bit for bit. Places outside
+ * [0, sortedRows) are left out; no two others may be equal. Rows of `sorted` without a slot stay as they are. */
+bool CbHipDispatchRows(int valueType, size_t rows, size_t width, int32_t perRow, const void* source, size_t sourceStride,
+                       const int32_t* places, void* sorted, size_t sortedRows, size_t sortedStride, void* hipStream);
+
+/* result[r] = sum over k of weights[r * perRow + k] * sorted[places[r * perRow + k]], in slot order in 32 bits (64 for
+ * CBHIP_FLOAT64), rounded once. weights: float, double for CBHIP_FLOAT64; NULL: all 1, which makes this the gradient of
+ * CbHipDispatchRows. Places outside [0, sortedRows) add nothing, whatever their weight. */
+bool CbHipCombineRows(int valueType, size_t rows, size_t width, int32_t perRow, const void* sorted, size_t sortedRows,
+                      size_t sortedStride, const int32_t* places, const void* weights, void* result, size_t resultStride,
+                      void* hipStream);
+
+/* Its gradients: sortedGradients[places[r * perRow + k]] = weights[r * perRow + k] * resultGradients[r] (rows without a
+ * slot stay as they are) and weightGradients[r * perRow + k] = the product of resultGradients[r] and
+ * sorted[places[r * perRow + k]], 0 for a place outside [0, sortedRows). Either output may be NULL; without
+ * weightGradients `sorted` is not read and may be NULL. No two places may be equal. */
+bool CbHipCombineRowsBackward(int valueType, size_t rows, size_t width, int32_t perRow, const void* resultGradients,
+                              size_t gradientStride, const void* sorted, size_t sortedRows, size_t sortedStride,
+                              const int32_t* places, const void* weights, void* sortedGradients,
+                              size_t sortedGradientStride, void* weightGradients, void* hipStream);
+
 /* ---- extensions on a ModelCalcerHandle (c_api.h) ------------------------------------------ */
 
 /* The evaluator bound to a model handle (created on first use on the enabled device). Owned by

@@ -1,0 +1,616 @@
+"""Operators on scores and on routed rows against their definitions in 64 bits and more. Needs an MI355X.
+
+Tolerances count roundings of half a step: U is half a step of what a kernel computes in (2^-24, 2^-53 for 64-bit values),
+HALF half a step of the type that it stores (with half of the smallest subnormal where values are that small)."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import catboost_amd as cb
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {cb.FLOAT64: torch.float64, cb.FLOAT32: torch.float32, cb.FLOAT16: torch.float16, cb.BFLOAT16: torch.bfloat16}
+NAMES = {cb.FLOAT64: "f64", cb.FLOAT32: "f32", cb.FLOAT16: "f16", cb.BFLOAT16: "bf16"}
+ALL = pytest.mark.parametrize("kind", list(TYPES), ids=NAMES.get)
+HALF = {cb.FLOAT64: 2.0 ** -53, cb.FLOAT32: 2.0 ** -24, cb.FLOAT16: 2.0 ** -11, cb.BFLOAT16: 2.0 ** -8}
+TINY = {cb.FLOAT64: 0.0, cb.FLOAT32: 2.0 ** -150, cb.FLOAT16: 2.0 ** -25, cb.BFLOAT16: 2.0 ** -134}
+
+
+def u(kind):
+    return 2.0 ** -53 if kind == cb.FLOAT64 else 2.0 ** -24
+
+
+def acc(kind):
+    return torch.float64 if kind == cb.FLOAT64 else torch.float32
+
+
+def ptr(t):
+    return 0 if t is None else t.data_ptr()
+
+
+def dev(a, dtype=None):
+    return None if a is None else torch.as_tensor(np.ascontiguousarray(a)).to("cuda", dtype)
+
+
+def table(values, kind, pad=0, fill=7.0):
+    """The values rounded to the type, as the first columns of a wider table of `fill`."""
+    rows, width = values.shape
+    wide = torch.full((rows, width + pad), fill, dtype=TYPES[kind], device="cuda")
+    wide[:, :width] = torch.from_numpy(values).cuda().to(TYPES[kind])
+    return wide[:, :width]
+
+
+def exactly(t):
+    return t.detach().to(torch.float64).cpu().numpy().astype(np.longdouble)
+
+
+def compare(got, expected, bound, kind):
+    """|got - expected| <= bound + one rounding to the type; infinities and NaN at the same places."""
+    got, expected = np.asarray(got, np.longdouble), np.asarray(expected, np.longdouble)
+    assert np.array_equal(np.isnan(got), np.isnan(expected))
+    finite = np.isfinite(expected)
+    assert np.array_equal(got[~finite & ~np.isnan(expected)], expected[~finite & ~np.isnan(expected)])
+    bound = np.broadcast_to(bound, expected.shape)[finite]
+    off = np.abs(got[finite] - expected[finite])
+    allowed = bound + HALF[kind] * (np.abs(expected[finite]) + bound) + TINY[kind]
+    worst = np.max(off - allowed, initial=-1.0)
+    assert worst <= 0, "off by %g where %g is allowed" % (off[np.argmax(off - allowed)], allowed[np.argmax(off - allowed)])
+
+
+# ---------------------------------------------------------------- penalties, biases, masks
+
+def history(rng, rows, classes, most, outside=True):
+    lengths = rng.integers(0, most + 1, rows)
+    lengths[rng.random(rows) < 0.2] = 0
+    offsets = np.concatenate([[0], np.cumsum(lengths)]).astype(np.int64)
+    ids = (classes * rng.random(int(offsets[-1])) ** 3).astype(np.int32)
+    if outside and len(ids):
+        ids[rng.random(len(ids)) < 0.05] = -1
+        ids[rng.random(len(ids)) < 0.03] = classes
+        ids[rng.random(len(ids)) < 0.02] = np.iinfo(np.int32).min
+    return offsets, ids
+
+
+def adjusted(x, p):
+    """The definition, row by row; and the largest of the values on the way to each result."""
+    rows, classes = x.shape
+    x, big = x.copy(), np.abs(np.where(np.isfinite(x), x, 0))
+    for r in range(rows):
+        if p.get("offsets") is not None:
+            entries = p["ids"][p["offsets"][r]:p["offsets"][r + 1]]
+            prompt = p["prompts"][r] if p.get("prompts") is not None else 0
+            given = set(int(c) for c in entries if 0 <= c < classes)
+            counts = {}
+            for c in entries[max(prompt, 0):]:
+                if 0 <= c < classes:
+                    counts[int(c)] = counts.get(int(c), 0) + 1
+            for c in given:
+                v = x[r, c]
+                if p.get("repetition") is not None:
+                    rep = np.longdouble(p["repetition"][r])
+                    v = v / rep if v > 0 else v * rep
+                    big[r, c] = max(big[r, c], abs(v) if np.isfinite(v) else 0)
+                n = counts.get(c, 0)
+                if n and p.get("frequency") is not None:
+                    v = v - np.longdouble(p["frequency"][r]) * n
+                    big[r, c] = max(big[r, c], abs(v) if np.isfinite(v) else 0) + abs(np.longdouble(p["frequency"][r]) * n)
+                if n and p.get("presence") is not None:
+                    v = v - np.longdouble(p["presence"][r])
+                    big[r, c] = max(big[r, c], abs(v) if np.isfinite(v) else 0)
+                x[r, c] = v
+        if p.get("class_bias") is not None:
+            x[r] += p["class_bias"][r if p["class_bias"].shape[0] > 1 else 0].astype(np.longdouble)
+            big[r] = np.maximum(big[r], np.abs(np.where(np.isfinite(x[r]), x[r], 0)))
+        if p.get("bias_offsets") is not None:
+            wanted = {}
+            for e in range(p["bias_offsets"][r], p["bias_offsets"][r + 1]):
+                wanted[int(p["bias_classes"][e])] = np.longdouble(p["bias_values"][e])
+            for c, v in wanted.items():
+                if 0 <= c < classes:
+                    x[r, c] += v
+                    big[r, c] = max(big[r, c], abs(x[r, c]) if np.isfinite(x[r, c]) else 0)
+        if p.get("allowed") is not None:
+            m = p["allowed_rows"][r] if p.get("allowed_rows") is not None else r
+            if 0 <= m < p["allowed"].shape[0]:
+                c = np.arange(classes)
+                x[r, (p["allowed"][m, c >> 5] >> (c & 31).astype(np.uint32)) & 1 == 0] = -np.inf
+    return x, big
+
+
+class Adjustment:
+    """The parts on the GPU, and the struct that points at them."""
+
+    def __init__(self, p):
+        d = {k: dev(v) for k, v in p.items() if v is not None and k != "allowed"}
+        if p.get("allowed") is not None:
+            d["allowed"] = dev(p["allowed"].view(np.int32))
+        self.keep = d
+        g = d.get
+        self.struct = cb.score_adjustment(
+            history_offsets_ptr=ptr(g("offsets")), history_ptr=ptr(g("ids")), history_count=len(p["ids"]) if "ids" in p else 0,
+            prompt_lengths_ptr=ptr(g("prompts")), repetition_ptr=ptr(g("repetition")), frequency_ptr=ptr(g("frequency")), presence_ptr=ptr(g("presence")),
+            class_bias_ptr=ptr(g("class_bias")), class_bias_stride=p["class_bias"].shape[1] if p.get("class_bias") is not None and p["class_bias"].shape[0] > 1 else 0,
+            bias_offsets_ptr=ptr(g("bias_offsets")), bias_classes_ptr=ptr(g("bias_classes")), bias_values_ptr=ptr(g("bias_values")),
+            bias_count=len(p["bias_classes"]) if "bias_classes" in p else 0, allowed_ptr=ptr(g("allowed")),
+            allowed_stride=p["allowed"].shape[1] if p.get("allowed") is not None else 0,
+            allowed_count=p["allowed"].shape[0] if p.get("allowed") is not None else 0, allowed_rows_ptr=ptr(g("allowed_rows")))
+
+
+def parts(rng, rows, classes, which, most=40):
+    p = {}
+    if "h" in which:
+        p["offsets"], p["ids"] = history(rng, rows, classes, most)
+        if "p" in which:
+            p["prompts"] = rng.integers(0, most, rows).astype(np.int32)
+        if "r" in which:
+            p["repetition"] = (1 + rng.random(rows)).astype(np.float32)
+        if "f" in which:
+            p["frequency"] = rng.normal(size=rows).astype(np.float32)
+        if "s" in which:
+            p["presence"] = rng.normal(size=rows).astype(np.float32)
+    if "c" in which:
+        p["class_bias"] = rng.normal(size=(1, classes)).astype(np.float32)
+    if "C" in which:
+        p["class_bias"] = rng.normal(size=(max(rows, 2), classes)).astype(np.float32)[:max(rows, 2)]
+    if "b" in which:
+        p["bias_offsets"], p["bias_classes"] = history(rng, rows, classes, 6)
+        p["bias_values"] = (rng.normal(size=len(p["bias_classes"])) * 10).astype(np.float32)
+    if "m" in which:
+        masks = rows if "M" not in which else 3
+        p["allowed"] = rng.integers(0, 1 << 32, (masks, (classes + 31) // 32), dtype=np.uint32)
+        p["allowed"][rng.random(masks) < 0.3] = 0  # nothing left
+        if "M" in which:
+            p["allowed_rows"] = rng.integers(-1, 5, rows).astype(np.int32)  # 3 and 4: behind the last mask
+    return p
+
+
+SHAPES = [(1, 1, 0), (3, 2, 1), (701, 10, 0), (1300, 10, 3), (5, 33, 0), (2, 4095, 0), (3, 4096, 0), (2, 4097, 5), (4, 20003, 0), (2, 70001, 7), (1, 131072, 0)]
+
+
+@ALL
+@pytest.mark.parametrize("rows,classes,pad", SHAPES)
+@pytest.mark.parametrize("which", ["", "hprfs", "hfs", "hr", "cb", "C", "mM", "m", "hprfscbmM"])
+def test_adjust_scores(kind, rows, classes, pad, which):
+    rng = np.random.default_rng(rows * 1000 + classes + len(which))
+    scores = table(rng.normal(size=(rows, classes)) * 4, kind, pad)
+    p = parts(rng, rows, classes, which)
+    a = Adjustment(p)
+    wide = torch.full((rows, classes + pad + 2), 3.0, dtype=TYPES[kind], device="cuda")
+    result = wide[:, :classes]
+    cb.adjust_scores(kind, rows, classes, scores.data_ptr(), scores.stride(0), a.struct, result.data_ptr(), result.stride(0))
+    expected, big = adjusted(exactly(scores), p)
+    # at most six roundings on the way, each of a value of at most `big`
+    compare(exactly(result), expected, 6.01 * u(kind) * big, kind)
+    assert bool((wide[:, classes:] == 3.0).all())
+
+
+@ALL
+def test_adjust_scores_of_infinite_and_undefined_values(kind):
+    rng = np.random.default_rng(5)
+    rows, classes = 6, 5001
+    x = rng.normal(size=(rows, classes))
+    low = float(torch.finfo(TYPES[kind]).min)
+    for value in (np.inf, -np.inf, np.nan, low, -low, 0.0, -0.0):
+        x[rng.random((rows, classes)) < 0.05] = value
+    scores = table(x, kind)
+    p = parts(rng, rows, classes, "hprfmM", 3000)
+    p["repetition"][:] = 1.0  # the largest value stays in range
+    a = Adjustment(p)
+    result = torch.empty_like(scores)
+    cb.adjust_scores(kind, rows, classes, scores.data_ptr(), classes, a.struct, result.data_ptr(), classes)
+    expected, big = adjusted(exactly(scores), p)
+    got = exactly(result)
+    # values next to the type's largest may round to it or to infinity: both are compared at the type's largest
+    most = np.longdouble(torch.finfo(TYPES[kind]).max)
+    near = np.isfinite(expected) & (np.abs(expected) >= most * (1 - HALF[kind] * 4))
+    assert np.array_equal(np.sign(got[near]), np.sign(expected[near])) and bool((np.abs(got[near]) >= most * (1 - HALF[kind] * 4)).all())
+    compare(got[~near], expected[~near], 6.01 * u(kind) * big[~near], kind)
+
+
+def test_adjust_scores_counts_and_last_biases():
+    """Many times the same class, in one row and in rows next to each other; the last of equal biases counts."""
+    rows, classes = 3, 100
+    lengths = [70_000, 0, 65_536]
+    offsets = np.concatenate([[0], np.cumsum(lengths)]).astype(np.int64)
+    ids = np.full(offsets[-1], 99, np.int32)
+    ids[::2] = 0
+    bias_classes = np.tile(np.array([5, 6, 5], np.int32), 1000)
+    p = dict(offsets=offsets, ids=ids, prompts=np.array([10, 5, 65_536], np.int32), frequency=np.ones(rows, np.float32),
+             bias_offsets=np.array([0, 3000, 3000, 3000]), bias_classes=bias_classes, bias_values=np.arange(3000, dtype=np.float32))
+    scores = torch.zeros(rows, classes, device="cuda")
+    a = Adjustment(p)
+    cb.adjust_scores(cb.FLOAT32, rows, classes, scores.data_ptr(), classes, a.struct, scores.data_ptr(), classes)  # in place
+    expected = np.zeros((rows, classes))
+    expected[0, 0], expected[0, 99] = -(35_000 - 5), -(35_000 - 5)
+    expected[0, 5], expected[0, 6] = 2999, 2998
+    np.testing.assert_array_equal(scores.cpu().numpy(), expected)
+
+
+def test_adjust_scores_of_offsets_that_lead_nowhere():
+    """Entries behind HistoryCount and BiasCount are not read, whatever the offsets say."""
+    rows, classes = 2, 40
+    p = dict(offsets=np.array([-5, 3, 1 << 40]), ids=np.array([1, 2, 3, 4], np.int32), presence=np.ones(rows, np.float32),
+             bias_offsets=np.array([0, 1, 1 << 50]), bias_classes=np.array([7, 8], np.int32), bias_values=np.array([1, 2], np.float32))
+    scores = torch.zeros(rows, classes, device="cuda")
+    a = Adjustment(p)
+    cb.adjust_scores(cb.FLOAT32, rows, classes, scores.data_ptr(), classes, a.struct, scores.data_ptr(), classes)
+    expected = np.zeros((rows, classes))
+    expected[0, [1, 2, 3]] = -1
+    expected[1, 4] = -1
+    expected[0, 7], expected[1, 8] = 1, 2
+    np.testing.assert_array_equal(scores.cpu().numpy(), expected)
+
+
+# ---------------------------------------------------------------- the best classes
+
+def best(x, count, among):
+    rows, classes = x.shape
+    index = np.full((rows, count), -1, np.int32)
+    weight = np.zeros((rows, count), np.longdouble)
+    p = np.zeros((rows, classes), np.longdouble)
+    for r in range(rows):
+        usable = [c for c in range(classes) if x[r, c] > -np.inf]  # (not for NaN)
+        order = sorted(usable, key=lambda c: (-x[r, c], c))[:count]
+        over = order if among else usable
+        if not usable:
+            continue
+        most = x[r, order[0]]
+        e = {c: np.longdouble(1) if x[r, c] == most else np.exp(x[r, c] - most) for c in over}
+        total = sum(e.values())
+        for c in over:
+            p[r, c] = e[c] / total
+        index[r, :len(order)] = order
+        weight[r, :len(order)] = [p[r, c] for c in order]
+    return index, weight, p
+
+
+def spread(x):
+    finite = x[np.isfinite(x)]
+    return float(finite.max() - finite.min()) if finite.size else 0.0
+
+
+def weight_error(kind, x):
+    """Relative: the difference to the largest is off by U times itself, the exponential by two, the sum by one for each of at
+    most `classes` additions; numerator and total alike, and a division."""
+    return u(kind) * (2 * (spread(x) + 2) + x.shape[1] + 2)
+
+
+@ALL
+@pytest.mark.parametrize("rows,classes,count,pad", [
+    (1, 1, 1, 0), (5, 2, 2, 0), (70, 3, 4, 1), (1001, 10, 3, 0), (300, 10, 10, 2), (9, 16, 8, 0), (9, 17, 8, 0), (130, 33, 32, 0), (7, 64, 2, 0), (65, 65, 8, 0), (33, 128, 8, 0),
+    (6, 129, 5, 0), (11, 256, 6, 0), (4, 300, 8, 3), (3, 512, 1, 0), (5, 513, 9, 0), (2, 1023, 32, 1), (3, 1024, 16, 0)])
+@pytest.mark.parametrize("among", [False, True])
+def test_select_top(kind, rows, classes, count, pad, among):
+    rng = np.random.default_rng(classes * 100 + count)
+    x = rng.normal(size=(rows, classes)) * 3
+    x[rng.random((rows, classes)) < 0.2] = 1.5  # equal ones
+    x[rng.random((rows, classes)) < 0.1] = -np.inf
+    x[rng.random((rows, classes)) < 0.02] = np.nan
+    if rows > 4:
+        x[1] = -np.inf
+        x[2, 1:] = np.nan
+        x[3] = float(torch.finfo(TYPES[kind]).min)  # the lowest value is a score like any other
+    scores = table(x, kind, pad)
+    indexes = torch.full((rows * count + 1,), 77, dtype=torch.int32, device="cuda")
+    weights = torch.full((rows * count + 1,), 77, dtype=acc(kind), device="cuda")
+    cb.select_top(kind, rows, classes, scores.data_ptr(), scores.stride(0), count, among, indexes.data_ptr(), weights.data_ptr())
+    exact = exactly(scores)
+    index, weight, p = best(exact, count, among)
+    np.testing.assert_array_equal(indexes[:-1].cpu().numpy().reshape(rows, count), index)
+    plain = np.delete(exact, 3, 0) if rows > 4 else exact
+    error = weight_error(kind, plain)
+    # weights below the smallest normal number may be lost
+    compare(exactly(weights[:-1]).reshape(rows, count), weight, error * weight + 2.0 ** -125, kind if kind == cb.FLOAT64 else cb.FLOAT32)
+    assert int(indexes[-1]) == 77 and float(weights[-1]) == 77
+
+    g = rng.normal(size=(rows, count))
+    gradients = torch.from_numpy(g).cuda().to(acc(kind))
+    wide = torch.full((rows, classes + pad + 1), 5.0, dtype=TYPES[kind], device="cuda")
+    cb.select_top_backward(kind, rows, classes, scores.data_ptr(), scores.stride(0), count, among, indexes.data_ptr(), weights.data_ptr(),
+                           gradients.data_ptr(), wide.data_ptr(), wide.stride(0))
+    g = np.where(index >= 0, exactly(gradients), 0)
+    mean = (g * weight).sum(1, keepdims=True)
+    sizes = (np.abs(g) * weight).sum(1, keepdims=True)
+    expected, bound = -p * mean, np.zeros_like(p)
+    # the mean is a sum of `count` products of weights that are off themselves
+    off_mean = sizes * (error + u(kind) * (count + 2))
+    bound = p * off_mean + np.abs(expected) * (error + 3 * u(kind))
+    for r in range(rows):
+        for k in range(count):
+            if index[r, k] >= 0:
+                c = index[r, k]
+                expected[r, c] += weight[r, k] * g[r, k]
+                bound[r, c] += weight[r, k] * abs(g[r, k]) * (error + 3 * u(kind)) + weight[r, k] * abs(mean[r, 0]) * 3 * u(kind)
+    compare(exactly(wide[:, :classes]), expected, bound + 2.0 ** -120, kind)
+    assert bool((wide[:, classes:] == 5.0).all())
+
+
+@ALL
+def test_select_top_of_infinite_scores(kind):
+    x = np.array([[np.inf, 1, np.inf, 0], [np.inf, np.inf, np.inf, np.inf], [1, np.inf, -np.inf, np.nan]])
+    scores = table(x, kind)
+    indexes = torch.empty(3, 3, dtype=torch.int32, device="cuda")
+    weights = torch.empty(3, 3, dtype=acc(kind), device="cuda")
+    for among in (False, True):
+        cb.select_top(kind, 3, 4, scores.data_ptr(), 4, 3, among, indexes.data_ptr(), weights.data_ptr())
+        assert indexes.tolist() == [[0, 2, 1], [0, 1, 2], [1, 0, -1]]
+        third = [1 / 3] * 3 if among else [0.25] * 3
+        np.testing.assert_allclose(weights.cpu().numpy(), [[0.5, 0.5, 0], third, [1, 0, 0]], rtol=2.0 ** -22)
+
+
+@pytest.mark.parametrize("among", [False, True])
+@pytest.mark.parametrize("classes,count", [(7, 3), (40, 5), (200, 8)])
+def test_select_top_gradient_by_differences(classes, count, among):
+    """Central differences in 64 bits: off by the third derivative (below 1 in size, over 6) times the step squared, and by
+    the weights' rounding over the step."""
+    rng = np.random.default_rng(classes)
+    rows, step = 3, 2.0 ** -17
+    x = rng.permutation(rows * classes).reshape(rows, classes) * (4.0 / classes)  # no two nearer than the steps
+    g = rng.normal(size=(rows, count))
+
+    def run(values):
+        scores = table(values, cb.FLOAT64)
+        i, w = torch.empty(rows, count, dtype=torch.int32, device="cuda"), torch.empty(rows, count, dtype=torch.float64, device="cuda")
+        cb.select_top(cb.FLOAT64, rows, classes, scores.data_ptr(), classes, count, among, i.data_ptr(), w.data_ptr())
+        return scores, i, w
+
+    scores, i, w = run(x)
+    dx = torch.empty(rows, classes, dtype=torch.float64, device="cuda")
+    gradients = dev(g)
+    cb.select_top_backward(cb.FLOAT64, rows, classes, 0 if among else scores.data_ptr(), classes, count, among, i.data_ptr(), w.data_ptr(),
+                           gradients.data_ptr(), dx.data_ptr(), classes)
+    size = np.abs(g).sum(1).max()
+    for c in range(0, classes, max(1, classes // 9)):
+        lower, upper = x.copy(), x.copy()
+        lower[:, c] -= step
+        upper[:, c] += step
+        difference = ((run(upper)[2] - run(lower)[2]).cpu().numpy() * g).sum(1) / (2 * step)
+        allowed = size * (step * step + weight_error(cb.FLOAT64, x) / step)
+        assert np.max(np.abs(difference - dx[:, c].cpu().numpy())) <= allowed
+
+
+# ---------------------------------------------------------------- rows sorted by expert and back
+
+def sort(ids, experts):
+    ids = dev(np.asarray(ids, np.int32).reshape(-1))
+    places = torch.full((ids.numel() + 1,), 123, dtype=torch.int32, device="cuda")
+    offsets = torch.full((experts + 2,), 123, dtype=torch.int32, device="cuda")
+    size = cb.sort_by_expert_bytes(ids.numel(), experts)
+    workspace = torch.full((size + 16,), 255, dtype=torch.uint8, device="cuda")
+    cb.sort_by_expert(ids.numel(), experts, ids.data_ptr(), places.data_ptr(), offsets.data_ptr(), workspace.data_ptr(), size)
+    assert int(places[-1]) == 123 and int(offsets[-1]) == 123 and bool((workspace[size:] == 255).all())
+    return places[:-1], offsets[:-1]
+
+
+@pytest.mark.parametrize("slots", [0, 1, 2, 63, 64, 65, 1000, 1023, 1024, 1025, 4095, 4096, 4097, 8192, 8193, 16384, 16385, 70_001, 1_200_000])
+@pytest.mark.parametrize("experts", [1, 2, 7, 64, 255, 256, 257, 1024])
+def test_sort_by_expert(slots, experts):
+    rng = np.random.default_rng(slots + experts)
+    ids = (experts * rng.random(slots) ** 2).astype(np.int32)
+    ids[rng.random(slots) < 0.05] = -1
+    ids[rng.random(slots) < 0.02] = experts
+    ids[rng.random(slots) < 0.01] = np.iinfo(np.int32).min
+    places, offsets = sort(ids, experts)
+    valid = (ids >= 0) & (ids < experts)
+    order = np.argsort(np.where(valid, ids, experts), kind="stable")
+    expected = np.empty(slots, np.int32)
+    expected[order] = np.arange(slots)
+    np.testing.assert_array_equal(places.cpu().numpy(), np.where(valid, expected, -1))
+    np.testing.assert_array_equal(offsets.cpu().numpy(), np.concatenate([[0], np.cumsum(np.bincount(ids[valid], minlength=experts))]))
+
+
+@pytest.mark.parametrize("slots", [500, 50_000])
+def test_sort_by_one_of_many_experts(slots):
+    for ids in (np.full(slots, 5), np.full(slots, -1), np.arange(slots) % 2 * 1023):
+        places, offsets = sort(ids, 1024)
+        valid = ids >= 0
+        order = np.argsort(ids, kind="stable")
+        expected = np.empty(slots, np.int32)
+        expected[order] = np.arange(slots)
+        np.testing.assert_array_equal(places.cpu().numpy(), np.where(valid, expected, -1))
+        assert int(offsets[-1]) == valid.sum()
+
+
+def routed(rng, rows, per_row, spare=3):
+    """Places as a sort gives them, some of none, some behind the last row; with room for more rows."""
+    slots = rows * per_row
+    places = rng.permutation(slots + spare)[:slots].astype(np.int32)
+    places[rng.random(slots) < 0.1] = -1
+    if slots > 3:
+        places[2] = slots + spare + 4
+        places[3] = np.iinfo(np.int32).max
+    return places.reshape(rows, per_row), slots + spare
+
+
+ROWS = [(1, 1, 1, 0), (1, 2, 5, 0), (3, 64, 8, 0), (700, 1, 200, 0), (501, 3, 7, 2), (40, 4, 1000, 0), (9, 2, 4096, 0), (5, 8, 4099, 1), (2, 5, 16384, 0), (1000, 2, 10, 0),
+        (33, 6, 63, 0), (20, 7, 65, 0), (300, 2, 1, 0), (64, 9, 514, 6), (3000, 2, 64, 0)]
+
+
+@ALL
+@pytest.mark.parametrize("rows,per_row,width,pad", ROWS)
+def test_dispatch_rows(kind, rows, per_row, width, pad):
+    rng = np.random.default_rng(rows + width)
+    places, sorted_rows = routed(rng, rows, per_row)
+    x = rng.normal(size=(rows, width))
+    x[rng.random((rows, width)) < 0.01] = np.nan
+    source = table(x, kind, pad)
+    wide = torch.full((sorted_rows, width + pad + 1), 9.0, dtype=TYPES[kind], device="cuda")
+    d = dev(places)
+    cb.dispatch_rows(kind, rows, width, per_row, source.data_ptr(), source.stride(0), d.data_ptr(), wide.data_ptr(), sorted_rows, wide.stride(0))
+    expected = torch.full_like(wide, 9.0)
+    there = (places >= 0) & (places < sorted_rows)
+    expected[torch.from_numpy(places[there].astype(np.int64)).cuda(), :width] = source[torch.from_numpy(np.nonzero(there)[0]).cuda()]
+    bits = torch.int64 if kind == cb.FLOAT64 else torch.int32 if kind == cb.FLOAT32 else torch.int16
+    assert torch.equal(wide.view(bits), expected.view(bits))
+
+
+@ALL
+@pytest.mark.parametrize("rows,per_row,width,pad", ROWS)
+@pytest.mark.parametrize("weighted", [True, False])
+def test_combine_rows_and_gradients(kind, rows, per_row, width, pad, weighted):
+    rng = np.random.default_rng(rows + width + 1)
+    places, sorted_rows = routed(rng, rows, per_row)
+    y = table(rng.normal(size=(sorted_rows, width)), kind, pad, fill=float("nan"))
+    unused = np.setdiff1d(np.arange(sorted_rows), places)
+    y[torch.from_numpy(unused).cuda()] = float("nan")  # what no place names is not read
+    there = (places >= 0) & (places < sorted_rows)
+    weights = rng.normal(size=(rows, per_row))
+    weights[~there] = np.nan  # nor is the weight of none
+    w = dev(weights, acc(kind)) if weighted else None
+    d = dev(places)
+    wide = torch.full((rows, width + pad + 1), 9.0, dtype=TYPES[kind], device="cuda")
+    cb.combine_rows(kind, rows, width, per_row, y.data_ptr(), sorted_rows, y.stride(0), d.data_ptr(), ptr(w), wide.data_ptr(), wide.stride(0))
+    exact_y, exact_w = exactly(y), exactly(w) if weighted else np.ones((rows, per_row), np.longdouble)
+    expected, size = np.zeros((rows, width), np.longdouble), np.zeros((rows, width), np.longdouble)
+    for k in range(per_row):
+        rs = np.nonzero(there[:, k])[0]
+        part = exact_w[rs, k, None] * exact_y[places[rs, k]]
+        expected[rs] += part
+        size[rs] += np.abs(part)
+    compare(exactly(wide[:, :width]), expected, u(kind) * (per_row + 1) * size, kind)  # a product and up to per_row additions each
+    assert bool((wide[:, width:] == 9.0).all())
+
+    g = table(rng.normal(size=(rows, width)), kind, pad, fill=float("nan"))
+    dy = torch.full((sorted_rows, width + pad + 2), 9.0, dtype=TYPES[kind], device="cuda")
+    dw = torch.full((rows * per_row + 1,), 9.0, dtype=acc(kind), device="cuda")
+    cb.combine_rows_backward(kind, rows, width, per_row, g.data_ptr(), g.stride(0), y.data_ptr(), sorted_rows, y.stride(0), d.data_ptr(), ptr(w),
+                             dy.data_ptr(), dy.stride(0), dw.data_ptr())
+    exact_g = exactly(g)
+    expected = np.full((sorted_rows, width), 9.0, np.longdouble)
+    product, size = np.zeros((rows, per_row), np.longdouble), np.zeros((rows, per_row), np.longdouble)
+    for k in range(per_row):
+        rs = np.nonzero(there[:, k])[0]
+        expected[places[rs, k]] = exact_w[rs, k, None] * exact_g[rs]
+        product[rs, k] = (exact_y[places[rs, k]] * exact_g[rs]).sum(1)
+        size[rs, k] = np.abs(exact_y[places[rs, k]] * exact_g[rs]).sum(1)
+    compare(exactly(dy[:, :width]), expected, u(kind) * np.abs(expected), kind)
+    assert bool((dy[:, width:] == 9.0).all())
+    # the columns are added in chains of at most width / 32 + 32 additions, whatever they are split into, after one product
+    compare(exactly(dw[:-1]).reshape(rows, per_row), product, u(kind) * (width // 32 + 33) * size, kind if kind == cb.FLOAT64 else cb.FLOAT32)
+    assert float(dw[-1]) == 9.0
+
+    # either alone
+    dy2, dw2 = torch.full_like(dy, 9.0), torch.full_like(dw, 9.0)
+    cb.combine_rows_backward(kind, rows, width, per_row, g.data_ptr(), g.stride(0), 0, sorted_rows, y.stride(0), d.data_ptr(), ptr(w), dy2.data_ptr(),
+                             dy2.stride(0), 0)
+    cb.combine_rows_backward(kind, rows, width, per_row, g.data_ptr(), g.stride(0), y.data_ptr(), sorted_rows, y.stride(0), d.data_ptr(), ptr(w), 0,
+                             0, dw2.data_ptr())
+    assert torch.equal(dy, dy2) and torch.equal(dw, dw2)
+
+
+@ALL
+def test_no_sorted_rows(kind):
+    places = torch.full((4, 2), -1, dtype=torch.int32, device="cuda")
+    result = torch.full((4, 8), 9.0, dtype=TYPES[kind], device="cuda")
+    cb.combine_rows(kind, 4, 8, 2, 0, 0, 8, places.data_ptr(), 0, result.data_ptr(), 8)
+    assert bool((result == 0).all())
+    dw = torch.full((4, 2), 9.0, dtype=acc(kind), device="cuda")
+    cb.combine_rows_backward(kind, 4, 8, 2, result.data_ptr(), 8, 0, 0, 8, places.data_ptr(), 0, 0, 8, dw.data_ptr())
+    assert bool((dw == 0).all())
+
+
+# ---------------------------------------------------------------- together, streams, graphs
+
+def mixture(kind, x, gate, bias, experts, per_row, stream, buffers):
+    """A layer of experts: gate scores with biases, the best experts, rows to them and back. Every expert doubles its rows."""
+    rows, width = x.shape
+    b = buffers
+    cb.adjust_scores(cb.FLOAT32, rows, experts, gate.data_ptr(), experts, bias.struct, b["scores"].data_ptr(), experts, stream)
+    cb.select_top(cb.FLOAT32, rows, experts, b["scores"].data_ptr(), experts, per_row, True, b["ids"].data_ptr(), b["weights"].data_ptr(), stream)
+    cb.sort_by_expert(rows * per_row, experts, b["ids"].data_ptr(), b["places"].data_ptr(), b["offsets"].data_ptr(), b["workspace"].data_ptr(),
+                      b["workspace"].numel(), stream)
+    cb.dispatch_rows(kind, rows, width, per_row, x.data_ptr(), width, b["places"].data_ptr(), b["sorted"].data_ptr(), rows * per_row, width, stream)
+    torch.mul(b["sorted"], 2, out=b["sorted"])
+    cb.combine_rows(kind, rows, width, per_row, b["sorted"].data_ptr(), rows * per_row, width, b["places"].data_ptr(), b["weights"].data_ptr(),
+                    b["result"].data_ptr(), width, stream)
+    cb.combine_rows_backward(kind, rows, width, per_row, x.data_ptr(), width, b["sorted"].data_ptr(), rows * per_row, width, b["places"].data_ptr(),
+                             b["weights"].data_ptr(), b["sorted_gradients"].data_ptr(), width, b["weight_gradients"].data_ptr(), stream)
+    cb.select_top_backward(cb.FLOAT32, rows, experts, b["scores"].data_ptr(), experts, per_row, True, b["ids"].data_ptr(), b["weights"].data_ptr(),
+                           b["weight_gradients"].data_ptr(), b["gate_gradients"].data_ptr(), experts, stream)
+    return b
+
+
+def mixture_buffers(kind, rows, width, experts, per_row):
+    def empty(*shape, dtype=torch.float32):
+        return torch.zeros(shape, dtype=dtype, device="cuda")
+
+    slots = rows * per_row
+    return dict(scores=empty(rows, experts), ids=empty(rows, per_row, dtype=torch.int32), weights=empty(rows, per_row), places=empty(slots, dtype=torch.int32),
+                offsets=empty(experts + 1, dtype=torch.int32), workspace=empty(cb.sort_by_expert_bytes(slots, experts), dtype=torch.uint8),
+                sorted=empty(slots, width, dtype=TYPES[kind]), result=empty(rows, width, dtype=TYPES[kind]),
+                sorted_gradients=empty(slots, width, dtype=TYPES[kind]), weight_gradients=empty(rows, per_row), gate_gradients=empty(rows, experts))
+
+
+def check_mixture(kind, x, b):
+    # weights add up to 1 (five roundings), experts double: the result is twice the input
+    exact = exactly(x)
+    compare(exactly(b["result"]), 2 * exact, 16 * u(kind) * np.abs(exact), kind)
+    # the product of a row and twice itself
+    norm = 2 * (exact * exact).sum(1, keepdims=True)
+    compare(exactly(b["weight_gradients"]), np.broadcast_to(norm, b["weight_gradients"].shape), u(kind) * (x.shape[1] // 32 + 33) * norm, cb.FLOAT32)
+
+
+@pytest.mark.parametrize("kind", [cb.FLOAT32, cb.BFLOAT16], ids=NAMES.get)
+@pytest.mark.parametrize("rows,width", [(3, 100), (2500, 64)])
+def test_a_layer_of_experts_on_a_stream_and_in_graphs(kind, rows, width):
+    experts, per_row = 9, 3
+    rng = np.random.default_rng(rows)
+    allowed = np.full((1, 1), 0b111011011, np.uint32)
+    bias = Adjustment(dict(class_bias=rng.normal(size=(1, experts)).astype(np.float32), allowed=allowed, allowed_rows=np.zeros(rows, np.int32)))
+    inputs = [(table(rng.normal(size=(rows, width)), kind), dev(rng.normal(size=(rows, experts)).astype(np.float32))) for _ in range(3)]
+    eager = []
+    for x, gate in inputs:
+        b = mixture(kind, x, gate, bias, experts, per_row, None, mixture_buffers(kind, rows, width, experts, per_row))
+        check_mixture(kind, x, b)
+        ids = b["ids"].cpu().numpy()
+        assert not np.isin(ids, [2, 5]).any() and (ids >= 0).all()
+        eager.append({k: v.clone() for k, v in b.items() if k != "workspace"})
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        b = mixture(kind, *inputs[1], bias, experts, per_row, side.cuda_stream, mixture_buffers(kind, rows, width, experts, per_row))
+    side.synchronize()
+    for k, v in eager[1].items():
+        assert torch.equal(b[k], v), k
+    # two graphs with buffers of their own, replayed in turn with eager work between
+    graphs = []
+    for _ in range(2):
+        x, gate = torch.zeros_like(inputs[0][0]), torch.zeros_like(inputs[0][1])
+        buffers = mixture_buffers(kind, rows, width, experts, per_row)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            mixture(kind, x, gate, bias, experts, per_row, torch.cuda.current_stream().cuda_stream, buffers)
+        graphs.append((graph, x, gate, buffers))
+    for turn in range(6):
+        at = turn % 3
+        graph, x, gate, buffers = graphs[turn % 2]
+        x.copy_(inputs[at][0])
+        gate.copy_(inputs[at][1])
+        graph.replay()
+        mixture(kind, *inputs[(at + 1) % 3], bias, experts, per_row, None, mixture_buffers(kind, rows, width, experts, per_row))
+        torch.cuda.synchronize()
+        for k, v in eager[at].items():
+            assert torch.equal(buffers[k], v), (turn, k)
+
+
+def test_a_stream_that_is_not_given_is_the_default_one():
+    x = torch.ones(1000, 100, device="cuda")
+    a = Adjustment(dict(class_bias=np.ones((1, 100), np.float32)))
+    for _ in range(5):
+        x.mul_(2)
+        cb.adjust_scores(cb.FLOAT32, 1000, 100, x.data_ptr(), 100, a.struct, x.data_ptr(), 100)
+    assert bool((x == 63).all())
+
+
+def test_host_memory_is_refused():
+    x = torch.ones(4, 4)
+    with pytest.raises(cb.CatBoostError, match="memory that a GPU can write"):
+        cb.adjust_scores(cb.FLOAT32, 4, 4, x.data_ptr(), 4, cb.score_adjustment(), x.data_ptr(), 4)
+    # and leaves no error behind for the next call
+    y = torch.ones(4, 4, device="cuda")
+    cb.adjust_scores(cb.FLOAT32, 4, 4, y.data_ptr(), 4, cb.score_adjustment(), y.data_ptr(), 4)
+    torch.cuda.synchronize()

@@ -5,10 +5,13 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
+#include <mutex>
 #include <string>
 #include <tuple>
 #include <utility>
+#include <vector>
 
 namespace cbamd {
 namespace op {
@@ -37,9 +40,10 @@ public:
             OP_HIP_CHECK(hipStreamGetDevice(Stream, &device));
             CBAMD_ENSURE(device == attributes.device, "the stream and the output are on different devices");
         }
+        Device = attributes.device;
         OP_HIP_CHECK(hipGetDevice(&Previous));
-        if (Previous != attributes.device) {
-            OP_HIP_CHECK(hipSetDevice(attributes.device));
+        if (Previous != Device) {
+            OP_HIP_CHECK(hipSetDevice(Device));
             Changed = true;
         }
     }
@@ -54,12 +58,29 @@ public:
     // (the launch's own status: hipGetLastError would also hand over what another library's call left behind)
     template <typename... TParams, typename... TArgs>
     void Launch(void (*kernel)(TParams...), size_t groups, uint32_t threads, size_t ldsBytes, TArgs&&... args) const {
-        std::pair<int, std::tuple<TParams...>> held(0, std::tuple<TParams...>(std::forward<TArgs>(args)...));
-        LaunchHeld(reinterpret_cast<const void*>(kernel), groups, threads, ldsBytes, held.second,
+        std::tuple<TParams...> held(std::forward<TArgs>(args)...);
+        LaunchHeld(reinterpret_cast<const void*>(kernel), groups, threads, ldsBytes, held,
                    std::index_sequence_for<TParams...>());
     }
 
+    // A kernel that uses more than 64 KB of dynamic LDS has to be told so, once for each device
+    void AllowLds(const void* kernel, size_t bytes) const {
+        if (bytes <= 64 * 1024) {
+            return;
+        }
+        static std::mutex lock;
+        static std::vector<std::pair<int, const void*>> told;
+        std::lock_guard<std::mutex> guard(lock);
+        const std::pair<int, const void*> item(Device, kernel);
+        if (std::find(told.begin(), told.end(), item) == told.end()) {
+            OP_HIP_CHECK(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kMaxLds));
+            told.push_back(item);
+        }
+    }
+
 private:
+    static constexpr int kMaxLds = 160 * 1024;
+
     template <typename TTuple, size_t... I>
     void LaunchHeld(const void* kernel, size_t groups, uint32_t threads, size_t ldsBytes, TTuple& held,
                     std::index_sequence<I...>) const {
@@ -68,6 +89,7 @@ private:
     }
 
     hipStream_t Stream = nullptr;
+    int Device = 0;
     int Previous = 0;
     bool Changed = false;
 };

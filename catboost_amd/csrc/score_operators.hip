@@ -16,7 +16,7 @@ struct TAdjustArgs {
     size_t ScoreStride, ResultStride;
     size_t Rows, Tiles;
     uint32_t Classes, Slices;
-    uint32_t RowsPerTile, LanesPerRow, Pitch;  // of AdjustRowsKernel
+    uint32_t RowsPerTile, Pitch, PiecesInverse;  // of AdjustRowsKernel
     CbHipScoreAdjustment A;
 };
 
@@ -24,25 +24,23 @@ __device__ __forceinline__ int64_t Clamped(int64_t at, size_t count) {
     return at < 0 ? 0 : at > static_cast<int64_t>(count) ? static_cast<int64_t>(count) : at;
 }
 
-// What a row's scores have in common
-template <typename A>
-struct TRowAdjustment {
-    A Repetition, Frequency, Presence;
-    const float* ClassBias;
-    const uint32_t* Allowed;  // null: no mask
+// The mask that a row has, -1: none
+__device__ __forceinline__ int64_t MaskOf(const CbHipScoreAdjustment& p, size_t row) {
+    if (p.Allowed == nullptr) {
+        return -1;
+    }
+    const int64_t mask = p.AllowedRows != nullptr ? static_cast<int64_t>(p.AllowedRows[row]) : static_cast<int64_t>(row);
+    return mask >= 0 && static_cast<size_t>(mask) < p.AllowedCount ? mask : -1;
+}
 
-    __device__ __forceinline__ TRowAdjustment(const CbHipScoreAdjustment& p, size_t row) {
-        Repetition = p.HistoryOffsets != nullptr && p.Repetition != nullptr ? p.Repetition[row] : 1.f;
-        Frequency = p.HistoryOffsets != nullptr && p.Frequency != nullptr ? p.Frequency[row] : 0.f;
-        Presence = p.HistoryOffsets != nullptr && p.Presence != nullptr ? p.Presence[row] : 0.f;
-        ClassBias = p.ClassBias != nullptr ? p.ClassBias + row * p.ClassBiasStride : nullptr;
-        Allowed = nullptr;
-        if (p.Allowed != nullptr) {
-            const int64_t mask = p.AllowedRows != nullptr ? static_cast<int64_t>(p.AllowedRows[row]) : static_cast<int64_t>(row);
-            if (mask >= 0 && static_cast<size_t>(mask) < p.AllowedCount) {
-                Allowed = p.Allowed + static_cast<size_t>(mask) * p.AllowedStride;
-            }
-        }
+// What a row's scores have in common. A part that a call leaves out has the value that changes nothing: a repetition penalty
+// of 1, a frequency and a presence penalty of 0
+struct TPenalties {
+    float Repetition, Frequency, Presence;
+
+    __device__ __forceinline__ static TPenalties Of(const CbHipScoreAdjustment& p, size_t row) {
+        return {p.Repetition != nullptr ? p.Repetition[row] : 1.f, p.Frequency != nullptr ? p.Frequency[row] : 0.f,
+                p.Presence != nullptr ? p.Presence[row] : 0.f};
     }
 };
 
@@ -57,11 +55,10 @@ __device__ __forceinline__ void CountEntry(uint32_t* word, bool given) {
     }
 }
 
-// N scores from class c on: `words` and `last` their places in the two tables, or null. (A part that a call leaves out has
-// the value that changes nothing: a repetition penalty of 1, a frequency and a presence penalty of 0.)
+// N scores from class c on: `words` and `last` their places in the two tables, or null; `mask` the row's words, or null
 template <typename T, int N>
-__device__ __forceinline__ void AdjustValues(TValues<T, N>& v, const TRowAdjustment<TAcc<T>>& row, const CbHipScoreAdjustment& p, uint32_t c, uint32_t classes,
-                                             const uint32_t* words, const uint32_t* last, int64_t firstBias) {
+__device__ __forceinline__ void AdjustValues(TValues<T, N>& v, const TPenalties& penalties, const CbHipScoreAdjustment& p, size_t row, uint32_t c,
+                                             uint32_t classes, const uint32_t* words, const uint32_t* last, int64_t firstBias, const uint32_t* mask) {
     using A = TAcc<T>;
     A x[N];
 #pragma unroll
@@ -79,20 +76,22 @@ __device__ __forceinline__ void AdjustValues(TValues<T, N>& v, const TRowAdjustm
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 if (w[i] != 0) {
-                    x[i] = x[i] > 0 ? x[i] / row.Repetition : x[i] * row.Repetition;
+                    const A repetition = penalties.Repetition;
+                    x[i] = x[i] > 0 ? x[i] / repetition : x[i] * repetition;
                 }
                 if (w[i] > 1) {
-                    x[i] -= row.Frequency * static_cast<A>(w[i] >> 1);
-                    x[i] -= row.Presence;
+                    x[i] -= static_cast<A>(penalties.Frequency) * static_cast<A>(w[i] >> 1);
+                    x[i] -= static_cast<A>(penalties.Presence);
                 }
             }
         }
     }
-    if (row.ClassBias != nullptr) {
+    if (p.ClassBias != nullptr) {
+        const float* bias = p.ClassBias + row * p.ClassBiasStride + c;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             if (c + i < classes) {
-                x[i] += row.ClassBias[c + i];
+                x[i] += bias[i];
             }
         }
     }
@@ -104,9 +103,9 @@ __device__ __forceinline__ void AdjustValues(TValues<T, N>& v, const TRowAdjustm
             }
         }
     }
-    if (row.Allowed != nullptr) {
+    if (mask != nullptr) {
         // (N classes from a multiple of N on are in one word)
-        const uint32_t bits = row.Allowed[c >> 5] >> (c & 31);
+        const uint32_t bits = mask[c >> 5] >> (c & 31);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             x[i] = (bits >> i & 1) != 0 ? x[i] : -std::numeric_limits<A>::infinity();
@@ -151,7 +150,6 @@ __device__ __forceinline__ void StoreUpTo(const TValues<T, N>& v, T* at, uint32_
 // they arrive meanwhile; every slice of a row looks through the row's whole history.
 template <typename T, int THREADS, int P>
 __global__ void __launch_bounds__(THREADS) AdjustSliceKernel(TAdjustArgs a) {
-    using A = TAcc<T>;
     constexpr int N = 16 / sizeof(T);
     constexpr uint32_t S = THREADS * P * N;
     extern __shared__ uint4 tables[];
@@ -208,21 +206,24 @@ __global__ void __launch_bounds__(THREADS) AdjustSliceKernel(TAdjustArgs a) {
             }
             __syncthreads();
         }
-        const TRowAdjustment<A> common(p, row);
+        const TPenalties penalties = history ? TPenalties::Of(p, row) : TPenalties{1, 0, 0};
+        const int64_t maskRow = MaskOf(p, row);
+        const uint32_t* mask = maskRow >= 0 ? p.Allowed + static_cast<size_t>(maskRow) * p.AllowedStride : nullptr;
         T* to = static_cast<T*>(a.Result) + row * a.ResultStride + c0;
 #pragma unroll
         for (int j = 0; j < P; ++j) {
             const uint32_t c = (j * THREADS + threadIdx.x) * N;
             if (c < width) {
-                AdjustValues<T, N>(v[j], common, p, c0 + c, a.Classes, history ? words + c : nullptr, biases ? last + c : nullptr, firstBias);
+                AdjustValues<T, N>(v[j], penalties, p, row, c0 + c, a.Classes, history ? words + c : nullptr, biases ? last + c : nullptr,
+                                   firstBias, mask);
                 StoreUpTo<T, N>(v[j], to + c, width - c);
             }
         }
     }
 }
 
-// Rows that are shorter than a slice: a workgroup for RowsPerTile of them, LanesPerRow threads for a row's pieces
-constexpr uint32_t kMaxRowsPerTile = 256;
+// Rows that are shorter than a slice: a workgroup for RowsPerTile of them
+constexpr uint32_t kMaxRowsPerTile = 512;
 
 // The row that entry `e` of a list with these offsets belongs to: the last one that begins at or before it
 __device__ __forceinline__ uint32_t RowOfEntry(const int64_t* offsets, uint32_t rows, int64_t e) {
@@ -238,72 +239,91 @@ __device__ __forceinline__ uint32_t RowOfEntry(const int64_t* offsets, uint32_t 
     return low;
 }
 
+// f(entry, row, class) for every entry of a tile's rows. A thread takes four entries at a time: it searches for the row of
+// the first and goes on from there.
+template <typename F>
+__device__ __forceinline__ void ForEntries(const int64_t* offsets, uint32_t rows, int64_t begin, int64_t end, const int32_t* classes, F&& f) {
+    for (int64_t e = begin + threadIdx.x * 4; e < end; e += 256 * 4) {
+        const uint32_t n = end - e < 4 ? static_cast<uint32_t>(end - e) : 4;
+        const TValues<int32_t, 4> c = LoadUpTo<int32_t, 4>(classes + e, n);
+        uint32_t r = RowOfEntry(offsets, rows, e);
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            if (i < n) {
+                while (r + 1 < rows && offsets[r + 1] <= e + i) {
+                    ++r;
+                }
+                f(e + i, r, static_cast<uint32_t>(c.V[i]));
+            }
+        }
+    }
+}
+
+// Pieces are taken in the order in which they are in memory, whatever the rows' length, so that a wave's stores fill whole
+// lines (a thread for a row, at ten 64-bit values each, wrote 413 MB for 160)
 template <typename T>
 __global__ void __launch_bounds__(256) AdjustRowsKernel(TAdjustArgs a) {
-    using A = TAcc<T>;
     constexpr int N = 16 / sizeof(T);
     extern __shared__ uint4 tables[];
     __shared__ int64_t offsets[kMaxRowsPerTile];
+    __shared__ int64_t given[kMaxRowsPerTile];  // where the generated entries begin
+    __shared__ TPenalties penalties[kMaxRowsPerTile];
+    __shared__ int64_t masks[kMaxRowsPerTile];
     const CbHipScoreAdjustment& p = a.A;
     const bool history = p.HistoryOffsets != nullptr, biases = p.BiasOffsets != nullptr;
+    const uint32_t pieces = a.Pitch / N;
     const uint32_t tableWords = a.RowsPerTile * a.Pitch;
     uint32_t* words = reinterpret_cast<uint32_t*>(tables);
     uint32_t* last = history ? words + tableWords : words;
-    const uint32_t lane = threadIdx.x & (a.LanesPerRow - 1), first = threadIdx.x / a.LanesPerRow;
     for (size_t tile = blockIdx.x; tile < a.Tiles; tile += gridDim.x) {
         const size_t r0 = tile * a.RowsPerTile;
         const uint32_t rows = static_cast<uint32_t>(a.Rows - r0 < a.RowsPerTile ? a.Rows - r0 : a.RowsPerTile);
         int64_t firstBias = 0;
-        if (history || biases) {
-            __syncthreads();  // the tile before this one is done with the tables
-            for (uint32_t i = threadIdx.x; i < tableWords * (history + biases); i += 256) {
-                words[i] = 0;
+        __syncthreads();  // the tile before this one is done with the tables
+        for (uint32_t i = threadIdx.x; i < (tableWords * (history + biases) + 3) / 4; i += 256) {
+            tables[i] = uint4{0, 0, 0, 0};
+        }
+        for (uint32_t r = threadIdx.x; r < rows; r += 256) {
+            masks[r] = MaskOf(p, r0 + r);
+            if (history) {
+                offsets[r] = p.HistoryOffsets[r0 + r];
+                given[r] = offsets[r] + (p.PromptLengths != nullptr ? p.PromptLengths[r0 + r] : 0);
+                penalties[r] = TPenalties::Of(p, r0 + r);
             }
         }
+        __syncthreads();
         if (history) {
-            if (threadIdx.x < rows) {
-                offsets[threadIdx.x] = p.HistoryOffsets[r0 + threadIdx.x];
-            }
+            ForEntries(offsets, rows, Clamped(offsets[0], p.HistoryCount), Clamped(p.HistoryOffsets[r0 + rows], p.HistoryCount), p.History,
+                       [&](int64_t e, uint32_t r, uint32_t c) {
+                           if (c < a.Classes) {
+                               CountEntry(&words[r * a.Pitch + c], e < given[r]);
+                           }
+                       });
             __syncthreads();
-            const int64_t begin = Clamped(offsets[0], p.HistoryCount);
-            const int64_t end = Clamped(p.HistoryOffsets[r0 + rows], p.HistoryCount);
-            for (int64_t e = begin + threadIdx.x; e < end; e += 256) {
-                const uint32_t c = static_cast<uint32_t>(p.History[e]);
-                if (c < a.Classes) {
-                    const uint32_t r = RowOfEntry(offsets, rows, e);
-                    CountEntry(&words[r * a.Pitch + c], p.PromptLengths != nullptr && e - offsets[r] < p.PromptLengths[r0 + r]);
-                }
-            }
         }
         if (biases) {
-            __syncthreads();
-            if (threadIdx.x < rows) {
-                offsets[threadIdx.x] = p.BiasOffsets[r0 + threadIdx.x];
+            for (uint32_t r = threadIdx.x; r < rows; r += 256) {
+                offsets[r] = p.BiasOffsets[r0 + r];
             }
             __syncthreads();
             firstBias = Clamped(offsets[0], p.BiasCount);
-            const int64_t end = Clamped(p.BiasOffsets[r0 + rows], p.BiasCount);
-            for (int64_t e = firstBias + threadIdx.x; e < end; e += 256) {
-                const uint32_t c = static_cast<uint32_t>(p.BiasClasses[e]);
-                if (c < a.Classes) {
-                    atomicMax(&last[RowOfEntry(offsets, rows, e) * a.Pitch + c], static_cast<uint32_t>(e - firstBias) + 1);
-                }
-            }
-        }
-        if (history || biases) {
+            ForEntries(offsets, rows, firstBias, Clamped(p.BiasOffsets[r0 + rows], p.BiasCount), p.BiasClasses,
+                       [&](int64_t e, uint32_t r, uint32_t c) {
+                           if (c < a.Classes) {
+                               atomicMax(&last[r * a.Pitch + c], static_cast<uint32_t>(e - firstBias) + 1);
+                           }
+                       });
             __syncthreads();
         }
-        for (uint32_t r = first; r < rows; r += 256 / a.LanesPerRow) {
+        for (uint32_t q = threadIdx.x; q < rows * pieces; q += 256) {
+            const uint32_t r = a.PiecesInverse != 0 ? __umulhi(q, a.PiecesInverse) : q;
+            const uint32_t c = (q - r * pieces) * N;
             const size_t row = r0 + r;
-            const TRowAdjustment<A> common(p, row);
-            const T* from = static_cast<const T*>(a.Scores) + row * a.ScoreStride;
-            T* to = static_cast<T*>(a.Result) + row * a.ResultStride;
-            for (uint32_t c = lane * N; c < a.Classes; c += a.LanesPerRow * N) {
-                TValues<T, N> v = LoadUpTo<T, N>(from + c, a.Classes - c);
-                AdjustValues<T, N>(v, common, p, c, a.Classes, history ? words + r * a.Pitch + c : nullptr, biases ? last + r * a.Pitch + c : nullptr,
-                                   firstBias);
-                StoreUpTo<T, N>(v, to + c, a.Classes - c);
-            }
+            TValues<T, N> v = LoadUpTo<T, N>(static_cast<const T*>(a.Scores) + row * a.ScoreStride + c, a.Classes - c);
+            const int64_t mask = masks[r];
+            AdjustValues<T, N>(v, penalties[r], p, row, c, a.Classes, history ? words + q * N : nullptr, biases ? last + q * N : nullptr, firstBias,
+                               mask >= 0 ? p.Allowed + static_cast<size_t>(mask) * p.AllowedStride : nullptr);
+            StoreUpTo<T, N>(v, static_cast<T*>(a.Result) + row * a.ResultStride + c, a.Classes - c);
         }
     }
 }
@@ -339,31 +359,47 @@ struct TRanked {
         bits = (bits & sign) != 0 ? static_cast<Bits>(bits & ~sign) : static_cast<Bits>(~bits);
         return IsNone() ? -std::numeric_limits<float>::infinity() : static_cast<float>(__builtin_bit_cast(T, bits));
     }
-    __device__ __forceinline__ TRanked Better(const TRanked& other) const { return other.K > K ? other : *this; }
-    __device__ __forceinline__ bool Same(const TRanked& other) const { return K == other.K; }
+    __device__ __forceinline__ TRanked Better(const TRanked& other) const { return {other.K > K ? other.K : K}; }
+    // the same for an `other` whose class is the higher one
+    __device__ __forceinline__ TRanked BetterLater(const TRanked& other) const { return Better(other); }
+    __device__ __forceinline__ TRanked Without(const TRanked& other) const { return {K == other.K ? Key(0) : K}; }
+    __device__ __forceinline__ TRanked Or(const TRanked& other, bool take) const { return {take ? other.K : K}; }
 };
 template <>
 struct TRanked<double> {
     double Value;
-    uint32_t C, Unused;
+    uint32_t C;
 
-    __device__ __forceinline__ static TRanked None() { return {-std::numeric_limits<double>::infinity(), ~0u, 0}; }
+    __device__ __forceinline__ static TRanked None() { return {-std::numeric_limits<double>::infinity(), ~0u}; }
     __device__ __forceinline__ static TRanked Of(double x, uint32_t c) {
-        return x > -std::numeric_limits<double>::infinity() ? TRanked{x, c, 0} : None();
+        const bool usable = x > -std::numeric_limits<double>::infinity();
+        return {usable ? x : -std::numeric_limits<double>::infinity(), usable ? c : ~0u};
     }
     __device__ __forceinline__ bool IsNone() const { return C == ~0u; }
     __device__ __forceinline__ uint32_t Class() const { return C; }
     __device__ __forceinline__ double Score() const { return Value; }
     __device__ __forceinline__ TRanked Better(const TRanked& other) const {
-        return other.Value > Value || (other.Value == Value && other.C < C) ? other : *this;
+        const bool take = other.Value > Value || (other.Value == Value && other.C < C);
+        return {take ? other.Value : Value, take ? other.C : C};
     }
-    __device__ __forceinline__ bool Same(const TRanked& other) const { return C == other.C; }
+    __device__ __forceinline__ TRanked BetterLater(const TRanked& other) const {
+        const bool take = other.Value > Value;
+        return {take ? other.Value : Value, take ? other.C : C};
+    }
+    __device__ __forceinline__ TRanked Without(const TRanked& other) const {
+        const bool gone = C == other.C;
+        return {gone ? -std::numeric_limits<double>::infinity() : Value, gone ? ~0u : C};
+    }
+    __device__ __forceinline__ TRanked Or(const TRanked& other, bool take) const { return {take ? other.Value : Value, take ? other.C : C}; }
 };
 
 // What a lane gets from another one: STEP lanes on, around in its row of 16 (a modifier of the instruction that uses it, and
 // no trip through LDS), or the lane whose number differs in the bit STEP
 template <int STEP, typename V>
 __device__ __forceinline__ V FromLane(const V& x) {
+    if constexpr (std::is_same_v<V, TRanked<double>>) {
+        return {FromLane<STEP>(x.Value), FromLane<STEP>(x.C)};
+    } else {
     V r;
     constexpr int words = sizeof(V) / 4;
     int from[words], to[words];
@@ -378,6 +414,7 @@ __device__ __forceinline__ V FromLane(const V& x) {
     }
     __builtin_memcpy(&r, to, sizeof(V));
     return r;
+    }
 }
 
 // f over the values of a group of 16 or 64 lanes, in the same order in each of them
@@ -445,25 +482,26 @@ __global__ void __launch_bounds__(256) SelectTopKernel(TTopArgs<T> a, int32_t* i
             R best = left[0];
 #pragma unroll
             for (int j = 1; j < V; ++j) {
-                best = best.Better(left[j]);
+                best = best.BetterLater(left[j]);
             }
             best = OverGroup<G>(best, [](const R& x, const R& y) { return x.Better(y); });
             if (k == 0) {
                 most = best.Score();
                 if (!a.Among) {
+                    // (what is never selected has a weight of 0; where nothing else is there the sum is not used)
 #pragma unroll
                     for (int j = 0; j < V; ++j) {
-                        total += left[j].IsNone() ? A(0) : WeightOf(left[j].Score(), most);
+                        total += WeightOf(left[j].Score(), most);
                     }
                 }
             }
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                left[j] = left[j].Same(best) ? R::None() : left[j];
+                left[j] = left[j].Without(best);
             }
 #pragma unroll
             for (int i = 0; i < kept; ++i) {
-                mine[i] = k == lane + i * G ? best : mine[i];
+                mine[i] = mine[i].Or(best, k == lane + i * G);
             }
         }
         A e[kept];
@@ -502,48 +540,68 @@ __device__ __forceinline__ TValues<T, C> LoadRow(const T* from, uint32_t classes
     return v;
 }
 
-// Rows of few classes: a thread for a row of at most C
+// Rows of few classes: a thread for a row of at most C (classes behind the row's last are left out by branches that every
+// lane takes alike). What is stored goes through LDS, so that a wave's stores fill whole lines.
 template <typename T, int C>
 __global__ void __launch_bounds__(256) SelectTopOfFewKernel(TTopArgs<T> a, int32_t* indexes, TAcc<T>* weights) {
     using A = TAcc<T>;
     using R = TRanked<T>;
-    for (size_t row = size_t(blockIdx.x) * 256 + threadIdx.x; row < a.Rows; row += size_t(gridDim.x) * 256) {
-        const TValues<T, C> v = LoadRow<T, C>(a.Scores + row * a.Stride, a.Classes);
-        R left[C];
-#pragma unroll
-        for (int j = 0; j < C; ++j) {
-            left[j] = static_cast<uint32_t>(j) < a.Classes ? R::Of(v.V[j], j) : R::None();
-        }
-        A most = 0, total = 0;
-        for (uint32_t k = 0; k < a.Count; ++k) {
-            R best = left[0];
-#pragma unroll
-            for (int j = 1; j < C; ++j) {
-                best = best.Better(left[j]);
-            }
-            if (k == 0) {
-                most = best.Score();
-                if (!a.Among) {
-#pragma unroll
-                    for (int j = 0; j < C; ++j) {
-                        total += left[j].IsNone() ? A(0) : WeightOf(left[j].Score(), most);
-                    }
-                }
-            }
+    extern __shared__ uint4 tables[];
+    A* outWeights = reinterpret_cast<A*>(tables);
+    int32_t* outIndexes = reinterpret_cast<int32_t*>(outWeights + 256 * a.Count);
+    for (size_t r0 = size_t(blockIdx.x) * 256; r0 < a.Rows; r0 += size_t(gridDim.x) * 256) {
+        const uint32_t rows = static_cast<uint32_t>(a.Rows - r0 < 256 ? a.Rows - r0 : 256);
+        if (threadIdx.x < rows) {
+            const TValues<T, C> v = LoadRow<T, C>(a.Scores + (r0 + threadIdx.x) * a.Stride, a.Classes);
+            R left[C];
 #pragma unroll
             for (int j = 0; j < C; ++j) {
-                left[j] = left[j].Same(best) ? R::None() : left[j];
+                left[j] = static_cast<uint32_t>(j) < a.Classes ? R::Of(v.V[j], j) : R::None();
             }
-            const A e = best.IsNone() ? A(0) : WeightOf(best.Score(), most);
-            indexes[row * a.Count + k] = best.IsNone() ? -1 : static_cast<int32_t>(best.Class());
-            weights[row * a.Count + k] = a.Among || best.IsNone() ? e : e / total;
-            total += a.Among ? e : A(0);
-        }
-        if (a.Among && total > 0) {
+            A* myWeights = outWeights + threadIdx.x * a.Count;
+            int32_t* myIndexes = outIndexes + threadIdx.x * a.Count;
+            A most = 0, total = 0;
             for (uint32_t k = 0; k < a.Count; ++k) {
-                weights[row * a.Count + k] /= total;
+                R best = left[0];
+#pragma unroll
+                for (int j = 1; j < C; ++j) {
+                    if (static_cast<uint32_t>(j) < a.Classes) {
+                        best = best.BetterLater(left[j]);
+                    }
+                }
+                if (k == 0) {
+                    most = best.Score();
+                    if (!a.Among) {
+                        // (what is never selected has a weight of 0; where nothing else is there the sum is not used)
+#pragma unroll
+                        for (int j = 0; j < C; ++j) {
+                            if (static_cast<uint32_t>(j) < a.Classes) {
+                                total += WeightOf(left[j].Score(), most);
+                            }
+                        }
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < C; ++j) {
+                    if (static_cast<uint32_t>(j) < a.Classes) {
+                        left[j] = left[j].Without(best);
+                    }
+                }
+                const A e = best.IsNone() ? A(0) : WeightOf(best.Score(), most);
+                myIndexes[k] = best.IsNone() ? -1 : static_cast<int32_t>(best.Class());
+                myWeights[k] = e;
+                total += a.Among ? e : A(0);
+            }
+            for (uint32_t k = 0; k < a.Count; ++k) {
+                myWeights[k] = myIndexes[k] < 0 ? A(0) : myWeights[k] / total;
             }
         }
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < rows * a.Count; i += 256) {
+            indexes[r0 * a.Count + i] = outIndexes[i];
+            weights[r0 * a.Count + i] = outWeights[i];
+        }
+        __syncthreads();
     }
 }
 
@@ -637,60 +695,69 @@ __global__ void __launch_bounds__(256) SelectTopBackwardKernel(TTopArgs<T> a, TT
 template <typename T, int C>
 __global__ void __launch_bounds__(256) SelectTopOfFewBackwardKernel(TTopArgs<T> a, TTopGradientArgs<T> b) {
     using A = TAcc<T>;
-    for (size_t row = size_t(blockIdx.x) * 256 + threadIdx.x; row < a.Rows; row += size_t(gridDim.x) * 256) {
-        const int32_t* indexes = b.Indexes + row * a.Count;
-        const A* weights = b.Weights + row * a.Count;
-        const A* gradients = b.WeightGradients + row * a.Count;
-        A mean = 0;
-        for (uint32_t k = 0; k < a.Count; ++k) {
-            mean += indexes[k] >= 0 ? weights[k] * gradients[k] : A(0);
-        }
-        A x[C];
-#pragma unroll
-        for (int j = 0; j < C; ++j) {
-            x[j] = 0;
-        }
-        if (!a.Among) {
-            const TValues<T, C> v = LoadRow<T, C>(a.Scores + row * a.Stride, a.Classes);
-            A most = -std::numeric_limits<A>::infinity(), total = 0;
+    __shared__ T out[256 * C];
+    for (size_t r0 = size_t(blockIdx.x) * 256; r0 < a.Rows; r0 += size_t(gridDim.x) * 256) {
+        const uint32_t rows = static_cast<uint32_t>(a.Rows - r0 < 256 ? a.Rows - r0 : 256);
+        if (threadIdx.x < rows) {
+            const size_t row = r0 + threadIdx.x;
+            const int32_t* indexes = b.Indexes + row * a.Count;
+            const A* weights = b.Weights + row * a.Count;
+            const A* gradients = b.WeightGradients + row * a.Count;
+            A mean = 0;
+            for (uint32_t k = 0; k < a.Count; ++k) {
+                mean += indexes[k] >= 0 ? weights[k] * gradients[k] : A(0);
+            }
+            A x[C];
 #pragma unroll
             for (int j = 0; j < C; ++j) {
-                const A s = static_cast<A>(v.V[j]);
-                x[j] = static_cast<uint32_t>(j) < a.Classes && s == s ? s : -std::numeric_limits<A>::infinity();
-                most = x[j] > most ? x[j] : most;
+                x[j] = 0;
             }
-#pragma unroll
-            for (int j = 0; j < C; ++j) {
-                x[j] = x[j] > -std::numeric_limits<A>::infinity() ? WeightOf(x[j], most) : A(0);
-                total += x[j];
-            }
-#pragma unroll
-            for (int j = 0; j < C; ++j) {
-                x[j] = total > 0 ? -(x[j] / total) * mean : A(0);
-            }
-        }
-        for (uint32_t k = 0; k < a.Count; ++k) {
-            const int32_t index = indexes[k];
-            if (index >= 0) {
-                const A part = a.Among ? weights[k] * (gradients[k] - mean) : weights[k] * gradients[k];
+            if (!a.Among) {
+                const TValues<T, C> v = LoadRow<T, C>(a.Scores + row * a.Stride, a.Classes);
+                A most = -std::numeric_limits<A>::infinity(), total = 0;
 #pragma unroll
                 for (int j = 0; j < C; ++j) {
-                    x[j] += index == j ? part : A(0);
+                    const A s = static_cast<A>(v.V[j]);
+                    x[j] = static_cast<uint32_t>(j) < a.Classes && s == s ? s : -std::numeric_limits<A>::infinity();
+                    most = x[j] > most ? x[j] : most;
+                }
+#pragma unroll
+                for (int j = 0; j < C; ++j) {
+                    if (static_cast<uint32_t>(j) < a.Classes) {
+                        x[j] = x[j] > -std::numeric_limits<A>::infinity() ? WeightOf(x[j], most) : A(0);
+                        total += x[j];
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < C; ++j) {
+                    if (static_cast<uint32_t>(j) < a.Classes) {
+                        x[j] = total > 0 ? -(x[j] / total) * mean : A(0);
+                    }
+                }
+            }
+            for (uint32_t k = 0; k < a.Count; ++k) {
+                const int32_t index = indexes[k];
+                if (index >= 0) {
+                    const A part = a.Among ? weights[k] * (gradients[k] - mean) : weights[k] * gradients[k];
+#pragma unroll
+                    for (int j = 0; j < C; ++j) {
+                        x[j] += index == j ? part : A(0);
+                    }
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < C; ++j) {
+                if (static_cast<uint32_t>(j) < a.Classes) {
+                    out[threadIdx.x * a.Classes + j] = static_cast<T>(x[j]);
                 }
             }
         }
-        constexpr int N = C < 16 / static_cast<int>(sizeof(T)) ? C : 16 / sizeof(T);
-#pragma unroll
-        for (int j = 0; j < C; j += N) {
-            if (static_cast<uint32_t>(j) < a.Classes) {
-                TValues<T, N> v;
-#pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    v.V[i] = static_cast<T>(x[j + i]);
-                }
-                StoreUpTo<T, N>(v, b.Gradients + row * b.GradientStride + j, a.Classes - j);
-            }
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < rows * a.Classes; i += 256) {
+            const uint32_t r = i / a.Classes;
+            b.Gradients[(r0 + r) * b.GradientStride + (i - r * a.Classes)] = out[i];
         }
+        __syncthreads();
     }
 }
 
@@ -741,16 +808,15 @@ void AdjustScores(int valueType, size_t rows, size_t classes, const void* scores
         using T = decltype(value);
         constexpr uint32_t N = 16 / sizeof(T);
         const size_t tables = size_t(history) + size_t(biases);
-        if (a.Classes <= kRowTileWords / 2) {
+        if (a.Classes <= kRowTileWords / 4) {
             const uint32_t pieces = (a.Classes + N - 1) / N;
-            a.Pitch = (pieces | 1) * N;  // an odd number of pieces: rows begin in different LDS banks
+            a.Pitch = pieces * N;
             a.RowsPerTile = std::min<uint32_t>(kMaxRowsPerTile, std::max<uint32_t>(1, kRowTileWords / a.Pitch));
-            a.LanesPerRow = 1;
-            while (a.LanesPerRow < 256 && a.LanesPerRow * 8 < pieces) {
-                a.LanesPerRow *= 2;
-            }
+            // floor(q / pieces) = floor(q m / 2^32) with m = floor(2^32 / pieces) + 1: q m / 2^32 is over q / pieces by q / 2^32 at most, and
+            // q / pieces is under the next integer by 1 / pieces at least, which is more for the q and pieces under 2^13 here
+            a.PiecesInverse = pieces > 1 ? static_cast<uint32_t>((uint64_t(1) << 32) / pieces + 1) : 0;
             a.Tiles = (rows + a.RowsPerTile - 1) / a.RowsPerTile;
-            call.Launch(AdjustRowsKernel<T>, std::min<size_t>(a.Tiles, 1u << 20), 256, size_t(a.RowsPerTile) * a.Pitch * 4 * tables, a);
+            call.Launch(AdjustRowsKernel<T>, std::min<size_t>(a.Tiles, 1u << 20), 256, (size_t(a.RowsPerTile) * a.Pitch * tables + 3) / 4 * 16, a);
             return;
         }
         const auto slices = [&](uint32_t size) { return (a.Classes + size - 1) / size; };
@@ -782,6 +848,7 @@ namespace {
 constexpr size_t kMaxTopClasses = 1024;
 constexpr int32_t kMaxTopCount = 32;
 constexpr size_t kRowsForThreads = 16384;  // a wave for each compute unit
+constexpr int32_t kCountForThreads = 8;    // 24 KB of LDS for what is stored
 
 void CheckTop(size_t rows, size_t classes, int32_t count) {
     CBAMD_ENSURE(classes <= kMaxTopClasses, "too many classes to select from: " + std::to_string(classes) + ", at most " + std::to_string(kMaxTopClasses));
@@ -793,10 +860,10 @@ void CheckTop(size_t rows, size_t classes, int32_t count) {
 // f(lanes of a row, classes of a lane), 1 lane: a thread has the row to itself. That reads each line of memory once as long
 // as a row is short, and needs rows enough to fill the chip with threads.
 template <typename F>
-void WithShape(size_t classes, size_t rows, F&& f) {
+void WithShape(size_t classes, size_t rows, int32_t count, F&& f) {
     using std::integral_constant;
     const auto shape = [&](auto lanes, auto perLane) { f(lanes, perLane); };
-    if (rows >= kRowsForThreads && classes <= 32) {
+    if (rows >= kRowsForThreads && classes <= 32 && count <= kCountForThreads) {
         const integral_constant<int, 1> alone;
         return classes <= 4 ? shape(alone, integral_constant<int, 4>()) : classes <= 8 ? shape(alone, integral_constant<int, 8>())
             : classes <= 16 ? shape(alone, integral_constant<int, 16>()) : shape(alone, integral_constant<int, 32>());
@@ -829,10 +896,11 @@ void SelectTop(int valueType, size_t rows, size_t classes, const void* scores, s
     WithType(valueType, [&](auto value) {
         using T = decltype(value);
         const TTopArgs<T> a{static_cast<const T*>(scores), scoreStride, rows, static_cast<uint32_t>(classes), static_cast<uint32_t>(count), amongSelected};
-        WithShape(classes, rows, [&](auto lanes, auto perLane) {
+        WithShape(classes, rows, count, [&](auto lanes, auto perLane) {
             constexpr int G = decltype(lanes)::value, V = decltype(perLane)::value;
             if constexpr (G == 1) {
-                call.Launch(SelectTopOfFewKernel<T, V>, GroupsOf(rows, G), 256, 0, a, indexes, static_cast<TAcc<T>*>(weights));
+                call.Launch(SelectTopOfFewKernel<T, V>, GroupsOf(rows, G), 256, size_t(256) * count * (sizeof(TAcc<T>) + 4), a, indexes,
+                            static_cast<TAcc<T>*>(weights));
             } else {
                 call.Launch(SelectTopKernel<T, G, V>, GroupsOf(rows, G), 256, 0, a, indexes, static_cast<TAcc<T>*>(weights));
             }
@@ -859,7 +927,7 @@ void SelectTopBackward(int valueType, size_t rows, size_t classes, const void* s
         const TTopArgs<T> a{static_cast<const T*>(scores), scoreStride, rows, static_cast<uint32_t>(classes), static_cast<uint32_t>(count), amongSelected};
         const TTopGradientArgs<T> b{indexes, static_cast<const TAcc<T>*>(weights), static_cast<const TAcc<T>*>(weightGradients),
                                     static_cast<T*>(scoreGradients), gradientStride};
-        WithShape(classes, rows, [&](auto lanes, auto perLane) {
+        WithShape(classes, rows, count, [&](auto lanes, auto perLane) {
             constexpr int G = decltype(lanes)::value, V = decltype(perLane)::value;
             if constexpr (G == 1) {
                 call.Launch(SelectTopOfFewBackwardKernel<T, V>, GroupsOf(rows, G), 256, 0, a, b);

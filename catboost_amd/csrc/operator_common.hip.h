@@ -5,13 +5,12 @@
 
 #include <hip/hip_runtime.h>
 
-#include <algorithm>
 #include <cstdint>
+#include <map>
 #include <mutex>
 #include <string>
 #include <tuple>
 #include <utility>
-#include <vector>
 
 namespace cbamd {
 namespace op {
@@ -63,24 +62,22 @@ public:
                    std::index_sequence_for<TParams...>());
     }
 
-    // A kernel that uses more than 64 KB of dynamic LDS has to be told so, once for each device
+    // A kernel that uses more than 64 KB of dynamic LDS has to be told so, for each device; the largest size so far is remembered
     void AllowLds(const void* kernel, size_t bytes) const {
         if (bytes <= 64 * 1024) {
             return;
         }
         static std::mutex lock;
-        static std::vector<std::pair<int, const void*>> told;
+        static std::map<std::pair<int, const void*>, size_t> allowed;
         std::lock_guard<std::mutex> guard(lock);
-        const std::pair<int, const void*> item(Device, kernel);
-        if (std::find(told.begin(), told.end(), item) == told.end()) {
-            OP_HIP_CHECK(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kMaxLds));
-            told.push_back(item);
+        size_t& most = allowed[{Device, kernel}];
+        if (most < bytes) {
+            OP_HIP_CHECK(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
+            most = bytes;
         }
     }
 
 private:
-    static constexpr int kMaxLds = 160 * 1024;
-
     template <typename TTuple, size_t... I>
     void LaunchHeld(const void* kernel, size_t groups, uint32_t threads, size_t ldsBytes, TTuple& held,
                     std::index_sequence<I...>) const {
@@ -144,6 +141,35 @@ struct TValues {
     }
     __device__ __forceinline__ void Store(T* at) const { __builtin_memcpy(at, this, sizeof(*this)); }
 };
+
+// The same for the `n` values that are left of a row, where those are fewer
+template <typename T, int N>
+__device__ __forceinline__ TValues<T, N> LoadUpTo(const T* at, size_t n) {
+    if (n >= N) {
+        return TValues<T, N>::Load(at);
+    }
+    TValues<T, N> v{};
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        if (static_cast<size_t>(i) < n) {
+            v.V[i] = at[i];
+        }
+    }
+    return v;
+}
+template <typename T, int N>
+__device__ __forceinline__ void StoreUpTo(const TValues<T, N>& v, T* at, size_t n) {
+    if (n >= N) {
+        v.Store(at);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        if (static_cast<size_t>(i) < n) {
+            at[i] = v.V[i];
+        }
+    }
+}
 
 }  // namespace op
 }  // namespace cbamd

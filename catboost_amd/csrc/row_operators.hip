@@ -2,6 +2,7 @@
 #include "operator_common.hip.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace cbamd {
 namespace op {
@@ -9,32 +10,72 @@ namespace op {
 // ---------------------------------------------------------------- slots sorted by expert ----
 
 constexpr int32_t kMaxExperts = 1024;
-constexpr uint32_t kSortWaves = 4;
-constexpr uint32_t kSortSteps = 16;                             // of 64 slots that a wave ranks
-constexpr uint32_t kSortSlots = kSortWaves * kSortSteps * 64;   // of a workgroup
+constexpr uint32_t kSortWaves = 16;
+constexpr uint32_t kSortThreads = kSortWaves * 64;
 
-// counts[expert][block]: how many of the block's slots go to the expert
-__global__ void __launch_bounds__(256) CountExpertsKernel(const int32_t* ids, uint32_t slots, uint32_t experts, uint32_t blocks, int32_t* counts) {
-    __shared__ int32_t count[kMaxExperts];
-    for (uint32_t e = threadIdx.x; e < experts; e += blockDim.x) {
-        count[e] = 0;
+// Lanes of a wave whose value is the caller's own, out of values of `bits` bits; every lane takes part
+__device__ __forceinline__ uint64_t LanesWithSame(uint32_t value, uint32_t bits) {
+    uint64_t same = ~uint64_t(0);
+    for (uint32_t b = 0; b < bits; ++b) {
+        const bool set = value >> b & 1;
+        const uint64_t with = __ballot(set);
+        same &= set ? with : ~with;
     }
-    __syncthreads();
-    const uint32_t begin = blockIdx.x * kSortSlots;
-    const uint32_t n = min(kSortSlots, slots - begin);
-    for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) {
-        const uint32_t e = static_cast<uint32_t>(ids[begin + i]);
-        if (e < experts) {
-            atomicAdd(&count[e], 1);
+    return same;
+}
+
+// A wave's slots, STEPS times 64 in a row, ranked: how many slots of the same step and expert come before each, and whether
+// it is the last one of them. `own` counts the wave's slots of each expert; one lane adds for all that are alike, which needs
+// no atomics (those of many lanes on few addresses take turns).
+template <int STEPS>
+struct TRankedSlots {
+    uint32_t Expert[STEPS];
+    uint32_t Rank[STEPS];  // bit 31: the last one
+
+    __device__ __forceinline__ TRankedSlots(const int32_t* ids, uint32_t begin, uint32_t slots, uint32_t experts, uint32_t bits, int32_t* own) {
+        const uint32_t lane = threadIdx.x & 63;
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+            const uint32_t slot = begin + s * 64 + lane;
+            const uint32_t e = slot < slots ? static_cast<uint32_t>(ids[slot]) : ~0u;
+            Expert[s] = e < experts ? e : experts;
+        }
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+            const uint64_t same = LanesWithSame(Expert[s], bits);
+            const bool last = (same >> lane >> 1) == 0;
+            Rank[s] = static_cast<uint32_t>(__popcll(same & ((uint64_t(1) << lane) - 1))) | (last ? 0x80000000u : 0u);
+            if (last && Expert[s] < experts) {
+                own[Expert[s]] += static_cast<int32_t>(Rank[s] & 0x7fffffffu) + 1;
+            }
+            __builtin_amdgcn_wave_barrier();  // the steps' additions stay in order
         }
     }
+};
+
+// counts[b * experts + e] (or [e * blocks + b] for the scan): how many slots of workgroup b go to expert e
+template <int STEPS>
+__global__ void __launch_bounds__(kSortThreads) CountExpertsKernel(const int32_t* ids, uint32_t slots, uint32_t experts, uint32_t bits, bool forScan,
+                                                                   int32_t* counts) {
+    extern __shared__ int32_t own[];  // [wave][expert]
+    for (uint32_t i = threadIdx.x; i < kSortWaves * experts; i += kSortThreads) {
+        own[i] = 0;
+    }
     __syncthreads();
-    for (uint32_t e = threadIdx.x; e < experts; e += blockDim.x) {
-        counts[size_t(e) * blocks + blockIdx.x] = count[e];
+    const uint32_t wave = threadIdx.x / 64;
+    const TRankedSlots<STEPS> ranked(ids, (blockIdx.x * kSortWaves + wave) * STEPS * 64, slots, experts, bits, own + wave * experts);
+    __syncthreads();
+    for (uint32_t e = threadIdx.x; e < experts; e += kSortThreads) {
+        int32_t sum = 0;
+        for (uint32_t w = 0; w < kSortWaves; ++w) {
+            sum += own[w * experts + e];
+        }
+        counts[forScan ? size_t(e) * gridDim.x + blockIdx.x : size_t(blockIdx.x) * experts + e] = sum;
     }
 }
 
-// The sum of the workgroup's values before a thread's own (256 threads)
+// The sum of the workgroup's values before a thread's own
+template <uint32_t WAVES>
 __device__ __forceinline__ int32_t SumBefore(int32_t x, int32_t* waveSums) {
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64;
     int32_t sum = x;
@@ -48,13 +89,13 @@ __device__ __forceinline__ int32_t SumBefore(int32_t x, int32_t* waveSums) {
     }
     __syncthreads();
     int32_t before = sum - x;
-    for (uint32_t w = 0; w < wave; ++w) {
-        before += waveSums[w];
+    for (uint32_t w = 0; w < WAVES; ++w) {
+        before += w < wave ? waveSums[w] : 0;
     }
     return before;
 }
 
-// A workgroup for an expert: its counts become the sums of the blocks before each; totals[expert] their sum
+// A workgroup for an expert: its counts become the sums of the workgroups before each; totals[expert] their sum
 __global__ void __launch_bounds__(256) ScanBlocksKernel(int32_t* counts, uint32_t blocks, int32_t* totals) {
     __shared__ int32_t waveSums[4];
     __shared__ int32_t carried;
@@ -63,7 +104,7 @@ __global__ void __launch_bounds__(256) ScanBlocksKernel(int32_t* counts, uint32_
     for (uint32_t begin = 0; begin < blocks; begin += 256) {
         const uint32_t b = begin + threadIdx.x;
         const int32_t x = b < blocks ? mine[b] : 0;
-        const int32_t before = SumBefore(x, waveSums) + carry;
+        const int32_t before = SumBefore<4>(x, waveSums) + carry;
         if (b < blocks) {
             mine[b] = before;
         }
@@ -78,248 +119,268 @@ __global__ void __launch_bounds__(256) ScanBlocksKernel(int32_t* counts, uint32_
     }
 }
 
-// Lanes of a wave whose value is the caller's own, out of values of `bits` bits; every lane takes part
-__device__ __forceinline__ uint64_t LanesWithSame(uint32_t value, uint32_t bits) {
-    uint64_t same = ~uint64_t(0);
-    for (uint32_t b = 0; b < bits; ++b) {
-        const bool set = value >> b & 1;
-        const uint64_t with = __ballot(set);
-        same &= set ? with : ~with;
-    }
-    return same;
-}
-
-// Places of a block's slots. A wave ranks its slots step by step: a slot's rank among the step's equal ids comes from
-// ballots, what comes before the step from the wave's own counters, which begin with what comes before the wave
-__global__ void __launch_bounds__(256) PlaceSlotsKernel(const int32_t* ids, uint32_t slots, uint32_t experts, uint32_t bits, uint32_t blocks,
-                                                        const int32_t* counts, const int32_t* totals, int32_t* places, int32_t* offsets) {
-    __shared__ int32_t next[kSortWaves][kMaxExperts];
-    __shared__ int32_t waveSums[4];
+// Places of a workgroup's slots: where the expert begins, what the workgroups before this one and the waves before the
+// slot's have, what the wave's steps before it have, its rank. A single workgroup counts for itself. Of few workgroups each
+// adds up all their counts (`totals` null), which takes less than a launch that does so; of many they come scanned.
+template <int STEPS>
+__global__ void __launch_bounds__(kSortThreads) PlaceSlotsKernel(const int32_t* ids, uint32_t slots, uint32_t experts, uint32_t bits,
+                                                                 const int32_t* counts, const int32_t* totals, int32_t* places, int32_t* offsets) {
+    extern __shared__ int32_t lds[];
+    __shared__ int32_t waveSums[kSortWaves];
+    int32_t* next = lds;                              // [wave][expert]
+    int32_t* sums = lds + kSortWaves * experts;       // the counts of all workgroups
+    int32_t* sumsBefore = sums + experts;             // and of those before this one
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64;
-    for (uint32_t e = threadIdx.x; e < experts; e += blockDim.x) {
-        for (uint32_t w = 0; w < kSortWaves; ++w) {
-            next[w][e] = 0;
+    for (uint32_t i = threadIdx.x; i < (kSortWaves + 2) * experts; i += kSortThreads) {
+        lds[i] = 0;
+    }
+    __syncthreads();
+    int32_t* own = next + wave * experts;
+    const uint32_t begin = (blockIdx.x * kSortWaves + wave) * STEPS * 64;
+    const TRankedSlots<STEPS> ranked(ids, begin, slots, experts, bits, own);
+    if (gridDim.x > 1 && totals == nullptr) {
+        for (uint32_t i = threadIdx.x; i < gridDim.x * experts; i += kSortThreads) {
+            const uint32_t b = i / experts;
+            const int32_t n = counts[i];
+            atomicAdd(&sums[i - b * experts], n);
+            if (b < blockIdx.x) {
+                atomicAdd(&sumsBefore[i - b * experts], n);
+            }
         }
     }
     __syncthreads();
-    const uint32_t begin = blockIdx.x * kSortSlots + wave * kSortSteps * 64;
-    for (uint32_t step = 0; step < kSortSteps; ++step) {
-        const uint32_t slot = begin + step * 64 + lane;
-        const uint32_t e = slot < slots ? static_cast<uint32_t>(ids[slot]) : ~0u;
-        if (e < experts) {
-            atomicAdd(&next[wave][e], 1);
-        }
-    }
-    // four experts a thread: where each begins, what the blocks before this one and the waves before each have
-    int32_t total[kMaxExperts / 256], sum = 0;
-    for (uint32_t i = 0; i < kMaxExperts / 256; ++i) {
-        const uint32_t e = threadIdx.x * (kMaxExperts / 256) + i;
-        total[i] = e < experts ? totals[e] : 0;
-        sum += total[i];
-    }
-    int32_t start = SumBefore(sum, waveSums);  // (its barriers stand behind the counting above)
-    for (uint32_t i = 0; i < kMaxExperts / 256; ++i) {
-        const uint32_t e = threadIdx.x * (kMaxExperts / 256) + i;
-        if (e < experts) {
-            int32_t at = start + counts[size_t(e) * blocks + blockIdx.x];
+    const uint32_t e = threadIdx.x;  // at most as many experts as threads
+    int32_t total = 0, before = 0;
+    if (e < experts) {
+        if (gridDim.x == 1) {
             for (uint32_t w = 0; w < kSortWaves; ++w) {
-                const int32_t n = next[w][e];
-                next[w][e] = at;
-                at += n;
+                total += next[w * experts + e];
             }
-            if (blockIdx.x == 0) {
-                offsets[e] = start;
-                if (e == experts - 1) {
-                    offsets[experts] = start + total[i];
-                }
+        } else {
+            total = totals != nullptr ? totals[e] : sums[e];
+            before = totals != nullptr ? counts[size_t(e) * gridDim.x + blockIdx.x] : sumsBefore[e];
+        }
+    }
+    const int32_t start = SumBefore<kSortWaves>(total, waveSums);
+    if (e < experts) {
+        int32_t at = start + before;
+        for (uint32_t w = 0; w < kSortWaves; ++w) {
+            const int32_t n = next[w * experts + e];
+            next[w * experts + e] = at;
+            at += n;
+        }
+        if (blockIdx.x == 0) {
+            offsets[e] = start;
+            if (e == experts - 1) {
+                offsets[experts] = start + total;
             }
         }
-        start += total[i];
     }
     __syncthreads();
-    for (uint32_t step = 0; step < kSortSteps; ++step) {
-        const uint32_t slot = begin + step * 64 + lane;
-        const uint32_t e = slot < slots ? static_cast<uint32_t>(ids[slot]) : ~0u;
-        const bool valid = e < experts;
-        const uint64_t same = LanesWithSame(valid ? e : experts, bits);
-        const uint32_t rank = __popcll(same & ((uint64_t(1) << lane) - 1));
-        const int32_t at = valid ? next[wave][e] : 0;
-        __builtin_amdgcn_wave_barrier();  // all lanes have read before the last one of each id writes
-        if (valid && (same >> lane >> 1) == 0) {
-            next[wave][e] = at + static_cast<int32_t>(rank) + 1;
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+        const bool valid = ranked.Expert[s] < experts;
+        const int32_t place = valid ? own[ranked.Expert[s]] + static_cast<int32_t>(ranked.Rank[s] & 0x7fffffffu) : -1;
+        __builtin_amdgcn_wave_barrier();  // all lanes have read before the last one of each expert writes
+        if (valid && (ranked.Rank[s] & 0x80000000u) != 0) {
+            own[ranked.Expert[s]] = place + 1;
         }
         __builtin_amdgcn_wave_barrier();
+        const uint32_t slot = begin + s * 64 + lane;
         if (slot < slots) {
-            places[slot] = valid ? at + static_cast<int32_t>(rank) : -1;
+            places[slot] = place;
         }
     }
 }
 
-// ---------------------------------------------------------------- rows to their places ----
+// ---------------------------------------------------------------- rows to their places and back ----
 
-// Where in a matrix of rows cut into `pieces` pieces each a thread's piece is: workgroups are 256 pieces long and may
-// begin inside a row
-struct TPiece {
-    size_t Row;
-    uint32_t Piece;
+// Rows are cut into pieces of 16 bytes (the last one of a row may be shorter), one for a thread, in the order in which they
+// are in memory
+struct TPieces {
+    size_t Rows, Width;   // values
+    uint32_t PerRow;      // slots
+    uint32_t Pieces;      // of a row
+    uint64_t Inverse;     // floor(i / Pieces) = floor(i Inverse / 2^64) as long as i Pieces < 2^64, which memory sees to
+    size_t Blocks;        // of 256 pieces
+
+    __device__ __forceinline__ bool Of(size_t block, size_t* row, size_t* column, uint32_t valuesPerPiece) const {
+        const uint64_t i = block * 256 + threadIdx.x;
+        *row = Inverse != 0 ? __umul64hi(i, Inverse) : i;
+        *column = (i - *row * Pieces) * valuesPerPiece;
+        return *row < Rows;
+    }
 };
 
-__device__ __forceinline__ TPiece PieceOf(size_t block, uint32_t pieces) {
-    const size_t first = block * 256;
-    const size_t row = first / pieces;
-    const uint32_t at = static_cast<uint32_t>(first - row * pieces) + threadIdx.x;
-    const uint32_t rows = at / pieces;
-    return {row + rows, at - rows * pieces};
-}
+// The next K places of a row from slot k on, -1 for those that are left out
+template <int K>
+struct TPlaces {
+    int32_t At[K];
+    __device__ __forceinline__ TPlaces(const int32_t* places, uint32_t k, uint32_t perRow, size_t sortedRows) {
+#pragma unroll
+        for (int j = 0; j < K; ++j) {
+            At[j] = k + j < perRow ? places[k + j] : -1;
+        }
+#pragma unroll
+        for (int j = 0; j < K; ++j) {
+            At[j] = static_cast<size_t>(At[j]) < sortedRows ? At[j] : -1;  // (negative ones are large)
+        }
+    }
+};
 
-// A piece of a row of E is N values, the last one of a row may be shorter
-template <typename T, int N>
-__global__ void __launch_bounds__(256) DispatchRowsKernel(const T* source, size_t sourceStride, size_t rows, size_t width, uint32_t pieces,
-                                                          uint32_t perRow, const int32_t* places, T* sorted, size_t sortedRows,
-                                                          size_t sortedStride, size_t blocks) {
-    for (size_t block = blockIdx.x; block < blocks; block += gridDim.x) {
-        const TPiece p = PieceOf(block, pieces);
-        if (p.Row >= rows) {
+// A row's places are requested K at a time, so that the stores do not wait for one after the other
+template <typename T, int K>
+__global__ void __launch_bounds__(256) DispatchRowsKernel(const T* source, size_t sourceStride, TPieces p, const int32_t* places, T* sorted,
+                                                          size_t sortedRows, size_t sortedStride) {
+    constexpr int N = 16 / sizeof(T);
+    for (size_t block = blockIdx.x; block < p.Blocks; block += gridDim.x) {
+        size_t row, c;
+        if (!p.Of(block, &row, &c, N)) {
             return;
         }
-        const size_t c = size_t(p.Piece) * N;
-        const T* from = source + p.Row * sourceStride + c;
-        const bool whole = c + N <= width;
-        TValues<T, N> v{};
-        if (whole) {
-            v = TValues<T, N>::Load(from);
-        } else {
-            for (int i = 0; i < N; ++i) {
-                if (c + i < width) {
-                    v.V[i] = from[i];
-                }
-            }
-        }
-        for (uint32_t k = 0; k < perRow; ++k) {
-            const int32_t place = places[p.Row * perRow + k];
-            if (place < 0 || static_cast<size_t>(place) >= sortedRows) {
-                continue;
-            }
-            T* to = sorted + static_cast<size_t>(place) * sortedStride + c;
-            if (whole) {
-                v.Store(to);
-            } else {
-                for (int i = 0; i < N; ++i) {
-                    if (c + i < width) {
-                        to[i] = v.V[i];
-                    }
+        const TValues<T, N> v = LoadUpTo<T, N>(source + row * sourceStride + c, p.Width - c);
+        for (uint32_t k = 0; k < p.PerRow; k += K) {
+            const TPlaces<K> to(places + row * p.PerRow, k, p.PerRow, sortedRows);
+#pragma unroll
+            for (int j = 0; j < K; ++j) {
+                if (to.At[j] >= 0) {
+                    StoreUpTo<T, N>(v, sorted + static_cast<size_t>(to.At[j]) * sortedStride + c, p.Width - c);
                 }
             }
         }
     }
 }
 
-// ---------------------------------------------------------------- rows from their places ----
-
-template <typename T, int N>
-__global__ void __launch_bounds__(256) CombineRowsKernel(const T* sorted, size_t sortedRows, size_t sortedStride, size_t rows, size_t width,
-                                                         uint32_t pieces, uint32_t perRow, const int32_t* places, const TAcc<T>* weights,
-                                                         T* result, size_t resultStride, size_t blocks) {
+template <typename T, int K>
+__global__ void __launch_bounds__(256) CombineRowsKernel(const T* sorted, size_t sortedRows, size_t sortedStride, TPieces p, const int32_t* places,
+                                                         const TAcc<T>* weights, T* result, size_t resultStride) {
     using A = TAcc<T>;
-    for (size_t block = blockIdx.x; block < blocks; block += gridDim.x) {
-        const TPiece p = PieceOf(block, pieces);
-        if (p.Row >= rows) {
+    constexpr int N = 16 / sizeof(T);
+    for (size_t block = blockIdx.x; block < p.Blocks; block += gridDim.x) {
+        size_t row, c;
+        if (!p.Of(block, &row, &c, N)) {
             return;
         }
-        const size_t c = size_t(p.Piece) * N;
-        const bool whole = c + N <= width;
         A sum[N] = {};
-        for (uint32_t k = 0; k < perRow; ++k) {
-            const int32_t place = places[p.Row * perRow + k];
-            if (place < 0 || static_cast<size_t>(place) >= sortedRows) {
-                continue;
+        for (uint32_t k = 0; k < p.PerRow; k += K) {
+            const TPlaces<K> from(places + row * p.PerRow, k, p.PerRow, sortedRows);
+            A w[K];
+            TValues<T, N> v[K];
+#pragma unroll
+            for (int j = 0; j < K; ++j) {
+                w[j] = weights != nullptr && from.At[j] >= 0 ? weights[row * p.PerRow + k + j] : A(1);
             }
-            const A w = weights != nullptr ? weights[p.Row * perRow + k] : A(1);
-            const T* from = sorted + static_cast<size_t>(place) * sortedStride + c;
-            if (whole) {
-                const TValues<T, N> v = TValues<T, N>::Load(from);
-                for (int i = 0; i < N; ++i) {
-                    sum[i] += w * static_cast<A>(v.V[i]);
+#pragma unroll
+            for (int j = 0; j < K; ++j) {
+                if (from.At[j] >= 0) {
+                    v[j] = LoadUpTo<T, N>(sorted + static_cast<size_t>(from.At[j]) * sortedStride + c, p.Width - c);
                 }
-            } else {
-                for (int i = 0; i < N; ++i) {
-                    if (c + i < width) {
-                        sum[i] += w * static_cast<A>(from[i]);
+            }
+#pragma unroll
+            for (int j = 0; j < K; ++j) {
+                if (from.At[j] >= 0) {
+#pragma unroll
+                    for (int i = 0; i < N; ++i) {
+                        sum[i] += w[j] * static_cast<A>(v[j].V[i]);
                     }
                 }
             }
         }
-        T* to = result + p.Row * resultStride + c;
-        TValues<T, N> v;
+        TValues<T, N> out;
+#pragma unroll
         for (int i = 0; i < N; ++i) {
-            v.V[i] = static_cast<T>(sum[i]);
+            out.V[i] = static_cast<T>(sum[i]);
         }
-        if (whole) {
-            v.Store(to);
-        } else {
-            for (int i = 0; i < N; ++i) {
-                if (c + i < width) {
-                    to[i] = v.V[i];
-                }
-            }
-        }
+        StoreUpTo<T, N>(out, result + row * resultStride + c, p.Width - c);
     }
 }
 
-// A wave for a row. Each lane adds the products of its own columns in their order, the lanes' sums are added by a
-// butterfly: the same order for every call
-template <typename T, int N>
+// L threads for a row. A thread takes every L-th piece of the row's gradient and, for K slots at a time, what is at their
+// places; its products are added in that order, then the threads' sums by a butterfly: the same order for every call.
+template <typename T, int L, int K>
 __global__ void __launch_bounds__(256) CombineRowsBackwardKernel(const T* gradients, size_t gradientStride, const T* sorted, size_t sortedRows,
                                                                  size_t sortedStride, size_t rows, size_t width, uint32_t perRow,
                                                                  const int32_t* places, const TAcc<T>* weights, T* sortedGradients,
                                                                  size_t sortedGradientStride, TAcc<T>* weightGradients) {
     using A = TAcc<T>;
-    const uint32_t lane = threadIdx.x & 63;
-    for (size_t row = size_t(blockIdx.x) * 4 + threadIdx.x / 64; row < rows; row += size_t(gridDim.x) * 4) {
-        const T* from = gradients + row * gradientStride;
-        for (uint32_t k = 0; k < perRow; ++k) {
-            const size_t slot = row * perRow + k;
-            const int32_t place = places[slot];
-            const bool there = place >= 0 && static_cast<size_t>(place) < sortedRows;
-            A product = 0;
+    constexpr int N = 16 / sizeof(T);
+    __shared__ A waveSums[4][K];
+    const uint32_t lane = threadIdx.x % L;
+    for (size_t first = size_t(blockIdx.x) * (256 / L); first < rows; first += size_t(gridDim.x) * (256 / L)) {
+        const size_t row = first + threadIdx.x / L;
+        const bool there = row < rows;  // (false for whole groups of L threads)
+        for (uint32_t k = 0; k < perRow; k += K) {
+            A product[K] = {};
             if (there) {
-                const A w = weights != nullptr ? weights[slot] : A(1);
-                const T* y = sorted + static_cast<size_t>(place) * sortedStride;
-                T* to = sortedGradients + static_cast<size_t>(place) * sortedGradientStride;
-                for (size_t c = size_t(lane) * N; c < width; c += 64 * N) {
-                    if (c + N <= width) {
-                        const TValues<T, N> g = TValues<T, N>::Load(from + c);
-                        if (weightGradients != nullptr) {
-                            const TValues<T, N> v = TValues<T, N>::Load(y + c);
-                            for (int i = 0; i < N; ++i) {
-                                product += static_cast<A>(g.V[i]) * static_cast<A>(v.V[i]);
+                const TPlaces<K> at(places + row * perRow, k, perRow, sortedRows);
+                A w[K];
+#pragma unroll
+                for (int j = 0; j < K; ++j) {
+                    w[j] = weights != nullptr && at.At[j] >= 0 ? weights[row * perRow + k + j] : A(1);
+                }
+                for (size_t c = size_t(lane) * N; c < width; c += L * N) {
+                    const TValues<T, N> g = LoadUpTo<T, N>(gradients + row * gradientStride + c, width - c);
+                    if (weightGradients != nullptr) {
+                        TValues<T, N> v[K];
+#pragma unroll
+                        for (int j = 0; j < K; ++j) {
+                            v[j] = at.At[j] >= 0 ? LoadUpTo<T, N>(sorted + static_cast<size_t>(at.At[j]) * sortedStride + c, width - c)
+                                                 : TValues<T, N>{};
+                        }
+#pragma unroll
+                        for (int j = 0; j < K; ++j) {
+                            if (at.At[j] >= 0) {
+#pragma unroll
+                                for (int i = 0; i < N; ++i) {
+                                    product[j] += static_cast<A>(g.V[i]) * static_cast<A>(v[j].V[i]);
+                                }
                             }
                         }
-                        if (sortedGradients != nullptr) {
-                            TValues<T, N> v;
-                            for (int i = 0; i < N; ++i) {
-                                v.V[i] = static_cast<T>(w * static_cast<A>(g.V[i]));
-                            }
-                            v.Store(to + c);
-                        }
-                    } else {
-                        for (size_t i = c; i < width; ++i) {
-                            if (weightGradients != nullptr) {
-                                product += static_cast<A>(from[i]) * static_cast<A>(y[i]);
-                            }
-                            if (sortedGradients != nullptr) {
-                                to[i] = static_cast<T>(w * static_cast<A>(from[i]));
+                    }
+                    if (sortedGradients != nullptr) {
+#pragma unroll
+                        for (int j = 0; j < K; ++j) {
+                            if (at.At[j] >= 0) {
+                                TValues<T, N> out;
+#pragma unroll
+                                for (int i = 0; i < N; ++i) {
+                                    out.V[i] = static_cast<T>(w[j] * static_cast<A>(g.V[i]));
+                                }
+                                StoreUpTo<T, N>(out, sortedGradients + static_cast<size_t>(at.At[j]) * sortedGradientStride + c, width - c);
                             }
                         }
                     }
                 }
             }
-            if (weightGradients != nullptr) {
-                for (int step = 32; step > 0; step /= 2) {
-                    product += __shfl_xor(product, step);
+            if (weightGradients == nullptr) {
+                continue;
+            }
+#pragma unroll
+            for (int j = 0; j < K; ++j) {
+                for (int step = (L < 64 ? L : 64) / 2; step > 0; step /= 2) {
+                    product[j] += __shfl_xor(product[j], step);
                 }
-                if (lane == 0) {
-                    weightGradients[slot] = product;
+            }
+            if constexpr (L > 64) {
+                __syncthreads();
+                if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+                    for (int j = 0; j < K; ++j) {
+                        waveSums[threadIdx.x / 64][j] = product[j];
+                    }
+                }
+                __syncthreads();
+#pragma unroll
+                for (int j = 0; j < K; ++j) {
+                    product[j] = (waveSums[0][j] + waveSums[1][j]) + (waveSums[2][j] + waveSums[3][j]);
+                }
+            }
+            if (there && lane == 0) {
+#pragma unroll
+                for (int j = 0; j < K; ++j) {
+                    if (k + j < perRow) {
+                        weightGradients[row * perRow + k + j] = product[j];
+                    }
                 }
             }
         }
@@ -332,8 +393,13 @@ using namespace op;
 
 namespace {
 
-uint32_t SortBlocks(size_t slots) {
-    return static_cast<uint32_t>((slots + kSortSlots - 1) / kSortSlots);
+constexpr uint32_t kStepsOfMany = 4;                                         // when there are several workgroups
+constexpr size_t kSlotsOfOne = 16 * kSortThreads;                            // that one workgroup sorts
+constexpr size_t kSlotsOfBlock = size_t(kStepsOfMany) * kSortThreads;
+constexpr size_t kCountsToAdd = 16384;                                       // by each workgroup, 16 for a thread
+
+size_t SortBlocks(size_t slots) {
+    return slots <= kSlotsOfOne ? 1 : (slots + kSlotsOfBlock - 1) / kSlotsOfBlock;
 }
 
 }  // namespace
@@ -342,7 +408,7 @@ size_t SortByExpertBytes(size_t slots, int32_t experts) {
     if (experts <= 0 || experts > kMaxExperts || slots > 0x7fffffffu) {
         return 0;
     }
-    return (size_t(std::max<uint32_t>(1, SortBlocks(slots))) + 1) * static_cast<size_t>(experts) * 4;
+    return (SortBlocks(slots) + 1) * static_cast<size_t>(experts) * 4;
 }
 
 void SortByExpert(size_t slots, int32_t experts, const int32_t* ids, int32_t* places, int32_t* offsets, void* workspace,
@@ -355,7 +421,7 @@ void SortByExpert(size_t slots, int32_t experts, const int32_t* ids, int32_t* pl
     CBAMD_ENSURE(workspace != nullptr && workspaceBytes >= needed, "workspace of " + std::to_string(workspaceBytes) + " bytes, " + std::to_string(needed) + " are needed");
     CBAMD_ENSURE(reinterpret_cast<uintptr_t>(workspace) % 4 == 0, "workspace pointer is not a multiple of 4");
     const TCallDevice call(offsets, stream);
-    const uint32_t blocks = std::max<uint32_t>(1, SortBlocks(slots));
+    const size_t blocks = SortBlocks(slots);
     int32_t* totals = static_cast<int32_t*>(workspace);
     int32_t* counts = totals + experts;
     const uint32_t e = static_cast<uint32_t>(experts), n = static_cast<uint32_t>(slots);
@@ -363,15 +429,27 @@ void SortByExpert(size_t slots, int32_t experts, const int32_t* ids, int32_t* pl
     while (e >> bits != 0) {
         ++bits;
     }
-    call.Launch(CountExpertsKernel, blocks, 256, 0, ids, n, e, blocks, counts);
-    call.Launch(ScanBlocksKernel, e, 256, 0, counts, blocks, totals);
-    call.Launch(PlaceSlotsKernel, blocks, 256, 0, ids, n, e, bits, blocks, counts, totals, places, offsets);
+    const auto place = [&](auto kernel, const int32_t* scannedTotals) {
+        const size_t lds = (kSortWaves + 2) * static_cast<size_t>(e) * 4;
+        call.AllowLds(reinterpret_cast<const void*>(kernel), lds);
+        call.Launch(kernel, blocks, kSortThreads, lds, ids, n, e, bits, static_cast<const int32_t*>(counts), scannedTotals, places, offsets);
+    };
+    if (blocks == 1) {
+        return slots <= kSortThreads ? place(PlaceSlotsKernel<1>, nullptr) : slots <= 4 * kSortThreads ? place(PlaceSlotsKernel<4>, nullptr)
+            : place(PlaceSlotsKernel<16>, nullptr);
+    }
+    const bool scan = blocks * e > kCountsToAdd;
+    call.Launch(CountExpertsKernel<kStepsOfMany>, blocks, kSortThreads, kSortWaves * static_cast<size_t>(e) * 4, ids, n, e, bits, scan, counts);
+    if (scan) {
+        call.Launch(ScanBlocksKernel, e, 256, 0, counts, static_cast<uint32_t>(blocks), totals);
+    }
+    place(PlaceSlotsKernel<kStepsOfMany>, scan ? totals : nullptr);
 }
 
 namespace {
 
 constexpr int32_t kMaxPerRow = 64;
-constexpr size_t kMaxGroups = size_t(1) << 20;
+constexpr size_t kMaxGroups = size_t(1) << 23;  // the workgroups go on from there
 
 void CheckRoutes(size_t rows, size_t width, int32_t perRow, const int32_t* places, size_t sortedRows) {
     CBAMD_ENSURE(perRow >= 1 && perRow <= kMaxPerRow, "slots per row: " + std::to_string(perRow) + ", 1 to " + std::to_string(kMaxPerRow) + " are supported");
@@ -379,6 +457,25 @@ void CheckRoutes(size_t rows, size_t width, int32_t perRow, const int32_t* place
     CBAMD_ENSURE(width < size_t(1) << 31, "rows are too wide: " + std::to_string(width));
     CBAMD_ENSURE(rows <= size_t(1) << 40, "too many rows");
     CBAMD_ENSURE(sortedRows <= 0x7fffffffu, "too many sorted rows: " + std::to_string(sortedRows));
+}
+
+TPieces PiecesOf(size_t rows, size_t width, int32_t perRow, size_t valueSize) {
+    TPieces p;
+    p.Rows = rows;
+    p.Width = width;
+    p.PerRow = static_cast<uint32_t>(perRow);
+    p.Pieces = static_cast<uint32_t>((width * valueSize + 15) / 16);
+    p.Inverse = p.Pieces > 1 ? ~uint64_t(0) / p.Pieces + 1 : 0;
+    p.Blocks = (rows * p.Pieces + 255) / 256;
+    return p;
+}
+
+// f(slots that are taken at a time)
+template <typename F>
+void WithSlots(int32_t perRow, F&& f) {
+    using std::integral_constant;
+    return perRow == 1 ? f(integral_constant<int, 1>()) : perRow == 2 ? f(integral_constant<int, 2>())
+        : perRow <= 4 ? f(integral_constant<int, 4>()) : f(integral_constant<int, 8>());
 }
 
 }  // namespace
@@ -393,13 +490,13 @@ void DispatchRows(int valueType, size_t rows, size_t width, int32_t perRow, cons
     CheckMatrix("source", source, rows, width, sourceStride, size);
     CheckMatrix("sorted rows", sorted, sortedRows, width, sortedStride, size);
     const TCallDevice call(sorted, stream);
+    const TPieces pieces = PiecesOf(rows, width, perRow, size);
     const auto launch = [&](auto value) {
         using T = decltype(value);
-        constexpr int N = 16 / sizeof(T);
-        const uint32_t pieces = static_cast<uint32_t>((width + N - 1) / N);
-        const size_t blocks = (rows * pieces + 255) / 256;
-        call.Launch(DispatchRowsKernel<T, N>, std::min(blocks, kMaxGroups), 256, 0, static_cast<const T*>(source), sourceStride, rows, width,
-                    pieces, static_cast<uint32_t>(perRow), places, static_cast<T*>(sorted), sortedRows, sortedStride, blocks);
+        WithSlots(perRow, [&](auto slots) {
+            call.Launch(DispatchRowsKernel<T, decltype(slots)::value>, std::min(pieces.Blocks, kMaxGroups), 256, 0, static_cast<const T*>(source),
+                        sourceStride, pieces, places, static_cast<T*>(sorted), sortedRows, sortedStride);
+        });
     };
     // the values' bits are moved as they are
     switch (size) {
@@ -424,12 +521,11 @@ void CombineRows(int valueType, size_t rows, size_t width, int32_t perRow, const
     const TCallDevice call(result, stream);
     WithType(valueType, [&](auto value) {
         using T = decltype(value);
-        constexpr int N = 16 / sizeof(T);
-        const uint32_t pieces = static_cast<uint32_t>((width + N - 1) / N);
-        const size_t blocks = (rows * pieces + 255) / 256;
-        call.Launch(CombineRowsKernel<T, N>, std::min(blocks, kMaxGroups), 256, 0, static_cast<const T*>(sorted), sortedRows, sortedStride, rows,
-                    width, pieces, static_cast<uint32_t>(perRow), places, static_cast<const TAcc<T>*>(weights), static_cast<T*>(result),
-                    resultStride, blocks);
+        const TPieces pieces = PiecesOf(rows, width, perRow, size);
+        WithSlots(perRow, [&](auto slots) {
+            call.Launch(CombineRowsKernel<T, decltype(slots)::value>, std::min(pieces.Blocks, kMaxGroups), 256, 0, static_cast<const T*>(sorted),
+                        sortedRows, sortedStride, pieces, places, static_cast<const TAcc<T>*>(weights), static_cast<T*>(result), resultStride);
+        });
     });
 }
 
@@ -454,11 +550,25 @@ void CombineRowsBackward(int valueType, size_t rows, size_t width, int32_t perRo
     const TCallDevice call(weightGradients != nullptr ? weightGradients : sortedGradients, stream);
     WithType(valueType, [&](auto value) {
         using T = decltype(value);
-        constexpr int N = 16 / sizeof(T);
-        call.Launch(CombineRowsBackwardKernel<T, N>, std::min((rows + 3) / 4, kMaxGroups), 256, 0, static_cast<const T*>(resultGradients),
-                    gradientStride, static_cast<const T*>(sorted), sortedRows, sortedStride, rows, width, static_cast<uint32_t>(perRow), places,
-                    static_cast<const TAcc<T>*>(weights), static_cast<T*>(sortedGradients), sortedGradientStride,
-                    static_cast<TAcc<T>*>(weightGradients));
+        const size_t pieces = (width * size + 15) / 16;
+        WithSlots(perRow, [&](auto slots) {
+            constexpr int K = decltype(slots)::value;
+            const auto launch = [&](auto kernel, size_t threadsPerRow) {
+                const size_t rowsPerGroup = 256 / threadsPerRow;
+                call.Launch(kernel, std::min((rows + rowsPerGroup - 1) / rowsPerGroup, kMaxGroups), 256, 0, static_cast<const T*>(resultGradients),
+                            gradientStride, static_cast<const T*>(sorted), sortedRows, sortedStride, rows, width, static_cast<uint32_t>(perRow),
+                            places, static_cast<const TAcc<T>*>(weights), static_cast<T*>(sortedGradients), sortedGradientStride,
+                            static_cast<TAcc<T>*>(weightGradients));
+            };
+            // two pieces for a thread at most as long as eight threads are enough, else one to four for a wave's
+            if (pieces <= 16) {
+                launch(CombineRowsBackwardKernel<T, 8, K>, 8);
+            } else if (pieces <= 256) {
+                launch(CombineRowsBackwardKernel<T, 64, K>, 64);
+            } else {
+                launch(CombineRowsBackwardKernel<T, 256, K>, 256);
+            }
+        });
     });
 }
 

@@ -117,35 +117,6 @@ __device__ __forceinline__ void AdjustValues(TValues<T, N>& v, const TPenalties&
     }
 }
 
-// What a load of N values at a row's end leaves out
-template <typename T, int N>
-__device__ __forceinline__ TValues<T, N> LoadUpTo(const T* at, uint32_t n) {
-    if (n >= N) {
-        return TValues<T, N>::Load(at);
-    }
-    TValues<T, N> v{};
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        if (static_cast<uint32_t>(i) < n) {
-            v.V[i] = at[i];
-        }
-    }
-    return v;
-}
-template <typename T, int N>
-__device__ __forceinline__ void StoreUpTo(const TValues<T, N>& v, T* at, uint32_t n) {
-    if (n >= N) {
-        v.Store(at);
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        if (static_cast<uint32_t>(i) < n) {
-            at[i] = v.V[i];
-        }
-    }
-}
-
 // A workgroup for THREADS * P pieces of 16 bytes of one row. The scores are requested before the tables are made, so that
 // they arrive meanwhile; every slice of a row looks through the row's whole history.
 template <typename T, int THREADS, int P>
@@ -367,9 +338,15 @@ struct TRanked {
 };
 template <>
 struct TRanked<double> {
-    double Value;
+    uint32_t Words[2];  // of the score (with a double here, the padding behind C kept arrays of these out of registers)
     uint32_t C;
 
+    __device__ __forceinline__ TRanked() {}
+    __device__ __forceinline__ TRanked(double x, uint32_t c)
+        : C(c)
+    {
+        __builtin_memcpy(Words, &x, 8);
+    }
     __device__ __forceinline__ static TRanked None() { return {-std::numeric_limits<double>::infinity(), ~0u}; }
     __device__ __forceinline__ static TRanked Of(double x, uint32_t c) {
         const bool usable = x > -std::numeric_limits<double>::infinity();
@@ -377,29 +354,23 @@ struct TRanked<double> {
     }
     __device__ __forceinline__ bool IsNone() const { return C == ~0u; }
     __device__ __forceinline__ uint32_t Class() const { return C; }
-    __device__ __forceinline__ double Score() const { return Value; }
+    __device__ __forceinline__ double Score() const {
+        double x;
+        __builtin_memcpy(&x, Words, 8);
+        return x;
+    }
+    __device__ __forceinline__ TRanked Or(const TRanked& other, bool take) const { return {take ? other.Score() : Score(), take ? other.C : C}; }
     __device__ __forceinline__ TRanked Better(const TRanked& other) const {
-        const bool take = other.Value > Value || (other.Value == Value && other.C < C);
-        return {take ? other.Value : Value, take ? other.C : C};
+        return Or(other, other.Score() > Score() || (other.Score() == Score() && other.C < C));
     }
-    __device__ __forceinline__ TRanked BetterLater(const TRanked& other) const {
-        const bool take = other.Value > Value;
-        return {take ? other.Value : Value, take ? other.C : C};
-    }
-    __device__ __forceinline__ TRanked Without(const TRanked& other) const {
-        const bool gone = C == other.C;
-        return {gone ? -std::numeric_limits<double>::infinity() : Value, gone ? ~0u : C};
-    }
-    __device__ __forceinline__ TRanked Or(const TRanked& other, bool take) const { return {take ? other.Value : Value, take ? other.C : C}; }
+    __device__ __forceinline__ TRanked BetterLater(const TRanked& other) const { return Or(other, other.Score() > Score()); }
+    __device__ __forceinline__ TRanked Without(const TRanked& other) const { return Or(None(), C == other.C); }
 };
 
 // What a lane gets from another one: STEP lanes on, around in its row of 16 (a modifier of the instruction that uses it, and
 // no trip through LDS), or the lane whose number differs in the bit STEP
 template <int STEP, typename V>
 __device__ __forceinline__ V FromLane(const V& x) {
-    if constexpr (std::is_same_v<V, TRanked<double>>) {
-        return {FromLane<STEP>(x.Value), FromLane<STEP>(x.C)};
-    } else {
     V r;
     constexpr int words = sizeof(V) / 4;
     int from[words], to[words];
@@ -414,7 +385,6 @@ __device__ __forceinline__ V FromLane(const V& x) {
     }
     __builtin_memcpy(&r, to, sizeof(V));
     return r;
-    }
 }
 
 // f over the values of a group of 16 or 64 lanes, in the same order in each of them

@@ -195,8 +195,10 @@ __global__ void __launch_bounds__(kSortThreads) PlaceSlotsKernel(const int32_t* 
 
 // ---------------------------------------------------------------- rows to their places and back ----
 
-// Rows are cut into pieces of 16 bytes (the last one of a row may be shorter), one for a thread, in the order in which they
-// are in memory
+// Rows are cut into pieces of 16 bytes, one for a thread, in the order in which they are in memory. The last piece of a row
+// ends with the row: it holds some values of the piece before it again, which then come from two threads, alike. (Loads and
+// stores of what is left of a row instead took branches that every load waited in: 164 us for 16384 rows of 8 KB to four
+// places each where whole pieces take 130.) Rows of less than 16 bytes have pieces of one value.
 struct TPieces {
     size_t Rows, Width;   // values
     uint32_t PerRow;      // slots
@@ -204,10 +206,13 @@ struct TPieces {
     uint64_t Inverse;     // floor(i / Pieces) = floor(i Inverse / 2^64) as long as i Pieces < 2^64, which memory sees to
     size_t Blocks;        // of 256 pieces
 
-    __device__ __forceinline__ bool Of(size_t block, size_t* row, size_t* column, uint32_t valuesPerPiece) const {
+    // of N values each
+    template <int N>
+    __device__ __forceinline__ bool Of(size_t block, size_t* row, size_t* column) const {
         const uint64_t i = block * 256 + threadIdx.x;
         *row = Inverse != 0 ? __umul64hi(i, Inverse) : i;
-        *column = (i - *row * Pieces) * valuesPerPiece;
+        const size_t c = (i - *row * Pieces) * N;
+        *column = N == 1 || c + N <= Width ? c : Width - N;
         return *row < Rows;
     }
 };
@@ -229,41 +234,50 @@ struct TPlaces {
 };
 
 // A row's places are requested K at a time, so that the stores do not wait for one after the other
-template <typename T, int K>
+template <typename T, int N, int K>
 __global__ void __launch_bounds__(256) DispatchRowsKernel(const T* source, size_t sourceStride, TPieces p, const int32_t* places, T* sorted,
                                                           size_t sortedRows, size_t sortedStride) {
-    constexpr int N = 16 / sizeof(T);
+    using TPiece = std::conditional_t<N == 1, TValues<T, 1>, TValues<uint32_t, 4>>;
     for (size_t block = blockIdx.x; block < p.Blocks; block += gridDim.x) {
         size_t row, c;
-        if (!p.Of(block, &row, &c, N)) {
+        if (!p.Of<N>(block, &row, &c)) {
             return;
         }
-        const TValues<T, N> v = LoadUpTo<T, N>(source + row * sourceStride + c, p.Width - c);
+        TPiece v;
+        __builtin_memcpy(&v, source + row * sourceStride + c, sizeof(v));
         for (uint32_t k = 0; k < p.PerRow; k += K) {
             const TPlaces<K> to(places + row * p.PerRow, k, p.PerRow, sortedRows);
 #pragma unroll
             for (int j = 0; j < K; ++j) {
                 if (to.At[j] >= 0) {
-                    StoreUpTo<T, N>(v, sorted + static_cast<size_t>(to.At[j]) * sortedStride + c, p.Width - c);
+                    __builtin_memcpy(sorted + static_cast<size_t>(to.At[j]) * sortedStride + c, &v, sizeof(v));
                 }
             }
         }
     }
 }
 
-template <typename T, int K>
+// Slots that are left out are read at the row's first place that is not, and add nothing: no load waits in a branch
+template <typename T, int N, int K>
 __global__ void __launch_bounds__(256) CombineRowsKernel(const T* sorted, size_t sortedRows, size_t sortedStride, TPieces p, const int32_t* places,
                                                          const TAcc<T>* weights, T* result, size_t resultStride) {
     using A = TAcc<T>;
-    constexpr int N = 16 / sizeof(T);
     for (size_t block = blockIdx.x; block < p.Blocks; block += gridDim.x) {
         size_t row, c;
-        if (!p.Of(block, &row, &c, N)) {
+        if (!p.Of<N>(block, &row, &c)) {
             return;
         }
         A sum[N] = {};
         for (uint32_t k = 0; k < p.PerRow; k += K) {
             const TPlaces<K> from(places + row * p.PerRow, k, p.PerRow, sortedRows);
+            int32_t any = -1;
+#pragma unroll
+            for (int j = 0; j < K; ++j) {
+                any = any >= 0 ? any : from.At[j];
+            }
+            if (any < 0) {
+                continue;
+            }
             A w[K];
             TValues<T, N> v[K];
 #pragma unroll
@@ -272,17 +286,14 @@ __global__ void __launch_bounds__(256) CombineRowsKernel(const T* sorted, size_t
             }
 #pragma unroll
             for (int j = 0; j < K; ++j) {
-                if (from.At[j] >= 0) {
-                    v[j] = LoadUpTo<T, N>(sorted + static_cast<size_t>(from.At[j]) * sortedStride + c, p.Width - c);
-                }
+                v[j] = TValues<T, N>::Load(sorted + static_cast<size_t>(from.At[j] >= 0 ? from.At[j] : any) * sortedStride + c);
             }
 #pragma unroll
             for (int j = 0; j < K; ++j) {
-                if (from.At[j] >= 0) {
 #pragma unroll
-                    for (int i = 0; i < N; ++i) {
-                        sum[i] += w[j] * static_cast<A>(v[j].V[i]);
-                    }
+                for (int i = 0; i < N; ++i) {
+                    const A term = w[j] * static_cast<A>(v[j].V[i]);
+                    sum[i] += from.At[j] >= 0 ? term : A(0);
                 }
             }
         }
@@ -291,19 +302,18 @@ __global__ void __launch_bounds__(256) CombineRowsKernel(const T* sorted, size_t
         for (int i = 0; i < N; ++i) {
             out.V[i] = static_cast<T>(sum[i]);
         }
-        StoreUpTo<T, N>(out, result + row * resultStride + c, p.Width - c);
+        out.Store(result + row * resultStride + c);
     }
 }
 
 // L threads for a row. A thread takes every L-th piece of the row's gradient and, for K slots at a time, what is at their
 // places; its products are added in that order, then the threads' sums by a butterfly: the same order for every call.
-template <typename T, int L, int K>
+template <typename T, int N, int L, int K>
 __global__ void __launch_bounds__(256) CombineRowsBackwardKernel(const T* gradients, size_t gradientStride, const T* sorted, size_t sortedRows,
                                                                  size_t sortedStride, size_t rows, size_t width, uint32_t perRow,
                                                                  const int32_t* places, const TAcc<T>* weights, T* sortedGradients,
                                                                  size_t sortedGradientStride, TAcc<T>* weightGradients) {
     using A = TAcc<T>;
-    constexpr int N = 16 / sizeof(T);
     __shared__ A waveSums[4][K];
     const uint32_t lane = threadIdx.x % L;
     for (size_t first = size_t(blockIdx.x) * (256 / L); first < rows; first += size_t(gridDim.x) * (256 / L)) {
@@ -313,28 +323,21 @@ __global__ void __launch_bounds__(256) CombineRowsBackwardKernel(const T* gradie
             A product[K] = {};
             if (there) {
                 const TPlaces<K> at(places + row * perRow, k, perRow, sortedRows);
+                int32_t any = -1;
                 A w[K];
 #pragma unroll
                 for (int j = 0; j < K; ++j) {
+                    any = any >= 0 ? any : at.At[j];
                     w[j] = weights != nullptr && at.At[j] >= 0 ? weights[row * perRow + k + j] : A(1);
                 }
-                for (size_t c = size_t(lane) * N; c < width; c += L * N) {
-                    const TValues<T, N> g = LoadUpTo<T, N>(gradients + row * gradientStride + c, width - c);
+                for (size_t begin = size_t(lane) * N; any >= 0 && begin < width; begin += L * N) {
+                    const size_t c = N == 1 || begin + N <= width ? begin : width - N;
+                    TValues<T, N> g = TValues<T, N>::Load(gradients + row * gradientStride + c);
+                    TValues<T, N> v[K];
                     if (weightGradients != nullptr) {
-                        TValues<T, N> v[K];
 #pragma unroll
                         for (int j = 0; j < K; ++j) {
-                            v[j] = at.At[j] >= 0 ? LoadUpTo<T, N>(sorted + static_cast<size_t>(at.At[j]) * sortedStride + c, width - c)
-                                                 : TValues<T, N>{};
-                        }
-#pragma unroll
-                        for (int j = 0; j < K; ++j) {
-                            if (at.At[j] >= 0) {
-#pragma unroll
-                                for (int i = 0; i < N; ++i) {
-                                    product[j] += static_cast<A>(g.V[i]) * static_cast<A>(v[j].V[i]);
-                                }
-                            }
+                            v[j] = TValues<T, N>::Load(sorted + static_cast<size_t>(at.At[j] >= 0 ? at.At[j] : any) * sortedStride + c);
                         }
                     }
                     if (sortedGradients != nullptr) {
@@ -346,7 +349,19 @@ __global__ void __launch_bounds__(256) CombineRowsBackwardKernel(const T* gradie
                                 for (int i = 0; i < N; ++i) {
                                     out.V[i] = static_cast<T>(w[j] * static_cast<A>(g.V[i]));
                                 }
-                                StoreUpTo<T, N>(out, sortedGradients + static_cast<size_t>(at.At[j]) * sortedGradientStride + c, width - c);
+                                out.Store(sortedGradients + static_cast<size_t>(at.At[j]) * sortedGradientStride + c);
+                            }
+                        }
+                    }
+                    if (weightGradients != nullptr) {
+                        // (of a row's last piece, only what the piece before it does not have)
+#pragma unroll
+                        for (int i = 0; i < N; ++i) {
+                            const A gi = c + i >= begin ? static_cast<A>(g.V[i]) : A(0);
+#pragma unroll
+                            for (int j = 0; j < K; ++j) {
+                                const A term = gi * static_cast<A>(v[j].V[i]);
+                                product[j] += c + i >= begin && at.At[j] >= 0 ? term : A(0);
                             }
                         }
                     }
@@ -460,22 +475,26 @@ void CheckRoutes(size_t rows, size_t width, int32_t perRow, const int32_t* place
 }
 
 TPieces PiecesOf(size_t rows, size_t width, int32_t perRow, size_t valueSize) {
-    TPieces p;
+    TPieces p{};
     p.Rows = rows;
     p.Width = width;
     p.PerRow = static_cast<uint32_t>(perRow);
-    p.Pieces = static_cast<uint32_t>((width * valueSize + 15) / 16);
+    p.Pieces = static_cast<uint32_t>(width * valueSize < 16 ? width : (width * valueSize + 15) / 16);
     p.Inverse = p.Pieces > 1 ? ~uint64_t(0) / p.Pieces + 1 : 0;
     p.Blocks = (rows * p.Pieces + 255) / 256;
     return p;
 }
 
-// f(slots that are taken at a time)
-template <typename F>
-void WithSlots(int32_t perRow, F&& f) {
+// f(values of a piece, slots that are taken at a time)
+template <typename T, typename F>
+void WithShape(size_t width, int32_t perRow, F&& f) {
     using std::integral_constant;
-    return perRow == 1 ? f(integral_constant<int, 1>()) : perRow == 2 ? f(integral_constant<int, 2>())
-        : perRow <= 4 ? f(integral_constant<int, 4>()) : f(integral_constant<int, 8>());
+    constexpr int N = 16 / sizeof(T);
+    const auto slots = [&](auto values) {
+        return perRow == 1 ? f(values, integral_constant<int, 1>()) : perRow == 2 ? f(values, integral_constant<int, 2>())
+            : perRow <= 4 ? f(values, integral_constant<int, 4>()) : f(values, integral_constant<int, 8>());
+    };
+    return width >= N ? slots(integral_constant<int, N>()) : slots(integral_constant<int, 1>());
 }
 
 }  // namespace
@@ -493,8 +512,8 @@ void DispatchRows(int valueType, size_t rows, size_t width, int32_t perRow, cons
     const TPieces pieces = PiecesOf(rows, width, perRow, size);
     const auto launch = [&](auto value) {
         using T = decltype(value);
-        WithSlots(perRow, [&](auto slots) {
-            call.Launch(DispatchRowsKernel<T, decltype(slots)::value>, std::min(pieces.Blocks, kMaxGroups), 256, 0, static_cast<const T*>(source),
+        WithShape<T>(width, perRow, [&](auto values, auto slots) {
+            call.Launch(DispatchRowsKernel<T, decltype(values)::value, decltype(slots)::value>, std::min(pieces.Blocks, kMaxGroups), 256, 0, static_cast<const T*>(source),
                         sourceStride, pieces, places, static_cast<T*>(sorted), sortedRows, sortedStride);
         });
     };
@@ -522,8 +541,8 @@ void CombineRows(int valueType, size_t rows, size_t width, int32_t perRow, const
     WithType(valueType, [&](auto value) {
         using T = decltype(value);
         const TPieces pieces = PiecesOf(rows, width, perRow, size);
-        WithSlots(perRow, [&](auto slots) {
-            call.Launch(CombineRowsKernel<T, decltype(slots)::value>, std::min(pieces.Blocks, kMaxGroups), 256, 0, static_cast<const T*>(sorted),
+        WithShape<T>(width, perRow, [&](auto values, auto slots) {
+            call.Launch(CombineRowsKernel<T, decltype(values)::value, decltype(slots)::value>, std::min(pieces.Blocks, kMaxGroups), 256, 0, static_cast<const T*>(sorted),
                         sortedRows, sortedStride, pieces, places, static_cast<const TAcc<T>*>(weights), static_cast<T*>(result), resultStride);
         });
     });
@@ -551,8 +570,8 @@ void CombineRowsBackward(int valueType, size_t rows, size_t width, int32_t perRo
     WithType(valueType, [&](auto value) {
         using T = decltype(value);
         const size_t pieces = (width * size + 15) / 16;
-        WithSlots(perRow, [&](auto slots) {
-            constexpr int K = decltype(slots)::value;
+        WithShape<T>(width, perRow, [&](auto values, auto slots) {
+            constexpr int N = decltype(values)::value, K = decltype(slots)::value;
             const auto launch = [&](auto kernel, size_t threadsPerRow) {
                 const size_t rowsPerGroup = 256 / threadsPerRow;
                 call.Launch(kernel, std::min((rows + rowsPerGroup - 1) / rowsPerGroup, kMaxGroups), 256, 0, static_cast<const T*>(resultGradients),
@@ -562,11 +581,11 @@ void CombineRowsBackward(int valueType, size_t rows, size_t width, int32_t perRo
             };
             // two pieces for a thread at most as long as eight threads are enough, else one to four for a wave's
             if (pieces <= 16) {
-                launch(CombineRowsBackwardKernel<T, 8, K>, 8);
+                launch(CombineRowsBackwardKernel<T, N, 8, K>, 8);
             } else if (pieces <= 256) {
-                launch(CombineRowsBackwardKernel<T, 64, K>, 64);
+                launch(CombineRowsBackwardKernel<T, N, 64, K>, 64);
             } else {
-                launch(CombineRowsBackwardKernel<T, 256, K>, 256);
+                launch(CombineRowsBackwardKernel<T, N, 256, K>, 256);
             }
         });
     });

@@ -16,7 +16,7 @@ struct TAdjustArgs {
     size_t ScoreStride, ResultStride;
     size_t Rows, Tiles;
     uint32_t Classes, Slices;
-    uint32_t RowsPerTile, Pitch, PiecesInverse;  // of AdjustRowsKernel
+    uint32_t RowsPerTile, Pieces, PiecesInverse;  // of AdjustRowsKernel
     CbHipScoreAdjustment A;
 };
 
@@ -24,23 +24,23 @@ __device__ __forceinline__ int64_t Clamped(int64_t at, size_t count) {
     return at < 0 ? 0 : at > static_cast<int64_t>(count) ? static_cast<int64_t>(count) : at;
 }
 
-// The mask that a row has, -1: none
-__device__ __forceinline__ int64_t MaskOf(const CbHipScoreAdjustment& p, size_t row) {
+// The mask that a row has, null: none
+__device__ __forceinline__ const uint32_t* MaskOf(const CbHipScoreAdjustment& p, size_t row) {
     if (p.Allowed == nullptr) {
-        return -1;
+        return nullptr;
     }
     const int64_t mask = p.AllowedRows != nullptr ? static_cast<int64_t>(p.AllowedRows[row]) : static_cast<int64_t>(row);
-    return mask >= 0 && static_cast<size_t>(mask) < p.AllowedCount ? mask : -1;
+    return mask >= 0 && static_cast<size_t>(mask) < p.AllowedCount ? p.Allowed + static_cast<size_t>(mask) * p.AllowedStride : nullptr;
 }
 
-// What a row's scores have in common. A part that a call leaves out has the value that changes nothing: a repetition penalty
-// of 1, a frequency and a presence penalty of 0
+// A row's penalties. A part that a call leaves out has the value that changes nothing: a repetition penalty of 1, a frequency
+// and a presence penalty of 0
 struct TPenalties {
-    float Repetition, Frequency, Presence;
+    float Repetition, Frequency, Presence, Unused;
 
     __device__ __forceinline__ static TPenalties Of(const CbHipScoreAdjustment& p, size_t row) {
         return {p.Repetition != nullptr ? p.Repetition[row] : 1.f, p.Frequency != nullptr ? p.Frequency[row] : 0.f,
-                p.Presence != nullptr ? p.Presence[row] : 0.f};
+                p.Presence != nullptr ? p.Presence[row] : 0.f, 0.f};
     }
 };
 
@@ -55,11 +55,23 @@ __device__ __forceinline__ void CountEntry(uint32_t* word, bool given) {
     }
 }
 
-// N scores from class c on: `words` and `last` their places in the two tables, or null; `mask` the row's words, or null
-template <typename T, int N>
-__device__ __forceinline__ void AdjustValues(TValues<T, N>& v, const TPenalties& penalties, const CbHipScoreAdjustment& p, size_t row, uint32_t c,
-                                             uint32_t classes, const uint32_t* words, const uint32_t* last, int64_t firstBias, const uint32_t* mask) {
+// Four entries of a list of `count` from entry e on
+__device__ __forceinline__ TValues<int32_t, 4> LoadEntries(const int32_t* list, int64_t e, size_t count) {
+    return LoadUpTo<int32_t, 4>(list + e, count - static_cast<size_t>(e));
+}
+
+// 16 bytes of scores as they are in memory. (As single 16-bit values they would take a register each.)
+using TRaw = TValues<uint32_t, 4>;
+
+// A piece of N scores from class c on: `words` and `last` are its places in the two tables, or null; `allowed` has a bit for
+// each of the N
+template <typename T>
+__device__ __forceinline__ TRaw Adjusted(const TRaw& raw, const TPenalties& penalties, const CbHipScoreAdjustment& p, size_t row, uint32_t c,
+                                         uint32_t classes, const uint32_t* words, const uint32_t* last, int64_t firstBias, uint32_t allowed) {
     using A = TAcc<T>;
+    constexpr int N = 16 / sizeof(T);
+    TValues<T, N> v;
+    __builtin_memcpy(&v, &raw, 16);
     A x[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -87,12 +99,10 @@ __device__ __forceinline__ void AdjustValues(TValues<T, N>& v, const TPenalties&
         }
     }
     if (p.ClassBias != nullptr) {
-        const float* bias = p.ClassBias + row * p.ClassBiasStride + c;
+        const TValues<float, N> bias = LoadUpTo<float, N>(p.ClassBias + row * p.ClassBiasStride + c, classes - c);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            if (c + i < classes) {
-                x[i] += bias[i];
-            }
+            x[i] += bias.V[i];
         }
     }
     if (last != nullptr) {
@@ -103,22 +113,33 @@ __device__ __forceinline__ void AdjustValues(TValues<T, N>& v, const TPenalties&
             }
         }
     }
-    if (mask != nullptr) {
-        // (N classes from a multiple of N on are in one word)
-        const uint32_t bits = mask[c >> 5] >> (c & 31);
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            x[i] = (bits >> i & 1) != 0 ? x[i] : -std::numeric_limits<A>::infinity();
-        }
-    }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        v.V[i] = static_cast<T>(x[i]);
+        v.V[i] = static_cast<T>((allowed >> i & 1) != 0 ? x[i] : -std::numeric_limits<A>::infinity());
     }
+    TRaw out;
+    __builtin_memcpy(&out, &v, 16);
+    return out;
 }
 
-// A workgroup for THREADS * P pieces of 16 bytes of one row. The scores are requested before the tables are made, so that
-// they arrive meanwhile; every slice of a row looks through the row's whole history.
+// The first n values of a piece (a row's last piece may have less than N)
+template <typename T>
+__device__ __forceinline__ TRaw LoadPiece(const T* at, uint32_t n) {
+    const TValues<T, 16 / sizeof(T)> v = LoadUpTo<T, 16 / sizeof(T)>(at, n);
+    TRaw raw;
+    __builtin_memcpy(&raw, &v, 16);
+    return raw;
+}
+template <typename T>
+__device__ __forceinline__ void StorePiece(const TRaw& raw, T* at, uint32_t n) {
+    TValues<T, 16 / sizeof(T)> v;
+    __builtin_memcpy(&v, &raw, 16);
+    StoreUpTo<T, 16 / sizeof(T)>(v, at, n);
+}
+
+// A workgroup for THREADS * P pieces of one row. What it reads is requested at once, as far as its place is known: the
+// scores, the mask's words, the first entries of the lists; the tables are made while they are on their way. Every slice
+// of a row looks through the row's whole history.
 template <typename T, int THREADS, int P>
 __global__ void __launch_bounds__(THREADS) AdjustSliceKernel(TAdjustArgs a) {
     constexpr int N = 16 / sizeof(T);
@@ -132,69 +153,94 @@ __global__ void __launch_bounds__(THREADS) AdjustSliceKernel(TAdjustArgs a) {
         const size_t row = tile / a.Slices;
         const uint32_t c0 = static_cast<uint32_t>(tile - row * a.Slices) * S;
         const uint32_t width = min(S, a.Classes - c0);
+        int64_t begin = 0, end = 0, given = 0, firstBias = 0, endBias = 0;
+        TPenalties penalties{1, 0, 0, 0};
+        if (history) {
+            given = p.HistoryOffsets[row];
+            begin = Clamped(given, p.HistoryCount);
+            end = Clamped(p.HistoryOffsets[row + 1], p.HistoryCount);
+            given += p.PromptLengths != nullptr ? p.PromptLengths[row] : 0;
+            penalties = TPenalties::Of(p, row);
+        }
+        if (biases) {
+            firstBias = Clamped(p.BiasOffsets[row], p.BiasCount);
+            endBias = Clamped(p.BiasOffsets[row + 1], p.BiasCount);
+        }
+        const uint32_t* mask = MaskOf(p, row);
         const T* from = static_cast<const T*>(a.Scores) + row * a.ScoreStride + c0;
-        TValues<T, N> v[P];
+        TRaw v[P];
+        uint32_t allowed[P];
+        if (width == S) {
+#pragma unroll
+            for (int j = 0; j < P; ++j) {
+                v[j] = TRaw::Load(reinterpret_cast<const uint32_t*>(from + (j * THREADS + threadIdx.x) * N));
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < P; ++j) {
+                const uint32_t c = (j * THREADS + threadIdx.x) * N;
+                if (c < width) {
+                    v[j] = LoadPiece<T>(from + c, width - c);
+                }
+            }
+        }
 #pragma unroll
         for (int j = 0; j < P; ++j) {
             const uint32_t c = (j * THREADS + threadIdx.x) * N;
-            if (c < width) {
-                v[j] = LoadUpTo<T, N>(from + c, width - c);
-            }
+            // (N classes from a multiple of N on are in one word)
+            allowed[j] = mask != nullptr && c < width ? mask[(c0 + c) >> 5] >> (c & 31) : ~0u;
         }
-        int64_t firstBias = 0;
         if (history || biases) {
+            int64_t e = begin + threadIdx.x * 4;
+            TValues<int32_t, 4> entries{};
+            if (e < end) {
+                entries = LoadEntries(p.History, e, p.HistoryCount);
+            }
             __syncthreads();  // the tile before this one is done with the tables
             for (uint32_t i = threadIdx.x; i < S / 4 * (history + biases); i += THREADS) {
                 tables[i] = uint4{0, 0, 0, 0};
             }
             __syncthreads();
-            if (history) {
-                const int64_t start = p.HistoryOffsets[row];
-                const int64_t begin = Clamped(start, p.HistoryCount);
-                const int64_t end = Clamped(p.HistoryOffsets[row + 1], p.HistoryCount);
-                const int64_t given = start + (p.PromptLengths != nullptr ? p.PromptLengths[row] : 0);
-                for (int64_t e = begin + threadIdx.x * 4; e < end; e += THREADS * 4) {
-                    const uint32_t n = end - e < 4 ? static_cast<uint32_t>(end - e) : 4;
-                    const TValues<int32_t, 4> entries = LoadUpTo<int32_t, 4>(p.History + e, n);
+            while (e < end) {
+                const int64_t next = e + THREADS * 4;
+                TValues<int32_t, 4> more{};
+                if (next < end) {
+                    more = LoadEntries(p.History, next, p.HistoryCount);
+                }
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const uint32_t c = static_cast<uint32_t>(entries.V[i]) - c0;  // outside of the slice: large
-                        if (c < width && static_cast<uint32_t>(i) < n) {
-                            CountEntry(&words[c], e + i < given);
-                        }
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t c = static_cast<uint32_t>(entries.V[i]) - c0;  // outside of the slice: large
+                    if (c < width && e + i < end) {
+                        CountEntry(&words[c], e + i < given);
                     }
                 }
+                entries = more;
+                e = next;
             }
-            if (biases) {
-                firstBias = Clamped(p.BiasOffsets[row], p.BiasCount);
-                const int64_t end = Clamped(p.BiasOffsets[row + 1], p.BiasCount);
-                for (int64_t e = firstBias + threadIdx.x; e < end; e += THREADS) {
-                    const uint32_t c = static_cast<uint32_t>(p.BiasClasses[e]) - c0;
-                    if (c < width) {
-                        atomicMax(&last[c], static_cast<uint32_t>(e - firstBias) + 1);
-                    }
+            for (int64_t b = firstBias + threadIdx.x; b < endBias; b += THREADS) {
+                const uint32_t c = static_cast<uint32_t>(p.BiasClasses[b]) - c0;
+                if (c < width) {
+                    atomicMax(&last[c], static_cast<uint32_t>(b - firstBias) + 1);
                 }
             }
             __syncthreads();
         }
-        const TPenalties penalties = history ? TPenalties::Of(p, row) : TPenalties{1, 0, 0};
-        const int64_t maskRow = MaskOf(p, row);
-        const uint32_t* mask = maskRow >= 0 ? p.Allowed + static_cast<size_t>(maskRow) * p.AllowedStride : nullptr;
         T* to = static_cast<T*>(a.Result) + row * a.ResultStride + c0;
 #pragma unroll
         for (int j = 0; j < P; ++j) {
             const uint32_t c = (j * THREADS + threadIdx.x) * N;
             if (c < width) {
-                AdjustValues<T, N>(v[j], penalties, p, row, c0 + c, a.Classes, history ? words + c : nullptr, biases ? last + c : nullptr,
-                                   firstBias, mask);
-                StoreUpTo<T, N>(v[j], to + c, width - c);
+                v[j] = Adjusted<T>(v[j], penalties, p, row, c0 + c, a.Classes, history ? words + c : nullptr, biases ? last + c : nullptr, firstBias,
+                                   allowed[j]);
+                if (width == S) {
+                    v[j].Store(reinterpret_cast<uint32_t*>(to + c));
+                } else {
+                    StorePiece<T>(v[j], to + c, width - c);
+                }
             }
         }
     }
 }
-
-// Rows that are shorter than a slice: a workgroup for RowsPerTile of them
-constexpr uint32_t kMaxRowsPerTile = 512;
 
 // The row that entry `e` of a list with these offsets belongs to: the last one that begins at or before it
 __device__ __forceinline__ uint32_t RowOfEntry(const int64_t* offsets, uint32_t rows, int64_t e) {
@@ -210,91 +256,133 @@ __device__ __forceinline__ uint32_t RowOfEntry(const int64_t* offsets, uint32_t 
     return low;
 }
 
-// f(entry, row, class) for every entry of a tile's rows. A thread takes four entries at a time: it searches for the row of
-// the first and goes on from there.
+// f(entry, row, class) for the entries of a tile's rows. A thread takes four entries at a time: it searches for the row of
+// the first and goes on from there. `entries`: its first four
 template <typename F>
-__device__ __forceinline__ void ForEntries(const int64_t* offsets, uint32_t rows, int64_t begin, int64_t end, const int32_t* classes, F&& f) {
-    for (int64_t e = begin + threadIdx.x * 4; e < end; e += 256 * 4) {
-        const uint32_t n = end - e < 4 ? static_cast<uint32_t>(end - e) : 4;
-        const TValues<int32_t, 4> c = LoadUpTo<int32_t, 4>(classes + e, n);
+__device__ __forceinline__ void ForEntries(const int64_t* offsets, uint32_t rows, int64_t begin, int64_t end, const int32_t* list, size_t count,
+                                           TValues<int32_t, 4> entries, F&& f) {
+    for (int64_t e = begin + threadIdx.x * 4; e < end;) {
+        const int64_t next = e + 256 * 4;
+        TValues<int32_t, 4> more{};
+        if (next < end) {
+            more = LoadEntries(list, next, count);
+        }
         uint32_t r = RowOfEntry(offsets, rows, e);
 #pragma unroll
         for (uint32_t i = 0; i < 4; ++i) {
-            if (i < n) {
+            if (e + i < end) {
                 while (r + 1 < rows && offsets[r + 1] <= e + i) {
                     ++r;
                 }
-                f(e + i, r, static_cast<uint32_t>(c.V[i]));
+                f(e + i, r, static_cast<uint32_t>(entries.V[i]));
             }
         }
+        entries = more;
+        e = next;
     }
 }
 
-// Pieces are taken in the order in which they are in memory, whatever the rows' length, so that a wave's stores fill whole
-// lines (a thread for a row, at ten 64-bit values each, wrote 413 MB for 160)
-template <typename T>
+// Rows that are shorter than a slice: a workgroup for RowsPerTile of them, P pieces for a thread. Pieces are taken in the
+// order in which they are in memory, whatever the rows' length, so that a wave's stores fill whole lines (a thread for a
+// row, at ten 64-bit values each, wrote 413 MB for 160). What is read is requested first, as in the kernel above.
+constexpr int kPiecesPerThread = 4;
+
+template <typename T, bool WHOLE>
 __global__ void __launch_bounds__(256) AdjustRowsKernel(TAdjustArgs a) {
-    constexpr int N = 16 / sizeof(T);
+    constexpr int N = 16 / sizeof(T), P = kPiecesPerThread;
     extern __shared__ uint4 tables[];
-    __shared__ int64_t offsets[kMaxRowsPerTile];
-    __shared__ int64_t given[kMaxRowsPerTile];  // where the generated entries begin
-    __shared__ TPenalties penalties[kMaxRowsPerTile];
-    __shared__ int64_t masks[kMaxRowsPerTile];
     const CbHipScoreAdjustment& p = a.A;
     const bool history = p.HistoryOffsets != nullptr, biases = p.BiasOffsets != nullptr;
-    const uint32_t pieces = a.Pitch / N;
-    const uint32_t tableWords = a.RowsPerTile * a.Pitch;
-    uint32_t* words = reinterpret_cast<uint32_t*>(tables);
+    TPenalties* penalties = reinterpret_cast<TPenalties*>(tables);
+    int64_t* offsets = reinterpret_cast<int64_t*>(penalties + (history ? a.RowsPerTile : 0));
+    int64_t* given = offsets + (history ? a.RowsPerTile : 0);  // where the generated entries begin
+    int64_t* biasOffsets = given + (history ? a.RowsPerTile : 0);
+    uint32_t* words = reinterpret_cast<uint32_t*>(biasOffsets + (biases ? a.RowsPerTile : 0));
+    const uint32_t tableWords = a.RowsPerTile * a.Pieces * N;
     uint32_t* last = history ? words + tableWords : words;
     for (size_t tile = blockIdx.x; tile < a.Tiles; tile += gridDim.x) {
         const size_t r0 = tile * a.RowsPerTile;
         const uint32_t rows = static_cast<uint32_t>(a.Rows - r0 < a.RowsPerTile ? a.Rows - r0 : a.RowsPerTile);
-        int64_t firstBias = 0;
-        __syncthreads();  // the tile before this one is done with the tables
-        for (uint32_t i = threadIdx.x; i < (tableWords * (history + biases) + 3) / 4; i += 256) {
-            tables[i] = uint4{0, 0, 0, 0};
-        }
-        for (uint32_t r = threadIdx.x; r < rows; r += 256) {
-            masks[r] = MaskOf(p, r0 + r);
-            if (history) {
-                offsets[r] = p.HistoryOffsets[r0 + r];
-                given[r] = offsets[r] + (p.PromptLengths != nullptr ? p.PromptLengths[r0 + r] : 0);
-                penalties[r] = TPenalties::Of(p, r0 + r);
-            }
-        }
-        __syncthreads();
+        int64_t begin = 0, end = 0, firstBias = 0, endBias = 0;
         if (history) {
-            ForEntries(offsets, rows, Clamped(offsets[0], p.HistoryCount), Clamped(p.HistoryOffsets[r0 + rows], p.HistoryCount), p.History,
-                       [&](int64_t e, uint32_t r, uint32_t c) {
-                           if (c < a.Classes) {
-                               CountEntry(&words[r * a.Pitch + c], e < given[r]);
-                           }
-                       });
-            __syncthreads();
+            begin = Clamped(p.HistoryOffsets[r0], p.HistoryCount);
+            end = Clamped(p.HistoryOffsets[r0 + rows], p.HistoryCount);
         }
         if (biases) {
-            for (uint32_t r = threadIdx.x; r < rows; r += 256) {
-                offsets[r] = p.BiasOffsets[r0 + r];
+            firstBias = Clamped(p.BiasOffsets[r0], p.BiasCount);
+            endBias = Clamped(p.BiasOffsets[r0 + rows], p.BiasCount);
+        }
+        uint32_t r[P], c[P], allowed[P];
+        const uint32_t* mask[P];
+        TRaw v[P];
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+            const uint32_t q = j * 256 + threadIdx.x;
+            r[j] = a.PiecesInverse != 0 ? __umulhi(q, a.PiecesInverse) : q;
+            c[j] = (q - r[j] * a.Pieces) * N;
+            r[j] = min(r[j], rows);
+            mask[j] = r[j] < rows ? MaskOf(p, r0 + r[j]) : nullptr;
+        }
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+            if (r[j] < rows) {
+                const T* from = static_cast<const T*>(a.Scores) + (r0 + r[j]) * a.ScoreStride + c[j];
+                v[j] = WHOLE ? TRaw::Load(reinterpret_cast<const uint32_t*>(from)) : LoadPiece<T>(from, a.Classes - c[j]);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+            allowed[j] = mask[j] != nullptr ? mask[j][c[j] >> 5] >> (c[j] & 31) : ~0u;
+        }
+        if (history || biases) {
+            TValues<int32_t, 4> entries{}, biasEntries{};
+            if (begin + threadIdx.x * 4 < end) {
+                entries = LoadEntries(p.History, begin + threadIdx.x * 4, p.HistoryCount);
+            }
+            if (firstBias + threadIdx.x * 4 < endBias) {
+                biasEntries = LoadEntries(p.BiasClasses, firstBias + threadIdx.x * 4, p.BiasCount);
+            }
+            __syncthreads();  // the tile before this one is done with the tables
+            for (uint32_t i = threadIdx.x; i < tableWords * (history + biases); i += 256) {
+                words[i] = 0;
+            }
+            for (uint32_t i = threadIdx.x; i < rows; i += 256) {
+                if (history) {
+                    offsets[i] = p.HistoryOffsets[r0 + i];
+                    given[i] = offsets[i] + (p.PromptLengths != nullptr ? p.PromptLengths[r0 + i] : 0);
+                    penalties[i] = TPenalties::Of(p, r0 + i);
+                }
+                if (biases) {
+                    biasOffsets[i] = p.BiasOffsets[r0 + i];
+                }
             }
             __syncthreads();
-            firstBias = Clamped(offsets[0], p.BiasCount);
-            ForEntries(offsets, rows, firstBias, Clamped(p.BiasOffsets[r0 + rows], p.BiasCount), p.BiasClasses,
-                       [&](int64_t e, uint32_t r, uint32_t c) {
-                           if (c < a.Classes) {
-                               atomicMax(&last[r * a.Pitch + c], static_cast<uint32_t>(e - firstBias) + 1);
-                           }
-                       });
+            const uint32_t pitch = a.Pieces * N;
+            ForEntries(offsets, rows, begin, end, p.History, p.HistoryCount, entries, [&](int64_t e, uint32_t i, uint32_t k) {
+                if (k < a.Classes) {
+                    CountEntry(&words[i * pitch + k], e < given[i]);
+                }
+            });
+            ForEntries(biasOffsets, rows, firstBias, endBias, p.BiasClasses, p.BiasCount, biasEntries, [&](int64_t e, uint32_t i, uint32_t k) {
+                if (k < a.Classes) {
+                    atomicMax(&last[i * pitch + k], static_cast<uint32_t>(e - firstBias) + 1);
+                }
+            });
             __syncthreads();
         }
-        for (uint32_t q = threadIdx.x; q < rows * pieces; q += 256) {
-            const uint32_t r = a.PiecesInverse != 0 ? __umulhi(q, a.PiecesInverse) : q;
-            const uint32_t c = (q - r * pieces) * N;
-            const size_t row = r0 + r;
-            TValues<T, N> v = LoadUpTo<T, N>(static_cast<const T*>(a.Scores) + row * a.ScoreStride + c, a.Classes - c);
-            const int64_t mask = masks[r];
-            AdjustValues<T, N>(v, penalties[r], p, row, c, a.Classes, history ? words + q * N : nullptr, biases ? last + q * N : nullptr, firstBias,
-                               mask >= 0 ? p.Allowed + static_cast<size_t>(mask) * p.AllowedStride : nullptr);
-            StoreUpTo<T, N>(v, static_cast<T*>(a.Result) + row * a.ResultStride + c, a.Classes - c);
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+            if (r[j] < rows) {
+                const uint32_t at = (j * 256 + threadIdx.x) * N;
+                v[j] = Adjusted<T>(v[j], history ? penalties[r[j]] : TPenalties{1, 0, 0, 0}, p, r0 + r[j], c[j], a.Classes,
+                                   history ? words + at : nullptr, biases ? last + at : nullptr, firstBias, allowed[j]);
+                T* to = static_cast<T*>(a.Result) + (r0 + r[j]) * a.ResultStride + c[j];
+                if (WHOLE) {
+                    v[j].Store(reinterpret_cast<uint32_t*>(to));
+                } else {
+                    StorePiece<T>(v[j], to, a.Classes - c[j]);
+                }
+            }
         }
     }
 }
@@ -737,7 +825,6 @@ using namespace op;
 
 namespace {
 
-constexpr uint32_t kRowTileWords = 4096;      // of a table of AdjustRowsKernel
 constexpr size_t kWorkgroupsWanted = 512;     // two for each compute unit
 
 }  // namespace
@@ -778,15 +865,26 @@ void AdjustScores(int valueType, size_t rows, size_t classes, const void* scores
         using T = decltype(value);
         constexpr uint32_t N = 16 / sizeof(T);
         const size_t tables = size_t(history) + size_t(biases);
-        if (a.Classes <= kRowTileWords / 4) {
-            const uint32_t pieces = (a.Classes + N - 1) / N;
-            a.Pitch = pieces * N;
-            a.RowsPerTile = std::min<uint32_t>(kMaxRowsPerTile, std::max<uint32_t>(1, kRowTileWords / a.Pitch));
+        const uint32_t pieces = (a.Classes + N - 1) / N;
+        constexpr uint32_t tilePieces = kPiecesPerThread * 256;
+        if (pieces <= tilePieces / 4) {
+            a.Pieces = pieces;
+            a.RowsPerTile = static_cast<uint32_t>(std::min<size_t>(tilePieces / pieces, rows));
             // floor(q / pieces) = floor(q m / 2^32) with m = floor(2^32 / pieces) + 1: q m / 2^32 is over q / pieces by q / 2^32 at most, and
-            // q / pieces is under the next integer by 1 / pieces at least, which is more for the q and pieces under 2^13 here
+            // q / pieces is under the next integer by 1 / pieces at least, which is more for the q and pieces under 2^11 here
             a.PiecesInverse = pieces > 1 ? static_cast<uint32_t>((uint64_t(1) << 32) / pieces + 1) : 0;
             a.Tiles = (rows + a.RowsPerTile - 1) / a.RowsPerTile;
-            call.Launch(AdjustRowsKernel<T>, std::min<size_t>(a.Tiles, 1u << 20), 256, (size_t(a.RowsPerTile) * a.Pitch * tables + 3) / 4 * 16, a);
+            const size_t perRow = (history ? sizeof(TPenalties) + 16 : 0) + (biases ? 8 : 0) + size_t(pieces) * N * 4 * tables;
+            const size_t lds = a.RowsPerTile * perRow;
+            const auto launch = [&](auto kernel) {
+                call.AllowLds(reinterpret_cast<const void*>(kernel), lds);
+                call.Launch(kernel, std::min<size_t>(a.Tiles, 1u << 20), 256, lds, a);
+            };
+            if (a.Classes % N == 0) {
+                launch(AdjustRowsKernel<T, true>);
+            } else {
+                launch(AdjustRowsKernel<T, false>);
+            }
             return;
         }
         const auto slices = [&](uint32_t size) { return (a.Classes + size - 1) / size; };

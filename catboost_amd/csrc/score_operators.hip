@@ -14,8 +14,8 @@ struct TAdjustArgs {
     const void* Scores;
     void* Result;
     size_t ScoreStride, ResultStride;
-    size_t Rows, Tiles;
-    uint32_t Classes, Slices;
+    size_t Rows, FirstTile;
+    uint32_t Classes, Slices, SliceClasses;       // of AdjustSliceKernel
     uint32_t RowsPerTile, Pieces, PiecesInverse;  // of AdjustRowsKernel
     CbHipScoreAdjustment A;
 };
@@ -24,13 +24,10 @@ __device__ __forceinline__ int64_t Clamped(int64_t at, size_t count) {
     return at < 0 ? 0 : at > static_cast<int64_t>(count) ? static_cast<int64_t>(count) : at;
 }
 
-// The mask that a row has, null: none
-__device__ __forceinline__ const uint32_t* MaskOf(const CbHipScoreAdjustment& p, size_t row) {
-    if (p.Allowed == nullptr) {
-        return nullptr;
-    }
+// The mask that a row has, -1: none
+__device__ __forceinline__ int64_t MaskOf(const CbHipScoreAdjustment& p, size_t row) {
     const int64_t mask = p.AllowedRows != nullptr ? static_cast<int64_t>(p.AllowedRows[row]) : static_cast<int64_t>(row);
-    return mask >= 0 && static_cast<size_t>(mask) < p.AllowedCount ? p.Allowed + static_cast<size_t>(mask) * p.AllowedStride : nullptr;
+    return mask >= 0 && static_cast<size_t>(mask) < p.AllowedCount ? mask : -1;
 }
 
 // A row's penalties. A part that a call leaves out has the value that changes nothing: a repetition penalty of 1, a frequency
@@ -63,21 +60,22 @@ __device__ __forceinline__ TValues<int32_t, 4> LoadEntries(const int32_t* list, 
 // 16 bytes of scores as they are in memory. (As single 16-bit values they would take a register each.)
 using TRaw = TValues<uint32_t, 4>;
 
-// A piece of N scores from class c on: `words` and `last` are its places in the two tables, or null; `allowed` has a bit for
-// each of the N
+// A piece's scores on their way
 template <typename T>
-__device__ __forceinline__ TRaw Adjusted(const TRaw& raw, const TPenalties& penalties, const CbHipScoreAdjustment& p, size_t row, uint32_t c,
-                                         uint32_t classes, const uint32_t* words, const uint32_t* last, int64_t firstBias, uint32_t allowed) {
+struct TPiece {
     using A = TAcc<T>;
-    constexpr int N = 16 / sizeof(T);
-    TValues<T, N> v;
-    __builtin_memcpy(&v, &raw, 16);
-    A x[N];
+    static constexpr int N = 16 / sizeof(T);
+    A X[N];
+
+    __device__ __forceinline__ explicit TPiece(const TRaw& raw) {
+        TValues<T, N> v;
+        __builtin_memcpy(&v, &raw, 16);
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        x[i] = static_cast<A>(v.V[i]);
+        for (int i = 0; i < N; ++i) {
+            X[i] = static_cast<A>(v.V[i]);
+        }
     }
-    if (words != nullptr) {
+    __device__ __forceinline__ void Penalize(const uint32_t* words, const TPenalties& penalties) {
         uint32_t w[N], any = 0;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
@@ -89,38 +87,42 @@ __device__ __forceinline__ TRaw Adjusted(const TRaw& raw, const TPenalties& pena
             for (int i = 0; i < N; ++i) {
                 if (w[i] != 0) {
                     const A repetition = penalties.Repetition;
-                    x[i] = x[i] > 0 ? x[i] / repetition : x[i] * repetition;
+                    X[i] = X[i] > 0 ? X[i] / repetition : X[i] * repetition;
                 }
                 if (w[i] > 1) {
-                    x[i] -= static_cast<A>(penalties.Frequency) * static_cast<A>(w[i] >> 1);
-                    x[i] -= static_cast<A>(penalties.Presence);
+                    X[i] -= static_cast<A>(penalties.Frequency) * static_cast<A>(w[i] >> 1);
+                    X[i] -= static_cast<A>(penalties.Presence);
                 }
             }
         }
     }
-    if (p.ClassBias != nullptr) {
-        const TValues<float, N> bias = LoadUpTo<float, N>(p.ClassBias + row * p.ClassBiasStride + c, classes - c);
+    __device__ __forceinline__ void Add(const TValues<float, N>& bias) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            x[i] += bias.V[i];
+            X[i] += bias.V[i];
         }
     }
-    if (last != nullptr) {
+    __device__ __forceinline__ void AddLast(const uint32_t* last, const float* values) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            if (last[i] != 0) {
-                x[i] += p.BiasValues[firstBias + last[i] - 1];
+            const uint32_t entry = last[i];
+            if (entry != 0) {
+                X[i] += values[entry - 1];
             }
         }
     }
+    // a bit of `allowed` for each of them
+    __device__ __forceinline__ TRaw Rounded(uint32_t allowed) const {
+        TValues<T, N> v;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        v.V[i] = static_cast<T>((allowed >> i & 1) != 0 ? x[i] : -std::numeric_limits<A>::infinity());
+        for (int i = 0; i < N; ++i) {
+            v.V[i] = static_cast<T>((allowed >> i & 1) != 0 ? X[i] : -std::numeric_limits<A>::infinity());
+        }
+        TRaw raw;
+        __builtin_memcpy(&raw, &v, 16);
+        return raw;
     }
-    TRaw out;
-    __builtin_memcpy(&out, &v, 16);
-    return out;
-}
+};
 
 // The first n values of a piece (a row's last piece may have less than N)
 template <typename T>
@@ -137,106 +139,118 @@ __device__ __forceinline__ void StorePiece(const TRaw& raw, T* at, uint32_t n) {
     StoreUpTo<T, 16 / sizeof(T)>(v, at, n);
 }
 
-// A workgroup for THREADS * P pieces of one row. What it reads is requested at once, as far as its place is known: the
-// scores, the mask's words, the first entries of the lists; the tables are made while they are on their way. Every slice
-// of a row looks through the row's whole history.
+// A workgroup for a slice of one row, at most THREADS * P pieces. What it reads is requested at once, as far as its place is
+// known, and without branches, which would wait for one load after the other: the scores, the mask's words, the first
+// entries of the history; the tables are made while they are on their way. The scores wait as they came (as 32-bit values
+// they would leave one workgroup for a compute unit instead of two). Every slice of a row looks through the row's whole
+// history; slices of a row are alike in length.
 template <typename T, int THREADS, int P>
 __global__ void __launch_bounds__(THREADS) AdjustSliceKernel(TAdjustArgs a) {
     constexpr int N = 16 / sizeof(T);
-    constexpr uint32_t S = THREADS * P * N;
     extern __shared__ uint4 tables[];
     const CbHipScoreAdjustment& p = a.A;
     const bool history = p.HistoryOffsets != nullptr, biases = p.BiasOffsets != nullptr;
     uint32_t* words = reinterpret_cast<uint32_t*>(tables);
-    uint32_t* last = history ? words + S : words;
-    for (size_t tile = blockIdx.x; tile < a.Tiles; tile += gridDim.x) {
-        const size_t row = tile / a.Slices;
-        const uint32_t c0 = static_cast<uint32_t>(tile - row * a.Slices) * S;
-        const uint32_t width = min(S, a.Classes - c0);
-        int64_t begin = 0, end = 0, given = 0, firstBias = 0, endBias = 0;
-        TPenalties penalties{1, 0, 0, 0};
-        if (history) {
-            given = p.HistoryOffsets[row];
-            begin = Clamped(given, p.HistoryCount);
-            end = Clamped(p.HistoryOffsets[row + 1], p.HistoryCount);
-            given += p.PromptLengths != nullptr ? p.PromptLengths[row] : 0;
-            penalties = TPenalties::Of(p, row);
-        }
-        if (biases) {
-            firstBias = Clamped(p.BiasOffsets[row], p.BiasCount);
-            endBias = Clamped(p.BiasOffsets[row + 1], p.BiasCount);
-        }
-        const uint32_t* mask = MaskOf(p, row);
-        const T* from = static_cast<const T*>(a.Scores) + row * a.ScoreStride + c0;
-        TRaw v[P];
-        uint32_t allowed[P];
-        if (width == S) {
-#pragma unroll
-            for (int j = 0; j < P; ++j) {
-                v[j] = TRaw::Load(reinterpret_cast<const uint32_t*>(from + (j * THREADS + threadIdx.x) * N));
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < P; ++j) {
-                const uint32_t c = (j * THREADS + threadIdx.x) * N;
-                if (c < width) {
-                    v[j] = LoadPiece<T>(from + c, width - c);
-                }
-            }
-        }
+    uint32_t* last = words + (history ? a.SliceClasses : 0);
+    const size_t tile = a.FirstTile + blockIdx.x;
+    const size_t row = tile / a.Slices;
+    const uint32_t c0 = static_cast<uint32_t>(tile - row * a.Slices) * a.SliceClasses;
+    const uint32_t width = min(a.SliceClasses, a.Classes - c0);
+    int64_t begin = 0, end = 0, given = 0, firstBias = 0, endBias = 0;
+    TPenalties penalties{1, 0, 0, 0};
+    if (history) {
+        given = p.HistoryOffsets[row];
+        begin = Clamped(given, p.HistoryCount);
+        end = Clamped(p.HistoryOffsets[row + 1], p.HistoryCount);
+        given += p.PromptLengths != nullptr ? p.PromptLengths[row] : 0;
+        penalties = TPenalties::Of(p, row);
+    }
+    if (biases) {
+        firstBias = Clamped(p.BiasOffsets[row], p.BiasCount);
+        endBias = Clamped(p.BiasOffsets[row + 1], p.BiasCount);
+    }
+    const int64_t mask = p.AllowedCount != 0 ? MaskOf(p, row) : -1;
+    const T* from = static_cast<const T*>(a.Scores) + row * a.ScoreStride + c0;
+    const bool whole = width % N == 0;  // only a row's last slice may end inside a piece
+    TRaw raw[P];
+    uint32_t allowed[P];
+    if (whole) {
 #pragma unroll
         for (int j = 0; j < P; ++j) {
-            const uint32_t c = (j * THREADS + threadIdx.x) * N;
-            // (N classes from a multiple of N on are in one word)
-            allowed[j] = mask != nullptr && c < width ? mask[(c0 + c) >> 5] >> (c & 31) : ~0u;
+            raw[j] = TRaw::Load(reinterpret_cast<const uint32_t*>(from + min((j * THREADS + threadIdx.x) * N, width - N)));
         }
-        if (history || biases) {
-            int64_t e = begin + threadIdx.x * 4;
-            TValues<int32_t, 4> entries{};
-            if (e < end) {
-                entries = LoadEntries(p.History, e, p.HistoryCount);
-            }
-            __syncthreads();  // the tile before this one is done with the tables
-            for (uint32_t i = threadIdx.x; i < S / 4 * (history + biases); i += THREADS) {
-                tables[i] = uint4{0, 0, 0, 0};
-            }
-            __syncthreads();
-            while (e < end) {
-                const int64_t next = e + THREADS * 4;
-                TValues<int32_t, 4> more{};
-                if (next < end) {
-                    more = LoadEntries(p.History, next, p.HistoryCount);
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t c = static_cast<uint32_t>(entries.V[i]) - c0;  // outside of the slice: large
-                    if (c < width && e + i < end) {
-                        CountEntry(&words[c], e + i < given);
-                    }
-                }
-                entries = more;
-                e = next;
-            }
-            for (int64_t b = firstBias + threadIdx.x; b < endBias; b += THREADS) {
-                const uint32_t c = static_cast<uint32_t>(p.BiasClasses[b]) - c0;
-                if (c < width) {
-                    atomicMax(&last[c], static_cast<uint32_t>(b - firstBias) + 1);
-                }
-            }
-            __syncthreads();
-        }
-        T* to = static_cast<T*>(a.Result) + row * a.ResultStride + c0;
+    } else {
 #pragma unroll
         for (int j = 0; j < P; ++j) {
             const uint32_t c = (j * THREADS + threadIdx.x) * N;
             if (c < width) {
-                v[j] = Adjusted<T>(v[j], penalties, p, row, c0 + c, a.Classes, history ? words + c : nullptr, biases ? last + c : nullptr, firstBias,
-                                   allowed[j]);
-                if (width == S) {
-                    v[j].Store(reinterpret_cast<uint32_t*>(to + c));
-                } else {
-                    StorePiece<T>(v[j], to + c, width - c);
+                raw[j] = LoadPiece<T>(from + c, width - c);
+            }
+        }
+    }
+    if (mask >= 0) {
+        const uint32_t* bits = p.Allowed + static_cast<size_t>(mask) * p.AllowedStride;
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+            // (N classes from a multiple of N on are in one word)
+            allowed[j] = bits[(c0 + min((j * THREADS + threadIdx.x) * N, width - 1)) >> 5];
+        }
+    }
+    if (history || biases) {
+        int64_t e = begin + threadIdx.x * 4;
+        TValues<int32_t, 4> entries{};
+        if (e < end) {
+            entries = LoadEntries(p.History, e, p.HistoryCount);
+        }
+        for (uint32_t i = threadIdx.x; i < a.SliceClasses / 4 * (history + biases); i += THREADS) {
+            tables[i] = uint4{0, 0, 0, 0};
+        }
+        __syncthreads();
+        while (e < end) {
+            const int64_t next = e + THREADS * 4;
+            TValues<int32_t, 4> more{};
+            if (next < end) {
+                more = LoadEntries(p.History, next, p.HistoryCount);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t c = static_cast<uint32_t>(entries.V[i]) - c0;  // outside of the slice: large
+                if (c < width && e + i < end) {
+                    CountEntry(&words[c], e + i < given);
                 }
+            }
+            entries = more;
+            e = next;
+        }
+        for (int64_t b = firstBias + threadIdx.x; b < endBias; b += THREADS) {
+            const uint32_t c = static_cast<uint32_t>(p.BiasClasses[b]) - c0;
+            if (c < width) {
+                atomicMax(&last[c], static_cast<uint32_t>(b - firstBias) + 1);
+            }
+        }
+        __syncthreads();
+    }
+    T* to = static_cast<T*>(a.Result) + row * a.ResultStride + c0;
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+        const uint32_t c = (j * THREADS + threadIdx.x) * N;
+        if (c < width) {
+            TPiece<T> x(raw[j]);
+            if (history) {
+                x.Penalize(words + c, penalties);
+            }
+            if (p.ClassBias != nullptr) {
+                const float* bias = p.ClassBias + row * p.ClassBiasStride + c0 + c;
+                x.Add(whole ? TValues<float, N>::Load(bias) : LoadUpTo<float, N>(bias, width - c));
+            }
+            if (biases) {
+                x.AddLast(last + c, p.BiasValues + firstBias);
+            }
+            const TRaw out = x.Rounded(mask >= 0 ? allowed[j] >> (c & 31) : ~0u);
+            if (whole) {
+                out.Store(reinterpret_cast<uint32_t*>(to + c));
+            } else {
+                StorePiece<T>(out, to + c, width - c);
             }
         }
     }
@@ -293,95 +307,111 @@ __global__ void __launch_bounds__(256) AdjustRowsKernel(TAdjustArgs a) {
     extern __shared__ uint4 tables[];
     const CbHipScoreAdjustment& p = a.A;
     const bool history = p.HistoryOffsets != nullptr, biases = p.BiasOffsets != nullptr;
+    const uint32_t pitch = a.Pieces * N;
     TPenalties* penalties = reinterpret_cast<TPenalties*>(tables);
     int64_t* offsets = reinterpret_cast<int64_t*>(penalties + (history ? a.RowsPerTile : 0));
     int64_t* given = offsets + (history ? a.RowsPerTile : 0);  // where the generated entries begin
     int64_t* biasOffsets = given + (history ? a.RowsPerTile : 0);
     uint32_t* words = reinterpret_cast<uint32_t*>(biasOffsets + (biases ? a.RowsPerTile : 0));
-    const uint32_t tableWords = a.RowsPerTile * a.Pieces * N;
-    uint32_t* last = history ? words + tableWords : words;
-    for (size_t tile = blockIdx.x; tile < a.Tiles; tile += gridDim.x) {
-        const size_t r0 = tile * a.RowsPerTile;
-        const uint32_t rows = static_cast<uint32_t>(a.Rows - r0 < a.RowsPerTile ? a.Rows - r0 : a.RowsPerTile);
-        int64_t begin = 0, end = 0, firstBias = 0, endBias = 0;
-        if (history) {
-            begin = Clamped(p.HistoryOffsets[r0], p.HistoryCount);
-            end = Clamped(p.HistoryOffsets[r0 + rows], p.HistoryCount);
-        }
-        if (biases) {
-            firstBias = Clamped(p.BiasOffsets[r0], p.BiasCount);
-            endBias = Clamped(p.BiasOffsets[r0 + rows], p.BiasCount);
-        }
-        uint32_t r[P], c[P], allowed[P];
-        const uint32_t* mask[P];
-        TRaw v[P];
+    uint32_t* last = words + (history ? a.RowsPerTile * pitch : 0);
+    const auto rowOf = [&](uint32_t q) { return a.PiecesInverse != 0 ? __umulhi(q, a.PiecesInverse) : q; };
+    const size_t tile = a.FirstTile + blockIdx.x;
+    const size_t r0 = tile * a.RowsPerTile;
+    const uint32_t rows = static_cast<uint32_t>(a.Rows - r0 < a.RowsPerTile ? a.Rows - r0 : a.RowsPerTile);
+    int64_t begin = 0, end = 0, firstBias = 0, endBias = 0;
+    if (history) {
+        begin = Clamped(p.HistoryOffsets[r0], p.HistoryCount);
+        end = Clamped(p.HistoryOffsets[r0 + rows], p.HistoryCount);
+    }
+    if (biases) {
+        firstBias = Clamped(p.BiasOffsets[r0], p.BiasCount);
+        endBias = Clamped(p.BiasOffsets[r0 + rows], p.BiasCount);
+    }
+    // a thread whose pieces are behind the tile's last row reads that row's instead
+    int32_t mask[P];
+    uint32_t allowed[P];
+    TRaw raw[P];
+    if (p.AllowedRows != nullptr) {
 #pragma unroll
         for (int j = 0; j < P; ++j) {
-            const uint32_t q = j * 256 + threadIdx.x;
-            r[j] = a.PiecesInverse != 0 ? __umulhi(q, a.PiecesInverse) : q;
-            c[j] = (q - r[j] * a.Pieces) * N;
-            r[j] = min(r[j], rows);
-            mask[j] = r[j] < rows ? MaskOf(p, r0 + r[j]) : nullptr;
+            mask[j] = p.AllowedRows[r0 + min(rowOf(j * 256 + threadIdx.x), rows - 1)];
         }
+    }
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+        const uint32_t q = j * 256 + threadIdx.x, r = rowOf(q), c = (q - r * a.Pieces) * N;
+        const T* from = static_cast<const T*>(a.Scores) + (r0 + min(r, rows - 1)) * a.ScoreStride + c;
+        raw[j] = WHOLE ? TRaw::Load(reinterpret_cast<const uint32_t*>(from)) : LoadPiece<T>(from, a.Classes - c);
+    }
+    if (p.AllowedCount != 0) {
 #pragma unroll
         for (int j = 0; j < P; ++j) {
-            if (r[j] < rows) {
-                const T* from = static_cast<const T*>(a.Scores) + (r0 + r[j]) * a.ScoreStride + c[j];
-                v[j] = WHOLE ? TRaw::Load(reinterpret_cast<const uint32_t*>(from)) : LoadPiece<T>(from, a.Classes - c[j]);
+            const uint32_t q = j * 256 + threadIdx.x, r = rowOf(q), c = (q - r * a.Pieces) * N;
+            size_t m = r0 + min(r, rows - 1);
+            if (p.AllowedRows != nullptr) {
+                const bool some = mask[j] >= 0 && static_cast<size_t>(mask[j]) < p.AllowedCount;
+                m = some ? mask[j] : 0;
+                mask[j] = some;
+            }
+            allowed[j] = p.Allowed[m * p.AllowedStride + (c >> 5)];
+        }
+    }
+    if (history || biases) {
+        TValues<int32_t, 4> entries{}, biasEntries{};
+        if (begin + threadIdx.x * 4 < end) {
+            entries = LoadEntries(p.History, begin + threadIdx.x * 4, p.HistoryCount);
+        }
+        if (firstBias + threadIdx.x * 4 < endBias) {
+            biasEntries = LoadEntries(p.BiasClasses, firstBias + threadIdx.x * 4, p.BiasCount);
+        }
+        for (uint32_t i = threadIdx.x; i < a.RowsPerTile * pitch * (history + biases); i += 256) {
+            words[i] = 0;
+        }
+        for (uint32_t i = threadIdx.x; i < rows; i += 256) {
+            if (history) {
+                offsets[i] = p.HistoryOffsets[r0 + i];
+                given[i] = offsets[i] + (p.PromptLengths != nullptr ? p.PromptLengths[r0 + i] : 0);
+                penalties[i] = TPenalties::Of(p, r0 + i);
+            }
+            if (biases) {
+                biasOffsets[i] = p.BiasOffsets[r0 + i];
             }
         }
+        __syncthreads();
+        ForEntries(offsets, rows, begin, end, p.History, p.HistoryCount, entries, [&](int64_t e, uint32_t i, uint32_t c) {
+            if (c < a.Classes) {
+                CountEntry(&words[i * pitch + c], e < given[i]);
+            }
+        });
+        ForEntries(biasOffsets, rows, firstBias, endBias, p.BiasClasses, p.BiasCount, biasEntries, [&](int64_t e, uint32_t i, uint32_t c) {
+            if (c < a.Classes) {
+                atomicMax(&last[i * pitch + c], static_cast<uint32_t>(e - firstBias) + 1);
+            }
+        });
+        __syncthreads();
+    }
 #pragma unroll
-        for (int j = 0; j < P; ++j) {
-            allowed[j] = mask[j] != nullptr ? mask[j][c[j] >> 5] >> (c[j] & 31) : ~0u;
-        }
-        if (history || biases) {
-            TValues<int32_t, 4> entries{}, biasEntries{};
-            if (begin + threadIdx.x * 4 < end) {
-                entries = LoadEntries(p.History, begin + threadIdx.x * 4, p.HistoryCount);
+    for (int j = 0; j < P; ++j) {
+        const uint32_t q = j * 256 + threadIdx.x, r = rowOf(q), c = (q - r * a.Pieces) * N;
+        if (r < rows) {
+            TPiece<T> x(raw[j]);
+            if (history) {
+                x.Penalize(words + q * N, penalties[r]);
             }
-            if (firstBias + threadIdx.x * 4 < endBias) {
-                biasEntries = LoadEntries(p.BiasClasses, firstBias + threadIdx.x * 4, p.BiasCount);
+            if (p.ClassBias != nullptr) {
+                const float* bias = p.ClassBias + (r0 + r) * p.ClassBiasStride + c;
+                x.Add(WHOLE ? TValues<float, N>::Load(bias) : LoadUpTo<float, N>(bias, a.Classes - c));
             }
-            __syncthreads();  // the tile before this one is done with the tables
-            for (uint32_t i = threadIdx.x; i < tableWords * (history + biases); i += 256) {
-                words[i] = 0;
+            if (biases) {
+                x.AddLast(last + q * N, p.BiasValues + firstBias);
             }
-            for (uint32_t i = threadIdx.x; i < rows; i += 256) {
-                if (history) {
-                    offsets[i] = p.HistoryOffsets[r0 + i];
-                    given[i] = offsets[i] + (p.PromptLengths != nullptr ? p.PromptLengths[r0 + i] : 0);
-                    penalties[i] = TPenalties::Of(p, r0 + i);
-                }
-                if (biases) {
-                    biasOffsets[i] = p.BiasOffsets[r0 + i];
-                }
-            }
-            __syncthreads();
-            const uint32_t pitch = a.Pieces * N;
-            ForEntries(offsets, rows, begin, end, p.History, p.HistoryCount, entries, [&](int64_t e, uint32_t i, uint32_t k) {
-                if (k < a.Classes) {
-                    CountEntry(&words[i * pitch + k], e < given[i]);
-                }
-            });
-            ForEntries(biasOffsets, rows, firstBias, endBias, p.BiasClasses, p.BiasCount, biasEntries, [&](int64_t e, uint32_t i, uint32_t k) {
-                if (k < a.Classes) {
-                    atomicMax(&last[i * pitch + k], static_cast<uint32_t>(e - firstBias) + 1);
-                }
-            });
-            __syncthreads();
-        }
-#pragma unroll
-        for (int j = 0; j < P; ++j) {
-            if (r[j] < rows) {
-                const uint32_t at = (j * 256 + threadIdx.x) * N;
-                v[j] = Adjusted<T>(v[j], history ? penalties[r[j]] : TPenalties{1, 0, 0, 0}, p, r0 + r[j], c[j], a.Classes,
-                                   history ? words + at : nullptr, biases ? last + at : nullptr, firstBias, allowed[j]);
-                T* to = static_cast<T*>(a.Result) + (r0 + r[j]) * a.ResultStride + c[j];
-                if (WHOLE) {
-                    v[j].Store(reinterpret_cast<uint32_t*>(to));
-                } else {
-                    StorePiece<T>(v[j], to, a.Classes - c[j]);
-                }
+            const bool masked = p.AllowedCount != 0 && (p.AllowedRows == nullptr || mask[j] != 0);
+            const TRaw out = x.Rounded(masked ? allowed[j] >> (c & 31) : ~0u);
+            T* to = static_cast<T*>(a.Result) + (r0 + r) * a.ResultStride + c;
+            if (WHOLE) {
+                out.Store(reinterpret_cast<uint32_t*>(to));
+            } else {
+                StorePiece<T>(out, to, a.Classes - c);
             }
         }
     }
@@ -826,6 +856,7 @@ using namespace op;
 namespace {
 
 constexpr size_t kWorkgroupsWanted = 512;     // two for each compute unit
+constexpr size_t kTilesPerLaunch = 1u << 21;  // 2^31 threads
 
 }  // namespace
 
@@ -860,11 +891,20 @@ void AdjustScores(int valueType, size_t rows, size_t classes, const void* scores
     a.Rows = rows;
     a.Classes = static_cast<uint32_t>(classes);
     a.A = p;
+    if (p.Allowed == nullptr) {
+        a.A.AllowedCount = 0;
+    }
     const TCallDevice call(result, stream);
     WithType(valueType, [&](auto value) {
         using T = decltype(value);
         constexpr uint32_t N = 16 / sizeof(T);
         const size_t tables = size_t(history) + size_t(biases);
+        // a workgroup has one tile: a loop over tiles in the kernels kept their arguments in registers all along
+        const auto launchTiles = [&](auto kernel, size_t tiles, uint32_t threads, size_t lds) {
+            for (a.FirstTile = 0; a.FirstTile < tiles; a.FirstTile += kTilesPerLaunch) {
+                call.Launch(kernel, std::min(tiles - a.FirstTile, kTilesPerLaunch), threads, lds, a);
+            }
+        };
         const uint32_t pieces = (a.Classes + N - 1) / N;
         constexpr uint32_t tilePieces = kPiecesPerThread * 256;
         if (pieces <= tilePieces / 4) {
@@ -873,12 +913,12 @@ void AdjustScores(int valueType, size_t rows, size_t classes, const void* scores
             // floor(q / pieces) = floor(q m / 2^32) with m = floor(2^32 / pieces) + 1: q m / 2^32 is over q / pieces by q / 2^32 at most, and
             // q / pieces is under the next integer by 1 / pieces at least, which is more for the q and pieces under 2^11 here
             a.PiecesInverse = pieces > 1 ? static_cast<uint32_t>((uint64_t(1) << 32) / pieces + 1) : 0;
-            a.Tiles = (rows + a.RowsPerTile - 1) / a.RowsPerTile;
+            const size_t tiles = (rows + a.RowsPerTile - 1) / a.RowsPerTile;
             const size_t perRow = (history ? sizeof(TPenalties) + 16 : 0) + (biases ? 8 : 0) + size_t(pieces) * N * 4 * tables;
             const size_t lds = a.RowsPerTile * perRow;
             const auto launch = [&](auto kernel) {
                 call.AllowLds(reinterpret_cast<const void*>(kernel), lds);
-                call.Launch(kernel, std::min<size_t>(a.Tiles, 1u << 20), 256, lds, a);
+                launchTiles(kernel, tiles, 256, lds);
             };
             if (a.Classes % N == 0) {
                 launch(AdjustRowsKernel<T, true>);
@@ -891,16 +931,17 @@ void AdjustScores(int valueType, size_t rows, size_t classes, const void* scores
         const auto launch = [&](auto threads, auto perThread) {
             constexpr int THREADS = decltype(threads)::value, P = decltype(perThread)::value;
             a.Slices = slices(THREADS * P * N);
-            a.Tiles = rows * a.Slices;
-            const auto kernel = AdjustSliceKernel<T, THREADS, P>;
-            const size_t lds = size_t(THREADS) * P * N * 4 * tables;
-            call.AllowLds(reinterpret_cast<const void*>(kernel), lds);
-            call.Launch(kernel, std::min<size_t>(a.Tiles, 1u << 20), THREADS, lds, a);
+            a.SliceClasses = ((a.Classes + a.Slices - 1) / a.Slices + 31) / 32 * 32;  // masks begin with a word
+            a.Slices = slices(a.SliceClasses);
+            const size_t tiles = rows * a.Slices;
+            const size_t lds = a.SliceClasses * 4 * tables;
+            launchTiles(AdjustSliceKernel<T, THREADS, P>, tiles, THREADS, lds);
         };
         const auto atLeast = [&](uint32_t size) { return rows >= (kWorkgroupsWanted + slices(size) - 1) / slices(size); };
         using std::integral_constant;
-        if (atLeast(16384)) {
-            launch(integral_constant<int, 1024>(), integral_constant<int, 16 / N>());
+        // the tables of two workgroups fit a compute unit (and their registers: 64-bit scores of 16384 classes would not)
+        if (sizeof(T) < 8 && tables < 2 && atLeast(16384)) {
+            launch(integral_constant<int, 1024>(), integral_constant<int, sizeof(T) < 8 ? 16 / N : 1>());
         } else if (atLeast(8192)) {
             launch(integral_constant<int, 1024>(), integral_constant<int, 8 / N>());
         } else if (atLeast(4096)) {

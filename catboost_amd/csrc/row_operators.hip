@@ -204,12 +204,11 @@ struct TPieces {
     uint32_t PerRow;      // slots
     uint32_t Pieces;      // of a row
     uint64_t Inverse;     // floor(i / Pieces) = floor(i Inverse / 2^64) as long as i Pieces < 2^64, which memory sees to
-    size_t Blocks;        // of 256 pieces
 
     // of N values each
     template <int N>
-    __device__ __forceinline__ bool Of(size_t block, size_t* row, size_t* column) const {
-        const uint64_t i = block * 256 + threadIdx.x;
+    __device__ __forceinline__ bool Of(size_t* row, size_t* column) const {
+        const uint64_t i = uint64_t(blockIdx.x) * 256 + threadIdx.x;
         *row = Inverse != 0 ? __umul64hi(i, Inverse) : i;
         const size_t c = (i - *row * Pieces) * N;
         *column = N == 1 || c + N <= Width ? c : Width - N;
@@ -238,20 +237,18 @@ template <typename T, int N, int K>
 __global__ void __launch_bounds__(256) DispatchRowsKernel(const T* source, size_t sourceStride, TPieces p, const int32_t* places, T* sorted,
                                                           size_t sortedRows, size_t sortedStride) {
     using TPiece = std::conditional_t<N == 1, TValues<T, 1>, TValues<uint32_t, 4>>;
-    for (size_t block = blockIdx.x; block < p.Blocks; block += gridDim.x) {
-        size_t row, c;
-        if (!p.Of<N>(block, &row, &c)) {
-            return;
-        }
-        TPiece v;
-        __builtin_memcpy(&v, source + row * sourceStride + c, sizeof(v));
-        for (uint32_t k = 0; k < p.PerRow; k += K) {
-            const TPlaces<K> to(places + row * p.PerRow, k, p.PerRow, sortedRows);
+    size_t row, c;
+    if (!p.Of<N>(&row, &c)) {
+        return;
+    }
+    TPiece v;
+    __builtin_memcpy(&v, source + row * sourceStride + c, sizeof(v));
+    for (uint32_t k = 0; k < p.PerRow; k += K) {
+        const TPlaces<K> to(places + row * p.PerRow, k, p.PerRow, sortedRows);
 #pragma unroll
-            for (int j = 0; j < K; ++j) {
-                if (to.At[j] >= 0) {
-                    __builtin_memcpy(sorted + static_cast<size_t>(to.At[j]) * sortedStride + c, &v, sizeof(v));
-                }
+        for (int j = 0; j < K; ++j) {
+            if (to.At[j] >= 0) {
+                __builtin_memcpy(sorted + static_cast<size_t>(to.At[j]) * sortedStride + c, &v, sizeof(v));
             }
         }
     }
@@ -262,48 +259,46 @@ template <typename T, int N, int K>
 __global__ void __launch_bounds__(256) CombineRowsKernel(const T* sorted, size_t sortedRows, size_t sortedStride, TPieces p, const int32_t* places,
                                                          const TAcc<T>* weights, T* result, size_t resultStride) {
     using A = TAcc<T>;
-    for (size_t block = blockIdx.x; block < p.Blocks; block += gridDim.x) {
-        size_t row, c;
-        if (!p.Of<N>(block, &row, &c)) {
-            return;
-        }
-        A sum[N] = {};
-        for (uint32_t k = 0; k < p.PerRow; k += K) {
-            const TPlaces<K> from(places + row * p.PerRow, k, p.PerRow, sortedRows);
-            int32_t any = -1;
-#pragma unroll
-            for (int j = 0; j < K; ++j) {
-                any = any >= 0 ? any : from.At[j];
-            }
-            if (any < 0) {
-                continue;
-            }
-            A w[K];
-            TValues<T, N> v[K];
-#pragma unroll
-            for (int j = 0; j < K; ++j) {
-                w[j] = weights != nullptr && from.At[j] >= 0 ? weights[row * p.PerRow + k + j] : A(1);
-            }
-#pragma unroll
-            for (int j = 0; j < K; ++j) {
-                v[j] = TValues<T, N>::Load(sorted + static_cast<size_t>(from.At[j] >= 0 ? from.At[j] : any) * sortedStride + c);
-            }
-#pragma unroll
-            for (int j = 0; j < K; ++j) {
-#pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    const A term = w[j] * static_cast<A>(v[j].V[i]);
-                    sum[i] += from.At[j] >= 0 ? term : A(0);
-                }
-            }
-        }
-        TValues<T, N> out;
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            out.V[i] = static_cast<T>(sum[i]);
-        }
-        out.Store(result + row * resultStride + c);
+    size_t row, c;
+    if (!p.Of<N>(&row, &c)) {
+        return;
     }
+    A sum[N] = {};
+    for (uint32_t k = 0; k < p.PerRow; k += K) {
+        const TPlaces<K> from(places + row * p.PerRow, k, p.PerRow, sortedRows);
+        int32_t any = -1;
+#pragma unroll
+        for (int j = 0; j < K; ++j) {
+            any = any >= 0 ? any : from.At[j];
+        }
+        if (any < 0) {
+            continue;
+        }
+        A w[K];
+        TValues<T, N> v[K];
+#pragma unroll
+        for (int j = 0; j < K; ++j) {
+            w[j] = weights != nullptr && from.At[j] >= 0 ? weights[row * p.PerRow + k + j] : A(1);
+        }
+#pragma unroll
+        for (int j = 0; j < K; ++j) {
+            v[j] = TValues<T, N>::Load(sorted + static_cast<size_t>(from.At[j] >= 0 ? from.At[j] : any) * sortedStride + c);
+        }
+#pragma unroll
+        for (int j = 0; j < K; ++j) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const A term = w[j] * static_cast<A>(v[j].V[i]);
+                sum[i] += from.At[j] >= 0 ? term : A(0);
+            }
+        }
+    }
+    TValues<T, N> out;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        out.V[i] = static_cast<T>(sum[i]);
+    }
+    out.Store(result + row * resultStride + c);
 }
 
 // L threads for a row. A thread takes every L-th piece of the row's gradient and, for K slots at a time, what is at their
@@ -316,86 +311,84 @@ __global__ void __launch_bounds__(256) CombineRowsBackwardKernel(const T* gradie
     using A = TAcc<T>;
     __shared__ A waveSums[4][K];
     const uint32_t lane = threadIdx.x % L;
-    for (size_t first = size_t(blockIdx.x) * (256 / L); first < rows; first += size_t(gridDim.x) * (256 / L)) {
-        const size_t row = first + threadIdx.x / L;
-        const bool there = row < rows;  // (false for whole groups of L threads)
-        for (uint32_t k = 0; k < perRow; k += K) {
-            A product[K] = {};
-            if (there) {
-                const TPlaces<K> at(places + row * perRow, k, perRow, sortedRows);
-                int32_t any = -1;
-                A w[K];
-#pragma unroll
-                for (int j = 0; j < K; ++j) {
-                    any = any >= 0 ? any : at.At[j];
-                    w[j] = weights != nullptr && at.At[j] >= 0 ? weights[row * perRow + k + j] : A(1);
-                }
-                for (size_t begin = size_t(lane) * N; any >= 0 && begin < width; begin += L * N) {
-                    const size_t c = N == 1 || begin + N <= width ? begin : width - N;
-                    TValues<T, N> g = TValues<T, N>::Load(gradients + row * gradientStride + c);
-                    TValues<T, N> v[K];
-                    if (weightGradients != nullptr) {
-#pragma unroll
-                        for (int j = 0; j < K; ++j) {
-                            v[j] = TValues<T, N>::Load(sorted + static_cast<size_t>(at.At[j] >= 0 ? at.At[j] : any) * sortedStride + c);
-                        }
-                    }
-                    if (sortedGradients != nullptr) {
-#pragma unroll
-                        for (int j = 0; j < K; ++j) {
-                            if (at.At[j] >= 0) {
-                                TValues<T, N> out;
-#pragma unroll
-                                for (int i = 0; i < N; ++i) {
-                                    out.V[i] = static_cast<T>(w[j] * static_cast<A>(g.V[i]));
-                                }
-                                out.Store(sortedGradients + static_cast<size_t>(at.At[j]) * sortedGradientStride + c);
-                            }
-                        }
-                    }
-                    if (weightGradients != nullptr) {
-                        // (of a row's last piece, only what the piece before it does not have)
-#pragma unroll
-                        for (int i = 0; i < N; ++i) {
-                            const A gi = c + i >= begin ? static_cast<A>(g.V[i]) : A(0);
-#pragma unroll
-                            for (int j = 0; j < K; ++j) {
-                                const A term = gi * static_cast<A>(v[j].V[i]);
-                                product[j] += c + i >= begin && at.At[j] >= 0 ? term : A(0);
-                            }
-                        }
-                    }
-                }
-            }
-            if (weightGradients == nullptr) {
-                continue;
-            }
+    const size_t row = size_t(blockIdx.x) * (256 / L) + threadIdx.x / L;
+    const bool there = row < rows;  // (false for whole groups of L threads)
+    for (uint32_t k = 0; k < perRow; k += K) {
+        A product[K] = {};
+        if (there) {
+            const TPlaces<K> at(places + row * perRow, k, perRow, sortedRows);
+            int32_t any = -1;
+            A w[K];
 #pragma unroll
             for (int j = 0; j < K; ++j) {
-                for (int step = (L < 64 ? L : 64) / 2; step > 0; step /= 2) {
-                    product[j] += __shfl_xor(product[j], step);
-                }
+                any = any >= 0 ? any : at.At[j];
+                w[j] = weights != nullptr && at.At[j] >= 0 ? weights[row * perRow + k + j] : A(1);
             }
-            if constexpr (L > 64) {
-                __syncthreads();
-                if ((threadIdx.x & 63) == 0) {
+            for (size_t begin = size_t(lane) * N; any >= 0 && begin < width; begin += L * N) {
+                const size_t c = N == 1 || begin + N <= width ? begin : width - N;
+                TValues<T, N> g = TValues<T, N>::Load(gradients + row * gradientStride + c);
+                TValues<T, N> v[K];
+                if (weightGradients != nullptr) {
 #pragma unroll
                     for (int j = 0; j < K; ++j) {
-                        waveSums[threadIdx.x / 64][j] = product[j];
+                        v[j] = TValues<T, N>::Load(sorted + static_cast<size_t>(at.At[j] >= 0 ? at.At[j] : any) * sortedStride + c);
                     }
                 }
-                __syncthreads();
+                if (sortedGradients != nullptr) {
 #pragma unroll
-                for (int j = 0; j < K; ++j) {
-                    product[j] = (waveSums[0][j] + waveSums[1][j]) + (waveSums[2][j] + waveSums[3][j]);
+                    for (int j = 0; j < K; ++j) {
+                        if (at.At[j] >= 0) {
+                            TValues<T, N> out;
+#pragma unroll
+                            for (int i = 0; i < N; ++i) {
+                                out.V[i] = static_cast<T>(w[j] * static_cast<A>(g.V[i]));
+                            }
+                            out.Store(sortedGradients + static_cast<size_t>(at.At[j]) * sortedGradientStride + c);
+                        }
+                    }
+                }
+                if (weightGradients != nullptr) {
+                    // (of a row's last piece, only what the piece before it does not have)
+#pragma unroll
+                    for (int i = 0; i < N; ++i) {
+                        const A gi = c + i >= begin ? static_cast<A>(g.V[i]) : A(0);
+#pragma unroll
+                        for (int j = 0; j < K; ++j) {
+                            const A term = gi * static_cast<A>(v[j].V[i]);
+                            product[j] += c + i >= begin && at.At[j] >= 0 ? term : A(0);
+                        }
+                    }
                 }
             }
-            if (there && lane == 0) {
+        }
+        if (weightGradients == nullptr) {
+            continue;
+        }
+#pragma unroll
+        for (int j = 0; j < K; ++j) {
+            for (int step = (L < 64 ? L : 64) / 2; step > 0; step /= 2) {
+                product[j] += __shfl_xor(product[j], step);
+            }
+        }
+        if constexpr (L > 64) {
+            __syncthreads();
+            if ((threadIdx.x & 63) == 0) {
 #pragma unroll
                 for (int j = 0; j < K; ++j) {
-                    if (k + j < perRow) {
-                        weightGradients[row * perRow + k + j] = product[j];
-                    }
+                    waveSums[threadIdx.x / 64][j] = product[j];
+                }
+            }
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < K; ++j) {
+                product[j] = (waveSums[0][j] + waveSums[1][j]) + (waveSums[2][j] + waveSums[3][j]);
+            }
+        }
+        if (there && lane == 0) {
+#pragma unroll
+            for (int j = 0; j < K; ++j) {
+                if (k + j < perRow) {
+                    weightGradients[row * perRow + k + j] = product[j];
                 }
             }
         }
@@ -464,7 +457,7 @@ void SortByExpert(size_t slots, int32_t experts, const int32_t* ids, int32_t* pl
 namespace {
 
 constexpr int32_t kMaxPerRow = 64;
-constexpr size_t kMaxGroups = size_t(1) << 23;  // the workgroups go on from there
+constexpr size_t kMaxGroups = size_t(1) << 23;  // of 256 threads in a launch
 
 void CheckRoutes(size_t rows, size_t width, int32_t perRow, const int32_t* places, size_t sortedRows) {
     CBAMD_ENSURE(perRow >= 1 && perRow <= kMaxPerRow, "slots per row: " + std::to_string(perRow) + ", 1 to " + std::to_string(kMaxPerRow) + " are supported");
@@ -481,8 +474,18 @@ TPieces PiecesOf(size_t rows, size_t width, int32_t perRow, size_t valueSize) {
     p.PerRow = static_cast<uint32_t>(perRow);
     p.Pieces = static_cast<uint32_t>(width * valueSize < 16 ? width : (width * valueSize + 15) / 16);
     p.Inverse = p.Pieces > 1 ? ~uint64_t(0) / p.Pieces + 1 : 0;
-    p.Blocks = (rows * p.Pieces + 255) / 256;
     return p;
+}
+
+// f(first row, rows, workgroups) for rows that one launch takes (a workgroup has one part of them: a loop would keep the
+// arguments in registers all along)
+template <typename F>
+void ForLaunches(size_t rows, size_t threadsPerRow, F&& f) {
+    const size_t most = std::max<size_t>(1, kMaxGroups * 256 / threadsPerRow);
+    for (size_t first = 0; first < rows; first += most) {
+        const size_t n = std::min(rows - first, most);
+        f(first, n, (n * threadsPerRow + 255) / 256);
+    }
 }
 
 // f(values of a piece, slots that are taken at a time)
@@ -509,12 +512,14 @@ void DispatchRows(int valueType, size_t rows, size_t width, int32_t perRow, cons
     CheckMatrix("source", source, rows, width, sourceStride, size);
     CheckMatrix("sorted rows", sorted, sortedRows, width, sortedStride, size);
     const TCallDevice call(sorted, stream);
-    const TPieces pieces = PiecesOf(rows, width, perRow, size);
     const auto launch = [&](auto value) {
         using T = decltype(value);
         WithShape<T>(width, perRow, [&](auto values, auto slots) {
-            call.Launch(DispatchRowsKernel<T, decltype(values)::value, decltype(slots)::value>, std::min(pieces.Blocks, kMaxGroups), 256, 0, static_cast<const T*>(source),
-                        sourceStride, pieces, places, static_cast<T*>(sorted), sortedRows, sortedStride);
+            ForLaunches(rows, PiecesOf(rows, width, perRow, size).Pieces, [&](size_t first, size_t n, size_t groups) {
+                call.Launch(DispatchRowsKernel<T, decltype(values)::value, decltype(slots)::value>, groups, 256, 0,
+                            static_cast<const T*>(source) + first * sourceStride, sourceStride, PiecesOf(n, width, perRow, size),
+                            places + first * perRow, static_cast<T*>(sorted), sortedRows, sortedStride);
+            });
         });
     };
     // the values' bits are moved as they are
@@ -540,10 +545,13 @@ void CombineRows(int valueType, size_t rows, size_t width, int32_t perRow, const
     const TCallDevice call(result, stream);
     WithType(valueType, [&](auto value) {
         using T = decltype(value);
-        const TPieces pieces = PiecesOf(rows, width, perRow, size);
         WithShape<T>(width, perRow, [&](auto values, auto slots) {
-            call.Launch(CombineRowsKernel<T, decltype(values)::value, decltype(slots)::value>, std::min(pieces.Blocks, kMaxGroups), 256, 0, static_cast<const T*>(sorted),
-                        sortedRows, sortedStride, pieces, places, static_cast<const TAcc<T>*>(weights), static_cast<T*>(result), resultStride);
+            ForLaunches(rows, PiecesOf(rows, width, perRow, size).Pieces, [&](size_t first, size_t n, size_t groups) {
+                call.Launch(CombineRowsKernel<T, decltype(values)::value, decltype(slots)::value>, groups, 256, 0, static_cast<const T*>(sorted),
+                            sortedRows, sortedStride, PiecesOf(n, width, perRow, size), places + first * perRow,
+                            weights != nullptr ? static_cast<const TAcc<T>*>(weights) + first * perRow : nullptr,
+                            static_cast<T*>(result) + first * resultStride, resultStride);
+            });
         });
     });
 }
@@ -573,11 +581,13 @@ void CombineRowsBackward(int valueType, size_t rows, size_t width, int32_t perRo
         WithShape<T>(width, perRow, [&](auto values, auto slots) {
             constexpr int N = decltype(values)::value, K = decltype(slots)::value;
             const auto launch = [&](auto kernel, size_t threadsPerRow) {
-                const size_t rowsPerGroup = 256 / threadsPerRow;
-                call.Launch(kernel, std::min((rows + rowsPerGroup - 1) / rowsPerGroup, kMaxGroups), 256, 0, static_cast<const T*>(resultGradients),
-                            gradientStride, static_cast<const T*>(sorted), sortedRows, sortedStride, rows, width, static_cast<uint32_t>(perRow),
-                            places, static_cast<const TAcc<T>*>(weights), static_cast<T*>(sortedGradients), sortedGradientStride,
-                            static_cast<TAcc<T>*>(weightGradients));
+                ForLaunches(rows, threadsPerRow, [&](size_t first, size_t n, size_t groups) {
+                    call.Launch(kernel, groups, 256, 0, static_cast<const T*>(resultGradients) + first * gradientStride, gradientStride,
+                                static_cast<const T*>(sorted), sortedRows, sortedStride, n, width, static_cast<uint32_t>(perRow),
+                                places + first * perRow, weights != nullptr ? static_cast<const TAcc<T>*>(weights) + first * perRow : nullptr,
+                                static_cast<T*>(sortedGradients), sortedGradientStride,
+                                weightGradients != nullptr ? static_cast<TAcc<T>*>(weightGradients) + first * perRow : nullptr);
+                });
             };
             // two pieces for a thread at most as long as eight threads are enough, else one to four for a wave's
             if (pieces <= 16) {

@@ -549,63 +549,65 @@ __global__ void __launch_bounds__(256) SelectTopKernel(TTopArgs<T> a, int32_t* i
     using R = TRanked<T>;
     constexpr int kept = 32 / G > 0 ? 32 / G : 1;
     const uint32_t lane = threadIdx.x & (G - 1);
-    for (size_t row = size_t(blockIdx.x) * (256 / G) + threadIdx.x / G; row < a.Rows; row += size_t(gridDim.x) * (256 / G)) {
-        const uint32_t c = lane * V;
-        TValues<T, V> v{};
-        if (c < a.Classes) {
-            v = LoadUpTo<T, V>(a.Scores + row * a.Stride + c, a.Classes - c);
+    const size_t row = size_t(blockIdx.x) * (256 / G) + threadIdx.x / G;
+    if (row >= a.Rows) {
+        return;
+    }
+    const uint32_t c = lane * V;
+    TValues<T, V> v{};
+    if (c < a.Classes) {
+        v = LoadUpTo<T, V>(a.Scores + row * a.Stride + c, a.Classes - c);
+    }
+    R left[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        left[j] = c + j < a.Classes ? R::Of(v.V[j], c + j) : R::None();
+    }
+    R mine[kept];
+#pragma unroll
+    for (int i = 0; i < kept; ++i) {
+        mine[i] = R::None();
+    }
+    A most = 0, total = 0;
+    for (uint32_t k = 0; k < a.Count; ++k) {
+        R best = left[0];
+#pragma unroll
+        for (int j = 1; j < V; ++j) {
+            best = best.BetterLater(left[j]);
         }
-        R left[V];
+        best = OverGroup<G>(best, [](const R& x, const R& y) { return x.Better(y); });
+        if (k == 0) {
+            most = best.Score();
+            if (!a.Among) {
+                // (what is never selected has a weight of 0; where nothing else is there the sum is not used)
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            left[j] = c + j < a.Classes ? R::Of(v.V[j], c + j) : R::None();
-        }
-        R mine[kept];
-#pragma unroll
-        for (int i = 0; i < kept; ++i) {
-            mine[i] = R::None();
-        }
-        A most = 0, total = 0;
-        for (uint32_t k = 0; k < a.Count; ++k) {
-            R best = left[0];
-#pragma unroll
-            for (int j = 1; j < V; ++j) {
-                best = best.BetterLater(left[j]);
-            }
-            best = OverGroup<G>(best, [](const R& x, const R& y) { return x.Better(y); });
-            if (k == 0) {
-                most = best.Score();
-                if (!a.Among) {
-                    // (what is never selected has a weight of 0; where nothing else is there the sum is not used)
-#pragma unroll
-                    for (int j = 0; j < V; ++j) {
-                        total += WeightOf(left[j].Score(), most);
-                    }
+                for (int j = 0; j < V; ++j) {
+                    total += WeightOf(left[j].Score(), most);
                 }
             }
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                left[j] = left[j].Without(best);
-            }
-#pragma unroll
-            for (int i = 0; i < kept; ++i) {
-                mine[i] = mine[i].Or(best, k == lane + i * G);
-            }
         }
-        A e[kept];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            left[j] = left[j].Without(best);
+        }
 #pragma unroll
         for (int i = 0; i < kept; ++i) {
-            e[i] = mine[i].IsNone() ? A(0) : WeightOf(mine[i].Score(), most);
-            total += a.Among ? e[i] : A(0);
+            mine[i] = mine[i].Or(best, k == lane + i * G);
         }
-        total = GroupSum<G>(total);
+    }
+    A e[kept];
 #pragma unroll
-        for (int i = 0; i < kept; ++i) {
-            const uint32_t k = lane + i * G;
-            if (k < a.Count) {
-                indexes[row * a.Count + k] = mine[i].IsNone() ? -1 : static_cast<int32_t>(mine[i].Class());
-                weights[row * a.Count + k] = mine[i].IsNone() ? A(0) : e[i] / total;
-            }
+    for (int i = 0; i < kept; ++i) {
+        e[i] = mine[i].IsNone() ? A(0) : WeightOf(mine[i].Score(), most);
+        total += a.Among ? e[i] : A(0);
+    }
+    total = GroupSum<G>(total);
+#pragma unroll
+    for (int i = 0; i < kept; ++i) {
+        const uint32_t k = lane + i * G;
+        if (k < a.Count) {
+            indexes[row * a.Count + k] = mine[i].IsNone() ? -1 : static_cast<int32_t>(mine[i].Class());
+            weights[row * a.Count + k] = mine[i].IsNone() ? A(0) : e[i] / total;
         }
     }
 }
@@ -637,59 +639,57 @@ __global__ void __launch_bounds__(256) SelectTopOfFewKernel(TTopArgs<T> a, int32
     extern __shared__ uint4 tables[];
     A* outWeights = reinterpret_cast<A*>(tables);
     int32_t* outIndexes = reinterpret_cast<int32_t*>(outWeights + 256 * a.Count);
-    for (size_t r0 = size_t(blockIdx.x) * 256; r0 < a.Rows; r0 += size_t(gridDim.x) * 256) {
-        const uint32_t rows = static_cast<uint32_t>(a.Rows - r0 < 256 ? a.Rows - r0 : 256);
-        if (threadIdx.x < rows) {
-            const TValues<T, C> v = LoadRow<T, C>(a.Scores + (r0 + threadIdx.x) * a.Stride, a.Classes);
-            R left[C];
+    const size_t r0 = size_t(blockIdx.x) * 256;
+    const uint32_t rows = static_cast<uint32_t>(a.Rows - r0 < 256 ? a.Rows - r0 : 256);
+    if (threadIdx.x < rows) {
+        const TValues<T, C> v = LoadRow<T, C>(a.Scores + (r0 + threadIdx.x) * a.Stride, a.Classes);
+        R left[C];
 #pragma unroll
-            for (int j = 0; j < C; ++j) {
-                left[j] = static_cast<uint32_t>(j) < a.Classes ? R::Of(v.V[j], j) : R::None();
-            }
-            A* myWeights = outWeights + threadIdx.x * a.Count;
-            int32_t* myIndexes = outIndexes + threadIdx.x * a.Count;
-            A most = 0, total = 0;
-            for (uint32_t k = 0; k < a.Count; ++k) {
-                R best = left[0];
+        for (int j = 0; j < C; ++j) {
+            left[j] = static_cast<uint32_t>(j) < a.Classes ? R::Of(v.V[j], j) : R::None();
+        }
+        A* myWeights = outWeights + threadIdx.x * a.Count;
+        int32_t* myIndexes = outIndexes + threadIdx.x * a.Count;
+        A most = 0, total = 0;
+        for (uint32_t k = 0; k < a.Count; ++k) {
+            R best = left[0];
 #pragma unroll
-                for (int j = 1; j < C; ++j) {
-                    if (static_cast<uint32_t>(j) < a.Classes) {
-                        best = best.BetterLater(left[j]);
-                    }
+            for (int j = 1; j < C; ++j) {
+                if (static_cast<uint32_t>(j) < a.Classes) {
+                    best = best.BetterLater(left[j]);
                 }
-                if (k == 0) {
-                    most = best.Score();
-                    if (!a.Among) {
-                        // (what is never selected has a weight of 0; where nothing else is there the sum is not used)
+            }
+            if (k == 0) {
+                most = best.Score();
+                if (!a.Among) {
+                    // (what is never selected has a weight of 0; where nothing else is there the sum is not used)
 #pragma unroll
-                        for (int j = 0; j < C; ++j) {
-                            if (static_cast<uint32_t>(j) < a.Classes) {
-                                total += WeightOf(left[j].Score(), most);
-                            }
+                    for (int j = 0; j < C; ++j) {
+                        if (static_cast<uint32_t>(j) < a.Classes) {
+                            total += WeightOf(left[j].Score(), most);
                         }
                     }
                 }
+            }
 #pragma unroll
-                for (int j = 0; j < C; ++j) {
-                    if (static_cast<uint32_t>(j) < a.Classes) {
-                        left[j] = left[j].Without(best);
-                    }
+            for (int j = 0; j < C; ++j) {
+                if (static_cast<uint32_t>(j) < a.Classes) {
+                    left[j] = left[j].Without(best);
                 }
-                const A e = best.IsNone() ? A(0) : WeightOf(best.Score(), most);
-                myIndexes[k] = best.IsNone() ? -1 : static_cast<int32_t>(best.Class());
-                myWeights[k] = e;
-                total += a.Among ? e : A(0);
             }
-            for (uint32_t k = 0; k < a.Count; ++k) {
-                myWeights[k] = myIndexes[k] < 0 ? A(0) : myWeights[k] / total;
-            }
+            const A e = best.IsNone() ? A(0) : WeightOf(best.Score(), most);
+            myIndexes[k] = best.IsNone() ? -1 : static_cast<int32_t>(best.Class());
+            myWeights[k] = e;
+            total += a.Among ? e : A(0);
         }
-        __syncthreads();
-        for (uint32_t i = threadIdx.x; i < rows * a.Count; i += 256) {
-            indexes[r0 * a.Count + i] = outIndexes[i];
-            weights[r0 * a.Count + i] = outWeights[i];
+        for (uint32_t k = 0; k < a.Count; ++k) {
+            myWeights[k] = myIndexes[k] < 0 ? A(0) : myWeights[k] / total;
         }
-        __syncthreads();
+    }
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < rows * a.Count; i += 256) {
+        indexes[r0 * a.Count + i] = outIndexes[i];
+        weights[r0 * a.Count + i] = outWeights[i];
     }
 }
 
@@ -712,71 +712,72 @@ __global__ void __launch_bounds__(256) SelectTopBackwardKernel(TTopArgs<T> a, TT
     __shared__ __align__(16) A sums[256 * V];
     const uint32_t lane = threadIdx.x & (G - 1);
     A* mySums = sums + threadIdx.x / G * (G * V);
-    for (size_t row = size_t(blockIdx.x) * (256 / G) + threadIdx.x / G; row < a.Rows; row += size_t(gridDim.x) * (256 / G)) {
-        const uint32_t c = lane * V;
-        int32_t index[kept];
-        A part[kept], mean = 0;
+    const size_t row = size_t(blockIdx.x) * (256 / G) + threadIdx.x / G;
+    if (row >= a.Rows) {
+        return;
+    }
+    const uint32_t c = lane * V;
+    int32_t index[kept];
+    A part[kept], mean = 0;
+#pragma unroll
+    for (int i = 0; i < kept; ++i) {
+        const uint32_t k = lane + i * G;
+        index[i] = k < a.Count ? b.Indexes[row * a.Count + k] : -1;
+        const A w = index[i] >= 0 ? b.Weights[row * a.Count + k] : A(0);
+        const A g = index[i] >= 0 ? b.WeightGradients[row * a.Count + k] : A(0);
+        part[i] = a.Among ? g : w * g;
+        mean += w * g;
+    }
+    mean = GroupSum<G>(mean);
+    if (a.Among) {
 #pragma unroll
         for (int i = 0; i < kept; ++i) {
-            const uint32_t k = lane + i * G;
-            index[i] = k < a.Count ? b.Indexes[row * a.Count + k] : -1;
-            const A w = index[i] >= 0 ? b.Weights[row * a.Count + k] : A(0);
-            const A g = index[i] >= 0 ? b.WeightGradients[row * a.Count + k] : A(0);
-            part[i] = a.Among ? g : w * g;
-            mean += w * g;
+            part[i] = index[i] >= 0 ? b.Weights[row * a.Count + lane + i * G] * (part[i] - mean) : A(0);
         }
-        mean = GroupSum<G>(mean);
-        if (a.Among) {
-#pragma unroll
-            for (int i = 0; i < kept; ++i) {
-                part[i] = index[i] >= 0 ? b.Weights[row * a.Count + lane + i * G] * (part[i] - mean) : A(0);
-            }
-        }
-        TValues<A, V> x{};
-        if (!a.Among) {
-            TValues<T, V> v{};
-            if (c < a.Classes) {
-                v = LoadUpTo<T, V>(a.Scores + row * a.Stride + c, a.Classes - c);
-            }
-            A most = -std::numeric_limits<A>::infinity();
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const A s = static_cast<A>(v.V[j]);
-                x.V[j] = c + j < a.Classes && s == s ? s : -std::numeric_limits<A>::infinity();
-                most = x.V[j] > most ? x.V[j] : most;
-            }
-            most = OverGroup<G>(most, [](A y, A z) { return z > y ? z : y; });
-            A total = 0;
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                x.V[j] = x.V[j] > -std::numeric_limits<A>::infinity() ? WeightOf(x.V[j], most) : A(0);
-                total += x.V[j];
-            }
-            total = GroupSum<G>(total);
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                x.V[j] = total > 0 ? -(x.V[j] / total) * mean : A(0);
-            }
-        }
-        x.Store(mySums + c);
-        __builtin_amdgcn_wave_barrier();  // a row's lanes are of one wave, whose LDS operations are done in order
-#pragma unroll
-        for (int i = 0; i < kept; ++i) {
-            if (static_cast<uint32_t>(index[i]) < a.Classes) {
-                mySums[index[i]] += part[i];
-            }
-        }
-        __builtin_amdgcn_wave_barrier();
-        x = TValues<A, V>::Load(mySums + c);
-        __builtin_amdgcn_wave_barrier();
+    }
+    TValues<A, V> x{};
+    if (!a.Among) {
+        TValues<T, V> v{};
         if (c < a.Classes) {
-            TValues<T, V> v;
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                v.V[j] = static_cast<T>(x.V[j]);
-            }
-            StoreUpTo<T, V>(v, b.Gradients + row * b.GradientStride + c, a.Classes - c);
+            v = LoadUpTo<T, V>(a.Scores + row * a.Stride + c, a.Classes - c);
         }
+        A most = -std::numeric_limits<A>::infinity();
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const A s = static_cast<A>(v.V[j]);
+            x.V[j] = c + j < a.Classes && s == s ? s : -std::numeric_limits<A>::infinity();
+            most = x.V[j] > most ? x.V[j] : most;
+        }
+        most = OverGroup<G>(most, [](A y, A z) { return z > y ? z : y; });
+        A total = 0;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            x.V[j] = x.V[j] > -std::numeric_limits<A>::infinity() ? WeightOf(x.V[j], most) : A(0);
+            total += x.V[j];
+        }
+        total = GroupSum<G>(total);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            x.V[j] = total > 0 ? -(x.V[j] / total) * mean : A(0);
+        }
+    }
+    x.Store(mySums + c);
+    __builtin_amdgcn_wave_barrier();  // a row's lanes are of one wave, whose LDS operations are done in order
+#pragma unroll
+    for (int i = 0; i < kept; ++i) {
+        if (static_cast<uint32_t>(index[i]) < a.Classes) {
+            mySums[index[i]] += part[i];
+        }
+    }
+    __builtin_amdgcn_wave_barrier();
+    x = TValues<A, V>::Load(mySums + c);
+    if (c < a.Classes) {
+        TValues<T, V> v;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            v.V[j] = static_cast<T>(x.V[j]);
+        }
+        StoreUpTo<T, V>(v, b.Gradients + row * b.GradientStride + c, a.Classes - c);
     }
 }
 
@@ -784,68 +785,66 @@ template <typename T, int C>
 __global__ void __launch_bounds__(256) SelectTopOfFewBackwardKernel(TTopArgs<T> a, TTopGradientArgs<T> b) {
     using A = TAcc<T>;
     __shared__ T out[256 * C];
-    for (size_t r0 = size_t(blockIdx.x) * 256; r0 < a.Rows; r0 += size_t(gridDim.x) * 256) {
-        const uint32_t rows = static_cast<uint32_t>(a.Rows - r0 < 256 ? a.Rows - r0 : 256);
-        if (threadIdx.x < rows) {
-            const size_t row = r0 + threadIdx.x;
-            const int32_t* indexes = b.Indexes + row * a.Count;
-            const A* weights = b.Weights + row * a.Count;
-            const A* gradients = b.WeightGradients + row * a.Count;
-            A mean = 0;
-            for (uint32_t k = 0; k < a.Count; ++k) {
-                mean += indexes[k] >= 0 ? weights[k] * gradients[k] : A(0);
-            }
-            A x[C];
+    const size_t r0 = size_t(blockIdx.x) * 256;
+    const uint32_t rows = static_cast<uint32_t>(a.Rows - r0 < 256 ? a.Rows - r0 : 256);
+    if (threadIdx.x < rows) {
+        const size_t row = r0 + threadIdx.x;
+        const int32_t* indexes = b.Indexes + row * a.Count;
+        const A* weights = b.Weights + row * a.Count;
+        const A* gradients = b.WeightGradients + row * a.Count;
+        A mean = 0;
+        for (uint32_t k = 0; k < a.Count; ++k) {
+            mean += indexes[k] >= 0 ? weights[k] * gradients[k] : A(0);
+        }
+        A x[C];
+#pragma unroll
+        for (int j = 0; j < C; ++j) {
+            x[j] = 0;
+        }
+        if (!a.Among) {
+            const TValues<T, C> v = LoadRow<T, C>(a.Scores + row * a.Stride, a.Classes);
+            A most = -std::numeric_limits<A>::infinity(), total = 0;
 #pragma unroll
             for (int j = 0; j < C; ++j) {
-                x[j] = 0;
+                const A s = static_cast<A>(v.V[j]);
+                x[j] = static_cast<uint32_t>(j) < a.Classes && s == s ? s : -std::numeric_limits<A>::infinity();
+                most = x[j] > most ? x[j] : most;
             }
-            if (!a.Among) {
-                const TValues<T, C> v = LoadRow<T, C>(a.Scores + row * a.Stride, a.Classes);
-                A most = -std::numeric_limits<A>::infinity(), total = 0;
 #pragma unroll
-                for (int j = 0; j < C; ++j) {
-                    const A s = static_cast<A>(v.V[j]);
-                    x[j] = static_cast<uint32_t>(j) < a.Classes && s == s ? s : -std::numeric_limits<A>::infinity();
-                    most = x[j] > most ? x[j] : most;
-                }
-#pragma unroll
-                for (int j = 0; j < C; ++j) {
-                    if (static_cast<uint32_t>(j) < a.Classes) {
-                        x[j] = x[j] > -std::numeric_limits<A>::infinity() ? WeightOf(x[j], most) : A(0);
-                        total += x[j];
-                    }
-                }
-#pragma unroll
-                for (int j = 0; j < C; ++j) {
-                    if (static_cast<uint32_t>(j) < a.Classes) {
-                        x[j] = total > 0 ? -(x[j] / total) * mean : A(0);
-                    }
-                }
-            }
-            for (uint32_t k = 0; k < a.Count; ++k) {
-                const int32_t index = indexes[k];
-                if (index >= 0) {
-                    const A part = a.Among ? weights[k] * (gradients[k] - mean) : weights[k] * gradients[k];
-#pragma unroll
-                    for (int j = 0; j < C; ++j) {
-                        x[j] += index == j ? part : A(0);
-                    }
+            for (int j = 0; j < C; ++j) {
+                if (static_cast<uint32_t>(j) < a.Classes) {
+                    x[j] = x[j] > -std::numeric_limits<A>::infinity() ? WeightOf(x[j], most) : A(0);
+                    total += x[j];
                 }
             }
 #pragma unroll
             for (int j = 0; j < C; ++j) {
                 if (static_cast<uint32_t>(j) < a.Classes) {
-                    out[threadIdx.x * a.Classes + j] = static_cast<T>(x[j]);
+                    x[j] = total > 0 ? -(x[j] / total) * mean : A(0);
                 }
             }
         }
-        __syncthreads();
-        for (uint32_t i = threadIdx.x; i < rows * a.Classes; i += 256) {
-            const uint32_t r = i / a.Classes;
-            b.Gradients[(r0 + r) * b.GradientStride + (i - r * a.Classes)] = out[i];
+        for (uint32_t k = 0; k < a.Count; ++k) {
+            const int32_t index = indexes[k];
+            if (index >= 0) {
+                const A part = a.Among ? weights[k] * (gradients[k] - mean) : weights[k] * gradients[k];
+#pragma unroll
+                for (int j = 0; j < C; ++j) {
+                    x[j] += index == j ? part : A(0);
+                }
+            }
         }
-        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < C; ++j) {
+            if (static_cast<uint32_t>(j) < a.Classes) {
+                out[threadIdx.x * a.Classes + j] = static_cast<T>(x[j]);
+            }
+        }
+    }
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < rows * a.Classes; i += 256) {
+        const uint32_t r = i / a.Classes;
+        b.Gradients[(r0 + r) * b.GradientStride + (i - r * a.Classes)] = out[i];
     }
 }
 
@@ -985,9 +984,18 @@ void WithShape(size_t classes, size_t rows, int32_t count, F&& f) {
         : shape(wave, integral_constant<int, 16>());
 }
 
+// f(first row, rows) for rows that one launch takes (a workgroup has one tile of them)
+template <typename F>
+void ForLaunches(size_t rows, F&& f) {
+    constexpr size_t most = size_t(1) << 24;
+    for (size_t first = 0; first < rows; first += most) {
+        f(first, std::min(rows - first, most));
+    }
+}
+
 size_t GroupsOf(size_t rows, int lanes) {
     const size_t rowsPerGroup = 256 / lanes;
-    return std::min<size_t>((rows + rowsPerGroup - 1) / rowsPerGroup, 1u << 20);
+    return (rows + rowsPerGroup - 1) / rowsPerGroup;
 }
 
 }  // namespace
@@ -1004,15 +1012,19 @@ void SelectTop(int valueType, size_t rows, size_t classes, const void* scores, s
     const TCallDevice call(indexes, stream);
     WithType(valueType, [&](auto value) {
         using T = decltype(value);
-        const TTopArgs<T> a{static_cast<const T*>(scores), scoreStride, rows, static_cast<uint32_t>(classes), static_cast<uint32_t>(count), amongSelected};
         WithShape(classes, rows, count, [&](auto lanes, auto perLane) {
             constexpr int G = decltype(lanes)::value, V = decltype(perLane)::value;
-            if constexpr (G == 1) {
-                call.Launch(SelectTopOfFewKernel<T, V>, GroupsOf(rows, G), 256, size_t(256) * count * (sizeof(TAcc<T>) + 4), a, indexes,
-                            static_cast<TAcc<T>*>(weights));
-            } else {
-                call.Launch(SelectTopKernel<T, G, V>, GroupsOf(rows, G), 256, 0, a, indexes, static_cast<TAcc<T>*>(weights));
-            }
+            ForLaunches(rows, [&](size_t first, size_t n) {
+                const TTopArgs<T> a{static_cast<const T*>(scores) + first * scoreStride, scoreStride, n, static_cast<uint32_t>(classes),
+                                    static_cast<uint32_t>(count), amongSelected};
+                int32_t* theIndexes = indexes + first * count;
+                TAcc<T>* theWeights = static_cast<TAcc<T>*>(weights) + first * count;
+                if constexpr (G == 1) {
+                    call.Launch(SelectTopOfFewKernel<T, V>, GroupsOf(n, G), 256, size_t(256) * count * (sizeof(TAcc<T>) + 4), a, theIndexes, theWeights);
+                } else {
+                    call.Launch(SelectTopKernel<T, G, V>, GroupsOf(n, G), 256, 0, a, theIndexes, theWeights);
+                }
+            });
         });
     });
 }
@@ -1033,16 +1045,20 @@ void SelectTopBackward(int valueType, size_t rows, size_t classes, const void* s
     const TCallDevice call(scoreGradients, stream);
     WithType(valueType, [&](auto value) {
         using T = decltype(value);
-        const TTopArgs<T> a{static_cast<const T*>(scores), scoreStride, rows, static_cast<uint32_t>(classes), static_cast<uint32_t>(count), amongSelected};
-        const TTopGradientArgs<T> b{indexes, static_cast<const TAcc<T>*>(weights), static_cast<const TAcc<T>*>(weightGradients),
-                                    static_cast<T*>(scoreGradients), gradientStride};
         WithShape(classes, rows, count, [&](auto lanes, auto perLane) {
             constexpr int G = decltype(lanes)::value, V = decltype(perLane)::value;
-            if constexpr (G == 1) {
-                call.Launch(SelectTopOfFewBackwardKernel<T, V>, GroupsOf(rows, G), 256, 0, a, b);
-            } else {
-                call.Launch(SelectTopBackwardKernel<T, G, V>, GroupsOf(rows, G), 256, 0, a, b);
-            }
+            ForLaunches(rows, [&](size_t first, size_t n) {
+                const TTopArgs<T> a{static_cast<const T*>(scores) + (amongSelected ? 0 : first * scoreStride), scoreStride, n,
+                                    static_cast<uint32_t>(classes), static_cast<uint32_t>(count), amongSelected};
+                const TTopGradientArgs<T> b{indexes + first * count, static_cast<const TAcc<T>*>(weights) + first * count,
+                                            static_cast<const TAcc<T>*>(weightGradients) + first * count,
+                                            static_cast<T*>(scoreGradients) + first * gradientStride, gradientStride};
+                if constexpr (G == 1) {
+                    call.Launch(SelectTopOfFewBackwardKernel<T, V>, GroupsOf(n, G), 256, 0, a, b);
+                } else {
+                    call.Launch(SelectTopBackwardKernel<T, G, V>, GroupsOf(n, G), 256, 0, a, b);
+                }
+            });
         });
     });
 }

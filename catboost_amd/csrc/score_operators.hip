@@ -67,7 +67,7 @@ struct TPiece {
     static constexpr int N = 16 / sizeof(T);
     A X[N];
 
-    __device__ __forceinline__ explicit TPiece(const TRaw& raw) {
+    __device__ __forceinline__ void From(const TRaw& raw) {
         TValues<T, N> v;
         __builtin_memcpy(&v, &raw, 16);
 #pragma unroll
@@ -141,8 +141,8 @@ __device__ __forceinline__ void StorePiece(const TRaw& raw, T* at, uint32_t n) {
 
 // A workgroup for a slice of one row, at most THREADS * P pieces. What it reads is requested at once, as far as its place is
 // known, and without branches, which would wait for one load after the other: the scores, the mask's words, the first
-// entries of the history; the tables are made while they are on their way. The scores wait as they came (as 32-bit values
-// they would leave one workgroup for a compute unit instead of two). Every slice of a row looks through the row's whole
+// entries of the lists; the tables are made while they are on their way. The tables of the history and of the biases take
+// turns in the same LDS, so that two workgroups fit a compute unit. Every slice of a row looks through the row's whole
 // history; slices of a row are alike in length.
 template <typename T, int THREADS, int P>
 __global__ void __launch_bounds__(THREADS) AdjustSliceKernel(TAdjustArgs a) {
@@ -151,7 +151,12 @@ __global__ void __launch_bounds__(THREADS) AdjustSliceKernel(TAdjustArgs a) {
     const CbHipScoreAdjustment& p = a.A;
     const bool history = p.HistoryOffsets != nullptr, biases = p.BiasOffsets != nullptr;
     uint32_t* words = reinterpret_cast<uint32_t*>(tables);
-    uint32_t* last = words + (history ? a.SliceClasses : 0);
+    const auto clear = [&] {
+        for (uint32_t i = threadIdx.x; i < a.SliceClasses / 4; i += THREADS) {
+            tables[i] = uint4{0, 0, 0, 0};
+        }
+        __syncthreads();
+    };
     const size_t tile = a.FirstTile + blockIdx.x;
     const size_t row = tile / a.Slices;
     const uint32_t c0 = static_cast<uint32_t>(tile - row * a.Slices) * a.SliceClasses;
@@ -196,16 +201,17 @@ __global__ void __launch_bounds__(THREADS) AdjustSliceKernel(TAdjustArgs a) {
             allowed[j] = bits[(c0 + min((j * THREADS + threadIdx.x) * N, width - 1)) >> 5];
         }
     }
-    if (history || biases) {
+    int32_t biasClass = 0;
+    if (firstBias + threadIdx.x < endBias) {
+        biasClass = p.BiasClasses[firstBias + threadIdx.x];
+    }
+    if (history) {
         int64_t e = begin + threadIdx.x * 4;
         TValues<int32_t, 4> entries{};
         if (e < end) {
             entries = LoadEntries(p.History, e, p.HistoryCount);
         }
-        for (uint32_t i = threadIdx.x; i < a.SliceClasses / 4 * (history + biases); i += THREADS) {
-            tables[i] = uint4{0, 0, 0, 0};
-        }
-        __syncthreads();
+        clear();
         while (e < end) {
             const int64_t next = e + THREADS * 4;
             TValues<int32_t, 4> more{};
@@ -222,10 +228,35 @@ __global__ void __launch_bounds__(THREADS) AdjustSliceKernel(TAdjustArgs a) {
             entries = more;
             e = next;
         }
+        __syncthreads();
+    }
+    TPiece<T> x[P];
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+        const uint32_t c = (j * THREADS + threadIdx.x) * N;
+        x[j].From(raw[j]);
+        if (c < width) {
+            if (history) {
+                x[j].Penalize(words + c, penalties);
+            }
+            if (p.ClassBias != nullptr) {
+                const float* bias = p.ClassBias + row * p.ClassBiasStride + c0 + c;
+                x[j].Add(whole ? TValues<float, N>::Load(bias) : LoadUpTo<float, N>(bias, width - c));
+            }
+        }
+    }
+    if (biases) {
+        if (history) {
+            __syncthreads();  // the history's words are read
+        }
+        clear();
         for (int64_t b = firstBias + threadIdx.x; b < endBias; b += THREADS) {
-            const uint32_t c = static_cast<uint32_t>(p.BiasClasses[b]) - c0;
+            const uint32_t c = static_cast<uint32_t>(biasClass) - c0;
             if (c < width) {
-                atomicMax(&last[c], static_cast<uint32_t>(b - firstBias) + 1);
+                atomicMax(&words[c], static_cast<uint32_t>(b - firstBias) + 1);
+            }
+            if (b + THREADS < endBias) {
+                biasClass = p.BiasClasses[b + THREADS];
             }
         }
         __syncthreads();
@@ -235,18 +266,10 @@ __global__ void __launch_bounds__(THREADS) AdjustSliceKernel(TAdjustArgs a) {
     for (int j = 0; j < P; ++j) {
         const uint32_t c = (j * THREADS + threadIdx.x) * N;
         if (c < width) {
-            TPiece<T> x(raw[j]);
-            if (history) {
-                x.Penalize(words + c, penalties);
-            }
-            if (p.ClassBias != nullptr) {
-                const float* bias = p.ClassBias + row * p.ClassBiasStride + c0 + c;
-                x.Add(whole ? TValues<float, N>::Load(bias) : LoadUpTo<float, N>(bias, width - c));
-            }
             if (biases) {
-                x.AddLast(last + c, p.BiasValues + firstBias);
+                x[j].AddLast(words + c, p.BiasValues + firstBias);
             }
-            const TRaw out = x.Rounded(mask >= 0 ? allowed[j] >> (c & 31) : ~0u);
+            const TRaw out = x[j].Rounded(mask >= 0 ? allowed[j] >> (c & 31) : ~0u);
             if (whole) {
                 out.Store(reinterpret_cast<uint32_t*>(to + c));
             } else {
@@ -394,7 +417,8 @@ __global__ void __launch_bounds__(256) AdjustRowsKernel(TAdjustArgs a) {
     for (int j = 0; j < P; ++j) {
         const uint32_t q = j * 256 + threadIdx.x, r = rowOf(q), c = (q - r * a.Pieces) * N;
         if (r < rows) {
-            TPiece<T> x(raw[j]);
+            TPiece<T> x;
+            x.From(raw[j]);
             if (history) {
                 x.Penalize(words + q * N, penalties[r]);
             }
@@ -422,38 +446,115 @@ __global__ void __launch_bounds__(256) AdjustRowsKernel(TAdjustArgs a) {
 // A score with its class as one value that orders them: larger scores first, of equal ones the lower class first. What is
 // never selected (minus infinity, NaN) comes behind all others. 16-bit scores and their class fit 32 bits, 32-bit ones 64.
 template <typename T>
-struct TRanked {
-    using Bits = std::conditional_t<sizeof(T) == 2, uint16_t, uint32_t>;
-    using Key = std::conditional_t<sizeof(T) == 2, uint32_t, uint64_t>;
-    static constexpr int kBits = 8 * sizeof(T);
-    Key K;
+struct TRanked;
+
+template <>
+struct TRanked<float> {
+    uint64_t K;
 
     __device__ __forceinline__ static TRanked None() { return {0}; }
-    __device__ __forceinline__ static TRanked Of(T score, uint32_t c) {
-        const float x = static_cast<float>(score);
-        if (!(x > -std::numeric_limits<float>::infinity())) {
-            return None();
-        }
-        Bits bits = __builtin_bit_cast(Bits, score);
-        bits = x == 0 ? Bits(0) : bits;  // zeros of both signs are equal
-        const Bits sign = Bits(1) << (kBits - 1);
-        bits = (bits & sign) != 0 ? static_cast<Bits>(~bits) : static_cast<Bits>(bits | sign);
-        return {static_cast<Key>(bits) << kBits | static_cast<Bits>(~c)};
+    __device__ __forceinline__ static TRanked Of(float x, uint32_t c) {
+        uint32_t bits = __float_as_uint(x + 0.f);  // zeros of both signs are equal
+        bits ^= static_cast<uint32_t>(static_cast<int32_t>(bits) >> 31) | 0x80000000u;
+        return {x > -std::numeric_limits<float>::infinity() ? static_cast<uint64_t>(bits) << 32 | ~c : 0};
     }
     __device__ __forceinline__ bool IsNone() const { return K == 0; }
-    __device__ __forceinline__ uint32_t Class() const { return static_cast<Bits>(~static_cast<Bits>(K)); }
+    __device__ __forceinline__ uint32_t Class() const { return ~static_cast<uint32_t>(K); }
     __device__ __forceinline__ float Score() const {
-        Bits bits = static_cast<Bits>(K >> kBits);
-        const Bits sign = Bits(1) << (kBits - 1);
-        bits = (bits & sign) != 0 ? static_cast<Bits>(bits & ~sign) : static_cast<Bits>(~bits);
-        return IsNone() ? -std::numeric_limits<float>::infinity() : static_cast<float>(__builtin_bit_cast(T, bits));
+        const uint32_t bits = static_cast<uint32_t>(K >> 32);
+        return IsNone() ? -std::numeric_limits<float>::infinity() : __uint_as_float(bits ^ (static_cast<uint32_t>(static_cast<int32_t>(~bits) >> 31) | 0x80000000u));
     }
     __device__ __forceinline__ TRanked Better(const TRanked& other) const { return {other.K > K ? other.K : K}; }
     // the same for an `other` whose class is the higher one
     __device__ __forceinline__ TRanked BetterLater(const TRanked& other) const { return Better(other); }
-    __device__ __forceinline__ TRanked Without(const TRanked& other) const { return {K == other.K ? Key(0) : K}; }
+    __device__ __forceinline__ TRanked Without(const TRanked& other) const { return {K == other.K ? 0 : K}; }
     __device__ __forceinline__ TRanked Or(const TRanked& other, bool take) const { return {take ? other.K : K}; }
 };
+
+// The upper half: the score as a number that has its order and is 0 for minus infinity. It is made of the magnitude with the
+// sign (zeros of both signs are equal), from which that of minus infinity is taken with a stop at 0, for two scores at a time.
+template <typename T>
+struct TRanked16 {
+    static constexpr uint32_t kInfinity = std::is_same_v<T, _Float16> ? 0x7c00 : 0x7f80;
+    uint32_t K;
+
+    __device__ __forceinline__ static TRanked16 None() { return {0}; }
+    __device__ __forceinline__ static TRanked16 Of(T x, uint32_t c) {
+        const uint32_t bits = __builtin_bit_cast(uint16_t, x), magnitude = bits & 0x7fff;
+        const uint32_t order = (bits & 0x8000) != 0 ? kInfinity - min(magnitude, kInfinity) : kInfinity + magnitude;
+        return {magnitude > kInfinity || order == 0 ? 0 : order << 16 | (~c & 0xffff)};
+    }
+    __device__ __forceinline__ bool IsNone() const { return K < 0x10000; }
+    __device__ __forceinline__ uint32_t Class() const { return ~K & 0xffff; }
+    __device__ __forceinline__ float Score() const {
+        const int32_t order = static_cast<int32_t>(K >> 16) - static_cast<int32_t>(kInfinity);
+        const uint16_t bits = order < 0 ? static_cast<uint16_t>(0x8000 - order) : static_cast<uint16_t>(order);
+        return static_cast<float>(__builtin_bit_cast(T, bits));
+    }
+    __device__ __forceinline__ TRanked16 Better(const TRanked16& other) const { return {max(K, other.K)}; }
+    __device__ __forceinline__ TRanked16 BetterLater(const TRanked16& other) const { return Better(other); }
+    __device__ __forceinline__ TRanked16 Without(const TRanked16& other) const { return {K == other.K ? 0 : K}; }
+    __device__ __forceinline__ TRanked16 Or(const TRanked16& other, bool take) const { return {take ? other.K : K}; }
+};
+template <>
+struct TRanked<_Float16> : TRanked16<_Float16> {
+    __device__ __forceinline__ TRanked() {}
+    __device__ __forceinline__ TRanked(const TRanked16<_Float16>& x) : TRanked16<_Float16>(x) {}
+};
+template <>
+struct TRanked<__bf16> : TRanked16<__bf16> {
+    __device__ __forceinline__ TRanked() {}
+    __device__ __forceinline__ TRanked(const TRanked16<__bf16>& x) : TRanked16<__bf16>(x) {}
+};
+
+// A lane's V scores from class c on, of which those before `classes` count
+template <typename T, int V>
+__device__ __forceinline__ void Rank(const TValues<T, V>& v, uint32_t c, uint32_t classes, TRanked<T> (&ranked)[V]) {
+    if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+        using TPair = uint16_t __attribute__((ext_vector_type(2)));
+        constexpr uint16_t infinity = TRanked<T>::kInfinity;
+        uint32_t most = 0;
+#pragma unroll
+        for (int j = 0; j < V; j += 2) {
+            uint32_t bits;
+            __builtin_memcpy(&bits, &v.V[j], 4);
+            const TPair sign = __builtin_bit_cast(TPair, bits) >> uint16_t(15);                       // 0 or 1
+            const uint32_t negative = __builtin_bit_cast(uint32_t, static_cast<TPair>(TPair(0) - sign));  // 0 or all bits
+            const TPair magnitude = __builtin_bit_cast(TPair, (bits & 0x7fff7fffu) ^ negative) + sign;
+            // from minus the largest magnitude on up, and then from minus infinity
+            const TPair order = __builtin_elementwise_sub_sat(static_cast<TPair>(magnitude + uint16_t(0x8000)), TPair(uint16_t(0x8000 - infinity)));
+            const uint32_t both = __builtin_bit_cast(uint32_t, order);
+            ranked[j].K = c + j < classes ? both << 16 | (~(c + j) & 0xffff) : 0;
+            ranked[j + 1].K = c + j + 1 < classes ? (both & 0xffff0000u) | (~(c + j + 1) & 0xffff) : 0;
+            most = max(most, max(ranked[j].K, ranked[j + 1].K));
+        }
+        if (most >> 16 > 2 * uint32_t(infinity)) {  // NaN of the sign that comes behind infinity
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                ranked[j].K = ranked[j].K >> 16 > 2 * uint32_t(infinity) ? 0 : ranked[j].K;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            ranked[j] = c + j < classes ? TRanked<T>::Of(v.V[j], c + j) : TRanked<T>::None();
+        }
+    }
+}
+
+// Larger keys first, by exchanges in a fixed order
+template <typename R>
+__device__ __forceinline__ void Sort8(R (&r)[8]) {
+    constexpr int pairs[19][2] = {{0, 1}, {2, 3}, {4, 5}, {6, 7}, {0, 2}, {1, 3}, {4, 6}, {5, 7}, {1, 2}, {5, 6},
+                                  {0, 4}, {1, 5}, {2, 6}, {3, 7}, {2, 4}, {3, 5}, {1, 2}, {3, 4}, {5, 6}};
+#pragma unroll
+    for (int i = 0; i < 19; ++i) {
+        const uint32_t x = r[pairs[i][0]].K, y = r[pairs[i][1]].K;
+        r[pairs[i][0]].K = max(x, y);
+        r[pairs[i][1]].K = min(x, y);
+    }
+}
+
 template <>
 struct TRanked<double> {
     uint32_t Words[2];  // of the score (with a double here, the padding behind C kept arrays of these out of registers)
@@ -559,9 +660,11 @@ __global__ void __launch_bounds__(256) SelectTopKernel(TTopArgs<T> a, int32_t* i
         v = LoadUpTo<T, V>(a.Scores + row * a.Stride + c, a.Classes - c);
     }
     R left[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        left[j] = c + j < a.Classes ? R::Of(v.V[j], c + j) : R::None();
+    Rank<T, V>(v, c, a.Classes, left);
+    // eight 32-bit keys of a lane are sorted first: a round's best is then the first, and taking it out moves the others up
+    constexpr bool sorted = sizeof(T) == 2 && V == 8;
+    if constexpr (sorted) {
+        Sort8(left);
     }
     R mine[kept];
 #pragma unroll
@@ -571,9 +674,11 @@ __global__ void __launch_bounds__(256) SelectTopKernel(TTopArgs<T> a, int32_t* i
     A most = 0, total = 0;
     for (uint32_t k = 0; k < a.Count; ++k) {
         R best = left[0];
+        if constexpr (!sorted) {
 #pragma unroll
-        for (int j = 1; j < V; ++j) {
-            best = best.BetterLater(left[j]);
+            for (int j = 1; j < V; ++j) {
+                best = best.BetterLater(left[j]);
+            }
         }
         best = OverGroup<G>(best, [](const R& x, const R& y) { return x.Better(y); });
         if (k == 0) {
@@ -586,9 +691,17 @@ __global__ void __launch_bounds__(256) SelectTopKernel(TTopArgs<T> a, int32_t* i
                 }
             }
         }
+        if constexpr (sorted) {
+            const bool taken = left[0].K == best.K;
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            left[j] = left[j].Without(best);
+            for (int j = 0; j < V; ++j) {
+                left[j] = j + 1 < V ? left[j].Or(left[j + 1 < V ? j + 1 : 0], taken) : left[j].Or(R::None(), taken);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                left[j] = left[j].Without(best);
+            }
         }
 #pragma unroll
         for (int i = 0; i < kept; ++i) {
@@ -644,10 +757,7 @@ __global__ void __launch_bounds__(256) SelectTopOfFewKernel(TTopArgs<T> a, int32
     if (threadIdx.x < rows) {
         const TValues<T, C> v = LoadRow<T, C>(a.Scores + (r0 + threadIdx.x) * a.Stride, a.Classes);
         R left[C];
-#pragma unroll
-        for (int j = 0; j < C; ++j) {
-            left[j] = static_cast<uint32_t>(j) < a.Classes ? R::Of(v.V[j], j) : R::None();
-        }
+        Rank<T, C>(v, 0, a.Classes, left);
         A* myWeights = outWeights + threadIdx.x * a.Count;
         int32_t* myIndexes = outIndexes + threadIdx.x * a.Count;
         A most = 0, total = 0;
@@ -933,13 +1043,13 @@ void AdjustScores(int valueType, size_t rows, size_t classes, const void* scores
             a.SliceClasses = ((a.Classes + a.Slices - 1) / a.Slices + 31) / 32 * 32;  // masks begin with a word
             a.Slices = slices(a.SliceClasses);
             const size_t tiles = rows * a.Slices;
-            const size_t lds = a.SliceClasses * 4 * tables;
+            const size_t lds = tables > 0 ? a.SliceClasses * 4 : 0;
             launchTiles(AdjustSliceKernel<T, THREADS, P>, tiles, THREADS, lds);
         };
         const auto atLeast = [&](uint32_t size) { return rows >= (kWorkgroupsWanted + slices(size) - 1) / slices(size); };
         using std::integral_constant;
         // the tables of two workgroups fit a compute unit (and their registers: 64-bit scores of 16384 classes would not)
-        if (sizeof(T) < 8 && tables < 2 && atLeast(16384)) {
+        if (sizeof(T) < 8 && atLeast(16384)) {
             launch(integral_constant<int, 1024>(), integral_constant<int, sizeof(T) < 8 ? 16 / N : 1>());
         } else if (atLeast(8192)) {
             launch(integral_constant<int, 1024>(), integral_constant<int, 8 / N>());

@@ -507,9 +507,9 @@ struct TRanked<__bf16> : TRanked16<__bf16> {
     __device__ __forceinline__ TRanked(const TRanked16<__bf16>& x) : TRanked16<__bf16>(x) {}
 };
 
-// A lane's V scores from class c on, of which those before `classes` count
+// A lane's V scores from class c on, of which those before `classes` count (all of every lane's, if `full`)
 template <typename T, int V>
-__device__ __forceinline__ void Rank(const TValues<T, V>& v, uint32_t c, uint32_t classes, TRanked<T> (&ranked)[V]) {
+__device__ __forceinline__ void Rank(const TValues<T, V>& v, uint32_t c, uint32_t classes, bool full, TRanked<T> (&ranked)[V]) {
     if constexpr (sizeof(T) == 2 && V % 2 == 0) {
         using TPair = uint16_t __attribute__((ext_vector_type(2)));
         constexpr uint16_t infinity = TRanked<T>::kInfinity;
@@ -524,9 +524,15 @@ __device__ __forceinline__ void Rank(const TValues<T, V>& v, uint32_t c, uint32_
             // from minus the largest magnitude on up, and then from minus infinity
             const TPair order = __builtin_elementwise_sub_sat(static_cast<TPair>(magnitude + uint16_t(0x8000)), TPair(uint16_t(0x8000 - infinity)));
             const uint32_t both = __builtin_bit_cast(uint32_t, order);
-            ranked[j].K = c + j < classes ? both << 16 | (~(c + j) & 0xffff) : 0;
-            ranked[j + 1].K = c + j + 1 < classes ? (both & 0xffff0000u) | (~(c + j + 1) & 0xffff) : 0;
+            ranked[j].K = both << 16 | (~(c + j) & 0xffff);
+            ranked[j + 1].K = (both & 0xffff0000u) | (~(c + j + 1) & 0xffff);
             most = max(most, max(ranked[j].K, ranked[j + 1].K));
+        }
+        if (!full) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                ranked[j].K = c + j < classes ? ranked[j].K : 0;
+            }
         }
         if (most >> 16 > 2 * uint32_t(infinity)) {  // NaN of the sign that comes behind infinity
 #pragma unroll
@@ -655,12 +661,15 @@ __global__ void __launch_bounds__(256) SelectTopKernel(TTopArgs<T> a, int32_t* i
         return;
     }
     const uint32_t c = lane * V;
+    const bool full = a.Classes == G * V;
     TValues<T, V> v{};
-    if (c < a.Classes) {
+    if (full) {
+        v = TValues<T, V>::Load(a.Scores + row * a.Stride + c);
+    } else if (c < a.Classes) {
         v = LoadUpTo<T, V>(a.Scores + row * a.Stride + c, a.Classes - c);
     }
     R left[V];
-    Rank<T, V>(v, c, a.Classes, left);
+    Rank<T, V>(v, c, a.Classes, full, left);
     // eight 32-bit keys of a lane are sorted first: a round's best is then the first, and taking it out moves the others up
     constexpr bool sorted = sizeof(T) == 2 && V == 8;
     if constexpr (sorted) {
@@ -705,14 +714,19 @@ __global__ void __launch_bounds__(256) SelectTopKernel(TTopArgs<T> a, int32_t* i
         }
 #pragma unroll
         for (int i = 0; i < kept; ++i) {
-            mine[i] = mine[i].Or(best, k == lane + i * G);
+            if (i * G < a.Count) {
+                mine[i] = mine[i].Or(best, k == lane + i * G);
+            }
         }
     }
     A e[kept];
 #pragma unroll
     for (int i = 0; i < kept; ++i) {
-        e[i] = mine[i].IsNone() ? A(0) : WeightOf(mine[i].Score(), most);
-        total += a.Among ? e[i] : A(0);
+        e[i] = 0;
+        if (i * G < a.Count) {
+            e[i] = mine[i].IsNone() ? A(0) : WeightOf(mine[i].Score(), most);
+            total += a.Among ? e[i] : A(0);
+        }
     }
     total = GroupSum<G>(total);
 #pragma unroll
@@ -757,7 +771,7 @@ __global__ void __launch_bounds__(256) SelectTopOfFewKernel(TTopArgs<T> a, int32
     if (threadIdx.x < rows) {
         const TValues<T, C> v = LoadRow<T, C>(a.Scores + (r0 + threadIdx.x) * a.Stride, a.Classes);
         R left[C];
-        Rank<T, C>(v, 0, a.Classes, left);
+        Rank<T, C>(v, 0, a.Classes, a.Classes == C, left);
         A* myWeights = outWeights + threadIdx.x * a.Count;
         int32_t* myIndexes = outIndexes + threadIdx.x * a.Count;
         A most = 0, total = 0;

@@ -739,26 +739,7 @@ __global__ void __launch_bounds__(256) SelectTopKernel(TTopArgs<T> a, int32_t* i
     }
 }
 
-// The row of C classes at most that a thread has to itself
-template <typename T, int C>
-__device__ __forceinline__ TValues<T, C> LoadRow(const T* from, uint32_t classes) {
-    constexpr int N = C < 16 / static_cast<int>(sizeof(T)) ? C : 16 / sizeof(T);
-    TValues<T, C> v{};
-#pragma unroll
-    for (int j = 0; j < C; j += N) {
-        if (static_cast<uint32_t>(j) < classes) {
-            const TValues<T, N> part = LoadUpTo<T, N>(from + j, classes - j);
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                v.V[j + i] = part.V[i];
-            }
-        }
-    }
-    return v;
-}
-
-// Rows of few classes: a thread for a row of at most C (classes behind the row's last are left out by branches that every
-// lane takes alike). What is stored goes through LDS, so that a wave's stores fill whole lines.
+// Rows of C classes, a thread for each. What is stored goes through LDS, so that a wave's stores fill whole lines.
 template <typename T, int C>
 __global__ void __launch_bounds__(256) SelectTopOfFewKernel(TTopArgs<T> a, int32_t* indexes, TAcc<T>* weights) {
     using A = TAcc<T>;
@@ -769,39 +750,36 @@ __global__ void __launch_bounds__(256) SelectTopOfFewKernel(TTopArgs<T> a, int32
     const size_t r0 = size_t(blockIdx.x) * 256;
     const uint32_t rows = static_cast<uint32_t>(a.Rows - r0 < 256 ? a.Rows - r0 : 256);
     if (threadIdx.x < rows) {
-        const TValues<T, C> v = LoadRow<T, C>(a.Scores + (r0 + threadIdx.x) * a.Stride, a.Classes);
+        const TValues<T, C> v = TValues<T, C>::Load(a.Scores + (r0 + threadIdx.x) * a.Stride);
         R left[C];
-        Rank<T, C>(v, 0, a.Classes, a.Classes == C, left);
+        Rank<T, C>(v, 0, C, true, left);
         A* myWeights = outWeights + threadIdx.x * a.Count;
         int32_t* myIndexes = outIndexes + threadIdx.x * a.Count;
-        A most = 0, total = 0;
+        R first = left[0];
+#pragma unroll
+        for (int j = 1; j < C; ++j) {
+            first = first.BetterLater(left[j]);
+        }
+        const A most = first.Score();
+        A total = 0;
+        if (!a.Among) {
+            // (what is never selected has a weight of 0; where nothing else is there the sum is not used)
+#pragma unroll
+            for (int j = 0; j < C; ++j) {
+                total += WeightOf(left[j].Score(), most);
+            }
+        }
         for (uint32_t k = 0; k < a.Count; ++k) {
             R best = left[0];
 #pragma unroll
             for (int j = 1; j < C; ++j) {
-                if (static_cast<uint32_t>(j) < a.Classes) {
-                    best = best.BetterLater(left[j]);
-                }
-            }
-            if (k == 0) {
-                most = best.Score();
-                if (!a.Among) {
-                    // (what is never selected has a weight of 0; where nothing else is there the sum is not used)
-#pragma unroll
-                    for (int j = 0; j < C; ++j) {
-                        if (static_cast<uint32_t>(j) < a.Classes) {
-                            total += WeightOf(left[j].Score(), most);
-                        }
-                    }
-                }
+                best = best.BetterLater(left[j]);
             }
 #pragma unroll
             for (int j = 0; j < C; ++j) {
-                if (static_cast<uint32_t>(j) < a.Classes) {
-                    left[j] = left[j].Without(best);
-                }
+                left[j] = left[j].Without(best);
             }
-            const A e = best.IsNone() ? A(0) : WeightOf(best.Score(), most);
+            const A e = best.IsNone() ? A(0) : k == 0 ? A(1) : WeightOf(best.Score(), most);
             myIndexes[k] = best.IsNone() ? -1 : static_cast<int32_t>(best.Class());
             myWeights[k] = e;
             total += a.Among ? e : A(0);
@@ -916,59 +894,52 @@ __global__ void __launch_bounds__(256) SelectTopOfFewBackwardKernel(TTopArgs<T> 
         const int32_t* indexes = b.Indexes + row * a.Count;
         const A* weights = b.Weights + row * a.Count;
         const A* gradients = b.WeightGradients + row * a.Count;
-        A mean = 0;
-        for (uint32_t k = 0; k < a.Count; ++k) {
-            mean += indexes[k] >= 0 ? weights[k] * gradients[k] : A(0);
-        }
         A x[C];
+        A mean = 0;
 #pragma unroll
         for (int j = 0; j < C; ++j) {
             x[j] = 0;
         }
+        for (uint32_t k = 0; k < a.Count; ++k) {
+            mean += indexes[k] >= 0 ? weights[k] * gradients[k] : A(0);
+        }
         if (!a.Among) {
-            const TValues<T, C> v = LoadRow<T, C>(a.Scores + row * a.Stride, a.Classes);
+            const TValues<T, C> v = TValues<T, C>::Load(a.Scores + row * a.Stride);
             A most = -std::numeric_limits<A>::infinity(), total = 0;
 #pragma unroll
             for (int j = 0; j < C; ++j) {
                 const A s = static_cast<A>(v.V[j]);
-                x[j] = static_cast<uint32_t>(j) < a.Classes && s == s ? s : -std::numeric_limits<A>::infinity();
+                x[j] = s == s ? s : -std::numeric_limits<A>::infinity();
                 most = x[j] > most ? x[j] : most;
             }
 #pragma unroll
             for (int j = 0; j < C; ++j) {
-                if (static_cast<uint32_t>(j) < a.Classes) {
-                    x[j] = x[j] > -std::numeric_limits<A>::infinity() ? WeightOf(x[j], most) : A(0);
-                    total += x[j];
-                }
+                x[j] = WeightOf(x[j], most);
+                total += x[j];
             }
+            const bool some = most > -std::numeric_limits<A>::infinity();
 #pragma unroll
             for (int j = 0; j < C; ++j) {
-                if (static_cast<uint32_t>(j) < a.Classes) {
-                    x[j] = total > 0 ? -(x[j] / total) * mean : A(0);
-                }
+                x[j] = some ? -(x[j] / total) * mean : A(0);
             }
         }
         for (uint32_t k = 0; k < a.Count; ++k) {
             const int32_t index = indexes[k];
-            if (index >= 0) {
-                const A part = a.Among ? weights[k] * (gradients[k] - mean) : weights[k] * gradients[k];
+            const A part = index >= 0 ? weights[k] * (a.Among ? gradients[k] - mean : gradients[k]) : A(0);
 #pragma unroll
-                for (int j = 0; j < C; ++j) {
-                    x[j] += index == j ? part : A(0);
-                }
+            for (int j = 0; j < C; ++j) {
+                x[j] += index == j ? part : A(0);
             }
         }
 #pragma unroll
         for (int j = 0; j < C; ++j) {
-            if (static_cast<uint32_t>(j) < a.Classes) {
-                out[threadIdx.x * a.Classes + j] = static_cast<T>(x[j]);
-            }
+            out[threadIdx.x * C + j] = static_cast<T>(x[j]);
         }
     }
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < rows * a.Classes; i += 256) {
-        const uint32_t r = i / a.Classes;
-        b.Gradients[(r0 + r) * b.GradientStride + (i - r * a.Classes)] = out[i];
+    for (uint32_t i = threadIdx.x; i < rows * C; i += 256) {
+        const uint32_t r = i / C;
+        b.Gradients[(r0 + r) * b.GradientStride + (i - r * C)] = out[i];
     }
 }
 
@@ -1081,6 +1052,7 @@ constexpr size_t kMaxTopClasses = 1024;
 constexpr int32_t kMaxTopCount = 32;
 constexpr size_t kRowsForThreads = 16384;  // a wave for each compute unit
 constexpr int32_t kCountForThreads = 8;    // 24 KB of LDS for what is stored
+constexpr int kClassesForThreads = 16;
 
 void CheckTop(size_t rows, size_t classes, int32_t count) {
     CBAMD_ENSURE(classes <= kMaxTopClasses, "too many classes to select from: " + std::to_string(classes) + ", at most " + std::to_string(kMaxTopClasses));
@@ -1089,23 +1061,25 @@ void CheckTop(size_t rows, size_t classes, int32_t count) {
     CBAMD_ENSURE(rows <= size_t(1) << 48, "too many rows");
 }
 
-// f(lanes of a row, classes of a lane), 1 lane: a thread has the row to itself. That reads each line of memory once as long
-// as a row is short, and needs rows enough to fill the chip with threads.
+template <typename F, int... C>
+bool WithExactClasses(size_t classes, F&& f, std::integer_sequence<int, C...>) {
+    return ((classes == C + 1 && (f(std::integral_constant<int, 1>(), std::integral_constant<int, C + 1>()), true)) || ...);
+}
+
+// f(lanes of a row, classes of a lane). 1 lane: a thread has a row of exactly so many classes to itself, without branches for
+// others. That reads each line of memory once as long as a row is short, and needs rows enough to fill the chip with threads.
 template <typename F>
 void WithShape(size_t classes, size_t rows, int32_t count, F&& f) {
     using std::integral_constant;
-    const auto shape = [&](auto lanes, auto perLane) { f(lanes, perLane); };
-    if (rows >= kRowsForThreads && classes <= 32 && count <= kCountForThreads) {
-        const integral_constant<int, 1> alone;
-        return classes <= 4 ? shape(alone, integral_constant<int, 4>()) : classes <= 8 ? shape(alone, integral_constant<int, 8>())
-            : classes <= 16 ? shape(alone, integral_constant<int, 16>()) : shape(alone, integral_constant<int, 32>());
+    if (rows >= kRowsForThreads && count <= kCountForThreads && WithExactClasses(classes, f, std::make_integer_sequence<int, kClassesForThreads>())) {
+        return;
     }
     const integral_constant<int, 16> sixteen;
     const integral_constant<int, 64> wave;
-    return classes <= 16 ? shape(sixteen, integral_constant<int, 1>()) : classes <= 32 ? shape(sixteen, integral_constant<int, 2>())
-        : classes <= 64 ? shape(sixteen, integral_constant<int, 4>()) : classes <= 128 ? shape(sixteen, integral_constant<int, 8>())
-        : classes <= 256 ? shape(sixteen, integral_constant<int, 16>()) : classes <= 512 ? shape(wave, integral_constant<int, 8>())
-        : shape(wave, integral_constant<int, 16>());
+    return classes <= 16 ? f(sixteen, integral_constant<int, 1>()) : classes <= 32 ? f(sixteen, integral_constant<int, 2>())
+        : classes <= 64 ? f(sixteen, integral_constant<int, 4>()) : classes <= 128 ? f(sixteen, integral_constant<int, 8>())
+        : classes <= 256 ? f(sixteen, integral_constant<int, 16>()) : classes <= 512 ? f(wave, integral_constant<int, 8>())
+        : f(wave, integral_constant<int, 16>());
 }
 
 // f(first row, rows) for rows that one launch takes (a workgroup has one tile of them)

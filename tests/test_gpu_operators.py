@@ -329,6 +329,53 @@ def test_select_top(kind, rows, classes, count, pad, among):
 
 
 @ALL
+@pytest.mark.parametrize("classes", range(1, 18))
+@pytest.mark.parametrize("among", [False, True])
+def test_select_top_of_few_classes_for_many_rows(kind, classes, among):
+    rng = np.random.default_rng(classes)
+    rows, count, pad = 16384 + 77, min(8, 1 + classes // 2), classes % 3
+    x = rng.normal(size=(rows, classes)) * 3
+    x[rng.random((rows, classes)) < 0.2] = 1.5
+    x[rng.random((rows, classes)) < 0.05] = -0.0
+    x[rng.random((rows, classes)) < 0.05] = 0.0
+    x[rng.random((rows, classes)) < 0.1] = -np.inf
+    x[rng.random((rows, classes)) < 0.02] = np.nan
+    scores = table(x, kind, pad)
+    indexes = torch.full((rows * count + 1,), 77, dtype=torch.int32, device="cuda")
+    weights = torch.full((rows * count + 1,), 77, dtype=acc(kind), device="cuda")
+    cb.select_top(kind, rows, classes, scores.data_ptr(), scores.stride(0), count, among, indexes.data_ptr(), weights.data_ptr())
+    exact = exactly(scores)
+    usable = np.where(np.isnan(exact), -np.inf, exact)
+    order = np.argsort(-usable, axis=1, kind="stable")[:, :count]
+    taken = np.take_along_axis(usable, order, 1) > -np.inf
+    picked = np.zeros(usable.shape, bool)
+    np.put_along_axis(picked, order, taken, 1)
+    most = usable.max(1, keepdims=True)
+    e = np.where(picked if among else usable > -np.inf, np.exp(usable - np.where(most > -np.inf, most, 0)), 0)
+    total = e.sum(1, keepdims=True)
+    p = e / np.where(total > 0, total, 1)
+    weight = np.where(taken, np.take_along_axis(p, order, 1), 0)
+    np.testing.assert_array_equal(indexes[:-1].cpu().numpy().reshape(rows, count), np.where(taken, order, -1))
+    error = weight_error(kind, exact)
+    compare(exactly(weights[:-1]).reshape(rows, count), weight, error * weight + 2.0 ** -125, kind if kind == cb.FLOAT64 else cb.FLOAT32)
+    assert int(indexes[-1]) == 77 and float(weights[-1]) == 77
+
+    gradients = torch.from_numpy(rng.normal(size=(rows, count))).cuda().to(acc(kind))
+    wide = torch.full((rows, classes + pad + 1), 5.0, dtype=TYPES[kind], device="cuda")
+    cb.select_top_backward(kind, rows, classes, scores.data_ptr(), scores.stride(0), count, among, indexes.data_ptr(), weights.data_ptr(),
+                           gradients.data_ptr(), wide.data_ptr(), wide.stride(0))
+    g = np.where(taken, exactly(gradients), 0)
+    mean, sizes = (g * weight).sum(1, keepdims=True), (np.abs(g) * weight).sum(1, keepdims=True)
+    part, part_size = np.zeros(p.shape, np.longdouble), np.zeros(p.shape, np.longdouble)
+    np.put_along_axis(part, order, weight * g, 1)
+    np.put_along_axis(part_size, order, weight * np.abs(g) * (error + 3 * u(kind)) + weight * np.abs(mean) * 3 * u(kind), 1)
+    expected = part - p * mean
+    bound = p * sizes * (error + u(kind) * (count + 2)) + np.abs(p * mean) * (error + 3 * u(kind)) + part_size
+    compare(exactly(wide[:, :classes]), expected, bound + 2.0 ** -120, kind)
+    assert bool((wide[:, classes:] == 5.0).all())
+
+
+@ALL
 def test_select_top_of_infinite_scores(kind):
     x = np.array([[np.inf, 1, np.inf, 0], [np.inf, np.inf, np.inf, np.inf], [1, np.inf, -np.inf, np.nan]])
     scores = table(x, kind)

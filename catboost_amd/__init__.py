@@ -180,6 +180,8 @@ def load_library():
         "CbHipDispatchRows": (ctypes.c_bool, [ctypes.c_int, sz, sz, ctypes.c_int32, vp, sz, vp, vp, sz, sz, vp]),
         "CbHipCombineRows": (ctypes.c_bool, [ctypes.c_int, sz, sz, ctypes.c_int32, vp, sz, sz, vp, vp, vp, sz, vp]),
         "CbHipCombineRowsBackward": (ctypes.c_bool, [ctypes.c_int, sz, sz, ctypes.c_int32, vp, sz, vp, sz, sz, vp, vp, vp, sz, vp, vp]),
+        "CbHipEvalRoutedBytes": (sz, [ctypes.POINTER(vp), sz, ctypes.c_int, sz, ctypes.c_int32]),
+        "CbHipEvalRouted": (ctypes.c_bool, [ctypes.POINTER(vp), sz, ctypes.POINTER(DeviceFeatures), sz, ctypes.c_int32, vp, vp, vp, vp, sz, vp]),
         "CbHipSynchronize": (ctypes.c_bool, [vp, vp]),
         "CbHipLastKernelTimes": (ctypes.c_bool, [vp, ctypes.POINTER(ctypes.c_float), ctypes.POINTER(ctypes.c_float)]),
         "CbHipDescribeKernels": (ctypes.c_bool, [vp, ctypes.c_int, sz, ctypes.c_char_p, sz]),
@@ -530,6 +532,24 @@ class DeviceEvaluator:
     def set_small_batch_slicing(self, enabled):
         """False: small batches are evaluated in one pass in tree order like large ones (CbHipEvaluatorSetSmallBatchSlicing)."""
         _check(self._lib.CbHipEvaluatorSetSmallBatchSlicing(self._h, bool(enabled)))
+
+
+def _handles(evaluators):
+    return (ctypes.c_void_p * max(len(evaluators), 1))(*[e._h for e in evaluators])
+
+
+def eval_routed_bytes(evaluators, layout, doc_count, per_doc):
+    """Bytes of workspace that eval_routed needs."""
+    size = load_library().CbHipEvalRoutedBytes(_handles(evaluators), len(evaluators), layout, doc_count, per_doc)
+    if not size:
+        raise CatBoostError(last_error())
+    return size
+
+
+def eval_routed(evaluators, features, doc_count, per_doc, experts_ptr, weights_ptr, results_ptr, workspace_ptr, workspace_bytes, stream=None):
+    """Every document by the DeviceEvaluators that its indexes name, their raw values added with its weights (CbHipEvalRouted)."""
+    _check(load_library().CbHipEvalRouted(_handles(evaluators), len(evaluators), ctypes.byref(features), doc_count, per_doc, experts_ptr,
+                                          weights_ptr, results_ptr, workspace_ptr, workspace_bytes, stream))
 
 
 class ModelCalcer:

@@ -11,6 +11,7 @@
 #include "model.h"
 #include "model_builder.h"
 #include "operators.h"
+#include "routed_evaluation.h"
 
 #include <algorithm>
 #include <cmath>
@@ -335,6 +336,15 @@ TFeatureBatch ToBatch(const CbHipFeatures* f) {
 THipEvaluator* E(CbHipEvaluatorHandle* e) {
     CBAMD_ENSURE(e != nullptr, "evaluator handle is null");
     return static_cast<THipEvaluator*>(e);
+}
+
+std::vector<THipEvaluator*> Evaluators(CbHipEvaluatorHandle* const* evaluators, size_t count) {
+    CBAMD_ENSURE(evaluators != nullptr || count == 0, "evaluator list is null");
+    std::vector<THipEvaluator*> list(count);
+    for (size_t i = 0; i < count; ++i) {
+        list[i] = E(evaluators[i]);
+    }
+    return list;
 }
 
 }  // namespace
@@ -925,6 +935,22 @@ bool CbHipCombineRowsBackward(int valueType, size_t rows, size_t width, int32_t 
     return Guard([&] {
         CombineRowsBackward(valueType, rows, width, perRow, resultGradients, gradientStride, sorted, sortedRows, sortedStride,
                             places, weights, sortedGradients, sortedGradientStride, weightGradients, hipStream);
+    });
+}
+
+size_t CbHipEvalRoutedBytes(CbHipEvaluatorHandle* const* evaluators, size_t evaluatorCount, int layout, size_t docCount,
+                            int32_t perDoc) {
+    size_t bytes = 0;
+    Guard([&] { bytes = EvalRoutedBytes(Evaluators(evaluators, evaluatorCount), layout, docCount, perDoc); });
+    return bytes;
+}
+
+bool CbHipEvalRouted(CbHipEvaluatorHandle* const* evaluators, size_t evaluatorCount, const CbHipFeatures* deviceFeatures,
+                     size_t docCount, int32_t perDoc, const int32_t* deviceExperts, const double* deviceWeights,
+                     double* deviceResults, void* deviceWorkspace, size_t workspaceBytes, void* hipStream) {
+    return Guard([&] {
+        EvalRouted(Evaluators(evaluators, evaluatorCount), ToBatch(deviceFeatures), docCount, perDoc, deviceExperts, deviceWeights,
+                   deviceResults, deviceWorkspace, workspaceBytes, hipStream);
     });
 }
 

@@ -47,6 +47,15 @@ public:
     size_t GetTreeCount() const { return TreeCount; }
     int GetApproxDimension() const { return ApproxDimension; }
     uint32_t GetBucketCount() const { return BucketCount; }
+    int GetDeviceId() const;
+    void* GetStream() const;  // the evaluator's own (a hipStream_t)
+    // values that a row has at least: of the flat layout, and of the float and categorical rows of the split one
+    struct TRowSizes {
+        size_t Flat, Floats, Cats;
+    };
+    TRowSizes GetRowSizes() const;
+    // what every launch that reads features asks of its batch
+    void CheckBatch(const TFeatureBatch& batch, size_t docCount) const;
 
     // Bytes of the quantized buffer for docCount documents:
     // ceil(docCount / 256) blocks x max(1, buckets) x 256 bytes.
@@ -106,6 +115,8 @@ public:
     void CalcDeviceNoAlloc(const TFeatureBatch& batch, size_t docCount, size_t treeStart, size_t treeEnd,
                            double* results, void* stream);
     void Synchronize(void* stream);
+    // waits for the stream
+    void CopyToHost(void* to, const void* from, size_t bytes, void* stream);
     TKernelTimes LastKernelTimes() const;
     // which kernels a whole-model call (CalcDevice, the host entry points) on docCount documents of the given
     // layout (TFeatureBatch::ELayout) and row stride (in values; 0: the model's own row width) launches:
@@ -129,8 +140,6 @@ public:
     struct TImpl;
 
 private:
-    // what every launch that reads features asks of its batch
-    void CheckBatch(const TFeatureBatch& batch, size_t docCount) const;
     void SetLastTimes(const TKernelTimes& times);
     // ... of a small-batch launch on a THostContext, whose clock stamps are read when the times are asked for
     void SetLastSmallTimes(void* smallContext);

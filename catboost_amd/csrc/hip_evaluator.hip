@@ -3316,6 +3316,24 @@ size_t THipEvaluator::QuantizedBytes(size_t docCount) const {
     return std::max<size_t>(blocks, 1) * Impl->LayoutBuckets * dev::kDocsPerBlock;
 }
 
+int THipEvaluator::GetDeviceId() const {
+    return Impl->DeviceId;
+}
+
+void* THipEvaluator::GetStream() const {
+    return Impl->Stream;
+}
+
+THipEvaluator::TRowSizes THipEvaluator::GetRowSizes() const {
+    return {Impl->FlatVectorSize, Impl->MinFloatSize, Impl->HasCats ? Impl->MinCatSize : 0};
+}
+
+void THipEvaluator::CopyToHost(void* to, const void* from, size_t bytes, void* stream) {
+    HIP_CHECK(hipSetDevice(Impl->DeviceId));
+    HIP_CHECK(hipMemcpyAsync(to, from, bytes, hipMemcpyDeviceToHost, Impl->Pick(stream)));
+    HIP_CHECK(hipStreamSynchronize(Impl->Pick(stream)));
+}
+
 void THipEvaluator::Synchronize(void* stream) {
     HIP_CHECK(hipStreamSynchronize(Impl->Pick(stream)));
 }

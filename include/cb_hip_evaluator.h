@@ -304,6 +304,20 @@ bool CbHipCombineRowsBackward(int valueType, size_t rows, size_t width, int32_t 
                               const int32_t* places, const void* weights, void* sortedGradients,
                               size_t sortedGradientStride, void* weightGradients, void* hipStream);
 
+/* Documents that are evaluated by models of their own: deviceResults[doc * dim + k] = sum over j, in their order, of
+ * deviceWeights[doc * perDoc + j] (NULL: 1) times raw value k of evaluator deviceExperts[doc * perDoc + j] (all its trees, as
+ * CbHipEvalData gives it); indexes outside [0, evaluatorCount) add nothing. At most 1024 evaluators of the same dimension, all on one
+ * device, and 64 for a document; features in CBHIP_FLAT_ROWS or CBHIP_SPLIT_ROWS, of which every model reads its own. The
+ * documents are sorted by evaluator (CbHipSortByExpert, CbHipDispatchRows), each evaluator has its own in one call, and the
+ * values are brought back (CbHipCombineRows). `hipStream` NULL: the first evaluator's own stream. Waits for the
+ * stream, so it may not be captured. The workspace (at a multiple of 8) holds the sorted features and results:
+ * CbHipEvalRoutedBytes, 0 for what CbHipEvalRouted would refuse. */
+size_t CbHipEvalRoutedBytes(CbHipEvaluatorHandle* const* evaluators, size_t evaluatorCount, int layout, size_t docCount,
+                            int32_t perDoc);
+bool CbHipEvalRouted(CbHipEvaluatorHandle* const* evaluators, size_t evaluatorCount, const CbHipFeatures* deviceFeatures,
+                     size_t docCount, int32_t perDoc, const int32_t* deviceExperts, const double* deviceWeights,
+                     double* deviceResults, void* deviceWorkspace, size_t workspaceBytes, void* hipStream);
+
 /* ---- extensions on a ModelCalcerHandle (c_api.h) ------------------------------------------ */
 
 /* The evaluator bound to a model handle (created on first use on the enabled device). Owned by

@@ -109,3 +109,10 @@ def test_routed_rows_with_nothing_to_do():
 def test_workspace_sizes():
     assert cb.sort_by_expert_bytes(0, 8) > 0
     assert cb.sort_by_expert_bytes(100, 0) == 0 and cb.sort_by_expert_bytes(1 << 31, 8) == 0
+
+
+def test_eval_routed_without_evaluators():
+    with pytest.raises(cb.CatBoostError, match="evaluators: 0"):
+        cb.eval_routed_bytes([], cb.LAYOUT_FLAT_ROWS, 10, 1)
+    with pytest.raises(cb.CatBoostError, match="evaluators: 0"):
+        cb.eval_routed([], cb.DeviceEvaluator.features(cb.LAYOUT_FLAT_ROWS, AT, 4), 10, 1, AT, 0, AT, AT, 1 << 20)

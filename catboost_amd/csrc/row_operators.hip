@@ -402,7 +402,8 @@ using namespace op;
 namespace {
 
 constexpr uint32_t kStepsOfMany = 4;                                         // when there are several workgroups
-constexpr size_t kSlotsOfOne = 16 * kSortThreads;                            // that one workgroup sorts
+// that one workgroup sorts: 8192 take it 9 us and two launches of several 9, which cost the host one more
+constexpr size_t kSlotsOfOne = 8 * kSortThreads;
 constexpr size_t kSlotsOfBlock = size_t(kStepsOfMany) * kSortThreads;
 constexpr size_t kCountsToAdd = 16384;                                       // by each workgroup, 16 for a thread
 
@@ -444,7 +445,7 @@ void SortByExpert(size_t slots, int32_t experts, const int32_t* ids, int32_t* pl
     };
     if (blocks == 1) {
         return slots <= kSortThreads ? place(PlaceSlotsKernel<1>, nullptr) : slots <= 4 * kSortThreads ? place(PlaceSlotsKernel<4>, nullptr)
-            : place(PlaceSlotsKernel<16>, nullptr);
+            : place(PlaceSlotsKernel<8>, nullptr);
     }
     const bool scan = blocks * e > kCountsToAdd;
     call.Launch(CountExpertsKernel<kStepsOfMany>, blocks, kSortThreads, kSortWaves * static_cast<size_t>(e) * 4, ids, n, e, bits, scan, counts);
@@ -457,6 +458,7 @@ void SortByExpert(size_t slots, int32_t experts, const int32_t* ids, int32_t* pl
 namespace {
 
 constexpr int32_t kMaxPerRow = 64;
+constexpr size_t kRowsOfWaves = 4096;            // 16 waves for each compute unit
 constexpr size_t kMaxGroups = size_t(1) << 23;  // of 256 threads in a launch
 
 void CheckRoutes(size_t rows, size_t width, int32_t perRow, const int32_t* places, size_t sortedRows) {
@@ -589,10 +591,11 @@ void CombineRowsBackward(int valueType, size_t rows, size_t width, int32_t perRo
                                 weightGradients != nullptr ? static_cast<TAcc<T>*>(weightGradients) + first * perRow : nullptr);
                 });
             };
-            // two pieces for a thread at most as long as eight threads are enough, else one to four for a wave's
+            // two pieces for a thread at most as long as eight threads are enough, else one for each of a wave's or, where the rows alone
+            // fill the chip, up to four
             if (pieces <= 16) {
                 launch(CombineRowsBackwardKernel<T, N, 8, K>, 8);
-            } else if (pieces <= 256) {
+            } else if (pieces <= 64 || (pieces <= 256 && rows >= kRowsOfWaves)) {
                 launch(CombineRowsBackwardKernel<T, N, 64, K>, 64);
             } else {
                 launch(CombineRowsBackwardKernel<T, N, 256, K>, 256);

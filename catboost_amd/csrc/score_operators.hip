@@ -1031,14 +1031,17 @@ void AdjustScores(int valueType, size_t rows, size_t classes, const void* scores
             const size_t lds = tables > 0 ? a.SliceClasses * 4 : 0;
             launchTiles(AdjustSliceKernel<T, THREADS, P>, tiles, THREADS, lds);
         };
-        const auto atLeast = [&](uint32_t size) { return rows >= (kWorkgroupsWanted + slices(size) - 1) / slices(size); };
+        // the longest slices that a row fills at least half of one of and of which there are workgroups enough
+        const auto suits = [&](uint32_t size) {
+            return a.Classes > size / 2 && rows >= (kWorkgroupsWanted + slices(size) - 1) / slices(size);
+        };
         using std::integral_constant;
         // the tables of two workgroups fit a compute unit (and their registers: 64-bit scores of 16384 classes would not)
-        if (sizeof(T) < 8 && atLeast(16384)) {
+        if (sizeof(T) < 8 && suits(16384)) {
             launch(integral_constant<int, 1024>(), integral_constant<int, sizeof(T) < 8 ? 16 / N : 1>());
-        } else if (atLeast(8192)) {
+        } else if (suits(8192)) {
             launch(integral_constant<int, 1024>(), integral_constant<int, 8 / N>());
-        } else if (atLeast(4096)) {
+        } else if (suits(4096)) {
             launch(integral_constant<int, (4096 / N < 1024 ? 4096 / N : 1024)>(), integral_constant<int, (4096 / N < 1024 ? 1 : 4096 / N / 1024)>());
         } else {
             launch(integral_constant<int, (2048 / N < 1024 ? 2048 / N : 1024)>(), integral_constant<int, (2048 / N < 1024 ? 1 : 2048 / N / 1024)>());

@@ -42,8 +42,8 @@ struct TPenalties {
 };
 
 // A tile's table in LDS has a word for each of its scores that counts the row's history: 1 for a class that was given, 2
-// for each time that it was generated, so that a word is 0 exactly for the classes outside the history. A second table
-// holds the last bias entry of each class, counted from 1. Both are made by integer atomics, whose order does not show.
+// for each time that it was generated, so that a word is 0 exactly for the classes outside the history. The row's biases have
+// the table afterwards. Both are made by integer atomics, whose order does not show.
 __device__ __forceinline__ void CountEntry(uint32_t* word, bool given) {
     if (given) {
         atomicOr(word, 1u);
@@ -102,13 +102,11 @@ struct TPiece {
             X[i] += bias.V[i];
         }
     }
-    __device__ __forceinline__ void AddLast(const uint32_t* last, const float* values) {
+    // (0 where there is none)
+    __device__ __forceinline__ void Add(const uint32_t* biasBits) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const uint32_t entry = last[i];
-            if (entry != 0) {
-                X[i] += values[entry - 1];
-            }
+            X[i] += __uint_as_float(biasBits[i]);
         }
     }
     // a bit of `allowed` for each of them
@@ -137,6 +135,35 @@ __device__ __forceinline__ void StorePiece(const TRaw& raw, T* at, uint32_t n) {
     TValues<T, 16 / sizeof(T)> v;
     __builtin_memcpy(&v, &raw, 16);
     StoreUpTo<T, 16 / sizeof(T)>(v, at, n);
+}
+
+// The table of biases: the last entry of each class, counted from 1, and then its value's bits in its place. Entries are
+// taken THREADS at a time, so that an entry looks whether it is the last one before any of the same class writes: the
+// ones after it are in its own batch or a later one. `word(i, entry)`: the word of entry i's class, null outside of the tile
+template <int THREADS, typename F>
+__device__ __forceinline__ void MakeBiases(uint32_t count, const int32_t* classes, const float* values, int32_t firstClass, float firstValue, F&& word) {
+    for (uint32_t i = threadIdx.x; i < count; i += THREADS) {
+        uint32_t* at = word(i, i == threadIdx.x ? firstClass : classes[i]);
+        if (at != nullptr) {
+            atomicMax(at, i + 1);
+        }
+    }
+    __syncthreads();
+    for (uint32_t begin = 0; begin < count; begin += THREADS) {
+        const uint32_t i = begin + threadIdx.x;
+        uint32_t* at = nullptr;
+        float value = firstValue;
+        if (i < count) {
+            at = word(i, begin == 0 ? firstClass : classes[i]);
+            value = begin == 0 ? firstValue : values[i];
+        }
+        const bool isLast = at != nullptr && *at == i + 1;
+        __syncthreads();
+        if (isLast) {
+            *at = __float_as_uint(value);
+        }
+    }
+    __syncthreads();
 }
 
 // A workgroup for a slice of one row, at most THREADS * P pieces. What it reads is requested at once, as far as its place is
@@ -172,7 +199,7 @@ __global__ void __launch_bounds__(THREADS) AdjustSliceKernel(TAdjustArgs a) {
     }
     if (biases) {
         firstBias = Clamped(p.BiasOffsets[row], p.BiasCount);
-        endBias = Clamped(p.BiasOffsets[row + 1], p.BiasCount);
+        endBias = max(firstBias, Clamped(p.BiasOffsets[row + 1], p.BiasCount));
     }
     const int64_t mask = p.AllowedCount != 0 ? MaskOf(p, row) : -1;
     const T* from = static_cast<const T*>(a.Scores) + row * a.ScoreStride + c0;
@@ -202,8 +229,10 @@ __global__ void __launch_bounds__(THREADS) AdjustSliceKernel(TAdjustArgs a) {
         }
     }
     int32_t biasClass = 0;
+    float biasValue = 0;
     if (firstBias + threadIdx.x < endBias) {
         biasClass = p.BiasClasses[firstBias + threadIdx.x];
+        biasValue = p.BiasValues[firstBias + threadIdx.x];
     }
     if (history) {
         int64_t e = begin + threadIdx.x * 4;
@@ -230,19 +259,29 @@ __global__ void __launch_bounds__(THREADS) AdjustSliceKernel(TAdjustArgs a) {
         }
         __syncthreads();
     }
+    TValues<float, N> classBias[P];
+    if (p.ClassBias != nullptr) {
+        const float* bias = p.ClassBias + row * p.ClassBiasStride + c0;
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+            const uint32_t c = (j * THREADS + threadIdx.x) * N;
+            if (whole) {
+                classBias[j] = TValues<float, N>::Load(bias + min(c, width - N));
+            } else if (c < width) {
+                classBias[j] = LoadUpTo<float, N>(bias + c, width - c);
+            }
+        }
+    }
     TPiece<T> x[P];
 #pragma unroll
     for (int j = 0; j < P; ++j) {
         const uint32_t c = (j * THREADS + threadIdx.x) * N;
         x[j].From(raw[j]);
-        if (c < width) {
-            if (history) {
-                x[j].Penalize(words + c, penalties);
-            }
-            if (p.ClassBias != nullptr) {
-                const float* bias = p.ClassBias + row * p.ClassBiasStride + c0 + c;
-                x[j].Add(whole ? TValues<float, N>::Load(bias) : LoadUpTo<float, N>(bias, width - c));
-            }
+        if (history && c < width) {
+            x[j].Penalize(words + c, penalties);
+        }
+        if (p.ClassBias != nullptr) {
+            x[j].Add(classBias[j]);
         }
     }
     if (biases) {
@@ -250,16 +289,11 @@ __global__ void __launch_bounds__(THREADS) AdjustSliceKernel(TAdjustArgs a) {
             __syncthreads();  // the history's words are read
         }
         clear();
-        for (int64_t b = firstBias + threadIdx.x; b < endBias; b += THREADS) {
-            const uint32_t c = static_cast<uint32_t>(biasClass) - c0;
-            if (c < width) {
-                atomicMax(&words[c], static_cast<uint32_t>(b - firstBias) + 1);
-            }
-            if (b + THREADS < endBias) {
-                biasClass = p.BiasClasses[b + THREADS];
-            }
-        }
-        __syncthreads();
+        MakeBiases<THREADS>(static_cast<uint32_t>(endBias - firstBias), p.BiasClasses + firstBias, p.BiasValues + firstBias, biasClass, biasValue,
+                            [&](uint32_t, int32_t entry) {
+                                const uint32_t c = static_cast<uint32_t>(entry) - c0;
+                                return c < width ? &words[c] : nullptr;
+                            });
     }
     T* to = static_cast<T*>(a.Result) + row * a.ResultStride + c0;
 #pragma unroll
@@ -267,7 +301,7 @@ __global__ void __launch_bounds__(THREADS) AdjustSliceKernel(TAdjustArgs a) {
         const uint32_t c = (j * THREADS + threadIdx.x) * N;
         if (c < width) {
             if (biases) {
-                x[j].AddLast(words + c, p.BiasValues + firstBias);
+                x[j].Add(words + c);
             }
             const TRaw out = x[j].Rounded(mask >= 0 ? allowed[j] >> (c & 31) : ~0u);
             if (whole) {
@@ -322,25 +356,29 @@ __device__ __forceinline__ void ForEntries(const int64_t* offsets, uint32_t rows
 // Rows that are shorter than a slice: a workgroup for RowsPerTile of them, P pieces for a thread. Pieces are taken in the
 // order in which they are in memory, whatever the rows' length, so that a wave's stores fill whole lines (a thread for a
 // row, at ten 64-bit values each, wrote 413 MB for 160). What is read is requested first, as in the kernel above.
-constexpr int kPiecesPerThread = 4;
+template <typename T>
+constexpr int kPiecesPerThread = sizeof(T) == 2 ? 2 : 4;  // 16 scores on their way, 8 of 64 bits
 
 template <typename T, bool WHOLE>
 __global__ void __launch_bounds__(256) AdjustRowsKernel(TAdjustArgs a) {
-    constexpr int N = 16 / sizeof(T), P = kPiecesPerThread;
+    constexpr int N = 16 / sizeof(T), P = kPiecesPerThread<T>;
     extern __shared__ uint4 tables[];
     const CbHipScoreAdjustment& p = a.A;
     const bool history = p.HistoryOffsets != nullptr, biases = p.BiasOffsets != nullptr;
     const uint32_t pitch = a.Pieces * N;
     TPenalties* penalties = reinterpret_cast<TPenalties*>(tables);
     int64_t* offsets = reinterpret_cast<int64_t*>(penalties + (history ? a.RowsPerTile : 0));
-    int64_t* given = offsets + (history ? a.RowsPerTile : 0);  // where the generated entries begin
-    int64_t* biasOffsets = given + (history ? a.RowsPerTile : 0);
-    uint32_t* words = reinterpret_cast<uint32_t*>(biasOffsets + (biases ? a.RowsPerTile : 0));
-    uint32_t* last = words + (history ? a.RowsPerTile * pitch : 0);
+    int64_t* given = offsets + (history || biases ? a.RowsPerTile : 0);  // where the generated entries begin
+    uint32_t* words = reinterpret_cast<uint32_t*>(given + (history ? a.RowsPerTile : 0));
     const auto rowOf = [&](uint32_t q) { return a.PiecesInverse != 0 ? __umulhi(q, a.PiecesInverse) : q; };
     const size_t tile = a.FirstTile + blockIdx.x;
     const size_t r0 = tile * a.RowsPerTile;
     const uint32_t rows = static_cast<uint32_t>(a.Rows - r0 < a.RowsPerTile ? a.Rows - r0 : a.RowsPerTile);
+    const auto clear = [&] {
+        for (uint32_t i = threadIdx.x; i < rows * pitch; i += 256) {
+            words[i] = 0;
+        }
+    };
     int64_t begin = 0, end = 0, firstBias = 0, endBias = 0;
     if (history) {
         begin = Clamped(p.HistoryOffsets[r0], p.HistoryCount);
@@ -348,7 +386,7 @@ __global__ void __launch_bounds__(256) AdjustRowsKernel(TAdjustArgs a) {
     }
     if (biases) {
         firstBias = Clamped(p.BiasOffsets[r0], p.BiasCount);
-        endBias = Clamped(p.BiasOffsets[r0 + rows], p.BiasCount);
+        endBias = max(firstBias, Clamped(p.BiasOffsets[r0 + rows], p.BiasCount));
     }
     // a thread whose pieces are behind the tile's last row reads that row's instead
     int32_t mask[P];
@@ -379,26 +417,22 @@ __global__ void __launch_bounds__(256) AdjustRowsKernel(TAdjustArgs a) {
             allowed[j] = p.Allowed[m * p.AllowedStride + (c >> 5)];
         }
     }
-    if (history || biases) {
-        TValues<int32_t, 4> entries{}, biasEntries{};
+    int32_t biasClass = 0;
+    float biasValue = 0;
+    if (firstBias + threadIdx.x < endBias) {
+        biasClass = p.BiasClasses[firstBias + threadIdx.x];
+        biasValue = p.BiasValues[firstBias + threadIdx.x];
+    }
+    if (history) {
+        TValues<int32_t, 4> entries{};
         if (begin + threadIdx.x * 4 < end) {
             entries = LoadEntries(p.History, begin + threadIdx.x * 4, p.HistoryCount);
         }
-        if (firstBias + threadIdx.x * 4 < endBias) {
-            biasEntries = LoadEntries(p.BiasClasses, firstBias + threadIdx.x * 4, p.BiasCount);
-        }
-        for (uint32_t i = threadIdx.x; i < a.RowsPerTile * pitch * (history + biases); i += 256) {
-            words[i] = 0;
-        }
+        clear();
         for (uint32_t i = threadIdx.x; i < rows; i += 256) {
-            if (history) {
-                offsets[i] = p.HistoryOffsets[r0 + i];
-                given[i] = offsets[i] + (p.PromptLengths != nullptr ? p.PromptLengths[r0 + i] : 0);
-                penalties[i] = TPenalties::Of(p, r0 + i);
-            }
-            if (biases) {
-                biasOffsets[i] = p.BiasOffsets[r0 + i];
-            }
+            offsets[i] = p.HistoryOffsets[r0 + i];
+            given[i] = offsets[i] + (p.PromptLengths != nullptr ? p.PromptLengths[r0 + i] : 0);
+            penalties[i] = TPenalties::Of(p, r0 + i);
         }
         __syncthreads();
         ForEntries(offsets, rows, begin, end, p.History, p.HistoryCount, entries, [&](int64_t e, uint32_t i, uint32_t c) {
@@ -406,31 +440,53 @@ __global__ void __launch_bounds__(256) AdjustRowsKernel(TAdjustArgs a) {
                 CountEntry(&words[i * pitch + c], e < given[i]);
             }
         });
-        ForEntries(biasOffsets, rows, firstBias, endBias, p.BiasClasses, p.BiasCount, biasEntries, [&](int64_t e, uint32_t i, uint32_t c) {
-            if (c < a.Classes) {
-                atomicMax(&last[i * pitch + c], static_cast<uint32_t>(e - firstBias) + 1);
-            }
-        });
         __syncthreads();
+    }
+    TValues<float, N> classBias[P];
+    if (p.ClassBias != nullptr) {
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+            const uint32_t q = j * 256 + threadIdx.x, r = rowOf(q), c = (q - r * a.Pieces) * N;
+            const float* bias = p.ClassBias + (r0 + min(r, rows - 1)) * p.ClassBiasStride + c;
+            classBias[j] = WHOLE ? TValues<float, N>::Load(bias) : LoadUpTo<float, N>(bias, a.Classes - c);
+        }
+    }
+    TPiece<T> x[P];
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+        const uint32_t q = j * 256 + threadIdx.x, r = rowOf(q);
+        x[j].From(raw[j]);
+        if (history && r < rows) {
+            x[j].Penalize(words + q * N, penalties[r]);
+        }
+        if (p.ClassBias != nullptr) {
+            x[j].Add(classBias[j]);
+        }
+    }
+    if (biases) {
+        if (history) {
+            __syncthreads();  // the history's words and offsets are read
+        }
+        clear();
+        for (uint32_t i = threadIdx.x; i < rows; i += 256) {
+            offsets[i] = p.BiasOffsets[r0 + i];
+        }
+        __syncthreads();
+        MakeBiases<256>(static_cast<uint32_t>(endBias - firstBias), p.BiasClasses + firstBias, p.BiasValues + firstBias, biasClass, biasValue,
+                        [&](uint32_t i, int32_t entry) {
+                            const uint32_t c = static_cast<uint32_t>(entry);
+                            return c < a.Classes ? &words[RowOfEntry(offsets, rows, firstBias + i) * pitch + c] : nullptr;
+                        });
     }
 #pragma unroll
     for (int j = 0; j < P; ++j) {
         const uint32_t q = j * 256 + threadIdx.x, r = rowOf(q), c = (q - r * a.Pieces) * N;
         if (r < rows) {
-            TPiece<T> x;
-            x.From(raw[j]);
-            if (history) {
-                x.Penalize(words + q * N, penalties[r]);
-            }
-            if (p.ClassBias != nullptr) {
-                const float* bias = p.ClassBias + (r0 + r) * p.ClassBiasStride + c;
-                x.Add(WHOLE ? TValues<float, N>::Load(bias) : LoadUpTo<float, N>(bias, a.Classes - c));
-            }
             if (biases) {
-                x.AddLast(last + q * N, p.BiasValues + firstBias);
+                x[j].Add(words + q * N);
             }
             const bool masked = p.AllowedCount != 0 && (p.AllowedRows == nullptr || mask[j] != 0);
-            const TRaw out = x.Rounded(masked ? allowed[j] >> (c & 31) : ~0u);
+            const TRaw out = x[j].Rounded(masked ? allowed[j] >> (c & 31) : ~0u);
             T* to = static_cast<T*>(a.Result) + (r0 + r) * a.ResultStride + c;
             if (WHOLE) {
                 out.Store(reinterpret_cast<uint32_t*>(to));
@@ -992,7 +1048,6 @@ void AdjustScores(int valueType, size_t rows, size_t classes, const void* scores
     WithType(valueType, [&](auto value) {
         using T = decltype(value);
         constexpr uint32_t N = 16 / sizeof(T);
-        const size_t tables = size_t(history) + size_t(biases);
         // a workgroup has one tile: a loop over tiles in the kernels kept their arguments in registers all along
         const auto launchTiles = [&](auto kernel, size_t tiles, uint32_t threads, size_t lds) {
             for (a.FirstTile = 0; a.FirstTile < tiles; a.FirstTile += kTilesPerLaunch) {
@@ -1000,15 +1055,15 @@ void AdjustScores(int valueType, size_t rows, size_t classes, const void* scores
             }
         };
         const uint32_t pieces = (a.Classes + N - 1) / N;
-        constexpr uint32_t tilePieces = kPiecesPerThread * 256;
-        if (pieces <= tilePieces / 4) {
+        constexpr uint32_t tilePieces = kPiecesPerThread<T> * 256;
+        if (pieces <= tilePieces) {
             a.Pieces = pieces;
             a.RowsPerTile = static_cast<uint32_t>(std::min<size_t>(tilePieces / pieces, rows));
             // floor(q / pieces) = floor(q m / 2^32) with m = floor(2^32 / pieces) + 1: q m / 2^32 is over q / pieces by q / 2^32 at most, and
             // q / pieces is under the next integer by 1 / pieces at least, which is more for the q and pieces under 2^11 here
             a.PiecesInverse = pieces > 1 ? static_cast<uint32_t>((uint64_t(1) << 32) / pieces + 1) : 0;
             const size_t tiles = (rows + a.RowsPerTile - 1) / a.RowsPerTile;
-            const size_t perRow = (history ? sizeof(TPenalties) + 16 : 0) + (biases ? 8 : 0) + size_t(pieces) * N * 4 * tables;
+            const size_t perRow = (history ? sizeof(TPenalties) + 16 : biases ? 8 : 0) + (history || biases ? size_t(pieces) * N * 4 : 0);
             const size_t lds = a.RowsPerTile * perRow;
             const auto launch = [&](auto kernel) {
                 call.AllowLds(reinterpret_cast<const void*>(kernel), lds);
@@ -1028,7 +1083,7 @@ void AdjustScores(int valueType, size_t rows, size_t classes, const void* scores
             a.SliceClasses = ((a.Classes + a.Slices - 1) / a.Slices + 31) / 32 * 32;  // masks begin with a word
             a.Slices = slices(a.SliceClasses);
             const size_t tiles = rows * a.Slices;
-            const size_t lds = tables > 0 ? a.SliceClasses * 4 : 0;
+            const size_t lds = history || biases ? a.SliceClasses * 4 : 0;
             launchTiles(AdjustSliceKernel<T, THREADS, P>, tiles, THREADS, lds);
         };
         // the longest slices that a row fills at least half of one of and of which there are workgroups enough

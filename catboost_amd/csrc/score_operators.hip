@@ -130,6 +130,18 @@ __device__ __forceinline__ TRaw LoadPiece(const T* at, uint32_t n) {
     __builtin_memcpy(&raw, &v, 16);
     return raw;
 }
+// The same in a row of at least N values, without branches: the load ends with the row, the values are shifted into place
+template <typename T>
+__device__ __forceinline__ TRaw LoadShifted(const T* at, uint32_t n) {
+    constexpr uint32_t N = 16 / sizeof(T);
+    const uint32_t back = n < N ? N - n : 0;
+    unsigned __int128 bits;
+    __builtin_memcpy(&bits, at - back, 16);
+    bits >>= back * (8 * sizeof(T));
+    TRaw raw;
+    __builtin_memcpy(&raw, &bits, 16);
+    return raw;
+}
 template <typename T>
 __device__ __forceinline__ void StorePiece(const TRaw& raw, T* at, uint32_t n) {
     TValues<T, 16 / sizeof(T)> v;
@@ -138,18 +150,18 @@ __device__ __forceinline__ void StorePiece(const TRaw& raw, T* at, uint32_t n) {
 }
 
 // The table of biases: the last entry of each class, counted from 1, and then its value's bits in its place. Entries are
-// taken THREADS at a time, so that an entry looks whether it is the last one before any of the same class writes: the
+// taken `threads` at a time, so that an entry looks whether it is the last one before any of the same class writes: the
 // ones after it are in its own batch or a later one. `word(i, entry)`: the word of entry i's class, null outside of the tile
-template <int THREADS, typename F>
-__device__ __forceinline__ void MakeBiases(uint32_t count, const int32_t* classes, const float* values, int32_t firstClass, float firstValue, F&& word) {
-    for (uint32_t i = threadIdx.x; i < count; i += THREADS) {
+template <typename F>
+__device__ __forceinline__ void MakeBiases(uint32_t threads, uint32_t count, const int32_t* classes, const float* values, int32_t firstClass, float firstValue, F&& word) {
+    for (uint32_t i = threadIdx.x; i < count; i += threads) {
         uint32_t* at = word(i, i == threadIdx.x ? firstClass : classes[i]);
         if (at != nullptr) {
             atomicMax(at, i + 1);
         }
     }
     __syncthreads();
-    for (uint32_t begin = 0; begin < count; begin += THREADS) {
+    for (uint32_t begin = 0; begin < count; begin += threads) {
         const uint32_t i = begin + threadIdx.x;
         uint32_t* at = nullptr;
         float value = firstValue;
@@ -166,20 +178,21 @@ __device__ __forceinline__ void MakeBiases(uint32_t count, const int32_t* classe
     __syncthreads();
 }
 
-// A workgroup for a slice of one row, at most THREADS * P pieces. What it reads is requested at once, as far as its place is
+// A workgroup for a slice of one row, at most P pieces for each of its threads. What it reads is requested at once, as far as its place is
 // known, and without branches, which would wait for one load after the other: the scores, the mask's words, the first
 // entries of the lists; the tables are made while they are on their way. The tables of the history and of the biases take
 // turns in the same LDS, so that two workgroups fit a compute unit. Every slice of a row looks through the row's whole
 // history; slices of a row are alike in length.
-template <typename T, int THREADS, int P>
-__global__ void __launch_bounds__(THREADS) AdjustSliceKernel(TAdjustArgs a) {
+template <typename T, int P>
+__global__ void __launch_bounds__(1024) AdjustSliceKernel(TAdjustArgs a) {
+    const uint32_t threads = blockDim.x;
     constexpr int N = 16 / sizeof(T);
     extern __shared__ uint4 tables[];
     const CbHipScoreAdjustment& p = a.A;
     const bool history = p.HistoryOffsets != nullptr, biases = p.BiasOffsets != nullptr;
     uint32_t* words = reinterpret_cast<uint32_t*>(tables);
     const auto clear = [&] {
-        for (uint32_t i = threadIdx.x; i < a.SliceClasses / 4; i += THREADS) {
+        for (uint32_t i = threadIdx.x; i < a.SliceClasses / 4; i += threads) {
             tables[i] = uint4{0, 0, 0, 0};
         }
         __syncthreads();
@@ -209,12 +222,12 @@ __global__ void __launch_bounds__(THREADS) AdjustSliceKernel(TAdjustArgs a) {
     if (whole) {
 #pragma unroll
         for (int j = 0; j < P; ++j) {
-            raw[j] = TRaw::Load(reinterpret_cast<const uint32_t*>(from + min((j * THREADS + threadIdx.x) * N, width - N)));
+            raw[j] = TRaw::Load(reinterpret_cast<const uint32_t*>(from + min((j * threads + threadIdx.x) * N, width - N)));
         }
     } else {
 #pragma unroll
         for (int j = 0; j < P; ++j) {
-            const uint32_t c = (j * THREADS + threadIdx.x) * N;
+            const uint32_t c = (j * threads + threadIdx.x) * N;
             if (c < width) {
                 raw[j] = LoadPiece<T>(from + c, width - c);
             }
@@ -225,7 +238,7 @@ __global__ void __launch_bounds__(THREADS) AdjustSliceKernel(TAdjustArgs a) {
 #pragma unroll
         for (int j = 0; j < P; ++j) {
             // (N classes from a multiple of N on are in one word)
-            allowed[j] = bits[(c0 + min((j * THREADS + threadIdx.x) * N, width - 1)) >> 5];
+            allowed[j] = bits[(c0 + min((j * threads + threadIdx.x) * N, width - 1)) >> 5];
         }
     }
     int32_t biasClass = 0;
@@ -242,7 +255,7 @@ __global__ void __launch_bounds__(THREADS) AdjustSliceKernel(TAdjustArgs a) {
         }
         clear();
         while (e < end) {
-            const int64_t next = e + THREADS * 4;
+            const int64_t next = e + threads * 4;
             TValues<int32_t, 4> more{};
             if (next < end) {
                 more = LoadEntries(p.History, next, p.HistoryCount);
@@ -264,7 +277,7 @@ __global__ void __launch_bounds__(THREADS) AdjustSliceKernel(TAdjustArgs a) {
         const float* bias = p.ClassBias + row * p.ClassBiasStride + c0;
 #pragma unroll
         for (int j = 0; j < P; ++j) {
-            const uint32_t c = (j * THREADS + threadIdx.x) * N;
+            const uint32_t c = (j * threads + threadIdx.x) * N;
             if (whole) {
                 classBias[j] = TValues<float, N>::Load(bias + min(c, width - N));
             } else if (c < width) {
@@ -275,7 +288,7 @@ __global__ void __launch_bounds__(THREADS) AdjustSliceKernel(TAdjustArgs a) {
     TPiece<T> x[P];
 #pragma unroll
     for (int j = 0; j < P; ++j) {
-        const uint32_t c = (j * THREADS + threadIdx.x) * N;
+        const uint32_t c = (j * threads + threadIdx.x) * N;
         x[j].From(raw[j]);
         if (history && c < width) {
             x[j].Penalize(words + c, penalties);
@@ -289,7 +302,7 @@ __global__ void __launch_bounds__(THREADS) AdjustSliceKernel(TAdjustArgs a) {
             __syncthreads();  // the history's words are read
         }
         clear();
-        MakeBiases<THREADS>(static_cast<uint32_t>(endBias - firstBias), p.BiasClasses + firstBias, p.BiasValues + firstBias, biasClass, biasValue,
+        MakeBiases(threads, static_cast<uint32_t>(endBias - firstBias), p.BiasClasses + firstBias, p.BiasValues + firstBias, biasClass, biasValue,
                             [&](uint32_t, int32_t entry) {
                                 const uint32_t c = static_cast<uint32_t>(entry) - c0;
                                 return c < width ? &words[c] : nullptr;
@@ -298,7 +311,7 @@ __global__ void __launch_bounds__(THREADS) AdjustSliceKernel(TAdjustArgs a) {
     T* to = static_cast<T*>(a.Result) + row * a.ResultStride + c0;
 #pragma unroll
     for (int j = 0; j < P; ++j) {
-        const uint32_t c = (j * THREADS + threadIdx.x) * N;
+        const uint32_t c = (j * threads + threadIdx.x) * N;
         if (c < width) {
             if (biases) {
                 x[j].Add(words + c);
@@ -359,8 +372,16 @@ __device__ __forceinline__ void ForEntries(const int64_t* offsets, uint32_t rows
 template <typename T>
 constexpr int kPiecesPerThread = sizeof(T) == 2 ? 2 : 4;  // 16 scores on their way, 8 of 64 bits
 
-template <typename T, bool WHOLE>
-__global__ void __launch_bounds__(256) AdjustRowsKernel(TAdjustArgs a) {
+enum ERests {
+    kNoRests,       // rows are whole pieces
+    kRests,         // a row's last piece may have less than N values
+    kLessThanOne,   // the only piece of a row has
+};
+
+// (64 registers, for eight waves a SIMD: 2M x 10 64-bit scores take 89 us, 93 with the 66 that the compiler chose. Where that
+// spills a dozen, 23391 x 513 of 64 bits take 67 us, 60 with 72 registers.)
+template <typename T, int RESTS>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 8 && RESTS == kRests ? 7 : 8))) AdjustRowsKernel(TAdjustArgs a) {
     constexpr int N = 16 / sizeof(T), P = kPiecesPerThread<T>;
     extern __shared__ uint4 tables[];
     const CbHipScoreAdjustment& p = a.A;
@@ -402,7 +423,8 @@ __global__ void __launch_bounds__(256) AdjustRowsKernel(TAdjustArgs a) {
     for (int j = 0; j < P; ++j) {
         const uint32_t q = j * 256 + threadIdx.x, r = rowOf(q), c = (q - r * a.Pieces) * N;
         const T* from = static_cast<const T*>(a.Scores) + (r0 + min(r, rows - 1)) * a.ScoreStride + c;
-        raw[j] = WHOLE ? TRaw::Load(reinterpret_cast<const uint32_t*>(from)) : LoadPiece<T>(from, a.Classes - c);
+        raw[j] = RESTS == kNoRests ? TRaw::Load(reinterpret_cast<const uint32_t*>(from))
+            : RESTS == kRests ? LoadShifted<T>(from, a.Classes - c) : LoadPiece<T>(from, a.Classes - c);
     }
     if (p.AllowedCount != 0) {
 #pragma unroll
@@ -447,8 +469,8 @@ __global__ void __launch_bounds__(256) AdjustRowsKernel(TAdjustArgs a) {
 #pragma unroll
         for (int j = 0; j < P; ++j) {
             const uint32_t q = j * 256 + threadIdx.x, r = rowOf(q), c = (q - r * a.Pieces) * N;
-            const float* bias = p.ClassBias + (r0 + min(r, rows - 1)) * p.ClassBiasStride + c;
-            classBias[j] = WHOLE ? TValues<float, N>::Load(bias) : LoadUpTo<float, N>(bias, a.Classes - c);
+            const float* bias = p.ClassBias + (r0 + min(r, rows - 1)) * p.ClassBiasStride;
+            classBias[j] = RESTS == kNoRests ? TValues<float, N>::Load(bias + c) : LoadUpTo<float, N>(bias + c, a.Classes - c);
         }
     }
     TPiece<T> x[P];
@@ -472,7 +494,7 @@ __global__ void __launch_bounds__(256) AdjustRowsKernel(TAdjustArgs a) {
             offsets[i] = p.BiasOffsets[r0 + i];
         }
         __syncthreads();
-        MakeBiases<256>(static_cast<uint32_t>(endBias - firstBias), p.BiasClasses + firstBias, p.BiasValues + firstBias, biasClass, biasValue,
+        MakeBiases(256, static_cast<uint32_t>(endBias - firstBias), p.BiasClasses + firstBias, p.BiasValues + firstBias, biasClass, biasValue,
                         [&](uint32_t i, int32_t entry) {
                             const uint32_t c = static_cast<uint32_t>(entry);
                             return c < a.Classes ? &words[RowOfEntry(offsets, rows, firstBias + i) * pitch + c] : nullptr;
@@ -488,7 +510,7 @@ __global__ void __launch_bounds__(256) AdjustRowsKernel(TAdjustArgs a) {
             const bool masked = p.AllowedCount != 0 && (p.AllowedRows == nullptr || mask[j] != 0);
             const TRaw out = x[j].Rounded(masked ? allowed[j] >> (c & 31) : ~0u);
             T* to = static_cast<T*>(a.Result) + (r0 + r) * a.ResultStride + c;
-            if (WHOLE) {
+            if (RESTS == kNoRests) {
                 out.Store(reinterpret_cast<uint32_t*>(to));
             } else {
                 StorePiece<T>(out, to, a.Classes - c);
@@ -1070,36 +1092,40 @@ void AdjustScores(int valueType, size_t rows, size_t classes, const void* scores
                 launchTiles(kernel, tiles, 256, lds);
             };
             if (a.Classes % N == 0) {
-                launch(AdjustRowsKernel<T, true>);
+                launch(AdjustRowsKernel<T, kNoRests>);
+            } else if (a.Classes > N) {
+                launch(AdjustRowsKernel<T, kRests>);
             } else {
-                launch(AdjustRowsKernel<T, false>);
+                launch(AdjustRowsKernel<T, kLessThanOne>);
             }
             return;
         }
         const auto slices = [&](uint32_t size) { return (a.Classes + size - 1) / size; };
-        const auto launch = [&](auto threads, auto perThread) {
-            constexpr int THREADS = decltype(threads)::value, P = decltype(perThread)::value;
-            a.Slices = slices(THREADS * P * N);
+        const auto launch = [&](uint32_t size, auto perThread) {
+            constexpr int P = decltype(perThread)::value;
+            a.Slices = slices(size);
             a.SliceClasses = ((a.Classes + a.Slices - 1) / a.Slices + 31) / 32 * 32;  // masks begin with a word
             a.Slices = slices(a.SliceClasses);
-            const size_t tiles = rows * a.Slices;
-            const size_t lds = history || biases ? a.SliceClasses * 4 : 0;
-            launchTiles(AdjustSliceKernel<T, THREADS, P>, tiles, THREADS, lds);
+            // as many threads as a slice has work for, more where long histories are looked through (384 rows of 100003 with 12000 entries:
+            // 85 us with 1024 threads, 89 with 896; 1411 of 17000 with 50: 48 with 1024, 44 with 576)
+            const bool longHistory = history && p.HistoryCount / rows > a.SliceClasses / 2;
+            const uint32_t threads = longHistory ? size / (P * N) : ((a.SliceClasses + P * N - 1) / (P * N) + 63) / 64 * 64;
+            launchTiles(AdjustSliceKernel<T, P>, rows * a.Slices, threads, history || biases ? a.SliceClasses * 4 : 0);
         };
         // the longest slices that a row fills at least half of one of and of which there are workgroups enough
         const auto suits = [&](uint32_t size) {
             return a.Classes > size / 2 && rows >= (kWorkgroupsWanted + slices(size) - 1) / slices(size);
         };
         using std::integral_constant;
-        // the tables of two workgroups fit a compute unit (and their registers: 64-bit scores of 16384 classes would not)
+        // the tables of two workgroups of 1024 threads fit a compute unit (and their registers: 64-bit scores of 16384 classes would not)
         if (sizeof(T) < 8 && suits(16384)) {
-            launch(integral_constant<int, 1024>(), integral_constant<int, sizeof(T) < 8 ? 16 / N : 1>());
+            launch(16384, integral_constant<int, sizeof(T) < 8 ? 16 / N : 1>());
         } else if (suits(8192)) {
-            launch(integral_constant<int, 1024>(), integral_constant<int, 8 / N>());
+            launch(8192, integral_constant<int, 8 / N>());
         } else if (suits(4096)) {
-            launch(integral_constant<int, (4096 / N < 1024 ? 4096 / N : 1024)>(), integral_constant<int, (4096 / N < 1024 ? 1 : 4096 / N / 1024)>());
+            launch(4096, integral_constant<int, N >= 4 ? 1 : 4 / N>());
         } else {
-            launch(integral_constant<int, (2048 / N < 1024 ? 2048 / N : 1024)>(), integral_constant<int, (2048 / N < 1024 ? 1 : 2048 / N / 1024)>());
+            launch(2048, integral_constant<int, N >= 2 ? 1 : 2 / N>());
         }
     });
 }

@@ -188,6 +188,47 @@ def test_adjust_scores(kind, rows, classes, pad, which):
 
 
 @ALL
+@pytest.mark.parametrize("rows,classes,most", [(40, 3, 5), (2000, 7, 2), (700, 12, 30), (300, 100, 3), (30, 2047, 900), (8, 4097, 20), (600, 4500, 4), (513, 8200, 40),
+                                               (270, 16400, 10), (90, 100003, 60_000)])
+def test_adjust_scores_in_place(kind, rows, classes, most):
+    """Every length of slices and tiles, histories of every length beside them, a result where the scores were."""
+    rng = np.random.default_rng(rows + classes)
+    scores = table(rng.normal(size=(rows, classes)) * 4, kind)
+    if rows * classes > 1_000_000:  # a few rows with what the others lack keep the definition quick
+        p = parts(rng, rows, classes, "hprfsbmM", 1)
+        few = np.concatenate([[0], np.cumsum(np.where(np.arange(rows) % 29 == 3, rng.integers(most // 2, most + 1, rows), 0))]).astype(np.int64)
+        p["offsets"], p["ids"] = few, (classes * rng.random(int(few[-1])) ** 3).astype(np.int32)
+        p["prompts"] = rng.integers(0, most, rows).astype(np.int32)
+    else:
+        p = parts(rng, rows, classes, "hprfscbmM", most)
+    a = Adjustment(p)
+    before = exactly(scores)
+    cb.adjust_scores(kind, rows, classes, scores.data_ptr(), classes, a.struct, scores.data_ptr(), classes)
+    expected, big = adjusted(before, p)
+    compare(exactly(scores), expected, 6.01 * u(kind) * big, kind)
+
+
+@pytest.mark.parametrize("classes", [10, 3000, 50_000])
+def test_adjust_scores_with_many_biases(classes):
+    """More bias entries than threads, most of them overridden by later ones, with values whose bits are small numbers."""
+    rng = np.random.default_rng(classes)
+    rows = 5
+    lengths = np.array([20_000, 0, 1, 7000, 300])
+    offsets = np.concatenate([[0], np.cumsum(lengths)]).astype(np.int64)
+    ids = rng.integers(0, classes, offsets[-1]).astype(np.int32)
+    values = rng.integers(1, 5000, offsets[-1]).astype(np.int32).view(np.float32)  # below the smallest normal number
+    values[::2] = rng.normal(size=len(values[::2]))
+    scores = torch.zeros(rows, classes, device="cuda")
+    a = Adjustment(dict(bias_offsets=offsets, bias_classes=ids, bias_values=values))
+    cb.adjust_scores(cb.FLOAT32, rows, classes, scores.data_ptr(), classes, a.struct, scores.data_ptr(), classes)
+    expected = np.zeros((rows, classes), np.float32)
+    for r in range(rows):
+        for e in range(offsets[r], offsets[r + 1]):
+            expected[r, ids[e]] = values[e]
+    np.testing.assert_array_equal(scores.cpu().numpy().view(np.int32), expected.view(np.int32))
+
+
+@ALL
 def test_adjust_scores_of_infinite_and_undefined_values(kind):
     rng = np.random.default_rng(5)
     rows, classes = 6, 5001

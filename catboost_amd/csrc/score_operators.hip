@@ -897,30 +897,37 @@ __global__ void __launch_bounds__(256) SelectTopBackwardKernel(TTopArgs<T> a, TT
         return;
     }
     const uint32_t c = lane * V;
+    const bool full = a.Classes == G * V;
+    TValues<T, V> v{};
+    if (!a.Among) {
+        if (full) {
+            v = TValues<T, V>::Load(a.Scores + row * a.Stride + c);
+        } else if (c < a.Classes) {
+            v = LoadUpTo<T, V>(a.Scores + row * a.Stride + c, a.Classes - c);
+        }
+    }
+    // (a lane without a slot reads the last one's, so that no load waits for another)
     int32_t index[kept];
-    A part[kept], mean = 0;
+    A w[kept], g[kept], part[kept], mean = 0;
 #pragma unroll
     for (int i = 0; i < kept; ++i) {
-        const uint32_t k = lane + i * G;
-        index[i] = k < a.Count ? b.Indexes[row * a.Count + k] : -1;
-        const A w = index[i] >= 0 ? b.Weights[row * a.Count + k] : A(0);
-        const A g = index[i] >= 0 ? b.WeightGradients[row * a.Count + k] : A(0);
-        part[i] = a.Among ? g : w * g;
-        mean += w * g;
+        const size_t at = row * a.Count + min(lane + i * G, a.Count - 1);
+        index[i] = b.Indexes[at];
+        w[i] = b.Weights[at];
+        g[i] = b.WeightGradients[at];
+    }
+#pragma unroll
+    for (int i = 0; i < kept; ++i) {
+        index[i] = lane + i * G < a.Count ? index[i] : -1;
+        mean += index[i] >= 0 ? w[i] * g[i] : A(0);
     }
     mean = GroupSum<G>(mean);
-    if (a.Among) {
 #pragma unroll
-        for (int i = 0; i < kept; ++i) {
-            part[i] = index[i] >= 0 ? b.Weights[row * a.Count + lane + i * G] * (part[i] - mean) : A(0);
-        }
+    for (int i = 0; i < kept; ++i) {
+        part[i] = a.Among ? w[i] * (g[i] - mean) : w[i] * g[i];
     }
     TValues<A, V> x{};
     if (!a.Among) {
-        TValues<T, V> v{};
-        if (c < a.Classes) {
-            v = LoadUpTo<T, V>(a.Scores + row * a.Stride + c, a.Classes - c);
-        }
         A most = -std::numeric_limits<A>::infinity();
 #pragma unroll
         for (int j = 0; j < V; ++j) {
@@ -951,12 +958,13 @@ __global__ void __launch_bounds__(256) SelectTopBackwardKernel(TTopArgs<T> a, TT
     }
     __builtin_amdgcn_wave_barrier();
     x = TValues<A, V>::Load(mySums + c);
-    if (c < a.Classes) {
-        TValues<T, V> v;
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            v.V[j] = static_cast<T>(x.V[j]);
-        }
+    for (int j = 0; j < V; ++j) {
+        v.V[j] = static_cast<T>(x.V[j]);
+    }
+    if (full) {
+        v.Store(b.Gradients + row * b.GradientStride + c);
+    } else if (c < a.Classes) {
         StoreUpTo<T, V>(v, b.Gradients + row * b.GradientStride + c, a.Classes - c);
     }
 }

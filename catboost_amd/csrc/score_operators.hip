@@ -1086,7 +1086,9 @@ void AdjustScores(int valueType, size_t rows, size_t classes, const void* scores
         };
         const uint32_t pieces = (a.Classes + N - 1) / N;
         constexpr uint32_t tilePieces = kPiecesPerThread<T> * 256;
-        if (pieces <= tilePieces) {
+        // rows that a tile holds eight of (48000 x 1000 16-bit scores: 54 us as a slice for each, 72 in tiles of 4 rows; 160000 x 300: 97 in tiles of
+        // 13, as slices the same)
+        if (pieces <= tilePieces / 8) {
             a.Pieces = pieces;
             a.RowsPerTile = static_cast<uint32_t>(std::min<size_t>(tilePieces / pieces, rows));
             // floor(q / pieces) = floor(q m / 2^32) with m = floor(2^32 / pieces) + 1: q m / 2^32 is over q / pieces by q / 2^32 at most, and
@@ -1125,8 +1127,16 @@ void AdjustScores(int valueType, size_t rows, size_t classes, const void* scores
             return a.Classes > size / 2 && rows >= (kWorkgroupsWanted + slices(size) - 1) / slices(size);
         };
         using std::integral_constant;
-        // the tables of two workgroups of 1024 threads fit a compute unit (and their registers: 64-bit scores of 16384 classes would not)
-        if (sizeof(T) < 8 && suits(16384)) {
+        // Slices of 16384 look through a history least often; the tables of two workgroups of 1024 threads fit a compute unit (and their
+        // registers: 64-bit scores would not). Where there are slices in plenty and histories are not long, smaller workgroups with as many
+        // pieces for a thread as it can hold are the better ones, of which more are at different steps at a time (256 x 131000 16-bit scores
+        // with 3000 entries a row: 46 us in slices of 8192, 50 in slices of 16384; with 12000 entries 61 and 60; 64 rows 18 and 17. 9600 x 5000:
+        // 64 us in two slices with two pieces for a thread, 103 in one with one).
+        const bool plenty = rows >= (4 * kWorkgroupsWanted + slices(8192) - 1) / slices(8192) && (!history || p.HistoryCount / rows <= 4096);
+        constexpr int most = kPiecesPerThread<T>;
+        if (plenty) {
+            launch(a.Classes > 4096 ? 8192 : a.Classes > 2048 ? 4096 : 2048, integral_constant<int, most>());
+        } else if (sizeof(T) < 8 && suits(16384)) {
             launch(16384, integral_constant<int, sizeof(T) < 8 ? 16 / N : 1>());
         } else if (suits(8192)) {
             launch(8192, integral_constant<int, 8 / N>());

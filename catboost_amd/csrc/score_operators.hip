@@ -183,13 +183,13 @@ __device__ __forceinline__ void MakeBiases(uint32_t threads, uint32_t count, con
 // entries of the lists; the tables are made while they are on their way. The tables of the history and of the biases take
 // turns in the same LDS, so that two workgroups fit a compute unit. Every slice of a row looks through the row's whole
 // history; slices of a row are alike in length.
-template <typename T, int P>
+template <typename T, int P, bool BIASES>
 __global__ void __launch_bounds__(1024) AdjustSliceKernel(TAdjustArgs a) {
     const uint32_t threads = blockDim.x;
     constexpr int N = 16 / sizeof(T);
     extern __shared__ uint4 tables[];
     const CbHipScoreAdjustment& p = a.A;
-    const bool history = p.HistoryOffsets != nullptr, biases = p.BiasOffsets != nullptr;
+    const bool history = p.HistoryOffsets != nullptr;
     uint32_t* words = reinterpret_cast<uint32_t*>(tables);
     const auto clear = [&] {
         for (uint32_t i = threadIdx.x; i < a.SliceClasses / 4; i += threads) {
@@ -210,7 +210,7 @@ __global__ void __launch_bounds__(1024) AdjustSliceKernel(TAdjustArgs a) {
         given += p.PromptLengths != nullptr ? p.PromptLengths[row] : 0;
         penalties = TPenalties::Of(p, row);
     }
-    if (biases) {
+    if (BIASES) {
         firstBias = Clamped(p.BiasOffsets[row], p.BiasCount);
         endBias = max(firstBias, Clamped(p.BiasOffsets[row + 1], p.BiasCount));
     }
@@ -285,6 +285,18 @@ __global__ void __launch_bounds__(1024) AdjustSliceKernel(TAdjustArgs a) {
             }
         }
     }
+    T* to = static_cast<T*>(a.Result) + row * a.ResultStride + c0;
+    const auto store = [&](int j, const TPiece<T>& x) {
+        const uint32_t c = (j * threads + threadIdx.x) * N;
+        if (c < width) {
+            const TRaw out = x.Rounded(mask >= 0 ? allowed[j] >> (c & 31) : ~0u);
+            if (whole) {
+                out.Store(reinterpret_cast<uint32_t*>(to + c));
+            } else {
+                StorePiece<T>(out, to + c, width - c);
+            }
+        }
+    };
     TPiece<T> x[P];
 #pragma unroll
     for (int j = 0; j < P; ++j) {
@@ -296,8 +308,11 @@ __global__ void __launch_bounds__(1024) AdjustSliceKernel(TAdjustArgs a) {
         if (p.ClassBias != nullptr) {
             x[j].Add(classBias[j]);
         }
+        if (!BIASES) {
+            store(j, x[j]);
+        }
     }
-    if (biases) {
+    if (BIASES) {
         if (history) {
             __syncthreads();  // the history's words are read
         }
@@ -307,20 +322,12 @@ __global__ void __launch_bounds__(1024) AdjustSliceKernel(TAdjustArgs a) {
                                 const uint32_t c = static_cast<uint32_t>(entry) - c0;
                                 return c < width ? &words[c] : nullptr;
                             });
-    }
-    T* to = static_cast<T*>(a.Result) + row * a.ResultStride + c0;
 #pragma unroll
-    for (int j = 0; j < P; ++j) {
-        const uint32_t c = (j * threads + threadIdx.x) * N;
-        if (c < width) {
-            if (biases) {
+        for (int j = 0; j < P; ++j) {
+            const uint32_t c = (j * threads + threadIdx.x) * N;
+            if (c < width) {
                 x[j].Add(words + c);
-            }
-            const TRaw out = x[j].Rounded(mask >= 0 ? allowed[j] >> (c & 31) : ~0u);
-            if (whole) {
-                out.Store(reinterpret_cast<uint32_t*>(to + c));
-            } else {
-                StorePiece<T>(out, to + c, width - c);
+                store(j, x[j]);
             }
         }
     }
@@ -380,16 +387,16 @@ enum ERests {
 
 // (64 registers, for eight waves a SIMD: 2M x 10 64-bit scores take 89 us, 93 with the 66 that the compiler chose. Where that
 // spills a dozen, 23391 x 513 of 64 bits take 67 us, 60 with 72 registers.)
-template <typename T, int RESTS>
+template <typename T, int RESTS, bool BIASES>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 8 && RESTS == kRests ? 7 : 8))) AdjustRowsKernel(TAdjustArgs a) {
     constexpr int N = 16 / sizeof(T), P = kPiecesPerThread<T>;
     extern __shared__ uint4 tables[];
     const CbHipScoreAdjustment& p = a.A;
-    const bool history = p.HistoryOffsets != nullptr, biases = p.BiasOffsets != nullptr;
+    const bool history = p.HistoryOffsets != nullptr;
     const uint32_t pitch = a.Pieces * N;
     TPenalties* penalties = reinterpret_cast<TPenalties*>(tables);
     int64_t* offsets = reinterpret_cast<int64_t*>(penalties + (history ? a.RowsPerTile : 0));
-    int64_t* given = offsets + (history || biases ? a.RowsPerTile : 0);  // where the generated entries begin
+    int64_t* given = offsets + (history || BIASES ? a.RowsPerTile : 0);  // where the generated entries begin
     uint32_t* words = reinterpret_cast<uint32_t*>(given + (history ? a.RowsPerTile : 0));
     const auto rowOf = [&](uint32_t q) { return a.PiecesInverse != 0 ? __umulhi(q, a.PiecesInverse) : q; };
     const size_t tile = a.FirstTile + blockIdx.x;
@@ -405,7 +412,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof
         begin = Clamped(p.HistoryOffsets[r0], p.HistoryCount);
         end = Clamped(p.HistoryOffsets[r0 + rows], p.HistoryCount);
     }
-    if (biases) {
+    if (BIASES) {
         firstBias = Clamped(p.BiasOffsets[r0], p.BiasCount);
         endBias = max(firstBias, Clamped(p.BiasOffsets[r0 + rows], p.BiasCount));
     }
@@ -473,6 +480,19 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof
             classBias[j] = RESTS == kNoRests ? TValues<float, N>::Load(bias + c) : LoadUpTo<float, N>(bias + c, a.Classes - c);
         }
     }
+    const auto store = [&](int j, const TPiece<T>& x) {
+        const uint32_t q = j * 256 + threadIdx.x, r = rowOf(q), c = (q - r * a.Pieces) * N;
+        if (r < rows) {
+            const bool masked = p.AllowedCount != 0 && (p.AllowedRows == nullptr || mask[j] != 0);
+            const TRaw out = x.Rounded(masked ? allowed[j] >> (c & 31) : ~0u);
+            T* to = static_cast<T*>(a.Result) + (r0 + r) * a.ResultStride + c;
+            if (RESTS == kNoRests) {
+                out.Store(reinterpret_cast<uint32_t*>(to));
+            } else {
+                StorePiece<T>(out, to, a.Classes - c);
+            }
+        }
+    };
     TPiece<T> x[P];
 #pragma unroll
     for (int j = 0; j < P; ++j) {
@@ -484,8 +504,11 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof
         if (p.ClassBias != nullptr) {
             x[j].Add(classBias[j]);
         }
+        if (!BIASES) {
+            store(j, x[j]);
+        }
     }
-    if (biases) {
+    if (BIASES) {
         if (history) {
             __syncthreads();  // the history's words and offsets are read
         }
@@ -499,22 +522,10 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof
                             const uint32_t c = static_cast<uint32_t>(entry);
                             return c < a.Classes ? &words[RowOfEntry(offsets, rows, firstBias + i) * pitch + c] : nullptr;
                         });
-    }
 #pragma unroll
-    for (int j = 0; j < P; ++j) {
-        const uint32_t q = j * 256 + threadIdx.x, r = rowOf(q), c = (q - r * a.Pieces) * N;
-        if (r < rows) {
-            if (biases) {
-                x[j].Add(words + q * N);
-            }
-            const bool masked = p.AllowedCount != 0 && (p.AllowedRows == nullptr || mask[j] != 0);
-            const TRaw out = x[j].Rounded(masked ? allowed[j] >> (c & 31) : ~0u);
-            T* to = static_cast<T*>(a.Result) + (r0 + r) * a.ResultStride + c;
-            if (RESTS == kNoRests) {
-                out.Store(reinterpret_cast<uint32_t*>(to));
-            } else {
-                StorePiece<T>(out, to, a.Classes - c);
-            }
+        for (int j = 0; j < P; ++j) {
+            x[j].Add(words + (j * 256 + threadIdx.x) * N);
+            store(j, x[j]);
         }
     }
 }
@@ -1101,12 +1112,20 @@ void AdjustScores(int valueType, size_t rows, size_t classes, const void* scores
                 call.AllowLds(reinterpret_cast<const void*>(kernel), lds);
                 launchTiles(kernel, tiles, 256, lds);
             };
+            const auto withBiases = [&](auto rests) {
+                constexpr int RESTS = decltype(rests)::value;
+                if (biases) {
+                    launch(AdjustRowsKernel<T, RESTS, true>);
+                } else {
+                    launch(AdjustRowsKernel<T, RESTS, false>);
+                }
+            };
             if (a.Classes % N == 0) {
-                launch(AdjustRowsKernel<T, kNoRests>);
+                withBiases(std::integral_constant<int, kNoRests>());
             } else if (a.Classes > N) {
-                launch(AdjustRowsKernel<T, kRests>);
+                withBiases(std::integral_constant<int, kRests>());
             } else {
-                launch(AdjustRowsKernel<T, kLessThanOne>);
+                withBiases(std::integral_constant<int, kLessThanOne>());
             }
             return;
         }
@@ -1120,7 +1139,12 @@ void AdjustScores(int valueType, size_t rows, size_t classes, const void* scores
             // 85 us with 1024 threads, 89 with 896; 1411 of 17000 with 50: 48 with 1024, 44 with 576)
             const bool longHistory = history && p.HistoryCount / rows > a.SliceClasses / 2;
             const uint32_t threads = longHistory ? size / (P * N) : ((a.SliceClasses + P * N - 1) / (P * N) + 63) / 64 * 64;
-            launchTiles(AdjustSliceKernel<T, P>, rows * a.Slices, threads, history || biases ? a.SliceClasses * 4 : 0);
+            const size_t lds = history || biases ? a.SliceClasses * 4 : 0;
+            if (biases) {
+                launchTiles(AdjustSliceKernel<T, P, true>, rows * a.Slices, threads, lds);
+            } else {
+                launchTiles(AdjustSliceKernel<T, P, false>, rows * a.Slices, threads, lds);
+            }
         };
         // the longest slices that a row fills at least half of one of and of which there are workgroups enough
         const auto suits = [&](uint32_t size) {

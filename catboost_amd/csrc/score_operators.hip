@@ -385,8 +385,8 @@ enum ERests {
     kLessThanOne,   // the only piece of a row has
 };
 
-// (64 registers, for eight waves a SIMD: 2M x 10 64-bit scores take 89 us, 93 with the 66 that the compiler chose. Where that
-// spills a dozen, 23391 x 513 of 64 bits take 67 us, 60 with 72 registers.)
+// (64 registers, for eight waves a SIMD: 2M x 10 64-bit scores take 90 us, 94 with the 66 that the compiler chose. Where that
+// spills a dozen, 23391 x 513 of 64 bits took 67 us, 60 with 72 registers.)
 template <typename T, int RESTS, bool BIASES>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 8 && RESTS == kRests ? 7 : 8))) AdjustRowsKernel(TAdjustArgs a) {
     constexpr int N = 16 / sizeof(T), P = kPiecesPerThread<T>;

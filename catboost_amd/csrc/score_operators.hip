@@ -524,8 +524,11 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof
                         });
 #pragma unroll
         for (int j = 0; j < P; ++j) {
-            x[j].Add(words + (j * 256 + threadIdx.x) * N);
-            store(j, x[j]);
+            const uint32_t q = j * 256 + threadIdx.x;
+            if (rowOf(q) < rows) {
+                x[j].Add(words + q * N);
+                store(j, x[j]);
+            }
         }
     }
 }

@@ -321,7 +321,7 @@ def weight_error(kind, x):
 
 @ALL
 @pytest.mark.parametrize("rows,classes,count,pad", [
-    (1, 1, 1, 0), (5, 2, 2, 0), (70, 3, 4, 1), (1001, 10, 3, 0), (300, 10, 10, 2), (9, 16, 8, 0), (9, 17, 8, 0), (130, 33, 32, 0), (7, 64, 2, 0), (65, 65, 8, 0), (33, 128, 8, 0),
+    (1, 1, 1, 0), (5, 2, 2, 0), (9, 3, 8, 0), (6, 20, 32, 1), (70, 3, 4, 1), (1001, 10, 3, 0), (300, 10, 10, 2), (9, 16, 8, 0), (9, 17, 8, 0), (130, 33, 32, 0), (7, 64, 2, 0), (65, 65, 8, 0), (33, 128, 8, 0),
     (6, 129, 5, 0), (11, 256, 6, 0), (4, 300, 8, 3), (3, 512, 1, 0), (5, 513, 9, 0), (2, 1023, 32, 1), (3, 1024, 16, 0)])
 @pytest.mark.parametrize("among", [False, True])
 def test_select_top(kind, rows, classes, count, pad, among):
@@ -374,7 +374,7 @@ def test_select_top(kind, rows, classes, count, pad, among):
 @pytest.mark.parametrize("among", [False, True])
 def test_select_top_of_few_classes_for_many_rows(kind, classes, among):
     rng = np.random.default_rng(classes)
-    rows, count, pad = 16384 + 77, min(8, 1 + classes // 2), classes % 3
+    rows, count, pad = 16384 + 77, 8 if classes % 5 == 0 else min(8, 1 + classes // 2), classes % 3
     x = rng.normal(size=(rows, classes)) * 3
     x[rng.random((rows, classes)) < 0.2] = 1.5
     x[rng.random((rows, classes)) < 0.05] = -0.0
@@ -389,6 +389,9 @@ def test_select_top_of_few_classes_for_many_rows(kind, classes, among):
     usable = np.where(np.isnan(exact), -np.inf, exact)
     order = np.argsort(-usable, axis=1, kind="stable")[:, :count]
     taken = np.take_along_axis(usable, order, 1) > -np.inf
+    if count > classes:  # what is not there: index -1, weight 0
+        assert bool((indexes[:-1].view(rows, count)[:, classes:] == -1).all()) and bool((weights[:-1].view(rows, count)[:, classes:] == 0).all())
+    there = order.shape[1]
     picked = np.zeros(usable.shape, bool)
     np.put_along_axis(picked, order, taken, 1)
     most = usable.max(1, keepdims=True)
@@ -396,16 +399,16 @@ def test_select_top_of_few_classes_for_many_rows(kind, classes, among):
     total = e.sum(1, keepdims=True)
     p = e / np.where(total > 0, total, 1)
     weight = np.where(taken, np.take_along_axis(p, order, 1), 0)
-    np.testing.assert_array_equal(indexes[:-1].cpu().numpy().reshape(rows, count), np.where(taken, order, -1))
+    np.testing.assert_array_equal(indexes[:-1].cpu().numpy().reshape(rows, count)[:, :there], np.where(taken, order, -1))
     error = weight_error(kind, exact)
-    compare(exactly(weights[:-1]).reshape(rows, count), weight, error * weight + 2.0 ** -125, kind if kind == cb.FLOAT64 else cb.FLOAT32)
+    compare(exactly(weights[:-1]).reshape(rows, count)[:, :there], weight, error * weight + 2.0 ** -125, kind if kind == cb.FLOAT64 else cb.FLOAT32)
     assert int(indexes[-1]) == 77 and float(weights[-1]) == 77
 
     gradients = torch.from_numpy(rng.normal(size=(rows, count))).cuda().to(acc(kind))
     wide = torch.full((rows, classes + pad + 1), 5.0, dtype=TYPES[kind], device="cuda")
     cb.select_top_backward(kind, rows, classes, scores.data_ptr(), scores.stride(0), count, among, indexes.data_ptr(), weights.data_ptr(),
                            gradients.data_ptr(), wide.data_ptr(), wide.stride(0))
-    g = np.where(taken, exactly(gradients), 0)
+    g = np.where(taken, exactly(gradients)[:, :there], 0)
     mean, sizes = (g * weight).sum(1, keepdims=True), (np.abs(g) * weight).sum(1, keepdims=True)
     part, part_size = np.zeros(p.shape, np.longdouble), np.zeros(p.shape, np.longdouble)
     np.put_along_axis(part, order, weight * g, 1)
@@ -683,6 +686,66 @@ def test_a_layer_of_experts_on_a_stream_and_in_graphs(kind, rows, width):
         torch.cuda.synchronize()
         for k, v in eager[at].items():
             assert torch.equal(buffers[k], v), (turn, k)
+
+
+def test_offsets_that_pass_32_bits():
+    """Histories and biases that lie behind 2^32 entries, rows that lie 2^32 values apart."""
+    far, rows, classes = (1 << 32) + 10, 3, 700
+    rng = np.random.default_rng(1)
+    scores = table(rng.normal(size=(rows, classes)), cb.FLOAT32)
+    p = dict(offsets=np.array([0, 4, 4, 9]), ids=rng.integers(0, classes, 9).astype(np.int32), frequency=np.ones(rows, np.float32))
+    expected, _ = adjusted(exactly(scores), p)
+    a = Adjustment(p)
+    entries = torch.empty(far + 16, dtype=torch.int32, device="cuda")
+    entries[far:far + 9] = a.keep["ids"]
+    a.keep["offsets"] += far
+    a.struct.History, a.struct.HistoryCount = entries.data_ptr(), far + 9
+    result = torch.empty_like(scores)
+    for few in (classes, 500):  # in tiles of rows and as slices
+        cb.adjust_scores(cb.FLOAT32, rows, few, scores.data_ptr(), classes, a.struct, result.data_ptr(), classes)
+        kept = [i for i in range(9) if p["ids"][i] < few]
+        assert kept
+        np.testing.assert_allclose(result[:, :few].cpu().numpy(), expected[:, :few].astype(np.float64), rtol=0, atol=16 * 2.0 ** -24)
+    del entries
+
+    stride = (1 << 32) + 3
+    wide = torch.empty(2 * stride + 64, dtype=torch.float16, device="cuda")
+    source = table(rng.normal(size=(3, 50)), cb.FLOAT16)
+    places = dev(np.array([[2], [0], [1]], np.int32))
+    cb.dispatch_rows(cb.FLOAT16, 3, 50, 1, source.data_ptr(), 50, places.data_ptr(), wide.data_ptr(), 3, stride)
+    for row, place in enumerate((2, 0, 1)):
+        assert torch.equal(wide[place * stride:place * stride + 50], source[row])
+    back = torch.empty_like(source)
+    cb.combine_rows(cb.FLOAT16, 3, 50, 1, wide.data_ptr(), 3, stride, places.data_ptr(), 0, back.data_ptr(), 50)
+    assert torch.equal(back, source)
+    doubled = torch.empty(3, dtype=torch.float32, device="cuda")
+    cb.combine_rows_backward(cb.FLOAT16, 3, 50, 1, source.data_ptr(), 50, wide.data_ptr(), 3, stride, places.data_ptr(), 0, 0, 50, doubled.data_ptr())
+    np.testing.assert_allclose(doubled.cpu().numpy(), (exactly(source) ** 2).sum(1).astype(np.float64), rtol=40 * 2.0 ** -24)
+    cb.adjust_scores(cb.FLOAT16, 3, 50, wide.data_ptr(), stride, cb.score_adjustment(), back.data_ptr(), 50)
+    assert torch.equal(back[torch.tensor([2, 0, 1])], source)
+    index, weight = torch.empty(3, dtype=torch.int32, device="cuda"), torch.empty(3, device="cuda")
+    cb.select_top(cb.FLOAT16, 3, 50, wide.data_ptr(), stride, 1, True, index.data_ptr(), weight.data_ptr())
+    assert torch.equal(index.long()[torch.tensor([2, 0, 1], device="cuda")], source.argmax(1))
+
+
+def test_two_streams_at_once():
+    """Calls of all kinds on two streams side by side, with buffers of their own."""
+    kind, rows, width, experts, per_row = cb.FLOAT32, 3000, 256, 40, 2
+    rng = np.random.default_rng(8)
+    bias = Adjustment(dict(class_bias=rng.normal(size=(1, experts)).astype(np.float32)))
+    inputs = [(table(rng.normal(size=(rows, width)), kind), dev(rng.normal(size=(rows, experts)).astype(np.float32))) for _ in range(2)]
+    alone = [mixture(kind, *i, bias, experts, per_row, None, mixture_buffers(kind, rows, width, experts, per_row)) for i in inputs]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    buffers = [mixture_buffers(kind, rows, width, experts, per_row) for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for i, s, b in zip(inputs, streams, buffers):
+            with torch.cuda.stream(s):
+                mixture(kind, *i, bias, experts, per_row, s.cuda_stream, b)
+    torch.cuda.synchronize()
+    for a, b in zip(alone, buffers):
+        for k in a:
+            assert k == "workspace" or torch.equal(a[k], b[k]), k
 
 
 def test_a_stream_that_is_not_given_is_the_default_one():

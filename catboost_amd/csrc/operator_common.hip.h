@@ -26,8 +26,9 @@ inline void Check(hipError_t e, const char* what) {
 // handle that knows a device, so the output's address tells it; a stream of another device is refused.
 class TCallDevice {
 public:
+    // (hipStreamLegacy is another name of the default stream, which hipStreamGetDevice takes for an address)
     TCallDevice(const void* output, void* stream)
-        : Stream(static_cast<hipStream_t>(stream))
+        : Stream(stream != static_cast<void*>(hipStreamLegacy) ? static_cast<hipStream_t>(stream) : nullptr)
     {
         hipPointerAttribute_t attributes;
         if (hipPointerGetAttributes(&attributes, output) != hipSuccess || attributes.type == hipMemoryTypeUnregistered) {
@@ -62,9 +63,10 @@ public:
                    std::index_sequence_for<TParams...>());
     }
 
-    // A kernel that uses more than 64 KB of dynamic LDS has to be told so, for each device; the largest size so far is remembered
+    // A kernel that uses more than 64 KB of LDS has to be told so, for each device; the largest size so far is remembered.
+    // `bytes`: the dynamic part (the kernels here have under 1 KB beside it)
     void AllowLds(const void* kernel, size_t bytes) const {
-        if (bytes <= 64 * 1024) {
+        if (bytes <= 63 * 1024) {
             return;
         }
         static std::mutex lock;

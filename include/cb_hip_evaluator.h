@@ -274,7 +274,7 @@ bool CbHipSelectTopBackward(int valueType, size_t rows, size_t classes, const vo
                             bool amongSelected, const int32_t* indexes, const void* weights, const void* weightGradients,
                             void* scoreGradients, size_t gradientStride, void* hipStream);
 
-/* Bytes of workspace (at any address that is a multiple of 4) that CbHipSortByExpert needs. */
+/* Bytes of workspace (at any address that is a multiple of 4) that CbHipSortByExpert needs, 0 for what it would refuse. */
 size_t CbHipSortByExpertBytes(size_t slots, int32_t experts);
 
 /* Sorts less than 2^31 slots by their expert ids[slot], of equal ones the first first: places[slot] is where the slot

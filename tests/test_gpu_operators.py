@@ -493,6 +493,15 @@ def test_sort_by_expert(slots, experts):
     np.testing.assert_array_equal(offsets.cpu().numpy(), np.concatenate([[0], np.cumsum(np.bincount(ids[valid], minlength=experts))]))
 
 
+@pytest.mark.parametrize("experts", [900, 909, 910, 911, 1000])  # tables of 64 KB more or less
+def test_sort_by_expert_around_64_kb(experts):
+    for slots in (300, 20_000):
+        ids = np.random.default_rng(slots).integers(0, experts, slots).astype(np.int32)
+        places, offsets = sort(ids, experts)
+        np.testing.assert_array_equal(places.cpu().numpy()[np.argsort(ids, kind="stable")], np.arange(slots))
+        assert int(offsets[-1]) == slots
+
+
 @pytest.mark.parametrize("slots", [500, 50_000])
 def test_sort_by_one_of_many_experts(slots):
     for ids in (np.full(slots, 5), np.full(slots, -1), np.arange(slots) % 2 * 1023):
@@ -728,6 +737,85 @@ def test_offsets_that_pass_32_bits():
     assert torch.equal(index.long()[torch.tensor([2, 0, 1], device="cuda")], source.argmax(1))
 
 
+@pytest.mark.parametrize("classes", [3, 20])
+def test_more_rows_to_select_from_than_one_launch_takes(classes):
+    rows, count = (1 << 24) + 77, 2
+    scores = torch.randn(rows, classes, device="cuda").half()
+    gradients = torch.randn(rows, count, device="cuda")
+
+    def run(begin, end):
+        n = end - begin
+        indexes, weights = torch.empty(n, count, dtype=torch.int32, device="cuda"), torch.empty(n, count, device="cuda")
+        cb.select_top(cb.FLOAT16, n, classes, scores[begin:].data_ptr(), classes, count, False, indexes.data_ptr(), weights.data_ptr())
+        out = torch.full((n, classes), 5.0, dtype=torch.float16, device="cuda")
+        cb.select_top_backward(cb.FLOAT16, n, classes, scores[begin:].data_ptr(), classes, count, False, indexes.data_ptr(), weights.data_ptr(),
+                               gradients[begin:].data_ptr(), out.data_ptr(), classes)
+        return indexes, weights, out
+
+    for whole, first, second in zip(run(0, rows), run(0, 8_000_000), run(8_000_000, rows)):
+        assert torch.equal(whole[:8_000_000], first) and torch.equal(whole[8_000_000:], second)
+
+
+def test_more_slices_than_one_launch_takes():
+    rows, classes = (1 << 21) + 9, 600
+    scores = torch.randn(rows, classes, device="cuda").half()
+    ids = torch.randint(0, classes, (rows,), dtype=torch.int32, device="cuda")
+    a = Adjustment(dict(offsets=np.arange(rows + 1), ids=ids.cpu().numpy(), presence=np.full(rows, 2.5, np.float32)))
+    result = torch.full_like(scores, 5.0)
+    cb.adjust_scores(cb.FLOAT16, rows, classes, scores.data_ptr(), classes, a.struct, result.data_ptr(), classes)
+    at = ids.long()[:, None]
+    expected = scores.scatter(1, at, (scores.gather(1, at).float() - 2.5).half())
+    assert torch.equal(result, expected)
+
+
+def test_more_tiles_of_rows_than_one_launch_takes():
+    rows = (1 << 30) + 700
+    scores = torch.randn(rows, device="cuda", dtype=torch.float16)
+    a = Adjustment(dict(class_bias=np.full((1, 1), 0.25, np.float32)))
+    result = torch.full_like(scores, 5.0)
+    cb.adjust_scores(cb.FLOAT16, rows, 1, scores.data_ptr(), 1, a.struct, result.data_ptr(), 1)
+    assert torch.equal(result, (scores.float() + 0.25).half())
+
+
+def test_more_pieces_of_rows_than_one_launch_takes():
+    width = 7
+    rows = (1 << 31) // width + 100
+    source = torch.randn(rows, width, device="cuda", dtype=torch.float16)
+    places = torch.arange(rows - 1, -1, -1, dtype=torch.int32, device="cuda")
+    moved = torch.full_like(source, 5.0)
+    cb.dispatch_rows(cb.FLOAT16, rows, width, 1, source.data_ptr(), width, places.data_ptr(), moved.data_ptr(), rows, width)
+    assert torch.equal(moved.flip(0), source)
+    result = torch.full_like(source, 5.0)
+    cb.combine_rows(cb.FLOAT16, rows, width, 1, moved.data_ptr(), rows, width, places.data_ptr(), 0, result.data_ptr(), width)
+    assert torch.equal(result, source)
+    result.fill_(5.0)
+    products = torch.full((rows,), 5.0, device="cuda")
+    cb.combine_rows_backward(cb.FLOAT16, rows, width, 1, source.data_ptr(), width, moved.data_ptr(), rows, width, places.data_ptr(), 0, result.data_ptr(),
+                             width, products.data_ptr())
+    assert torch.equal(result, moved)
+    for begin in range(0, rows, 1 << 26):  # 7 products, 7 sums
+        exact = source[begin:begin + (1 << 26)].double().square().sum(1)
+        assert bool(((products[begin:begin + (1 << 26)].double() - exact).abs() <= 14 * 2.0 ** -24 * exact).all())
+
+
+def test_the_most_slots():
+    slots = (1 << 31) - 1
+    ids = torch.empty(slots, dtype=torch.int32, device="cuda")
+    for begin in range(0, slots, 1 << 28):
+        part = ids[begin:begin + (1 << 28)]
+        part.copy_(torch.arange(begin, begin + part.numel(), device="cuda") % 3)
+    places, offsets = torch.empty_like(ids), torch.empty(3, dtype=torch.int32, device="cuda")
+    size = cb.sort_by_expert_bytes(slots, 2)
+    workspace = torch.empty(size, dtype=torch.uint8, device="cuda")
+    cb.sort_by_expert(slots, 2, ids.data_ptr(), places.data_ptr(), offsets.data_ptr(), workspace.data_ptr(), size)
+    zeros = (slots + 2) // 3
+    assert offsets.tolist() == [0, zeros, zeros + (slots + 1) // 3]
+    for begin in range(0, slots, 1 << 28):
+        i = torch.arange(begin, min(begin + (1 << 28), slots), device="cuda")
+        expected = torch.where(i % 3 == 2, -1, i // 3 + (i % 3) * zeros)
+        assert torch.equal(places[begin:begin + (1 << 28)].long(), expected)
+
+
 def test_two_streams_at_once():
     """Calls of all kinds on two streams side by side, with buffers of their own."""
     kind, rows, width, experts, per_row = cb.FLOAT32, 3000, 256, 40, 2
@@ -755,6 +843,17 @@ def test_a_stream_that_is_not_given_is_the_default_one():
         x.mul_(2)
         cb.adjust_scores(cb.FLOAT32, 1000, 100, x.data_ptr(), 100, a.struct, x.data_ptr(), 100)
     assert bool((x == 63).all())
+
+
+@pytest.mark.parametrize("stream", [1, 2])  # hipStreamLegacy, hipStreamPerThread
+def test_named_streams(stream):
+    x = torch.ones(1000, 100, device="cuda")
+    a = Adjustment(dict(class_bias=np.ones((1, 100), np.float32)))
+    torch.cuda.synchronize()
+    for _ in range(5):
+        cb.adjust_scores(cb.FLOAT32, 1000, 100, x.data_ptr(), 100, a.struct, x.data_ptr(), 100, stream)
+    torch.cuda.synchronize()
+    assert bool((x == 6).all())
 
 
 def test_host_memory_is_refused():

@@ -116,3 +116,13 @@ def test_eval_routed_without_evaluators():
         cb.eval_routed_bytes([], cb.LAYOUT_FLAT_ROWS, 10, 1)
     with pytest.raises(cb.CatBoostError, match="evaluators: 0"):
         cb.eval_routed([], cb.DeviceEvaluator.features(cb.LAYOUT_FLAT_ROWS, AT, 4), 10, 1, AT, 0, AT, AT, 1 << 20)
+
+
+def test_eval_routed_with_a_closed_evaluator():
+    class Closed:
+        _h = None
+
+    with pytest.raises(cb.CatBoostError, match="evaluator 0 is null"):
+        cb.eval_routed_bytes([Closed()], cb.LAYOUT_FLAT_ROWS, 10, 1)
+    with pytest.raises(cb.CatBoostError, match="evaluator 0 is null"):
+        cb.eval_routed([Closed(), Closed()], cb.DeviceEvaluator.features(cb.LAYOUT_FLAT_ROWS, AT, 4), 10, 1, AT, 0, AT, AT, 1 << 20)

@@ -342,7 +342,6 @@ std::vector<THipEvaluator*> Evaluators(CbHipEvaluatorHandle* const* evaluators, 
     CBAMD_ENSURE(evaluators != nullptr || count == 0, "evaluator list is null");
     std::vector<THipEvaluator*> list(count);
     for (size_t i = 0; i < count; ++i) {
-        CBAMD_ENSURE(evaluators[i] != nullptr, "evaluator " + std::to_string(i) + " is null");
         list[i] = E(evaluators[i]);
     }
     return list;

@@ -122,7 +122,7 @@ def test_eval_routed_with_a_closed_evaluator():
     class Closed:
         _h = None
 
-    with pytest.raises(cb.CatBoostError, match="evaluator 0 is null"):
+    with pytest.raises(cb.CatBoostError, match="handle is null"):
         cb.eval_routed_bytes([Closed()], cb.LAYOUT_FLAT_ROWS, 10, 1)
-    with pytest.raises(cb.CatBoostError, match="evaluator 0 is null"):
+    with pytest.raises(cb.CatBoostError, match="handle is null"):
         cb.eval_routed([Closed(), Closed()], cb.DeviceEvaluator.features(cb.LAYOUT_FLAT_ROWS, AT, 4), 10, 1, AT, 0, AT, AT, 1 << 20)

@@ -401,11 +401,13 @@ using namespace op;
 
 namespace {
 
-constexpr uint32_t kStepsOfMany = 4;                                         // when there are several workgroups
-// that one workgroup sorts: 8192 take it 9 us and two launches of several 9, which cost the host one more
+constexpr uint32_t kStepsOfMany = 4;  // when there are several workgroups
+// that one workgroup sorts (8192 of 64 experts: 8.4 us, 9.7 in two launches of several workgroups, which also cost the host one more)
 constexpr size_t kSlotsOfOne = 8 * kSortThreads;
 constexpr size_t kSlotsOfBlock = size_t(kStepsOfMany) * kSortThreads;
-constexpr size_t kCountsToAdd = 16384;                                       // by each workgroup, 16 for a thread
+// by each workgroup, eight for a thread (131072 slots of 256 experts, as many counts: 13.6 us, 14.1 with a launch that scans them; 65536 of
+// 1024, twice as many: 18.5 and 17.1)
+constexpr size_t kCountsToAdd = 8192;
 
 size_t SortBlocks(size_t slots) {
     return slots <= kSlotsOfOne ? 1 : (slots + kSlotsOfBlock - 1) / kSlotsOfBlock;
@@ -458,7 +460,7 @@ void SortByExpert(size_t slots, int32_t experts, const int32_t* ids, int32_t* pl
 namespace {
 
 constexpr int32_t kMaxPerRow = 64;
-constexpr size_t kRowsOfWaves = 4096;            // 16 waves for each compute unit
+constexpr size_t kRowsOfWaves = 4096, kRowsOfLanes = 16384;
 constexpr size_t kMaxGroups = size_t(1) << 23;  // of 256 threads in a launch
 
 void CheckRoutes(size_t rows, size_t width, int32_t perRow, const int32_t* places, size_t sortedRows) {
@@ -595,11 +597,12 @@ void CombineRowsBackward(int valueType, size_t rows, size_t width, int32_t perRo
                                 weightGradients != nullptr ? static_cast<TAcc<T>*>(weightGradients) + first * perRow : nullptr);
                 });
             };
-            // two pieces for a thread at most as long as eight threads are enough, else one for each of a wave's or, where the rows alone
-            // fill the chip, up to four
-            if (pieces <= 16) {
+            // eight threads for a row with two pieces each at most or, where the rows alone fill the chip, four (two slots of 32-bit values: 65536
+            // rows of 512 bytes 29 us, 32 with a wave for each; 4096 rows 5.8 and 5.1); a wave up to one piece for a thread or, of more rows,
+            // under four (4096 rows of 2 KB 8.8 us, 10.6 with four waves for each; 512 rows 5.0 and 4.7; 65536 rows of 4 KB 276 and 267)
+            if (pieces <= 16 || (pieces <= 32 && rows >= kRowsOfLanes)) {
                 launch(CombineRowsBackwardKernel<T, N, 8, K>, 8);
-            } else if (pieces <= 64 || (pieces <= 256 && rows >= kRowsOfWaves)) {
+            } else if (pieces <= 64 || (pieces < 256 && rows >= kRowsOfWaves)) {
                 launch(CombineRowsBackwardKernel<T, N, 64, K>, 64);
             } else {
                 launch(CombineRowsBackwardKernel<T, N, 256, K>, 256);

@@ -983,28 +983,40 @@ __global__ void __launch_bounds__(256) SelectTopBackwardKernel(TTopArgs<T> a, TT
     }
 }
 
+// Rows of C classes, a thread for each. What is loaded and stored goes through LDS (a thread that loaded its own row's selected
+// classes, one after the other, took 76 us for 262144 rows, 8 of 16 64-bit classes selected).
 template <typename T, int C>
 __global__ void __launch_bounds__(256) SelectTopOfFewBackwardKernel(TTopArgs<T> a, TTopGradientArgs<T> b) {
     using A = TAcc<T>;
-    __shared__ T out[256 * C];
+    extern __shared__ uint4 tables[];
     const size_t r0 = size_t(blockIdx.x) * 256;
     const uint32_t rows = static_cast<uint32_t>(a.Rows - r0 < 256 ? a.Rows - r0 : 256);
-    if (threadIdx.x < rows) {
-        const size_t row = r0 + threadIdx.x;
-        const int32_t* indexes = b.Indexes + row * a.Count;
-        const A* weights = b.Weights + row * a.Count;
-        const A* gradients = b.WeightGradients + row * a.Count;
-        A x[C];
-        A mean = 0;
+    const bool there = threadIdx.x < rows;
+    TValues<T, C> v{};
+    if (!a.Among) {
+        v = TValues<T, C>::Load(a.Scores + (r0 + min(threadIdx.x, rows - 1)) * a.Stride);
+    }
+    A* weights = reinterpret_cast<A*>(tables);
+    A* gradients = weights + 256 * a.Count;
+    int32_t* indexes = reinterpret_cast<int32_t*>(gradients + 256 * a.Count);
+    for (uint32_t i = threadIdx.x; i < rows * a.Count; i += 256) {
+        weights[i] = b.Weights[r0 * a.Count + i];
+        gradients[i] = b.WeightGradients[r0 * a.Count + i];
+        indexes[i] = b.Indexes[r0 * a.Count + i];
+    }
+    __syncthreads();
+    A x[C];
 #pragma unroll
-        for (int j = 0; j < C; ++j) {
-            x[j] = 0;
-        }
-        for (uint32_t k = 0; k < a.Count; ++k) {
+    for (int j = 0; j < C; ++j) {
+        x[j] = 0;
+    }
+    if (there) {
+        const uint32_t first = threadIdx.x * a.Count;
+        A mean = 0;
+        for (uint32_t k = first; k < first + a.Count; ++k) {
             mean += indexes[k] >= 0 ? weights[k] * gradients[k] : A(0);
         }
         if (!a.Among) {
-            const TValues<T, C> v = TValues<T, C>::Load(a.Scores + row * a.Stride);
             A most = -std::numeric_limits<A>::infinity(), total = 0;
 #pragma unroll
             for (int j = 0; j < C; ++j) {
@@ -1023,7 +1035,7 @@ __global__ void __launch_bounds__(256) SelectTopOfFewBackwardKernel(TTopArgs<T> 
                 x[j] = some ? -(x[j] / total) * mean : A(0);
             }
         }
-        for (uint32_t k = 0; k < a.Count; ++k) {
+        for (uint32_t k = first; k < first + a.Count; ++k) {
             const int32_t index = indexes[k];
             const A part = index >= 0 ? weights[k] * (a.Among ? gradients[k] - mean : gradients[k]) : A(0);
 #pragma unroll
@@ -1031,6 +1043,10 @@ __global__ void __launch_bounds__(256) SelectTopOfFewBackwardKernel(TTopArgs<T> 
                 x[j] += index == j ? part : A(0);
             }
         }
+    }
+    __syncthreads();  // what was loaded is read: the gradients have its place
+    T* out = reinterpret_cast<T*>(tables);
+    if (there) {
 #pragma unroll
         for (int j = 0; j < C; ++j) {
             out[threadIdx.x * C + j] = static_cast<T>(x[j]);
@@ -1179,9 +1195,15 @@ namespace {
 
 constexpr size_t kMaxTopClasses = 1024;
 constexpr int32_t kMaxTopCount = 32;
-constexpr size_t kRowsForThreads = 16384;  // a wave for each compute unit
-constexpr int32_t kCountForThreads = 8;    // 24 KB of LDS for what is stored
 constexpr int kClassesForThreads = 16;
+struct TForThreads {
+    size_t Rows;
+    int32_t Count;
+};
+// (16384 rows of 16 32-bit classes, 8 of them selected: 6.3 us by threads, 4.4 by lanes; 65536: 6.8 and 10.1; a million, 2 of 10: 11.4 and 50)
+constexpr TForThreads kForwardByThreads{32768, 8};
+// (65536 rows, 2 of 10 32-bit classes: 4.2 us by threads, 3.5 by lanes; 262144: 6.3 and 8.7; 8 of 10: 12.2 and 9.7)
+constexpr TForThreads kBackwardByThreads{131072, 4};
 
 void CheckTop(size_t rows, size_t classes, int32_t count) {
     CBAMD_ENSURE(classes <= kMaxTopClasses, "too many classes to select from: " + std::to_string(classes) + ", at most " + std::to_string(kMaxTopClasses));
@@ -1198,9 +1220,9 @@ bool WithExactClasses(size_t classes, F&& f, std::integer_sequence<int, C...>) {
 // f(lanes of a row, classes of a lane). 1 lane: a thread has a row of exactly so many classes to itself, without branches for
 // others. That reads each line of memory once as long as a row is short, and needs rows enough to fill the chip with threads.
 template <typename F>
-void WithShape(size_t classes, size_t rows, int32_t count, F&& f) {
+void WithShape(size_t classes, size_t rows, int32_t count, const TForThreads& threads, F&& f) {
     using std::integral_constant;
-    if (rows >= kRowsForThreads && count <= kCountForThreads && WithExactClasses(classes, f, std::make_integer_sequence<int, kClassesForThreads>())) {
+    if (rows >= threads.Rows && count <= threads.Count && WithExactClasses(classes, f, std::make_integer_sequence<int, kClassesForThreads>())) {
         return;
     }
     const integral_constant<int, 16> sixteen;
@@ -1239,7 +1261,7 @@ void SelectTop(int valueType, size_t rows, size_t classes, const void* scores, s
     const TCallDevice call(indexes, stream);
     WithType(valueType, [&](auto value) {
         using T = decltype(value);
-        WithShape(classes, rows, count, [&](auto lanes, auto perLane) {
+        WithShape(classes, rows, count, kForwardByThreads, [&](auto lanes, auto perLane) {
             constexpr int G = decltype(lanes)::value, V = decltype(perLane)::value;
             ForLaunches(rows, [&](size_t first, size_t n) {
                 const TTopArgs<T> a{static_cast<const T*>(scores) + first * scoreStride, scoreStride, n, static_cast<uint32_t>(classes),
@@ -1272,7 +1294,7 @@ void SelectTopBackward(int valueType, size_t rows, size_t classes, const void* s
     const TCallDevice call(scoreGradients, stream);
     WithType(valueType, [&](auto value) {
         using T = decltype(value);
-        WithShape(classes, rows, count, [&](auto lanes, auto perLane) {
+        WithShape(classes, rows, count, kBackwardByThreads, [&](auto lanes, auto perLane) {
             constexpr int G = decltype(lanes)::value, V = decltype(perLane)::value;
             ForLaunches(rows, [&](size_t first, size_t n) {
                 const TTopArgs<T> a{static_cast<const T*>(scores) + (amongSelected ? 0 : first * scoreStride), scoreStride, n,
@@ -1281,7 +1303,8 @@ void SelectTopBackward(int valueType, size_t rows, size_t classes, const void* s
                                             static_cast<const TAcc<T>*>(weightGradients) + first * count,
                                             static_cast<T*>(scoreGradients) + first * gradientStride, gradientStride};
                 if constexpr (G == 1) {
-                    call.Launch(SelectTopOfFewBackwardKernel<T, V>, GroupsOf(n, G), 256, 0, a, b);
+                    const size_t lds = 256 * std::max(count * (2 * sizeof(TAcc<T>) + 4), V * sizeof(T));
+                    call.Launch(SelectTopOfFewBackwardKernel<T, V>, GroupsOf(n, G), 256, lds, a, b);
                 } else {
                     call.Launch(SelectTopBackwardKernel<T, G, V>, GroupsOf(n, G), 256, 0, a, b);
                 }

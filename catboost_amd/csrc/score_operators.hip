@@ -600,16 +600,31 @@ struct TRanked<__bf16> : TRanked16<__bf16> {
 };
 
 // A lane's V scores from class c on, of which those before `classes` count (all of every lane's, if `full`)
+// (Those of 16 bits in pairs as they are in memory: single ones would take a register each.)
 template <typename T, int V>
-__device__ __forceinline__ void Rank(const TValues<T, V>& v, uint32_t c, uint32_t classes, bool full, TRanked<T> (&ranked)[V]) {
+using TLaneScores = std::conditional_t<sizeof(T) == 2 && V % 2 == 0, TValues<uint32_t, (V + 1) / 2>, TValues<T, V>>;
+
+template <typename T, int V>
+__device__ __forceinline__ TLaneScores<T, V> LoadLane(const T* at, uint32_t c, uint32_t classes, bool full) {
+    TLaneScores<T, V> raw{};
+    if (full) {
+        __builtin_memcpy(&raw, at + c, sizeof(raw));
+    } else if (c < classes) {
+        const TValues<T, V> v = LoadUpTo<T, V>(at + c, classes - c);
+        __builtin_memcpy(&raw, &v, sizeof(raw));
+    }
+    return raw;
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void Rank(const TLaneScores<T, V>& v, uint32_t c, uint32_t classes, bool full, TRanked<T> (&ranked)[V]) {
     if constexpr (sizeof(T) == 2 && V % 2 == 0) {
         using TPair = uint16_t __attribute__((ext_vector_type(2)));
         constexpr uint16_t infinity = TRanked<T>::kInfinity;
         uint32_t most = 0;
 #pragma unroll
         for (int j = 0; j < V; j += 2) {
-            uint32_t bits;
-            __builtin_memcpy(&bits, &v.V[j], 4);
+            const uint32_t bits = v.V[j / 2];
             const TPair sign = __builtin_bit_cast(TPair, bits) >> uint16_t(15);                       // 0 or 1
             const uint32_t negative = __builtin_bit_cast(uint32_t, static_cast<TPair>(TPair(0) - sign));  // 0 or all bits
             const TPair magnitude = __builtin_bit_cast(TPair, (bits & 0x7fff7fffu) ^ negative) + sign;
@@ -754,14 +769,8 @@ __global__ void __launch_bounds__(256) SelectTopKernel(TTopArgs<T> a, int32_t* i
     }
     const uint32_t c = lane * V;
     const bool full = a.Classes == G * V;
-    TValues<T, V> v{};
-    if (full) {
-        v = TValues<T, V>::Load(a.Scores + row * a.Stride + c);
-    } else if (c < a.Classes) {
-        v = LoadUpTo<T, V>(a.Scores + row * a.Stride + c, a.Classes - c);
-    }
     R left[V];
-    Rank<T, V>(v, c, a.Classes, full, left);
+    Rank<T, V>(LoadLane<T, V>(a.Scores + row * a.Stride, c, a.Classes, full), c, a.Classes, full, left);
     // eight 32-bit keys of a lane are sorted first: a round's best is then the first, and taking it out moves the others up
     constexpr bool sorted = sizeof(T) == 2 && V == 8;
     if constexpr (sorted) {
@@ -773,7 +782,8 @@ __global__ void __launch_bounds__(256) SelectTopKernel(TTopArgs<T> a, int32_t* i
         mine[i] = R::None();
     }
     A most = 0, total = 0;
-    for (uint32_t k = 0; k < a.Count; ++k) {
+    // `keys`: of a lane's sorted ones, how many later rounds may ask for
+    const auto round = [&](uint32_t k, int keys) {
         R best = left[0];
         if constexpr (!sorted) {
 #pragma unroll
@@ -796,7 +806,9 @@ __global__ void __launch_bounds__(256) SelectTopKernel(TTopArgs<T> a, int32_t* i
             const bool taken = left[0].K == best.K;
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                left[j] = j + 1 < V ? left[j].Or(left[j + 1 < V ? j + 1 : 0], taken) : left[j].Or(R::None(), taken);
+                if (j < keys) {
+                    left[j] = j + 1 < V ? left[j].Or(left[j + 1 < V ? j + 1 : 0], taken) : left[j].Or(R::None(), taken);
+                }
             }
         } else {
 #pragma unroll
@@ -809,6 +821,18 @@ __global__ void __launch_bounds__(256) SelectTopKernel(TTopArgs<T> a, int32_t* i
             if (i * G < a.Count) {
                 mine[i] = mine[i].Or(best, k == lane + i * G);
             }
+        }
+    };
+    if (sorted && a.Count <= V) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            if (static_cast<uint32_t>(k) < a.Count) {
+                round(k, V - 1 - k);
+            }
+        }
+    } else {
+        for (uint32_t k = 0; k < a.Count; ++k) {
+            round(k, V);
         }
     }
     A e[kept];
@@ -842,9 +866,8 @@ __global__ void __launch_bounds__(256) SelectTopOfFewKernel(TTopArgs<T> a, int32
     const size_t r0 = size_t(blockIdx.x) * 256;
     const uint32_t rows = static_cast<uint32_t>(a.Rows - r0 < 256 ? a.Rows - r0 : 256);
     if (threadIdx.x < rows) {
-        const TValues<T, C> v = TValues<T, C>::Load(a.Scores + (r0 + threadIdx.x) * a.Stride);
         R left[C];
-        Rank<T, C>(v, 0, C, true, left);
+        Rank<T, C>(LoadLane<T, C>(a.Scores + (r0 + threadIdx.x) * a.Stride, 0, C, true), 0, C, true, left);
         A* myWeights = outWeights + threadIdx.x * a.Count;
         int32_t* myIndexes = outIndexes + threadIdx.x * a.Count;
         R first = left[0];

@@ -182,7 +182,9 @@ __device__ __forceinline__ void MakeBiases(uint32_t threads, uint32_t count, con
 // known, and without branches, which would wait for one load after the other: the scores, the mask's words, the first
 // entries of the lists; the tables are made while they are on their way. The tables of the history and of the biases take
 // turns in the same LDS, so that two workgroups fit a compute unit. Every slice of a row looks through the row's whole
-// history; slices of a row are alike in length.
+// history; slices of a row are alike in length. Memory bounds it when there is much: 384 x 100003 32-bit scores with
+// 12000 entries a row take 80 us (4.1 TB/s); 64 x 131000 of 16 bits with 3000 entries, biases and masks 16, where the steps wait
+// for each other.
 template <typename T, int P, bool BIASES>
 __global__ void __launch_bounds__(1024) AdjustSliceKernel(TAdjustArgs a) {
     const uint32_t threads = blockDim.x;
@@ -375,7 +377,8 @@ __device__ __forceinline__ void ForEntries(const int64_t* offsets, uint32_t rows
 
 // Rows that are shorter than a slice: a workgroup for RowsPerTile of them, P pieces for a thread. Pieces are taken in the
 // order in which they are in memory, whatever the rows' length, so that a wave's stores fill whole lines (a thread for a
-// row, at ten 64-bit values each, wrote 413 MB for 160). What is read is requested first, as in the kernel above.
+// row, at ten 64-bit values each, wrote 413 MB for 160). What is read is requested first, as in the kernel above. Memory bounds it:
+// 2M x 10 64-bit scores with histories, biases of classes and masks take 88 us (4.6 TB/s).
 template <typename T>
 constexpr int kPiecesPerThread = sizeof(T) == 2 ? 2 : 4;  // 16 scores on their way, 8 of 64 bits
 
@@ -756,7 +759,8 @@ struct TTopArgs {
 };
 
 // G lanes for a row, V classes next to each other for each of them. A round finds the best class that is left: in the
-// lane's own, then over the group; whoever has it takes it out. Lane k % G keeps what round k finds.
+// lane's own, then over the group; whoever has it takes it out. Lane k % G keeps what round k finds. Arithmetic bounds it: 131072
+// rows, 8 of 128 16-bit classes take 17 us, for 42 MB.
 template <typename T, int G, int V>
 __global__ void __launch_bounds__(256) SelectTopKernel(TTopArgs<T> a, int32_t* indexes, TAcc<T>* weights) {
     using A = TAcc<T>;
@@ -855,7 +859,8 @@ __global__ void __launch_bounds__(256) SelectTopKernel(TTopArgs<T> a, int32_t* i
     }
 }
 
-// Rows of C classes, a thread for each. What is stored goes through LDS, so that a wave's stores fill whole lines.
+// Rows of C classes, a thread for each. What is stored goes through LDS, so that a wave's stores fill whole lines. Memory bounds it:
+// 2M rows, 3 of 10 64-bit classes take 52 us (4.5 TB/s).
 template <typename T, int C>
 __global__ void __launch_bounds__(256) SelectTopOfFewKernel(TTopArgs<T> a, int32_t* indexes, TAcc<T>* weights) {
     using A = TAcc<T>;
@@ -921,11 +926,14 @@ struct TTopGradientArgs {
 
 // With w the weights, p the softmax over all classes and g the weights' gradients, m = sum of g w over the selected:
 // among the selected only w_k (g_k - m) and 0 elsewhere, else w_k g_k - p m with the first part 0 elsewhere.
-// A row's gradients are put together in LDS, where the selected classes' lanes add their parts.
+// G lanes for a row, which take its pieces of 16 bytes in turn, V classes each in all (V next to each other instead took 43 us for
+// 131072 rows of 256 32-bit classes, and these 20). The gradients are put together in LDS, where the selected classes' lanes add
+// their parts. Memory bounds it: 8 of 128 16-bit classes 8.8 us for 46 MB, which the caches still have in part.
 template <typename T, int G, int V>
 __global__ void __launch_bounds__(256) SelectTopBackwardKernel(TTopArgs<T> a, TTopGradientArgs<T> b) {
     using A = TAcc<T>;
     constexpr int kept = 32 / G > 0 ? 32 / G : 1;
+    constexpr int N = V * sizeof(T) <= 16 ? V : 16 / sizeof(T), P = V / N;
     __shared__ __align__(16) A sums[256 * V];
     const uint32_t lane = threadIdx.x & (G - 1);
     A* mySums = sums + threadIdx.x / G * (G * V);
@@ -933,14 +941,18 @@ __global__ void __launch_bounds__(256) SelectTopBackwardKernel(TTopArgs<T> a, TT
     if (row >= a.Rows) {
         return;
     }
-    const uint32_t c = lane * V;
+    const auto classOf = [&](int i) { return (i * G + lane) * N; };
     const bool full = a.Classes == G * V;
-    TValues<T, V> v{};
+    TValues<T, N> v[P]{};
     if (!a.Among) {
-        if (full) {
-            v = TValues<T, V>::Load(a.Scores + row * a.Stride + c);
-        } else if (c < a.Classes) {
-            v = LoadUpTo<T, V>(a.Scores + row * a.Stride + c, a.Classes - c);
+        const T* scores = a.Scores + row * a.Stride;
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            if (full) {
+                v[i] = TValues<T, N>::Load(scores + classOf(i));
+            } else if (classOf(i) < a.Classes) {
+                v[i] = LoadUpTo<T, N>(scores + classOf(i), a.Classes - classOf(i));
+            }
         }
     }
     // (a lane without a slot reads the last one's, so that no load waits for another)
@@ -963,29 +975,41 @@ __global__ void __launch_bounds__(256) SelectTopBackwardKernel(TTopArgs<T> a, TT
     for (int i = 0; i < kept; ++i) {
         part[i] = a.Among ? w[i] * (g[i] - mean) : w[i] * g[i];
     }
-    TValues<A, V> x{};
+    TValues<A, N> x[P]{};
     if (!a.Among) {
         A most = -std::numeric_limits<A>::infinity();
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const A s = static_cast<A>(v.V[j]);
-            x.V[j] = c + j < a.Classes && s == s ? s : -std::numeric_limits<A>::infinity();
-            most = x.V[j] > most ? x.V[j] : most;
+        for (int i = 0; i < P; ++i) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const A s = static_cast<A>(v[i].V[j]);
+                x[i].V[j] = classOf(i) + j < a.Classes && s == s ? s : -std::numeric_limits<A>::infinity();
+                most = x[i].V[j] > most ? x[i].V[j] : most;
+            }
         }
         most = OverGroup<G>(most, [](A y, A z) { return z > y ? z : y; });
         A total = 0;
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            x.V[j] = x.V[j] > -std::numeric_limits<A>::infinity() ? WeightOf(x.V[j], most) : A(0);
-            total += x.V[j];
+        for (int i = 0; i < P; ++i) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                x[i].V[j] = x[i].V[j] > -std::numeric_limits<A>::infinity() ? WeightOf(x[i].V[j], most) : A(0);
+                total += x[i].V[j];
+            }
         }
         total = GroupSum<G>(total);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            x.V[j] = total > 0 ? -(x.V[j] / total) * mean : A(0);
+        for (int i = 0; i < P; ++i) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                x[i].V[j] = total > 0 ? -(x[i].V[j] / total) * mean : A(0);
+            }
         }
     }
-    x.Store(mySums + c);
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+        x[i].Store(mySums + classOf(i));
+    }
     __builtin_amdgcn_wave_barrier();  // a row's lanes are of one wave, whose LDS operations are done in order
 #pragma unroll
     for (int i = 0; i < kept; ++i) {
@@ -994,15 +1018,19 @@ __global__ void __launch_bounds__(256) SelectTopBackwardKernel(TTopArgs<T> a, TT
         }
     }
     __builtin_amdgcn_wave_barrier();
-    x = TValues<A, V>::Load(mySums + c);
+    T* gradients = b.Gradients + row * b.GradientStride;
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-        v.V[j] = static_cast<T>(x.V[j]);
-    }
-    if (full) {
-        v.Store(b.Gradients + row * b.GradientStride + c);
-    } else if (c < a.Classes) {
-        StoreUpTo<T, V>(v, b.Gradients + row * b.GradientStride + c, a.Classes - c);
+    for (int i = 0; i < P; ++i) {
+        x[i] = TValues<A, N>::Load(mySums + classOf(i));
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            v[i].V[j] = static_cast<T>(x[i].V[j]);
+        }
+        if (full) {
+            v[i].Store(gradients + classOf(i));
+        } else if (classOf(i) < a.Classes) {
+            StoreUpTo<T, N>(v[i], gradients + classOf(i), a.Classes - classOf(i));
+        }
     }
 }
 
@@ -1088,7 +1116,8 @@ using namespace op;
 
 namespace {
 
-constexpr size_t kWorkgroupsWanted = 512;     // two for each compute unit
+// One for each compute unit (64 x 50021 32-bit scores 8.1 us, 9.5 where two were wanted; 512 x 2000: 4.4, 5.9 where half were)
+constexpr size_t kWorkgroupsWanted = 256;
 constexpr size_t kTilesPerLaunch = 1u << 21;  // 2^31 threads
 
 }  // namespace
@@ -1195,8 +1224,8 @@ void AdjustScores(int valueType, size_t rows, size_t classes, const void* scores
         using std::integral_constant;
         // Slices of 16384 look through a history least often; the tables of two workgroups of 1024 threads fit a compute unit (and their
         // registers: 64-bit scores would not). Where there are slices in plenty and histories are not long, smaller workgroups with as many
-        // pieces for a thread as it can hold are the better ones, of which more are at different steps at a time (256 x 131000 16-bit scores
-        // with 3000 entries a row: 46 us in slices of 8192, 50 in slices of 16384; with 12000 entries 61 and 60; 64 rows 18 and 17. 9600 x 5000:
+        // pieces for a thread as it can hold are the better ones, of which more are at different steps at a time (256 x 50021 32-bit scores:
+        // 22.6 us in slices of 8192, 26.4 in slices of 16384; 256 x 131000 of 16 bits with 3000 entries a row: 46 us in slices of 8192, 50 in slices of 16384; with 12000 entries 61 and 60; 64 rows 18 and 17. 9600 x 5000:
         // 64 us in two slices with two pieces for a thread, 103 in one with one).
         const bool plenty = rows >= (4 * kWorkgroupsWanted + slices(8192) - 1) / slices(8192) && (!history || p.HistoryCount / rows <= 4096);
         constexpr int most = kPiecesPerThread<T>;
@@ -1241,7 +1270,9 @@ bool WithExactClasses(size_t classes, F&& f, std::integer_sequence<int, C...>) {
 }
 
 // f(lanes of a row, classes of a lane). 1 lane: a thread has a row of exactly so many classes to itself, without branches for
-// others. That reads each line of memory once as long as a row is short, and needs rows enough to fill the chip with threads.
+// others. That reads each line of memory once as long as a row is short, and needs rows enough to fill the chip with threads. 16 lanes
+// as long as their registers hold the row: sums and best ones of a group cost the same for four rows of a wave as for one (131072 rows
+// of 256 32-bit classes, 2 of them selected: 25 us, 42 with 64 lanes; of 64 classes 12 and 33).
 template <typename F>
 void WithShape(size_t classes, size_t rows, int32_t count, const TForThreads& threads, F&& f) {
     using std::integral_constant;

@@ -1,5 +1,6 @@
 """Documents evaluated by models of their own, and the operators on scores and rows around it, against the oracle. Needs an MI355X."""
 import ctypes
+import threading
 
 import numpy as np
 import pytest
@@ -101,6 +102,41 @@ def test_on_a_stream_with_slices_and_no_documents():
     got = routed(models, cb.LAYOUT_FLAT_ROWS, f, docs, ids, None, 1, stream.cuda_stream)
     np.testing.assert_allclose(got, mixed(models, x, 1, ids, None), rtol=1e-9, atol=1e-12)  # the slices' own bar
     cb.eval_routed([m.evaluator() for m, _ in models], f, 0, 1, 0, 0, 0, 0, 0)
+
+
+def test_from_two_threads_at_once():
+    rng = np.random.default_rng(6)
+    models = [model(s, 10, 2) for s in range(3)]
+    docs = 3000
+    x = rng.normal(size=(2, docs, 10)).astype(np.float32)
+    ids = rng.integers(0, 3, size=(2, docs, 2))
+    data = [dev(a) for a in x]
+    features = [cb.DeviceEvaluator.features(cb.LAYOUT_FLAT_ROWS, d.data_ptr(), 10) for d in data]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    evaluators = [m.evaluator() for m, _ in models]
+    size = cb.eval_routed_bytes(evaluators, cb.LAYOUT_FLAT_ROWS, docs, 2)
+    spaces = [torch.empty(size, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    indexes = [dev(i.astype(np.int32)) for i in ids]
+    results = [torch.empty(docs, 2, dtype=torch.float64, device="cuda") for _ in range(2)]
+    torch.cuda.synchronize()
+    failures = []
+
+    def work(i):
+        try:
+            for _ in range(10):
+                cb.eval_routed(evaluators, features[i], docs, 2, indexes[i].data_ptr(), 0, results[i].data_ptr(), spaces[i].data_ptr(), size,
+                               streams[i].cuda_stream)
+        except Exception as e:
+            failures.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures
+    for i in range(2):
+        np.testing.assert_array_equal(results[i].cpu().numpy(), mixed(models, x[i], 2, ids[i], None))
 
 
 def test_refusals():

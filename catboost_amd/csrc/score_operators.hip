@@ -52,6 +52,26 @@ __device__ __forceinline__ void CountEntry(uint32_t* word, bool given) {
     }
 }
 
+// N words of a table, and whether any is not 0
+template <int N>
+struct TWords : TValues<uint32_t, N> {
+    uint32_t Any = 0;
+
+    __device__ __forceinline__ TWords() {}
+    __device__ __forceinline__ explicit TWords(const uint32_t* words) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            this->V[i] = words[i];
+            Any |= words[i];
+        }
+    }
+};
+
+// A row of up to this many biases needs no table of them: the word of a class that has one names it in its upper bits, if the
+// history is short enough for its counts to leave those free (64 x 131000 16-bit scores with 20 biases a row 13.5 us, with a table 16)
+constexpr uint32_t kNamedBiases = 1024, kNameShift = 21;
+constexpr int64_t kNamedHistory = int64_t(1) << (kNameShift - 2);
+
 // Four entries of a list of `count` from entry e on
 __device__ __forceinline__ TValues<int32_t, 4> LoadEntries(const int32_t* list, int64_t e, size_t count) {
     return LoadUpTo<int32_t, 4>(list + e, count - static_cast<size_t>(e));
@@ -75,24 +95,18 @@ struct TPiece {
             X[i] = static_cast<A>(v.V[i]);
         }
     }
-    __device__ __forceinline__ void Penalize(const uint32_t* words, const TPenalties& penalties) {
-        uint32_t w[N], any = 0;
+    // (`counts`: the bits of a word that count)
+    __device__ __forceinline__ void Penalize(const TValues<uint32_t, N>& words, const TPenalties& penalties, uint32_t counts = ~0u) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            w[i] = words[i];
-            any |= w[i];
-        }
-        if (any != 0) {
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                if (w[i] != 0) {
-                    const A repetition = penalties.Repetition;
-                    X[i] = X[i] > 0 ? X[i] / repetition : X[i] * repetition;
-                }
-                if (w[i] > 1) {
-                    X[i] -= static_cast<A>(penalties.Frequency) * static_cast<A>(w[i] >> 1);
-                    X[i] -= static_cast<A>(penalties.Presence);
-                }
+            const uint32_t w = words.V[i] & counts;
+            if (w != 0) {
+                const A repetition = penalties.Repetition;
+                X[i] = X[i] > 0 ? X[i] / repetition : X[i] * repetition;
+            }
+            if (w > 1) {
+                X[i] -= static_cast<A>(penalties.Frequency) * static_cast<A>(w >> 1);
+                X[i] -= static_cast<A>(penalties.Presence);
             }
         }
     }
@@ -180,11 +194,11 @@ __device__ __forceinline__ void MakeBiases(uint32_t threads, uint32_t count, con
 
 // A workgroup for a slice of one row, at most P pieces for each of its threads. What it reads is requested at once, as far as its place is
 // known, and without branches, which would wait for one load after the other: the scores, the mask's words, the first
-// entries of the lists; the tables are made while they are on their way. The tables of the history and of the biases take
-// turns in the same LDS, so that two workgroups fit a compute unit. Every slice of a row looks through the row's whole
-// history; slices of a row are alike in length. Memory bounds it when there is much: 384 x 100003 32-bit scores with
-// 12000 entries a row take 80 us (4.1 TB/s); 64 x 131000 of 16 bits with 3000 entries, biases and masks 16, where the steps wait
-// for each other.
+// entries of the lists; the table is made while they are on their way. Its words count the history and name the biases' classes;
+// where that does not fit, the table of the biases has its place afterwards. Two workgroups fit a compute unit either way. Every slice
+// of a row looks through the row's whole history; slices of a row are alike in length. Memory bounds it when there is much: 384 x
+// 100003 32-bit scores with 12000 entries a row take 80 us (4.1 TB/s); 64 x 131000 of 16 bits with 3000 entries, biases and masks 14,
+// where the steps wait for each other.
 template <typename T, int P, bool BIASES>
 __global__ void __launch_bounds__(1024) AdjustSliceKernel(TAdjustArgs a) {
     const uint32_t threads = blockDim.x;
@@ -193,6 +207,7 @@ __global__ void __launch_bounds__(1024) AdjustSliceKernel(TAdjustArgs a) {
     const CbHipScoreAdjustment& p = a.A;
     const bool history = p.HistoryOffsets != nullptr;
     uint32_t* words = reinterpret_cast<uint32_t*>(tables);
+    float* biasValues = reinterpret_cast<float*>(words + a.SliceClasses);
     const auto clear = [&] {
         for (uint32_t i = threadIdx.x; i < a.SliceClasses / 4; i += threads) {
             tables[i] = uint4{0, 0, 0, 0};
@@ -249,13 +264,27 @@ __global__ void __launch_bounds__(1024) AdjustSliceKernel(TAdjustArgs a) {
         biasClass = p.BiasClasses[firstBias + threadIdx.x];
         biasValue = p.BiasValues[firstBias + threadIdx.x];
     }
-    if (history) {
+    const bool few = BIASES && endBias - firstBias <= kNamedBiases && end - begin < kNamedHistory;
+    const uint32_t named = few ? static_cast<uint32_t>(endBias - firstBias) : 0;
+    const bool table = history || named > 0;
+    if (table) {
         int64_t e = begin + threadIdx.x * 4;
         TValues<int32_t, 4> entries{};
         if (e < end) {
             entries = LoadEntries(p.History, e, p.HistoryCount);
         }
         clear();
+        if (named > 0) {
+            for (uint32_t i = threadIdx.x; i < named; i += threads) {
+                const bool first = i == threadIdx.x;
+                const uint32_t c = static_cast<uint32_t>(first ? biasClass : p.BiasClasses[firstBias + i]) - c0;
+                if (c < width) {
+                    atomicMax(&words[c], 1u << 31 | i << kNameShift);  // the last one of a class stays
+                }
+                biasValues[i] = first ? biasValue : p.BiasValues[firstBias + i];
+            }
+            __syncthreads();
+        }
         while (e < end) {
             const int64_t next = e + threads * 4;
             TValues<int32_t, 4> more{};
@@ -304,17 +333,29 @@ __global__ void __launch_bounds__(1024) AdjustSliceKernel(TAdjustArgs a) {
     for (int j = 0; j < P; ++j) {
         const uint32_t c = (j * threads + threadIdx.x) * N;
         x[j].From(raw[j]);
-        if (history && c < width) {
-            x[j].Penalize(words + c, penalties);
+        TWords<N> w;
+        if (table && c < width) {
+            w = TWords<N>(words + c);
+            if (w.Any != 0) {
+                x[j].Penalize(w, penalties, few ? (1u << kNameShift) - 1 : ~0u);
+            }
         }
         if (p.ClassBias != nullptr) {
             x[j].Add(classBias[j]);
         }
-        if (!BIASES) {
+        if (BIASES && named > 0 && w.Any >> 31 != 0) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                if (w.V[i] >> 31 != 0) {
+                    x[j].X[i] += biasValues[w.V[i] >> kNameShift & (kNamedBiases - 1)];
+                }
+            }
+        }
+        if (!BIASES || few) {
             store(j, x[j]);
         }
     }
-    if (BIASES) {
+    if (BIASES && !few) {
         if (history) {
             __syncthreads();  // the history's words are read
         }
@@ -502,7 +543,10 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof
         const uint32_t q = j * 256 + threadIdx.x, r = rowOf(q);
         x[j].From(raw[j]);
         if (history && r < rows) {
-            x[j].Penalize(words + q * N, penalties[r]);
+            const TWords<N> w(words + q * N);
+            if (w.Any != 0) {
+                x[j].Penalize(w, penalties[r]);
+            }
         }
         if (p.ClassBias != nullptr) {
             x[j].Add(classBias[j]);
@@ -1210,11 +1254,15 @@ void AdjustScores(int valueType, size_t rows, size_t classes, const void* scores
             // 85 us with 1024 threads, 89 with 896; 1411 of 17000 with 50: 48 with 1024, 44 with 576)
             const bool longHistory = history && p.HistoryCount / rows > a.SliceClasses / 2;
             const uint32_t threads = longHistory ? size / (P * N) : ((a.SliceClasses + P * N - 1) / (P * N) + 63) / 64 * 64;
-            const size_t lds = history || biases ? a.SliceClasses * 4 : 0;
+            const size_t lds = (history || biases ? a.SliceClasses * 4 : 0) + (biases ? kNamedBiases * 4 : 0);
+            const auto launchSlices = [&](auto kernel) {
+                call.AllowLds(reinterpret_cast<const void*>(kernel), lds);
+                launchTiles(kernel, rows * a.Slices, threads, lds);
+            };
             if (biases) {
-                launchTiles(AdjustSliceKernel<T, P, true>, rows * a.Slices, threads, lds);
+                launchSlices(AdjustSliceKernel<T, P, true>);
             } else {
-                launchTiles(AdjustSliceKernel<T, P, false>, rows * a.Slices, threads, lds);
+                launchSlices(AdjustSliceKernel<T, P, false>);
             }
         };
         // the longest slices that a row fills at least half of one of and of which there are workgroups enough

@@ -229,6 +229,53 @@ def test_adjust_scores_with_many_biases(classes):
 
 
 @ALL
+@pytest.mark.parametrize("classes", [2048, 5003, 40_001])
+@pytest.mark.parametrize("with_history", [False, True])
+def test_adjust_scores_with_named_biases_or_a_table(kind, classes, with_history):
+    """Up to 1024 biases of a row are named: rows around that many, classes next to each other and the same ones again."""
+    rng = np.random.default_rng(classes)
+    lengths = np.array([64, 1025, 0, 1023, 1, 1024, 200, 2])
+    rows = len(lengths)
+    offsets = np.concatenate([[0], np.cumsum(lengths)]).astype(np.int64)
+    ids = (rng.choice([0, 1000, 2040, classes - 12], offsets[-1]) + rng.integers(0, 12, offsets[-1])).astype(np.int32)
+    ids[rng.random(len(ids)) < 0.1] = -1
+    ids[rng.random(len(ids)) < 0.1] = classes
+    p = dict(bias_offsets=offsets, bias_classes=ids, bias_values=(rng.normal(size=offsets[-1]) * 4).astype(np.float32))
+    if with_history:
+        p.update(offsets=np.arange(rows + 1) * 30, ids=rng.integers(0, classes, 30 * rows).astype(np.int32), presence=np.full(rows, 0.5, np.float32))
+    scores = table(rng.normal(size=(rows, classes)), kind, classes % 2)
+    a = Adjustment(p)
+    result = torch.empty(rows, classes, dtype=TYPES[kind], device="cuda")
+    cb.adjust_scores(kind, rows, classes, scores.data_ptr(), scores.stride(0), a.struct, result.data_ptr(), classes)
+    expected, size = adjusted(exactly(scores), p)
+    compare(exactly(result), expected, 8 * u(kind) * size, kind)
+
+
+def test_adjust_scores_with_a_history_too_long_for_named_biases():
+    """Some 2^19 entries, the most that leave room for names, and one more; counted exactly, with a few biases beside them."""
+    classes = 5000
+    rng = np.random.default_rng(4)
+    lengths = np.array([(1 << 19) - 1, 1 << 19, 3])
+    offsets = np.concatenate([[0], np.cumsum(lengths)]).astype(np.int64)
+    ids = rng.integers(0, classes, offsets[-1]).astype(np.int32)
+    ids[:(1 << 19) - 1] = 7  # the largest count that a word with a name holds
+    bias_ids = np.array([7, 8, 7, 4999, 8, 7, 0, 7], np.int32)
+    values = np.array([9, 9, 1 / 4, -1, 2, 1 / 2, 3, 1], np.float32)
+    p = dict(offsets=offsets, ids=ids, frequency=np.full(3, 2.0 ** -6, np.float32), bias_offsets=np.array([0, 3, 6, 8]), bias_classes=bias_ids, bias_values=values)
+    a = Adjustment(p)
+    scores = torch.zeros(3, classes, device="cuda")
+    result = torch.empty_like(scores)
+    cb.adjust_scores(cb.FLOAT32, 3, classes, scores.data_ptr(), classes, a.struct, result.data_ptr(), classes)
+    expected = np.zeros((3, classes))
+    for r in range(3):
+        expected[r] -= np.bincount(ids[offsets[r]:offsets[r + 1]], minlength=classes) * 2.0 ** -6
+        for c in {7, 8, 4999, 0}:
+            at = [e for e in range(p["bias_offsets"][r], p["bias_offsets"][r + 1]) if bias_ids[e] == c]
+            expected[r, c] += values[at[-1]] if at else 0
+    np.testing.assert_array_equal(result.cpu().numpy(), expected.astype(np.float32))  # every sum has few enough bits
+
+
+@ALL
 def test_adjust_scores_of_infinite_and_undefined_values(kind):
     rng = np.random.default_rng(5)
     rows, classes = 6, 5001

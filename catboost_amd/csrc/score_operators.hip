@@ -16,7 +16,7 @@ struct TAdjustArgs {
     size_t ScoreStride, ResultStride;
     size_t Rows, FirstTile;
     uint32_t Classes, Slices, SliceClasses;       // of AdjustSliceKernel
-    uint32_t RowsPerTile, Pieces, PiecesInverse;  // of AdjustRowsKernel
+    uint32_t RowsPerTile, Pieces, PiecesInverse, RowLanesLog2;  // of AdjustRowsKernel
     CbHipScoreAdjustment A;
 };
 
@@ -67,15 +67,15 @@ struct TWords : TValues<uint32_t, N> {
     }
 };
 
-// A row of up to this many biases needs no table of them: the word of a class that has one names it in its upper bits, if the
-// history is short enough for its counts to leave those free (64 x 131000 16-bit scores with 20 biases a row 13.5 us, with a table 16)
-constexpr uint32_t kNamedBiases = 1024, kNameShift = 21;
-constexpr int64_t kNamedHistory = int64_t(1) << (kNameShift - 2);
-
 // Four entries of a list of `count` from entry e on
 __device__ __forceinline__ TValues<int32_t, 4> LoadEntries(const int32_t* list, int64_t e, size_t count) {
     return LoadUpTo<int32_t, 4>(list + e, count - static_cast<size_t>(e));
 }
+
+// A row of up to this many biases needs no table of them: the word of a class that has one names it in its upper bits, if the
+// history is short enough for its counts to leave those free (64 x 131000 16-bit scores with 20 biases a row 13.5 us, with a table 16)
+constexpr uint32_t kNamedBiases = 1024, kNameShift = 21;
+constexpr int64_t kNamedHistory = int64_t(1) << (kNameShift - 2);
 
 // 16 bytes of scores as they are in memory. (As single 16-bit values they would take a register each.)
 using TRaw = TValues<uint32_t, 4>;
@@ -114,6 +114,14 @@ struct TPiece {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             X[i] += bias.V[i];
+        }
+    }
+    __device__ __forceinline__ void AddNamed(const TValues<uint32_t, N>& words, const float* biasValues) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if (words.V[i] >> 31 != 0) {
+                X[i] += biasValues[words.V[i] >> kNameShift & (kNamedBiases - 1)];
+            }
         }
     }
     // (0 where there is none)
@@ -344,12 +352,7 @@ __global__ void __launch_bounds__(1024) AdjustSliceKernel(TAdjustArgs a) {
             x[j].Add(classBias[j]);
         }
         if (BIASES && named > 0 && w.Any >> 31 != 0) {
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                if (w.V[i] >> 31 != 0) {
-                    x[j].X[i] += biasValues[w.V[i] >> kNameShift & (kNamedBiases - 1)];
-                }
-            }
+            x[j].AddNamed(w, biasValues);
         }
         if (!BIASES || few) {
             store(j, x[j]);
@@ -418,8 +421,10 @@ __device__ __forceinline__ void ForEntries(const int64_t* offsets, uint32_t rows
 
 // Rows that are shorter than a slice: a workgroup for RowsPerTile of them, P pieces for a thread. Pieces are taken in the
 // order in which they are in memory, whatever the rows' length, so that a wave's stores fill whole lines (a thread for a
-// row, at ten 64-bit values each, wrote 413 MB for 160). What is read is requested first, as in the kernel above. Memory bounds it:
-// 2M x 10 64-bit scores with histories, biases of classes and masks take 88 us (4.6 TB/s).
+// row, at ten 64-bit values each, wrote 413 MB for 160). What is read is requested first, as in the kernel above. A row's first entries
+// are counted by lanes of its own, which know whose they are; a search for the row of each (all threads of the tile, as for what is
+// left of long histories) took 73 us for 2M x 10 32-bit scores and these 65. Memory bounds it: 2M x 10 64-bit scores with histories,
+// biases of classes and masks take 88 us (4.6 TB/s).
 template <typename T>
 constexpr int kPiecesPerThread = sizeof(T) == 2 ? 2 : 4;  // 16 scores on their way, 8 of 64 bits
 
@@ -429,19 +434,22 @@ enum ERests {
     kLessThanOne,   // the only piece of a row has
 };
 
-// (64 registers, for eight waves a SIMD: 2M x 10 64-bit scores take 90 us, 94 with the 66 that the compiler chose. Where that
-// spills a dozen, 23391 x 513 of 64 bits took 67 us, 60 with 72 registers.)
-template <typename T, int RESTS, bool BIASES>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 8 && RESTS == kRests ? 7 : 8))) AdjustRowsKernel(TAdjustArgs a) {
+// (Eight waves a SIMD, seven where the 64 registers of those would spill: 2M x 10 32-bit scores 64 us, 76 with eight. Kernels with and
+// without histories: 2M x 10 64-bit scores without one 60 us, 74 by a kernel of both.)
+template <typename T, int RESTS, bool HISTORY, bool BIASES>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) > 2 && HISTORY ? 7 : 8))) AdjustRowsKernel(TAdjustArgs a) {
     constexpr int N = 16 / sizeof(T), P = kPiecesPerThread<T>;
     extern __shared__ uint4 tables[];
     const CbHipScoreAdjustment& p = a.A;
-    const bool history = p.HistoryOffsets != nullptr;
+    constexpr bool history = HISTORY;
     const uint32_t pitch = a.Pieces * N;
     TPenalties* penalties = reinterpret_cast<TPenalties*>(tables);
     int64_t* offsets = reinterpret_cast<int64_t*>(penalties + (history ? a.RowsPerTile : 0));
-    int64_t* given = offsets + (history || BIASES ? a.RowsPerTile : 0);  // where the generated entries begin
-    uint32_t* words = reinterpret_cast<uint32_t*>(given + (history ? a.RowsPerTile : 0));
+    int64_t* given = offsets + (history ? a.RowsPerTile : 0);  // where the generated entries begin
+    int64_t* biasOffsets = given + (history ? a.RowsPerTile : 0);
+    uint32_t* more = reinterpret_cast<uint32_t*>(biasOffsets + (BIASES ? a.RowsPerTile : 0));  // a row has a longer history
+    float* biasValues = reinterpret_cast<float*>(more + 1);
+    uint32_t* words = reinterpret_cast<uint32_t*>(biasValues + (BIASES ? kNamedBiases : 0));
     const auto rowOf = [&](uint32_t q) { return a.PiecesInverse != 0 ? __umulhi(q, a.PiecesInverse) : q; };
     const size_t tile = a.FirstTile + blockIdx.x;
     const size_t r0 = tile * a.RowsPerTile;
@@ -452,6 +460,24 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof
         }
     };
     int64_t begin = 0, end = 0, firstBias = 0, endBias = 0;
+    // a row's first entries are counted by lanes of its own, which know whose they are: this thread's row, where its history begins, how long it
+    // is and how much of it is given
+    const uint32_t rowLanes = 1u << a.RowLanesLog2, myRow = threadIdx.x >> a.RowLanesLog2, myLane = threadIdx.x & (rowLanes - 1);
+    int64_t myBegin = 0;
+    int32_t myLength = 0, myGiven = 0;
+    const auto loadOffsets = [&](uint32_t i) {
+        const size_t r = r0 + min(i, rows - 1);
+        const int64_t first = p.HistoryOffsets[r];
+        myBegin = Clamped(first, p.HistoryCount);
+        myLength = static_cast<int32_t>(Clamped(p.HistoryOffsets[r + 1], p.HistoryCount) - myBegin);
+        const int64_t end = first + (p.PromptLengths != nullptr ? p.PromptLengths[r] : 0);
+        myGiven = static_cast<int32_t>(max(min(end - myBegin, int64_t(0x7fffffff)), int64_t(0)));
+        if (myLane == 0 && i < rows) {
+            offsets[i] = myBegin;
+            given[i] = end;
+            penalties[i] = TPenalties::Of(p, r);
+        }
+    };
     if (history) {
         begin = Clamped(p.HistoryOffsets[r0], p.HistoryCount);
         end = Clamped(p.HistoryOffsets[r0 + rows], p.HistoryCount);
@@ -496,24 +522,75 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof
         biasClass = p.BiasClasses[firstBias + threadIdx.x];
         biasValue = p.BiasValues[firstBias + threadIdx.x];
     }
-    if (history) {
+    const bool few = BIASES && endBias - firstBias <= kNamedBiases && end - begin < kNamedHistory;
+    const uint32_t named = few ? static_cast<uint32_t>(endBias - firstBias) : 0;
+    const bool table = history || named > 0;
+    if (table) {
         TValues<int32_t, 4> entries{};
-        if (begin + threadIdx.x * 4 < end) {
-            entries = LoadEntries(p.History, begin + threadIdx.x * 4, p.HistoryCount);
+        const auto loadEntries = [&](uint32_t i) {
+            if (i < rows && static_cast<int32_t>(myLane * 4) < myLength) {
+                entries = LoadEntries(p.History, myBegin + myLane * 4, p.HistoryCount);
+            }
+        };
+        if (history) {
+            loadOffsets(myRow);
+            loadEntries(myRow);
         }
         clear();
-        for (uint32_t i = threadIdx.x; i < rows; i += 256) {
-            offsets[i] = p.HistoryOffsets[r0 + i];
-            given[i] = offsets[i] + (p.PromptLengths != nullptr ? p.PromptLengths[r0 + i] : 0);
-            penalties[i] = TPenalties::Of(p, r0 + i);
+        if (threadIdx.x == 0) {
+            *more = 0;
+        }
+        if (BIASES) {
+            for (uint32_t i = threadIdx.x; i < rows; i += 256) {
+                biasOffsets[i] = p.BiasOffsets[r0 + i];
+            }
         }
         __syncthreads();
-        ForEntries(offsets, rows, begin, end, p.History, p.HistoryCount, entries, [&](int64_t e, uint32_t i, uint32_t c) {
-            if (c < a.Classes) {
-                CountEntry(&words[i * pitch + c], e < given[i]);
+        if (named > 0) {
+            for (uint32_t i = threadIdx.x; i < named; i += 256) {
+                const bool first = i == threadIdx.x;
+                const uint32_t c = static_cast<uint32_t>(first ? biasClass : p.BiasClasses[firstBias + i]);
+                if (c < a.Classes) {
+                    // the last one of a class stays
+                    atomicMax(&words[RowOfEntry(biasOffsets, rows, firstBias + i) * pitch + c], 1u << 31 | i << kNameShift);
+                }
+                biasValues[i] = first ? biasValue : p.BiasValues[firstBias + i];
             }
-        });
-        __syncthreads();
+            __syncthreads();
+        }
+        if (history) {
+            for (uint32_t i = myRow; i < rows; i += 256 >> a.RowLanesLog2) {
+                if (i != myRow) {
+                    loadOffsets(i);
+                    loadEntries(i);
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int32_t e = myLane * 4 + k;
+                    const uint32_t c = static_cast<uint32_t>(entries.V[k]);
+                    if (e < myLength && c < a.Classes) {
+                        CountEntry(&words[i * pitch + c], e < myGiven);
+                    }
+                }
+                if (myLength > static_cast<int32_t>(4 * rowLanes)) {
+                    *more = 1;
+                }
+            }
+            __syncthreads();
+            if (*more != 0) {
+                // the others by all threads
+                TValues<int32_t, 4> four{};
+                if (begin + threadIdx.x * 4 < end) {
+                    four = LoadEntries(p.History, begin + threadIdx.x * 4, p.HistoryCount);
+                }
+                ForEntries(offsets, rows, begin, end, p.History, p.HistoryCount, four, [&](int64_t e, uint32_t i, uint32_t c) {
+                    if (c < a.Classes && e - offsets[i] >= 4 * rowLanes) {
+                        CountEntry(&words[i * pitch + c], e < given[i]);
+                    }
+                });
+                __syncthreads();
+            }
+        }
     }
     TValues<float, N> classBias[P];
     if (p.ClassBias != nullptr) {
@@ -542,32 +619,37 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof
     for (int j = 0; j < P; ++j) {
         const uint32_t q = j * 256 + threadIdx.x, r = rowOf(q);
         x[j].From(raw[j]);
-        if (history && r < rows) {
-            const TWords<N> w(words + q * N);
-            if (w.Any != 0) {
-                x[j].Penalize(w, penalties[r]);
+        TWords<N> w;
+        if (table && r < rows) {
+            w = TWords<N>(words + q * N);
+            if (history && w.Any != 0) {
+                x[j].Penalize(w, penalties[r], few ? (1u << kNameShift) - 1 : ~0u);
             }
         }
         if (p.ClassBias != nullptr) {
             x[j].Add(classBias[j]);
         }
-        if (!BIASES) {
+        if (BIASES && named > 0 && w.Any >> 31 != 0) {
+            x[j].AddNamed(w, biasValues);
+        }
+        if (!BIASES || few) {
             store(j, x[j]);
         }
     }
-    if (BIASES) {
+    if (BIASES && !few) {
         if (history) {
-            __syncthreads();  // the history's words and offsets are read
+            __syncthreads();  // the history's words are read
+        } else {
+            for (uint32_t i = threadIdx.x; i < rows; i += 256) {
+                biasOffsets[i] = p.BiasOffsets[r0 + i];
+            }
         }
         clear();
-        for (uint32_t i = threadIdx.x; i < rows; i += 256) {
-            offsets[i] = p.BiasOffsets[r0 + i];
-        }
         __syncthreads();
         MakeBiases(256, static_cast<uint32_t>(endBias - firstBias), p.BiasClasses + firstBias, p.BiasValues + firstBias, biasClass, biasValue,
                         [&](uint32_t i, int32_t entry) {
                             const uint32_t c = static_cast<uint32_t>(entry);
-                            return c < a.Classes ? &words[RowOfEntry(offsets, rows, firstBias + i) * pitch + c] : nullptr;
+                            return c < a.Classes ? &words[RowOfEntry(biasOffsets, rows, firstBias + i) * pitch + c] : nullptr;
                         });
 #pragma unroll
         for (int j = 0; j < P; ++j) {
@@ -1221,18 +1303,22 @@ void AdjustScores(int valueType, size_t rows, size_t classes, const void* scores
             // q / pieces is under the next integer by 1 / pieces at least, which is more for the q and pieces under 2^11 here
             a.PiecesInverse = pieces > 1 ? static_cast<uint32_t>((uint64_t(1) << 32) / pieces + 1) : 0;
             const size_t tiles = (rows + a.RowsPerTile - 1) / a.RowsPerTile;
-            const size_t perRow = (history ? sizeof(TPenalties) + 16 : biases ? 8 : 0) + (history || biases ? size_t(pieces) * N * 4 : 0);
-            const size_t lds = a.RowsPerTile * perRow;
+            const size_t perRow = (history ? sizeof(TPenalties) + 16 : 0) + (biases ? 8 : 0) + (history || biases ? size_t(pieces) * N * 4 : 0);
+            const size_t lds = history || biases ? a.RowsPerTile * perRow + 4 + (biases ? kNamedBiases * 4 : 0) : 0;
+            a.RowLanesLog2 = 0;
+            while ((a.RowsPerTile << (a.RowLanesLog2 + 1)) <= 256) {
+                ++a.RowLanesLog2;
+            }
             const auto launch = [&](auto kernel) {
                 call.AllowLds(reinterpret_cast<const void*>(kernel), lds);
                 launchTiles(kernel, tiles, 256, lds);
             };
             const auto withBiases = [&](auto rests) {
                 constexpr int RESTS = decltype(rests)::value;
-                if (biases) {
-                    launch(AdjustRowsKernel<T, RESTS, true>);
+                if (history) {
+                    biases ? launch(AdjustRowsKernel<T, RESTS, true, true>) : launch(AdjustRowsKernel<T, RESTS, true, false>);
                 } else {
-                    launch(AdjustRowsKernel<T, RESTS, false>);
+                    biases ? launch(AdjustRowsKernel<T, RESTS, false, true>) : launch(AdjustRowsKernel<T, RESTS, false, false>);
                 }
             };
             if (a.Classes % N == 0) {

@@ -251,15 +251,15 @@ def test_adjust_scores_with_named_biases_or_a_table(kind, classes, with_history)
     compare(exactly(result), expected, 8 * u(kind) * size, kind)
 
 
-def test_adjust_scores_with_a_history_too_long_for_named_biases():
+@pytest.mark.parametrize("classes", [60, 5000])
+def test_adjust_scores_with_a_history_too_long_for_named_biases(classes):
     """Some 2^19 entries, the most that leave room for names, and one more; counted exactly, with a few biases beside them."""
-    classes = 5000
     rng = np.random.default_rng(4)
     lengths = np.array([(1 << 19) - 1, 1 << 19, 3])
     offsets = np.concatenate([[0], np.cumsum(lengths)]).astype(np.int64)
     ids = rng.integers(0, classes, offsets[-1]).astype(np.int32)
     ids[:(1 << 19) - 1] = 7  # the largest count that a word with a name holds
-    bias_ids = np.array([7, 8, 7, 4999, 8, 7, 0, 7], np.int32)
+    bias_ids = np.array([7, 8, 7, classes - 1, 8, 7, 0, 7], np.int32)
     values = np.array([9, 9, 1 / 4, -1, 2, 1 / 2, 3, 1], np.float32)
     p = dict(offsets=offsets, ids=ids, frequency=np.full(3, 2.0 ** -6, np.float32), bias_offsets=np.array([0, 3, 6, 8]), bias_classes=bias_ids, bias_values=values)
     a = Adjustment(p)
@@ -269,10 +269,31 @@ def test_adjust_scores_with_a_history_too_long_for_named_biases():
     expected = np.zeros((3, classes))
     for r in range(3):
         expected[r] -= np.bincount(ids[offsets[r]:offsets[r + 1]], minlength=classes) * 2.0 ** -6
-        for c in {7, 8, 4999, 0}:
+        for c in {7, 8, classes - 1, 0}:
             at = [e for e in range(p["bias_offsets"][r], p["bias_offsets"][r + 1]) if bias_ids[e] == c]
             expected[r, c] += values[at[-1]] if at else 0
     np.testing.assert_array_equal(result.cpu().numpy(), expected.astype(np.float32))  # every sum has few enough bits
+    result.fill_(5)
+    cb.adjust_scores(cb.FLOAT32, 1, classes, scores.data_ptr(), classes, a.struct, result.data_ptr(), classes)
+    np.testing.assert_array_equal(result[:1].cpu().numpy(), expected[:1].astype(np.float32))
+
+
+@ALL
+@pytest.mark.parametrize("rows,classes,most,biases", [(3000, 1, 3, 0), (3000, 1, 3, 3), (700, 2, 9, 4), (64, 40, 2, 3), (64, 40, 30, 30), (5, 7, 700, 300), (300, 9, 40, 2), (1, 10, 5000, 900),
+                                                      (1, 10, 30, 2000), (33, 64, 65, 33)])
+def test_adjust_scores_of_short_rows_with_histories_and_biases_of_all_lengths(kind, rows, classes, most, biases):
+    """A row's own lanes count up to four entries each, all threads of the tile the others; more biases than names."""
+    rng = np.random.default_rng(rows + classes + most)
+    p = parts(rng, rows, classes, "hpfrs", most)
+    if biases:
+        p["bias_offsets"], p["bias_classes"] = history(rng, rows, classes, biases)
+        p["bias_values"] = rng.normal(size=len(p["bias_classes"])).astype(np.float32)
+    scores = table(rng.normal(size=(rows, classes)), kind)
+    a = Adjustment(p)
+    result = torch.empty_like(scores)
+    cb.adjust_scores(kind, rows, classes, scores.data_ptr(), classes, a.struct, result.data_ptr(), classes)
+    expected, big = adjusted(exactly(scores), p)
+    compare(exactly(result), expected, 6.01 * u(kind) * big, kind)
 
 
 @ALL

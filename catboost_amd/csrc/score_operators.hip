@@ -52,18 +52,23 @@ __device__ __forceinline__ void CountEntry(uint32_t* word, bool given) {
     }
 }
 
-// N words of a table, and whether any is not 0
+// The N words of a piece in a table, which begins at a multiple of 16 bytes, and whether any is not 0
 template <int N>
 struct TWords : TValues<uint32_t, N> {
     uint32_t Any = 0;
+    static constexpr int Alignment = N * 4 < 16 ? N * 4 : 16;
 
     __device__ __forceinline__ TWords() {}
     __device__ __forceinline__ explicit TWords(const uint32_t* words) {
+        __builtin_memcpy(this->V, __builtin_assume_aligned(words, Alignment), sizeof(this->V));
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            this->V[i] = words[i];
-            Any |= words[i];
+            Any |= this->V[i];
         }
+    }
+    __device__ __forceinline__ static void Clear(uint32_t* words) {
+        const TValues<uint32_t, N> none{};
+        __builtin_memcpy(__builtin_assume_aligned(words, Alignment), &none, sizeof(none));
     }
 };
 
@@ -446,17 +451,17 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof
     TPenalties* penalties = reinterpret_cast<TPenalties*>(tables);
     int64_t* offsets = reinterpret_cast<int64_t*>(penalties + (history ? a.RowsPerTile : 0));
     int64_t* given = offsets + (history ? a.RowsPerTile : 0);  // where the generated entries begin
-    int64_t* biasOffsets = given + (history ? a.RowsPerTile : 0);
-    uint32_t* more = reinterpret_cast<uint32_t*>(biasOffsets + (BIASES ? a.RowsPerTile : 0));  // a row has a longer history
-    float* biasValues = reinterpret_cast<float*>(more + 1);
-    uint32_t* words = reinterpret_cast<uint32_t*>(biasValues + (BIASES ? kNamedBiases : 0));
+    uint32_t* words = reinterpret_cast<uint32_t*>(given + (history ? a.RowsPerTile : 0));
+    int64_t* biasOffsets = reinterpret_cast<int64_t*>(words + a.RowsPerTile * pitch);  // (pieces have an even number of values)
+    float* biasValues = reinterpret_cast<float*>(biasOffsets + (BIASES ? a.RowsPerTile : 0));
+    uint32_t* more = reinterpret_cast<uint32_t*>(biasValues + (BIASES ? kNamedBiases : 0));  // a row has a longer history
     const auto rowOf = [&](uint32_t q) { return a.PiecesInverse != 0 ? __umulhi(q, a.PiecesInverse) : q; };
     const size_t tile = a.FirstTile + blockIdx.x;
     const size_t r0 = tile * a.RowsPerTile;
     const uint32_t rows = static_cast<uint32_t>(a.Rows - r0 < a.RowsPerTile ? a.Rows - r0 : a.RowsPerTile);
     const auto clear = [&] {
-        for (uint32_t i = threadIdx.x; i < rows * pitch; i += 256) {
-            words[i] = 0;
+        for (uint32_t i = threadIdx.x; i < rows * a.Pieces; i += 256) {
+            TWords<N>::Clear(words + i * N);
         }
     };
     int64_t begin = 0, end = 0, firstBias = 0, endBias = 0;

@@ -385,7 +385,8 @@ __global__ void __launch_bounds__(1024) AdjustSliceKernel(TAdjustArgs a) {
 }
 
 // The row that entry `e` of a list with these offsets belongs to: the last one that begins at or before it
-__device__ __forceinline__ uint32_t RowOfEntry(const int64_t* offsets, uint32_t rows, int64_t e) {
+template <typename TOffset>
+__device__ __forceinline__ uint32_t RowOfEntry(const TOffset* offsets, uint32_t rows, TOffset e) {
     uint32_t low = 0, high = rows;
     while (high - low > 1) {
         const uint32_t middle = (low + high) / 2;
@@ -448,11 +449,12 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof
     const CbHipScoreAdjustment& p = a.A;
     constexpr bool history = HISTORY;
     const uint32_t pitch = a.Pieces * N;
-    TPenalties* penalties = reinterpret_cast<TPenalties*>(tables);
+    // (in the order of their alignments: a piece's words, 8 bytes, 4)
+    uint32_t* words = reinterpret_cast<uint32_t*>(tables);
+    TPenalties* penalties = reinterpret_cast<TPenalties*>(words + a.RowsPerTile * pitch);
     int64_t* offsets = reinterpret_cast<int64_t*>(penalties + (history ? a.RowsPerTile : 0));
-    int64_t* given = offsets + (history ? a.RowsPerTile : 0);  // where the generated entries begin
-    uint32_t* words = reinterpret_cast<uint32_t*>(given + (history ? a.RowsPerTile : 0));
-    int64_t* biasOffsets = reinterpret_cast<int64_t*>(words + a.RowsPerTile * pitch);  // (pieces have an even number of values)
+    int32_t* given = reinterpret_cast<int32_t*>(offsets + (history ? a.RowsPerTile : 0));  // how many of a row's entries are
+    uint32_t* biasOffsets = reinterpret_cast<uint32_t*>(given + (history ? a.RowsPerTile : 0));  // from the tile's first on
     float* biasValues = reinterpret_cast<float*>(biasOffsets + (BIASES ? a.RowsPerTile : 0));
     uint32_t* more = reinterpret_cast<uint32_t*>(biasValues + (BIASES ? kNamedBiases : 0));  // a row has a longer history
     const auto rowOf = [&](uint32_t q) { return a.PiecesInverse != 0 ? __umulhi(q, a.PiecesInverse) : q; };
@@ -479,7 +481,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof
         myGiven = static_cast<int32_t>(max(min(end - myBegin, int64_t(0x7fffffff)), int64_t(0)));
         if (myLane == 0 && i < rows) {
             offsets[i] = myBegin;
-            given[i] = end;
+            given[i] = myGiven;
             penalties[i] = TPenalties::Of(p, r);
         }
     };
@@ -527,6 +529,11 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof
         biasClass = p.BiasClasses[firstBias + threadIdx.x];
         biasValue = p.BiasValues[firstBias + threadIdx.x];
     }
+    const auto loadBiasOffsets = [&] {
+        for (uint32_t i = threadIdx.x; i < rows; i += 256) {
+            biasOffsets[i] = static_cast<uint32_t>(max(Clamped(p.BiasOffsets[r0 + i], p.BiasCount) - firstBias, int64_t(0)));
+        }
+    };
     const bool few = BIASES && endBias - firstBias <= kNamedBiases && end - begin < kNamedHistory;
     const uint32_t named = few ? static_cast<uint32_t>(endBias - firstBias) : 0;
     const bool table = history || named > 0;
@@ -546,9 +553,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof
             *more = 0;
         }
         if (BIASES) {
-            for (uint32_t i = threadIdx.x; i < rows; i += 256) {
-                biasOffsets[i] = p.BiasOffsets[r0 + i];
-            }
+            loadBiasOffsets();
         }
         __syncthreads();
         if (named > 0) {
@@ -557,7 +562,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof
                 const uint32_t c = static_cast<uint32_t>(first ? biasClass : p.BiasClasses[firstBias + i]);
                 if (c < a.Classes) {
                     // the last one of a class stays
-                    atomicMax(&words[RowOfEntry(biasOffsets, rows, firstBias + i) * pitch + c], 1u << 31 | i << kNameShift);
+                    atomicMax(&words[RowOfEntry(biasOffsets, rows, i) * pitch + c], 1u << 31 | i << kNameShift);
                 }
                 biasValues[i] = first ? biasValue : p.BiasValues[firstBias + i];
             }
@@ -590,7 +595,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof
                 }
                 ForEntries(offsets, rows, begin, end, p.History, p.HistoryCount, four, [&](int64_t e, uint32_t i, uint32_t c) {
                     if (c < a.Classes && e - offsets[i] >= 4 * rowLanes) {
-                        CountEntry(&words[i * pitch + c], e < given[i]);
+                        CountEntry(&words[i * pitch + c], e - offsets[i] < given[i]);
                     }
                 });
                 __syncthreads();
@@ -645,16 +650,14 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof
         if (history) {
             __syncthreads();  // the history's words are read
         } else {
-            for (uint32_t i = threadIdx.x; i < rows; i += 256) {
-                biasOffsets[i] = p.BiasOffsets[r0 + i];
-            }
+            loadBiasOffsets();
         }
         clear();
         __syncthreads();
         MakeBiases(256, static_cast<uint32_t>(endBias - firstBias), p.BiasClasses + firstBias, p.BiasValues + firstBias, biasClass, biasValue,
                         [&](uint32_t i, int32_t entry) {
                             const uint32_t c = static_cast<uint32_t>(entry);
-                            return c < a.Classes ? &words[RowOfEntry(biasOffsets, rows, firstBias + i) * pitch + c] : nullptr;
+                            return c < a.Classes ? &words[RowOfEntry(biasOffsets, rows, i) * pitch + c] : nullptr;
                         });
 #pragma unroll
         for (int j = 0; j < P; ++j) {
@@ -1308,7 +1311,7 @@ void AdjustScores(int valueType, size_t rows, size_t classes, const void* scores
             // q / pieces is under the next integer by 1 / pieces at least, which is more for the q and pieces under 2^11 here
             a.PiecesInverse = pieces > 1 ? static_cast<uint32_t>((uint64_t(1) << 32) / pieces + 1) : 0;
             const size_t tiles = (rows + a.RowsPerTile - 1) / a.RowsPerTile;
-            const size_t perRow = (history ? sizeof(TPenalties) + 16 : 0) + (biases ? 8 : 0) + (history || biases ? size_t(pieces) * N * 4 : 0);
+            const size_t perRow = (history ? sizeof(TPenalties) + 12 : 0) + (biases ? 4 : 0) + (history || biases ? size_t(pieces) * N * 4 : 0);
             const size_t lds = history || biases ? a.RowsPerTile * perRow + 4 + (biases ? kNamedBiases * 4 : 0) : 0;
             a.RowLanesLog2 = 0;
             while ((a.RowsPerTile << (a.RowLanesLog2 + 1)) <= 256) {

@@ -210,7 +210,7 @@ __device__ __forceinline__ void MakeBiases(uint32_t threads, uint32_t count, con
 // entries of the lists; the table is made while they are on their way. Its words count the history and name the biases' classes;
 // where that does not fit, the table of the biases has its place afterwards. Two workgroups fit a compute unit either way. Every slice
 // of a row looks through the row's whole history; slices of a row are alike in length. Memory bounds it when there is much: 384 x
-// 100003 32-bit scores with 12000 entries a row take 80 us (4.1 TB/s); 64 x 131000 of 16 bits with 3000 entries, biases and masks 14,
+// 100003 32-bit scores with 12000 entries a row take 80 us (4.1 TB/s); 64 x 131000 of 16 bits with 3000 entries, biases and masks 15,
 // where the steps wait for each other.
 template <typename T, int P, bool BIASES>
 __global__ void __launch_bounds__(1024) AdjustSliceKernel(TAdjustArgs a) {
@@ -429,8 +429,8 @@ __device__ __forceinline__ void ForEntries(const int64_t* offsets, uint32_t rows
 // order in which they are in memory, whatever the rows' length, so that a wave's stores fill whole lines (a thread for a
 // row, at ten 64-bit values each, wrote 413 MB for 160). What is read is requested first, as in the kernel above. A row's first entries
 // are counted by lanes of its own, which know whose they are; a search for the row of each (all threads of the tile, as for what is
-// left of long histories) took 73 us for 2M x 10 32-bit scores and these 65. Memory bounds it: 2M x 10 64-bit scores with histories,
-// biases of classes and masks take 88 us (4.6 TB/s).
+// left of long histories) took 73 us for 2M x 10 32-bit scores where these took 65 (60 with smaller tables). Memory bounds it: 2M x 10 64-bit scores with histories,
+// biases of classes and masks take 83 us (4.8 TB/s).
 template <typename T>
 constexpr int kPiecesPerThread = sizeof(T) == 2 ? 2 : 4;  // 16 scores on their way, 8 of 64 bits
 
@@ -440,7 +440,7 @@ enum ERests {
     kLessThanOne,   // the only piece of a row has
 };
 
-// (Eight waves a SIMD, seven where the 64 registers of those would spill: 2M x 10 32-bit scores 64 us, 76 with eight. Kernels with and
+// (Eight waves a SIMD, seven where the 64 registers of those would spill: 2M x 10 32-bit scores 60 us, with eight 12 more. Kernels with and
 // without histories: 2M x 10 64-bit scores without one 60 us, 74 by a kernel of both.)
 template <typename T, int RESTS, bool HISTORY, bool BIASES>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) > 2 && HISTORY ? 7 : 8))) AdjustRowsKernel(TAdjustArgs a) {

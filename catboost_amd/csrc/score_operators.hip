@@ -82,6 +82,9 @@ __device__ __forceinline__ TValues<int32_t, 4> LoadEntries(const int32_t* list, 
 constexpr uint32_t kNamedBiases = 1024, kNameShift = 21;
 constexpr int64_t kNamedHistory = int64_t(1) << (kNameShift - 2);
 
+// The bits of -0, which changes no score when it is added (0 would make a score of -0 a 0)
+constexpr uint32_t kNoBias = 0x80000000u;
+
 // 16 bytes of scores as they are in memory. (As single 16-bit values they would take a register each.)
 using TRaw = TValues<uint32_t, 4>;
 
@@ -129,11 +132,11 @@ struct TPiece {
             }
         }
     }
-    // (0 where there is none)
-    __device__ __forceinline__ void Add(const uint32_t* biasBits) {
+    // (from a table, see MakeBiases)
+    __device__ __forceinline__ void Add(const uint32_t* words) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            X[i] += __uint_as_float(biasBits[i]);
+            X[i] += __uint_as_float(words[i] ^ kNoBias);
         }
     }
     // a bit of `allowed` for each of them
@@ -176,9 +179,10 @@ __device__ __forceinline__ void StorePiece(const TRaw& raw, T* at, uint32_t n) {
     StoreUpTo<T, 16 / sizeof(T)>(v, at, n);
 }
 
-// The table of biases: the last entry of each class, counted from 1, and then its value's bits in its place. Entries are
-// taken `threads` at a time, so that an entry looks whether it is the last one before any of the same class writes: the
-// ones after it are in its own batch or a later one. `word(i, entry)`: the word of entry i's class, null outside of the tile
+// The table of biases: the last entry of each class, counted from 1, and then its value's bits in its place, with the sign
+// the other way around, so that 0, the word of a class without an entry, stands for -0. Entries are taken `threads` at a time,
+// so that an entry looks whether it is the last one before any of the same class writes: the ones after it are in its own
+// batch or a later one. `word(i, entry)`: the word of entry i's class, null outside of the tile
 template <typename F>
 __device__ __forceinline__ void MakeBiases(uint32_t threads, uint32_t count, const int32_t* classes, const float* values, int32_t firstClass, float firstValue, F&& word) {
     for (uint32_t i = threadIdx.x; i < count; i += threads) {
@@ -199,7 +203,7 @@ __device__ __forceinline__ void MakeBiases(uint32_t threads, uint32_t count, con
         const bool isLast = at != nullptr && *at == i + 1;
         __syncthreads();
         if (isLast) {
-            *at = __float_as_uint(value);
+            *at = __float_as_uint(value) ^ kNoBias;
         }
     }
     __syncthreads();

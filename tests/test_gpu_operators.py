@@ -251,6 +251,39 @@ def test_adjust_scores_with_named_biases_or_a_table(kind, classes, with_history)
     compare(exactly(result), expected, 8 * u(kind) * size, kind)
 
 
+@ALL
+@pytest.mark.parametrize("classes", [10, 100, 5003])
+@pytest.mark.parametrize("with_history", [False, True])
+def test_adjust_scores_of_a_row_is_the_same_beside_other_rows(kind, classes, with_history):
+    """Bit for bit, zeros' signs too: classes without a bias keep -0, whether the rows around have biases enough for a table or not."""
+    rng = np.random.default_rng(classes)
+    lengths = np.array([3, 1100, 0, 2, 5])  # more than 1024: of the second row, and of a tile that has it
+    rows = len(lengths)
+    offsets = np.concatenate([[0], np.cumsum(lengths)]).astype(np.int64)
+    ids = rng.integers(0, classes // 2, offsets[-1]).astype(np.int32)  # the other half has none
+    values = rng.normal(size=offsets[-1]).astype(np.float32)
+    values[::3], values[1::7] = 0.0, -0.0
+    x = rng.normal(size=(rows, classes))
+    x[rng.random((rows, classes)) < 0.5] = -0.0
+    scores = table(x, kind)
+
+    def run(first, n, biases):
+        p = dict(bias_offsets=offsets[first:first + n + 1], bias_classes=ids[:biases], bias_values=values[:biases])
+        if with_history:
+            p.update(offsets=np.arange(first, first + n + 1) * 4, ids=(np.arange(4 * rows) % classes).astype(np.int32), presence=np.zeros(n, np.float32))
+        a = Adjustment(p)
+        result = torch.empty(n, classes, dtype=TYPES[kind], device="cuda")
+        cb.adjust_scores(kind, n, classes, scores[first:].data_ptr(), classes, a.struct, result.data_ptr(), classes)
+        return exactly(result)
+
+    together = run(0, rows, offsets[-1])
+    for r in range(rows):
+        alone = run(r, 1, offsets[-1])[0]
+        assert np.array_equal(alone, together[r]) and np.array_equal(np.signbit(alone), np.signbit(together[r])), r
+    untouched = np.signbit(exactly(scores)[:, classes // 2:])
+    assert np.array_equal(np.signbit(together[:, classes // 2:]), untouched)
+
+
 @pytest.mark.parametrize("classes", [60, 5000])
 def test_adjust_scores_with_a_history_too_long_for_named_biases(classes):
     """Some 2^19 entries, the most that leave room for names, and one more; counted exactly, with a few biases beside them."""

@@ -208,6 +208,30 @@ def test_adjust_scores_in_place(kind, rows, classes, most):
     compare(exactly(scores), expected, 6.01 * u(kind) * big, kind)
 
 
+@ALL
+@pytest.mark.parametrize("classes,pad", [(517, 3), (1024, 0), (2049, 0), (4099, 3)])
+def test_adjust_scores_of_slices_in_plenty(kind, classes, pad):
+    """Rows enough for the smaller workgroups, some with a history longer than a slice, some with more biases than names."""
+    rng = np.random.default_rng(classes + pad)
+    rows = 1030
+    scores = table(rng.normal(size=(rows, classes)) * 4, kind, pad)
+    p = parts(rng, rows, classes, "hprfscmM", 5)
+    few = np.where(np.arange(rows) % 97 == 5, rng.integers(1025, 1400, rows), rng.integers(0, 4, rows))
+    p["bias_offsets"] = np.concatenate([[0], np.cumsum(few)]).astype(np.int64)
+    p["bias_classes"] = rng.integers(-1, classes + 1, int(p["bias_offsets"][-1])).astype(np.int32)
+    p["bias_values"] = rng.normal(size=len(p["bias_classes"])).astype(np.float32)
+    long = np.where(np.arange(rows) % 101 == 7, rng.integers(classes, 6000, rows), np.diff(p["offsets"]))
+    p["offsets"] = np.concatenate([[0], np.cumsum(long)]).astype(np.int64)
+    p["ids"] = (classes * rng.random(int(p["offsets"][-1])) ** 3).astype(np.int32)
+    a = Adjustment(p)
+    wide = torch.full((rows, classes + pad + 2), 3.0, dtype=TYPES[kind], device="cuda")
+    result = wide[:, :classes]
+    cb.adjust_scores(kind, rows, classes, scores.data_ptr(), scores.stride(0), a.struct, result.data_ptr(), result.stride(0))
+    expected, big = adjusted(exactly(scores), p)
+    compare(exactly(result), expected, 6.01 * u(kind) * big, kind)
+    assert bool((wide[:, classes:] == 3.0).all())
+
+
 @pytest.mark.parametrize("classes", [10, 3000, 50_000])
 def test_adjust_scores_with_many_biases(classes):
     """More bias entries than threads, most of them overridden by later ones, with values whose bits are small numbers."""
@@ -520,6 +544,70 @@ def test_select_top_of_few_classes_for_many_rows(kind, classes, among):
     assert bool((wide[:, classes:] == 5.0).all())
 
 
+def of_few_classes(kind, rows, classes, count, pad, among):
+    """The first rows against the definition; what has rows enough is these rows again and again, all with the same results."""
+    rng = np.random.default_rng(classes * 10 + count)
+    different = 1001
+    x = rng.normal(size=(different, classes)) * 3
+    x[rng.random(x.shape) < 0.2] = 1.5
+    x[rng.random(x.shape) < 0.05] = -0.0
+    x[rng.random(x.shape) < 0.05] = 0.0
+    x[rng.random(x.shape) < 0.1] = -np.inf
+    x[rng.random(x.shape) < 0.02] = np.nan
+    x[1], x[2], x[3, 1:] = -np.inf, np.nan, np.nan
+    again = torch.arange(rows, device="cuda") % different
+    wide = torch.full((rows, classes + pad), 7.0, dtype=TYPES[kind], device="cuda")
+    wide[:, :classes] = dev(x).to(TYPES[kind])[again]
+    scores = wide[:, :classes]
+    g = rng.normal(size=(different, count))
+    g[rng.random(g.shape) < 0.1] = 0.0
+    gradients = dev(g).to(acc(kind))[again].contiguous()
+    indexes = torch.full((rows * count + 1,), 77, dtype=torch.int32, device="cuda")
+    weights = torch.full((rows * count + 1,), 77, dtype=acc(kind), device="cuda")
+    out = torch.full((rows, classes + pad + 1), 5.0, dtype=TYPES[kind], device="cuda")
+    cb.select_top(kind, rows, classes, scores.data_ptr(), scores.stride(0), count, among, indexes.data_ptr(), weights.data_ptr())
+    cb.select_top_backward(kind, rows, classes, scores.data_ptr(), scores.stride(0), count, among, indexes.data_ptr(), weights.data_ptr(),
+                           gradients.data_ptr(), out.data_ptr(), out.stride(0))
+    assert int(indexes[-1]) == 77 and float(weights[-1]) == 77 and bool((out[:, classes:] == 5.0).all())
+    indexes, weights = indexes[:-1].view(rows, count), weights[:-1].view(rows, count)
+    for got in (indexes, weights, out[:, :classes]):
+        assert torch.equal(got, got[:different][again])
+
+    index, weight, p = best(exactly(scores[:different]), count, among)
+    np.testing.assert_array_equal(indexes[:different].cpu().numpy(), index)
+    error = weight_error(kind, exactly(scores[:different]))
+    compare(exactly(weights[:different]), weight, error * weight + 2.0 ** -125, kind if kind == cb.FLOAT64 else cb.FLOAT32)
+    # as in test_select_top
+    g = np.where(index >= 0, exactly(gradients[:different]), 0)
+    mean, sizes = (g * weight).sum(1, keepdims=True), (np.abs(g) * weight).sum(1, keepdims=True)
+    expected = -p * mean
+    if among:
+        expected[:] = 0
+    bound = p * sizes * (error + u(kind) * (count + 2)) + np.abs(expected) * (error + 3 * u(kind))
+    for k in range(count):
+        r = np.nonzero(index[:, k] >= 0)[0]
+        part = weight[r, k] * (g[r, k] - mean[r, 0] if among else g[r, k])
+        expected[r, index[r, k]] += part
+        bound[r, index[r, k]] += weight[r, k] * (np.abs(g[r, k]) * (error + 3 * u(kind)) + np.abs(mean[r, 0]) * (error + 3 * u(kind)))
+    compare(exactly(out[:different, :classes]), expected, bound + 2.0 ** -120, kind)
+
+
+@ALL
+@pytest.mark.parametrize("classes", range(1, 17))
+@pytest.mark.parametrize("among", [False, True])
+def test_select_top_of_few_classes_by_threads(kind, classes, among):
+    """Rows enough that every row has a thread to itself: forward with 8 classes selected, forward and backward with fewer."""
+    of_few_classes(kind, 32768 + 77, classes, 8, classes % 3, among)
+    of_few_classes(kind, 131072 + 77, classes, 4 if classes % 4 == 1 else 1 + classes % 4, classes % 2, among)
+
+
+@ALL
+@pytest.mark.parametrize("rows", [32767, 32768, 131071, 131072])
+@pytest.mark.parametrize("count", [4, 5, 8, 9])
+def test_select_top_of_few_classes_around_the_rows_for_threads(kind, rows, count):
+    of_few_classes(kind, rows, 10, count, 0, count % 2 == 0)
+
+
 @ALL
 def test_select_top_of_infinite_scores(kind):
     x = np.array([[np.inf, 1, np.inf, 0], [np.inf, np.inf, np.inf, np.inf], [1, np.inf, -np.inf, np.nan]])
@@ -700,6 +788,14 @@ def test_combine_rows_and_gradients(kind, rows, per_row, width, pad, weighted):
     cb.combine_rows_backward(kind, rows, width, per_row, g.data_ptr(), g.stride(0), y.data_ptr(), sorted_rows, y.stride(0), d.data_ptr(), ptr(w), 0,
                              0, dw2.data_ptr())
     assert torch.equal(dy, dy2) and torch.equal(dw, dw2)
+
+
+@ALL
+@pytest.mark.parametrize("rows,per_row,pieces", [(16383, 2, 20), (16384, 2, 20), (16400, 1, 17), (16390, 3, 32), (4095, 2, 70), (4096, 2, 70), (4100, 1, 100), (4097, 2, 255), (4100, 1, 256)])
+def test_combine_rows_and_gradients_of_many_rows(kind, rows, per_row, pieces):
+    """Around the numbers of rows from which eight threads and a wave have a row's gradients; rows that end inside a piece."""
+    in_piece = 2 if kind == cb.FLOAT64 else 4 if kind == cb.FLOAT32 else 8
+    test_combine_rows_and_gradients(kind, rows, per_row, pieces * in_piece - 1, per_row % 2, True)
 
 
 @ALL

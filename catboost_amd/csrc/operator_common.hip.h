@@ -131,17 +131,22 @@ inline void CheckMatrix(const char* name, const void* data, size_t rows, size_t 
     CBAMD_ENSURE(rows <= 1 || stride <= (size_t(1) << 60) / valueSize / rows, std::string(name) + " is too large");
 }
 
-// N values in a row, at any alignment of a value: one wide load or store where N values make one (the hardware's
-// unaligned mode takes any address)
+// N values in a row, at any alignment of what they are loaded from or stored to, whose type the pointer says (words of a
+// row of 16-bit values are at multiples of 2): one wide load or store where N values make one (the hardware's unaligned
+// mode takes any address)
 template <typename T, int N>
 struct TValues {
     T V[N];
-    __device__ __forceinline__ static TValues Load(const T* at) {
+    template <typename TFrom>
+    __device__ __forceinline__ static TValues Load(const TFrom* at) {
         TValues r;
         __builtin_memcpy(&r, at, sizeof(r));
         return r;
     }
-    __device__ __forceinline__ void Store(T* at) const { __builtin_memcpy(at, this, sizeof(*this)); }
+    template <typename TTo>
+    __device__ __forceinline__ void Store(TTo* at) const {
+        __builtin_memcpy(at, this, sizeof(*this));
+    }
 };
 
 // The same for the `n` values that are left of a row, where those are fewer

@@ -238,19 +238,18 @@ struct TPlaces {
 template <typename T, int N, int K>
 __global__ void __launch_bounds__(256) DispatchRowsKernel(const T* source, size_t sourceStride, TPieces p, const int32_t* places, T* sorted,
                                                           size_t sortedRows, size_t sortedStride) {
-    using TWord = std::conditional_t<N == 1, T, uint32_t>;
-    using TPiece = TValues<TWord, N == 1 ? 1 : 4>;
+    using TPiece = std::conditional_t<N == 1, TValues<T, 1>, TValues<uint32_t, 4>>;
     size_t row, c;
     if (!p.Of<N>(&row, &c)) {
         return;
     }
-    const TPiece v = TPiece::Load(reinterpret_cast<const TWord*>(source + row * sourceStride + c));
+    const TPiece v = TPiece::Load(source + row * sourceStride + c);
     for (uint32_t k = 0; k < p.PerRow; k += K) {
         const TPlaces<K> to(places + row * p.PerRow, k, p.PerRow, sortedRows);
 #pragma unroll
         for (int j = 0; j < K; ++j) {
             if (to.At[j] >= 0) {
-                v.Store(reinterpret_cast<TWord*>(sorted + static_cast<size_t>(to.At[j]) * sortedStride + c));
+                v.Store(sorted + static_cast<size_t>(to.At[j]) * sortedStride + c);
             }
         }
     }

@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(1024) AdjustSliceKernel(TAdjustArgs a) {
     if (whole) {
 #pragma unroll
         for (int j = 0; j < P; ++j) {
-            raw[j] = TRaw::Load(reinterpret_cast<const uint32_t*>(from + min((j * threads + threadIdx.x) * N, width - N)));
+            raw[j] = TRaw::Load(from + min((j * threads + threadIdx.x) * N, width - N));
         }
     } else {
 #pragma unroll
@@ -339,7 +339,7 @@ __global__ void __launch_bounds__(1024) AdjustSliceKernel(TAdjustArgs a) {
         if (c < width) {
             const TRaw out = x.Rounded(mask >= 0 ? allowed[j] >> (c & 31) : ~0u);
             if (whole) {
-                out.Store(reinterpret_cast<uint32_t*>(to + c));
+                out.Store(to + c);
             } else {
                 StorePiece<T>(out, to + c, width - c);
             }
@@ -511,7 +511,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof
     for (int j = 0; j < P; ++j) {
         const uint32_t q = j * 256 + threadIdx.x, r = rowOf(q), c = (q - r * a.Pieces) * N;
         const T* from = static_cast<const T*>(a.Scores) + (r0 + min(r, rows - 1)) * a.ScoreStride + c;
-        raw[j] = RESTS == kNoRests ? TRaw::Load(reinterpret_cast<const uint32_t*>(from))
+        raw[j] = RESTS == kNoRests ? TRaw::Load(from)
             : RESTS == kRests ? LoadShifted<T>(from, a.Classes - c) : LoadPiece<T>(from, a.Classes - c);
     }
     if (p.AllowedCount != 0) {
@@ -622,7 +622,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof
             const TRaw out = x.Rounded(masked ? allowed[j] >> (c & 31) : ~0u);
             T* to = static_cast<T*>(a.Result) + (r0 + r) * a.ResultStride + c;
             if (RESTS == kNoRests) {
-                out.Store(reinterpret_cast<uint32_t*>(to));
+                out.Store(to);
             } else {
                 StorePiece<T>(out, to, a.Classes - c);
             }

@@ -131,6 +131,14 @@ inline void CheckMatrix(const char* name, const void* data, size_t rows, size_t 
     CBAMD_ENSURE(rows <= 1 || stride <= (size_t(1) << 60) / valueSize / rows, std::string(name) + " is too large");
 }
 
+// What lanes of a wave hand each other through LDS: a wave's LDS operations are done in order, so that there is nothing to
+// wait for; the fences keep the compiler from moving them across (they cost no instruction)
+__device__ __forceinline__ void WaveHandover() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // N values in a row, at any alignment of what they are loaded from or stored to, whose type the pointer says (words of a
 // row of 16-bit values are at multiples of 2): one wide load or store where N values make one (the hardware's unaligned
 // mode takes any address)

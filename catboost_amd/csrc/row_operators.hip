@@ -48,7 +48,7 @@ struct TRankedSlots {
             if (last && Expert[s] < experts) {
                 own[Expert[s]] += static_cast<int32_t>(Rank[s] & 0x7fffffffu) + 1;
             }
-            __builtin_amdgcn_wave_barrier();  // the steps' additions stay in order
+            WaveHandover();  // the steps' additions stay in order
         }
     }
 };
@@ -182,11 +182,11 @@ __global__ void __launch_bounds__(kSortThreads) PlaceSlotsKernel(const int32_t* 
     for (int s = 0; s < STEPS; ++s) {
         const bool valid = ranked.Expert[s] < experts;
         const int32_t place = valid ? own[ranked.Expert[s]] + static_cast<int32_t>(ranked.Rank[s] & 0x7fffffffu) : -1;
-        __builtin_amdgcn_wave_barrier();  // all lanes have read before the last one of each expert writes
+        WaveHandover();  // all lanes have read before the last one of each expert writes
         if (valid && (ranked.Rank[s] & 0x80000000u) != 0) {
             own[ranked.Expert[s]] = place + 1;
         }
-        __builtin_amdgcn_wave_barrier();
+        WaveHandover();
         const uint32_t slot = begin + s * 64 + lane;
         if (slot < slots) {
             places[slot] = place;

@@ -1148,14 +1148,14 @@ __global__ void __launch_bounds__(256) SelectTopBackwardKernel(TTopArgs<T> a, TT
     for (int i = 0; i < P; ++i) {
         x[i].Store(mySums + classOf(i));
     }
-    __builtin_amdgcn_wave_barrier();  // a row's lanes are of one wave, whose LDS operations are done in order
+    WaveHandover();  // a row's lanes are of one wave
 #pragma unroll
     for (int i = 0; i < kept; ++i) {
         if (static_cast<uint32_t>(index[i]) < a.Classes) {
             mySums[index[i]] += part[i];
         }
     }
-    __builtin_amdgcn_wave_barrier();
+    WaveHandover();
     T* gradients = b.Gradients + row * b.GradientStride;
 #pragma unroll
     for (int i = 0; i < P; ++i) {

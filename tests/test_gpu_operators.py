@@ -232,6 +232,50 @@ def test_adjust_scores_of_slices_in_plenty(kind, classes, pad):
     assert bool((wide[:, classes:] == 3.0).all())
 
 
+@ALL
+def test_adjust_scores_of_slices_in_plenty_with_histories_longer_than_they_are(kind):
+    """As many threads as a slice may have, more than it has scores for: they look through the histories."""
+    rng = np.random.default_rng(3)
+    rows, classes = 1025, 517
+    scores = table(rng.normal(size=(rows, classes)) * 4, kind, 1)
+    p = parts(rng, rows, classes, "hprfsbm", 700)
+    assert len(p["ids"]) > rows * 272
+    a = Adjustment(p)
+    result = torch.empty(rows, classes, dtype=TYPES[kind], device="cuda")
+    cb.adjust_scores(kind, rows, classes, scores.data_ptr(), scores.stride(0), a.struct, result.data_ptr(), classes)
+    expected, big = adjusted(exactly(scores), p)
+    compare(exactly(result), expected, 6.01 * u(kind) * big, kind)
+
+
+def test_adjust_scores_of_the_most_classes():
+    """One row of 2^31 - 1: what is adjusted is at both ends, in the middle and around slices; everything else stays."""
+    classes = (1 << 31) - 1
+    scores = torch.empty(classes, dtype=torch.float16, device="cuda")
+    for begin in range(0, classes, 1 << 28):
+        scores[begin:begin + (1 << 28)].normal_()
+    at = np.array([0, 1, 16383, 16384, 1 << 24, (1 << 30) + 5, classes - 16384, classes - 2, classes - 1])
+    ids = np.concatenate([at, at[::2], [-1, np.iinfo(np.int32).min]]).astype(np.int32)
+    p = dict(offsets=np.array([0, len(ids)]), ids=ids, frequency=np.array([0.5], np.float32), bias_offsets=np.array([0, 3]),
+             bias_classes=np.array([classes - 1, 7, 1 << 30], np.int32), bias_values=np.array([4, 2, 1], np.float32),
+             allowed=np.full((1, (classes + 31) // 32), 0xffffffff, np.uint32))
+    off = np.array([5, 1 << 29, classes - 3])
+    for c in off:
+        p["allowed"][0, c >> 5] &= np.uint32(0xffffffff ^ 1 << (c & 31))
+    a = Adjustment(p)
+    result = torch.full_like(scores, 9.0)
+    cb.adjust_scores(cb.FLOAT16, 1, classes, scores.data_ptr(), classes, a.struct, result.data_ptr(), classes)
+    changed = np.concatenate([at, [7, 1 << 30], off])
+    expected = scores[torch.from_numpy(changed).cuda()].float().cpu().numpy()
+    expected[:len(at)] -= 0.5 * (1 + (np.arange(len(at)) % 2 == 0))
+    expected[len(at) - 1] += 4
+    expected[len(at):len(at) + 2] += [2, 1]
+    expected[len(at) + 2:] = -np.inf
+    where = torch.from_numpy(changed).cuda()
+    np.testing.assert_array_equal(result[where].float().cpu().numpy(), torch.from_numpy(expected).half().float().numpy())
+    result[where] = scores[where]
+    assert torch.equal(result, scores)
+
+
 @pytest.mark.parametrize("classes", [10, 3000, 50_000])
 def test_adjust_scores_with_many_biases(classes):
     """More bias entries than threads, most of them overridden by later ones, with values whose bits are small numbers."""
@@ -892,6 +936,35 @@ def test_a_layer_of_experts_on_a_stream_and_in_graphs(kind, rows, width):
         torch.cuda.synchronize()
         for k, v in eager[at].items():
             assert torch.equal(buffers[k], v), (turn, k)
+
+
+def test_a_first_call_with_large_tables_is_captured():
+    """More than 64 KB of LDS, which a kernel has to be allowed once for each device (in a process that runs this test alone, in the capture)."""
+    slots, experts, rows, classes = 3000, 1021, 200, 90_001
+    rng = np.random.default_rng(2)
+    ids = rng.integers(0, experts, slots).astype(np.int32)
+    d, places, offsets = dev(ids), torch.empty(slots, dtype=torch.int32, device="cuda"), torch.empty(experts + 1, dtype=torch.int32, device="cuda")
+    size = cb.sort_by_expert_bytes(slots, experts)
+    workspace = torch.empty(size, dtype=torch.uint8, device="cuda")
+    scores = table(rng.normal(size=(rows, classes)), cb.BFLOAT16)
+    p = parts(rng, rows, classes, "hsb", 3)
+    a = Adjustment(p)
+    result = torch.zeros_like(scores)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        stream = torch.cuda.current_stream().cuda_stream
+        cb.sort_by_expert(slots, experts, d.data_ptr(), places.data_ptr(), offsets.data_ptr(), workspace.data_ptr(), size, stream)
+        cb.adjust_scores(cb.BFLOAT16, rows, classes, scores.data_ptr(), classes, a.struct, result.data_ptr(), classes, stream)
+    eager = torch.zeros_like(scores)
+    cb.adjust_scores(cb.BFLOAT16, rows, classes, scores.data_ptr(), classes, a.struct, eager.data_ptr(), classes)
+    for _ in range(3):
+        result.zero_()
+        places.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(result, eager)
+        np.testing.assert_array_equal(places.cpu().numpy()[np.argsort(ids, kind="stable")], np.arange(slots))
 
 
 def test_offsets_that_pass_32_bits():

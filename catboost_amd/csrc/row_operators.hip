@@ -520,8 +520,10 @@ void DispatchRows(int valueType, size_t rows, size_t width, int32_t perRow, cons
     CheckMatrix("sorted rows", sorted, sortedRows, width, sortedStride, size);
     const TCallDevice call(sorted, stream);
     // LDS that no one uses keeps a compute unit to four workgroups, six where a row is stored to one or two places: fewer
-    // stores on their way at a time are faster (with the sort, 16384 rows of 8 KB to four places 127 us, 136 with the eight that there
-    // is room for; a million rows of 800 bytes to one 301 and 306, 311 with four)
+    // stores on their way at a time are faster once they go to memory (16384 rows of 8 KB to four places 114 us, 117 with six and 139
+    // with the eight that there is room for; 300000 rows of 800 bytes to one 93.3, 94.0 with four, 94.5 with eight), and make little
+    // difference where the caches hold them (4096 rows of 8 KB to four places 32.6 and 33.9 with eight, 1024 rows 8.0 and 7.7; 65536
+    // rows of 512 bytes to one 11.8, 12.8 with four, 11.6 with eight)
     const size_t unusedLds = (160 * 1024) / (perRow <= 2 ? 6 : 4) / 1024 * 1024;
     const auto launch = [&](auto value) {
         using T = decltype(value);

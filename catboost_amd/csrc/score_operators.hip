@@ -78,7 +78,8 @@ __device__ __forceinline__ TValues<int32_t, 4> LoadEntries(const int32_t* list, 
 }
 
 // A row of up to this many biases needs no table of them: the word of a class that has one names it in its upper bits, if the
-// history is short enough for its counts to leave those free (64 x 131000 16-bit scores with 20 biases a row 13.5 us, with a table 16)
+// history is short enough for its counts to leave those free (64 x 131000 16-bit scores with 3000 entries and 20 biases a row 15.1 us, with a
+// table 16.5; 2M x 10 32-bit ones with two of each 95 and 108)
 constexpr uint32_t kNamedBiases = 1024, kNameShift = 21;
 constexpr int64_t kNamedHistory = int64_t(1) << (kNameShift - 2);
 
@@ -898,7 +899,7 @@ struct TTopArgs {
 
 // G lanes for a row, V classes next to each other for each of them. A round finds the best class that is left: in the
 // lane's own, then over the group; whoever has it takes it out. Lane k % G keeps what round k finds. Arithmetic bounds it: 131072
-// rows, 8 of 128 16-bit classes take 17 us, for 42 MB.
+// rows, 8 of 128 16-bit classes take 15 us, for 42 MB.
 template <typename T, int G, int V>
 __global__ void __launch_bounds__(256) SelectTopKernel(TTopArgs<T> a, int32_t* indexes, TAcc<T>* weights) {
     using A = TAcc<T>;
@@ -998,7 +999,7 @@ __global__ void __launch_bounds__(256) SelectTopKernel(TTopArgs<T> a, int32_t* i
 }
 
 // Rows of C classes, a thread for each. What is stored goes through LDS, so that a wave's stores fill whole lines. Memory bounds it:
-// 2M rows, 3 of 10 64-bit classes take 52 us (4.5 TB/s).
+// 2M rows, 3 of 10 64-bit classes take 54 us (4.3 TB/s).
 template <typename T, int C>
 __global__ void __launch_bounds__(256) SelectTopOfFewKernel(TTopArgs<T> a, int32_t* indexes, TAcc<T>* weights) {
     using A = TAcc<T>;
@@ -1066,7 +1067,7 @@ struct TTopGradientArgs {
 // among the selected only w_k (g_k - m) and 0 elsewhere, else w_k g_k - p m with the first part 0 elsewhere.
 // G lanes for a row, which take its pieces of 16 bytes in turn, V classes each in all (V next to each other instead took 43 us for
 // 131072 rows of 256 32-bit classes, and these 20). The gradients are put together in LDS, where the selected classes' lanes add
-// their parts. Memory bounds it: 8 of 128 16-bit classes 8.8 us for 46 MB, which the caches still have in part.
+// their parts. Memory bounds it: 8 of 128 16-bit classes 9.5 us for 46 MB, which the caches still have in part.
 template <typename T, int G, int V>
 __global__ void __launch_bounds__(256) SelectTopBackwardKernel(TTopArgs<T> a, TTopGradientArgs<T> b) {
     using A = TAcc<T>;
@@ -1173,7 +1174,8 @@ __global__ void __launch_bounds__(256) SelectTopBackwardKernel(TTopArgs<T> a, TT
 }
 
 // Rows of C classes, a thread for each. What is loaded and stored goes through LDS (a thread that loaded its own row's selected
-// classes, one after the other, took 76 us for 262144 rows, 8 of 16 64-bit classes selected).
+// classes, one after the other, took 76 us for 262144 rows, 8 of 16 64-bit classes selected). Memory bounds it: 2M rows, 3 of 10 64-bit
+// classes over all take 86 us (5.1 TB/s).
 template <typename T, int C>
 __global__ void __launch_bounds__(256) SelectTopOfFewBackwardKernel(TTopArgs<T> a, TTopGradientArgs<T> b) {
     using A = TAcc<T>;

@@ -104,6 +104,43 @@ def test_on_a_stream_with_slices_and_no_documents():
     cb.eval_routed([m.evaluator() for m, _ in models], f, 0, 1, 0, 0, 0, 0, 0)
 
 
+@pytest.mark.parametrize("docs", [4001, 300_000])
+def test_models_rows_at_any_address(docs):
+    """An odd number of features and a workspace at a multiple of 8: a model's first document is at any multiple of 4."""
+    rng = np.random.default_rng(docs)
+    models = [model(s, n, 1, trees=60) for s, n in enumerate((51, 37, 51))]
+    x = rng.normal(size=(docs, 53)).astype(np.float32)
+    ids = rng.integers(0, 3, size=(docs, 1)).astype(np.int32)
+    ids[rng.random(docs) < 0.3] = 2
+    d, i = dev(x), dev(ids)
+    evaluators = [m.evaluator() for m, _ in models]
+    size = cb.eval_routed_bytes(evaluators, cb.LAYOUT_FLAT_ROWS, docs, 1)
+    results = torch.full((docs,), 7.0, dtype=torch.float64, device="cuda")
+    f = cb.DeviceEvaluator.features(cb.LAYOUT_FLAT_ROWS, d.data_ptr(), 53)
+    expected = mixed(models, x, 1, ids, None)[:, 0]
+    for at in (8, 24, 0):
+        workspace = torch.full((size + 64,), 255, dtype=torch.uint8, device="cuda")
+        torch.cuda.synchronize()
+        cb.eval_routed(evaluators, f, docs, 1, i.data_ptr(), 0, results.data_ptr(), workspace.data_ptr() + at, size)
+        np.testing.assert_allclose(results.cpu().numpy(), expected, rtol=1e-9, atol=1e-12)  # the models' own bar
+        assert bool((workspace[:at] == 255).all()) and bool((workspace[at + size:] == 255).all())
+
+
+def test_the_most_evaluators_and_the_most_for_a_document():
+    """1024 of them, most of a few models again and again, 64 for each document, the same ones several times."""
+    rng = np.random.default_rng(5)
+    models = [model(s, 10, 2) for s in range(3)]
+    docs, count, per_doc = 150, 1024, 64
+    x = rng.normal(size=(docs, 10)).astype(np.float32)
+    ids = rng.integers(-1, count + 1, size=(docs, per_doc))
+    weights = rng.normal(size=(docs, per_doc))
+    d = dev(x)
+    f = cb.DeviceEvaluator.features(cb.LAYOUT_FLAT_ROWS, d.data_ptr(), 10)
+    inside = np.where((ids >= 0) & (ids < count), ids % 3, -1)
+    got = routed([models[e % 3] for e in range(count)], cb.LAYOUT_FLAT_ROWS, f, docs, ids, weights, 2)
+    np.testing.assert_array_equal(got, mixed(models, x, 2, inside, weights))
+
+
 def test_from_two_threads_at_once():
     rng = np.random.default_rng(6)
     models = [model(s, 10, 2) for s in range(3)]

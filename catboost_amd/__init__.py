@@ -17,6 +17,7 @@ LIB_PATH = os.path.join(_HERE, "lib", "libcatboostmodel.so")
 APT_RAW_FORMULA_VAL, APT_EXPONENT, APT_RMSE_WITH_UNCERTAINTY, APT_PROBABILITY, APT_CLASS, APT_MULTI_PROBABILITY = range(6)
 LAYOUT_FLAT_ROWS, LAYOUT_FLAT_COLUMNS, LAYOUT_SPLIT_ROWS = range(3)
 FLOAT64, FLOAT32, FLOAT16, BFLOAT16 = range(4)
+SILU, GELU, GELU_TANH, RELU = range(4)  # activations (ECbHipActivation)
 
 _lib = None
 
@@ -94,6 +95,16 @@ class ScoreAdjustment(ctypes.Structure):
         ("AllowedStride", ctypes.c_size_t),
         ("AllowedCount", ctypes.c_size_t),
         ("AllowedRows", ctypes.c_void_p),
+    ]
+
+
+class Sampling(ctypes.Structure):
+    """CbHipSampling of include/cb_hip_evaluator.h."""
+    _fields_ = [
+        ("Temperature", ctypes.c_void_p),
+        ("TopK", ctypes.c_void_p),
+        ("TopP", ctypes.c_void_p),
+        ("MinP", ctypes.c_void_p),
     ]
 
 
@@ -180,6 +191,13 @@ def load_library():
         "CbHipDispatchRows": (ctypes.c_bool, [ctypes.c_int, sz, sz, ctypes.c_int32, vp, sz, vp, vp, sz, sz, vp]),
         "CbHipCombineRows": (ctypes.c_bool, [ctypes.c_int, sz, sz, ctypes.c_int32, vp, sz, sz, vp, vp, vp, sz, vp]),
         "CbHipCombineRowsBackward": (ctypes.c_bool, [ctypes.c_int, sz, sz, ctypes.c_int32, vp, sz, vp, sz, sz, vp, vp, vp, sz, vp, vp]),
+        "CbHipSampleClassesBytes": (sz, [ctypes.c_int, sz, sz]),
+        "CbHipSampleClasses": (ctypes.c_bool, [ctypes.c_int, sz, sz, vp, sz, ctypes.POINTER(Sampling), vp, vp, vp, vp, sz, vp]),
+        "CbHipGatedRows": (ctypes.c_bool, [ctypes.c_int, ctypes.c_int, sz, sz, sz, ctypes.c_int32, vp, vp, sz, vp, vp, sz, vp, sz, vp, vp]),
+        "CbHipGatedRowsBackward": (ctypes.c_bool, [ctypes.c_int, ctypes.c_int, sz, sz, sz, ctypes.c_int32, vp, vp, sz, vp, sz, vp, vp, sz, vp, vp, vp, sz, vp,
+                                                   vp, sz, vp]),
+        "CbHipMultiplyRows": (ctypes.c_bool, [ctypes.c_int, sz, sz, sz, ctypes.c_int32, vp, vp, sz, vp, sz, vp, sz, vp]),
+        "CbHipMultiplyRowsBackward": (ctypes.c_bool, [ctypes.c_int, sz, sz, sz, ctypes.c_int32, vp, vp, sz, vp, sz, vp, sz, vp, sz, vp, sz, vp]),
         "CbHipEvalRoutedBytes": (sz, [ctypes.POINTER(vp), sz, ctypes.c_int, sz, ctypes.c_int32]),
         "CbHipEvalRouted": (ctypes.c_bool, [ctypes.POINTER(vp), sz, ctypes.POINTER(DeviceFeatures), sz, ctypes.c_int32, vp, vp, vp, vp, sz, vp]),
         "CbHipSynchronize": (ctypes.c_bool, [vp, vp]),
@@ -408,6 +426,23 @@ def select_top_backward(value_type, rows, classes, scores_ptr, score_stride, cou
                                                  weights_ptr, weight_gradients_ptr, score_gradients_ptr, gradient_stride, stream))
 
 
+def sampling(temperature_ptr=0, top_k_ptr=0, top_p_ptr=0, min_p_ptr=0):
+    """How sample_classes draws (CbHipSampling); parts that are left out do not limit it."""
+    return Sampling(temperature_ptr, top_k_ptr, top_p_ptr, min_p_ptr)
+
+
+def sample_classes_bytes(value_type, rows, classes):
+    """Bytes of workspace that sample_classes needs."""
+    return load_library().CbHipSampleClassesBytes(value_type, rows, classes)
+
+
+def sample_classes(value_type, rows, classes, scores_ptr, score_stride, sampling, uniform_ptr, indexes_ptr, weights_ptr=0, workspace_ptr=0,
+                   workspace_bytes=0, stream=None):
+    """A class of every row, drawn by the softmax of its scores with the given random numbers (CbHipSampleClasses)."""
+    _check(load_library().CbHipSampleClasses(value_type, rows, classes, scores_ptr, score_stride, ctypes.byref(sampling), uniform_ptr, indexes_ptr,
+                                             weights_ptr, workspace_ptr, workspace_bytes, stream))
+
+
 def sort_by_expert_bytes(slots, experts):
     """Bytes of workspace that sort_by_expert needs."""
     return load_library().CbHipSortByExpertBytes(slots, experts)
@@ -437,6 +472,39 @@ def combine_rows_backward(value_type, rows, width, per_row, gradients_ptr, gradi
     _check(load_library().CbHipCombineRowsBackward(value_type, rows, width, per_row, gradients_ptr, gradient_stride, sorted_ptr, sorted_rows,
                                                    sorted_stride, places_ptr, weights_ptr, sorted_gradients_ptr, sorted_gradient_stride,
                                                    weight_gradients_ptr, stream))
+
+
+def gated_rows(value_type, activation, rows, width, hidden, experts, offsets_ptr, source_ptr, source_stride, gate_ptr, up_ptr, expert_stride,
+               result_ptr, result_stride, kept_ptr=0, stream=None):
+    """Rows sorted by expert through their experts' gated projections (CbHipGatedRows)."""
+    _check(load_library().CbHipGatedRows(value_type, activation, rows, width, hidden, experts, offsets_ptr, source_ptr, source_stride, gate_ptr, up_ptr,
+                                         expert_stride, result_ptr, result_stride, kept_ptr, stream))
+
+
+def gated_rows_backward(value_type, activation, rows, width, hidden, experts, offsets_ptr, gradients_ptr, gradient_stride, source_ptr, source_stride,
+                        gate_ptr, up_ptr, expert_stride, kept_ptr, pre_gradients_ptr, source_gradients_ptr, source_gradient_stride,
+                        gate_gradients_ptr, up_gradients_ptr, expert_gradient_stride, stream=None):
+    """The gradients of gated_rows (CbHipGatedRowsBackward)."""
+    _check(load_library().CbHipGatedRowsBackward(value_type, activation, rows, width, hidden, experts, offsets_ptr, gradients_ptr, gradient_stride,
+                                                 source_ptr, source_stride, gate_ptr, up_ptr, expert_stride, kept_ptr, pre_gradients_ptr,
+                                                 source_gradients_ptr, source_gradient_stride, gate_gradients_ptr, up_gradients_ptr,
+                                                 expert_gradient_stride, stream))
+
+
+def multiply_rows(value_type, rows, width, outputs, experts, offsets_ptr, source_ptr, source_stride, weights_ptr, expert_stride, result_ptr,
+                  result_stride, stream=None):
+    """Rows sorted by expert times their experts' weights (CbHipMultiplyRows)."""
+    _check(load_library().CbHipMultiplyRows(value_type, rows, width, outputs, experts, offsets_ptr, source_ptr, source_stride, weights_ptr, expert_stride,
+                                            result_ptr, result_stride, stream))
+
+
+def multiply_rows_backward(value_type, rows, width, outputs, experts, offsets_ptr, gradients_ptr, gradient_stride, source_ptr, source_stride,
+                           weights_ptr, expert_stride, source_gradients_ptr, source_gradient_stride, weight_gradients_ptr,
+                           expert_gradient_stride, stream=None):
+    """The gradients of multiply_rows (CbHipMultiplyRowsBackward)."""
+    _check(load_library().CbHipMultiplyRowsBackward(value_type, rows, width, outputs, experts, offsets_ptr, gradients_ptr, gradient_stride, source_ptr,
+                                                    source_stride, weights_ptr, expert_stride, source_gradients_ptr, source_gradient_stride,
+                                                    weight_gradients_ptr, expert_gradient_stride, stream))
 
 
 class DeviceEvaluator:

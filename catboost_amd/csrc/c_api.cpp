@@ -903,6 +903,18 @@ bool CbHipSelectTopBackward(int valueType, size_t rows, size_t classes, const vo
     });
 }
 
+size_t CbHipSampleClassesBytes(int valueType, size_t rows, size_t classes) {
+    return SampleClassesBytes(valueType, rows, classes);
+}
+
+bool CbHipSampleClasses(int valueType, size_t rows, size_t classes, const void* scores, size_t scoreStride, const CbHipSampling* sampling,
+                        const float* uniform, int32_t* indexes, void* weights, void* workspace, size_t workspaceBytes, void* hipStream) {
+    return Guard([&] {
+        CBAMD_ENSURE(sampling != nullptr, "sampling is null");
+        SampleClasses(valueType, rows, classes, scores, scoreStride, *sampling, uniform, indexes, weights, workspace, workspaceBytes, hipStream);
+    });
+}
+
 size_t CbHipSortByExpertBytes(size_t slots, int32_t experts) {
     return SortByExpertBytes(slots, experts);
 }
@@ -935,6 +947,47 @@ bool CbHipCombineRowsBackward(int valueType, size_t rows, size_t width, int32_t 
     return Guard([&] {
         CombineRowsBackward(valueType, rows, width, perRow, resultGradients, gradientStride, sorted, sortedRows, sortedStride,
                             places, weights, sortedGradients, sortedGradientStride, weightGradients, hipStream);
+    });
+}
+
+bool CbHipGatedRows(int valueType, int activation, size_t rows, size_t width, size_t hidden, int32_t experts, const int32_t* offsets,
+                    const void* source, size_t sourceStride, const void* gateWeights, const void* upWeights, size_t expertStride,
+                    void* result, size_t resultStride, void* kept, void* hipStream) {
+    return Guard([&] {
+        GatedRows(valueType, activation, rows, width, hidden, experts, offsets, source, sourceStride, gateWeights, upWeights, expertStride,
+                  result, resultStride, kept, hipStream);
+    });
+}
+
+bool CbHipGatedRowsBackward(int valueType, int activation, size_t rows, size_t width, size_t hidden, int32_t experts,
+                            const int32_t* offsets, const void* resultGradients, size_t gradientStride, const void* source,
+                            size_t sourceStride, const void* gateWeights, const void* upWeights, size_t expertStride,
+                            const void* kept, void* preGradients, void* sourceGradients, size_t sourceGradientStride,
+                            void* gateGradients, void* upGradients, size_t expertGradientStride, void* hipStream) {
+    return Guard([&] {
+        GatedRowsBackward(valueType, activation, rows, width, hidden, experts, offsets, resultGradients, gradientStride, source,
+                          sourceStride, gateWeights, upWeights, expertStride, kept, preGradients, sourceGradients,
+                          sourceGradientStride, gateGradients, upGradients, expertGradientStride, hipStream);
+    });
+}
+
+bool CbHipMultiplyRows(int valueType, size_t rows, size_t width, size_t outputs, int32_t experts, const int32_t* offsets,
+                       const void* source, size_t sourceStride, const void* weights, size_t expertStride, void* result,
+                       size_t resultStride, void* hipStream) {
+    return Guard([&] {
+        MultiplyRows(valueType, rows, width, outputs, experts, offsets, source, sourceStride, weights, expertStride, result, resultStride,
+                     hipStream);
+    });
+}
+
+bool CbHipMultiplyRowsBackward(int valueType, size_t rows, size_t width, size_t outputs, int32_t experts, const int32_t* offsets,
+                               const void* resultGradients, size_t gradientStride, const void* source, size_t sourceStride,
+                               const void* weights, size_t expertStride, void* sourceGradients, size_t sourceGradientStride,
+                               void* weightGradients, size_t expertGradientStride, void* hipStream) {
+    return Guard([&] {
+        MultiplyRowsBackward(valueType, rows, width, outputs, experts, offsets, resultGradients, gradientStride, source, sourceStride,
+                             weights, expertStride, sourceGradients, sourceGradientStride, weightGradients, expertGradientStride,
+                             hipStream);
     });
 }
 

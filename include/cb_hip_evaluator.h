@@ -207,8 +207,8 @@ bool CbHipSetSmallBatchSlicing(void* modelHandle, bool enabled);
 
 /* ---- operators on scores and on routed rows -----------------------------------------------------------------
  * What stands before, between and behind models: scores (raw values, a gate's, a language model's) with penalties,
- * biases and masks; the best classes with their weights; rows sorted by the model or expert that each goes to, and
- * brought back. None has a counterpart in the reference. All take DEVICE memory, are asynchronous on `hipStream` (a
+ * biases and masks; the best classes with their weights; a class drawn; rows sorted by the model or expert that each goes to,
+ * multiplied by their experts' weights and brought back. None has a counterpart in the reference. All take DEVICE memory, are asynchronous on `hipStream` (a
  * hipStream_t, NULL: the default stream of the device that the output is on) and, but for CbHipEvalRouted, only launch
  * kernels, so they may be captured into HIP graphs; memory that they work in comes from the caller. All operands of a
  * call are on one device, which need not be the current one. Results are the same for every call on the same inputs.
@@ -274,6 +274,31 @@ bool CbHipSelectTopBackward(int valueType, size_t rows, size_t classes, const vo
                             bool amongSelected, const int32_t* indexes, const void* weights, const void* weightGradients,
                             void* scoreGradients, size_t gradientStride, void* hipStream);
 
+/* How CbHipSampleClasses draws: one value per row each; a part whose pointer is NULL is left out. */
+typedef struct CbHipSampling {
+    /* Scores are divided by it (NULL: 1). 0, less or NaN: the best class is taken, of equal ones the lowest. */
+    const float* Temperature;
+    /* The TopK best classes take part, of equal ones the lowest first; 0 or less: all. */
+    const int32_t* TopK;
+    /* Of those, best first, as many as it takes for their weights to add up to TopP of their sum, one at least; 1, more or
+     * NaN: all. */
+    const float* TopP;
+    /* And only those of at least MinP times the best one's weight; 0, less or NaN: all, more than 1: as 1. */
+    const float* MinP;
+} CbHipSampling;
+
+/* Bytes of workspace (at a multiple of 8) that CbHipSampleClasses needs; 0 where it needs none. */
+size_t CbHipSampleClassesBytes(int valueType, size_t rows, size_t classes);
+
+/* indexes[r] = a class of row r, drawn with the softmax weights of the classes that take part: best first (of equal ones the
+ * lowest), the first whose weights, its own among them, add up to more than uniform[r] (in [0, 1), what is outside counts as the
+ * nearest) of their sum. weights[r] (float, double for CBHIP_FLOAT64; NULL: not wanted) = its weight among them. Minus infinity
+ * and NaN never take part; a row that has nothing else gets -1 and weight 0. Classes of plus infinity share the whole
+ * weight. At most 2^24 classes. Weights are computed in 64 bits for every type and added as whole numbers of 2^-45 of the best
+ * one's (131072 classes; a bit less for each doubling), so that the order of additions changes nothing. */
+bool CbHipSampleClasses(int valueType, size_t rows, size_t classes, const void* scores, size_t scoreStride, const CbHipSampling* sampling,
+                        const float* uniform, int32_t* indexes, void* weights, void* workspace, size_t workspaceBytes, void* hipStream);
+
 /* Bytes of workspace (at any address that is a multiple of 4) that CbHipSortByExpert needs, 0 for what it would refuse. */
 size_t CbHipSortByExpertBytes(size_t slots, int32_t experts);
 
@@ -303,6 +328,49 @@ bool CbHipCombineRowsBackward(int valueType, size_t rows, size_t width, int32_t 
                               size_t gradientStride, const void* sorted, size_t sortedRows, size_t sortedStride,
                               const int32_t* places, const void* weights, void* sortedGradients,
                               size_t sortedGradientStride, void* weightGradients, void* hipStream);
+
+/* act of a gated projection */
+enum ECbHipActivation {
+    CBHIP_SILU = 0,      /* x / (1 + exp(-x)) */
+    CBHIP_GELU = 1,      /* x * (1 + erf(x / sqrt(2))) / 2 */
+    CBHIP_GELU_TANH = 2, /* x * (1 + tanh(sqrt(2 / pi) * (x + 0.044715 * x^3))) / 2 */
+    CBHIP_RELU = 3,
+};
+
+/* The products of rows sorted by expert, between CbHipDispatchRows and CbHipCombineRows. Expert e (1 to 1024 of them) has rows
+ * offsets[e] to offsets[e + 1] - 1 of the matrices (experts + 1 offsets in device memory, as CbHipSortByExpert gives them; NULL:
+ * one expert has all rows); rows without an expert stay as they are. An expert's weights have a row of `width` values for
+ * each output, without gaps, and begin expertStride values behind those of the expert before it. Products and what follows
+ * them are computed in 32 bits (64 for CBHIP_FLOAT64) and rounded once. Less than 2^31 rows, 2^30 inputs and outputs. */
+
+/* result[r][c] = act(gate) * up, gate = the product of source[r] and row c of its expert's gateWeights, up of its upWeights.
+ * kept (float, double for CBHIP_FLOAT64; NULL: not wanted) = the values that the gradient needs: gate at
+ * kept[r * 2 * hidden + c], up `hidden` behind it. */
+bool CbHipGatedRows(int valueType, int activation, size_t rows, size_t width, size_t hidden, int32_t experts, const int32_t* offsets,
+                    const void* source, size_t sourceStride, const void* gateWeights, const void* upWeights, size_t expertStride,
+                    void* result, size_t resultStride, void* kept, void* hipStream);
+
+/* Its gradients, from what it kept: preGradients of the gate and up values, laid out as `kept` but in the value type (32-bit and
+ * 64-bit ones may be `kept` itself); from those sourceGradients (NULL: not wanted; `gateWeights` and `upWeights` are not read then), and
+ * gateGradients and upGradients (both or neither; `source` is not read then), which are written for experts without rows, and
+ * without rows at all, too. */
+bool CbHipGatedRowsBackward(int valueType, int activation, size_t rows, size_t width, size_t hidden, int32_t experts,
+                            const int32_t* offsets, const void* resultGradients, size_t gradientStride, const void* source,
+                            size_t sourceStride, const void* gateWeights, const void* upWeights, size_t expertStride,
+                            const void* kept, void* preGradients, void* sourceGradients, size_t sourceGradientStride,
+                            void* gateGradients, void* upGradients, size_t expertGradientStride, void* hipStream);
+
+/* result[r][c] = the product of source[r] and row c of its expert's weights. */
+bool CbHipMultiplyRows(int valueType, size_t rows, size_t width, size_t outputs, int32_t experts, const int32_t* offsets,
+                       const void* source, size_t sourceStride, const void* weights, size_t expertStride, void* result,
+                       size_t resultStride, void* hipStream);
+
+/* Its gradients: sourceGradients (NULL: not wanted; `weights` is not read then) and weightGradients (NULL: not wanted; `source` is
+ * not read then), which are written for experts without rows, and without rows at all, too. */
+bool CbHipMultiplyRowsBackward(int valueType, size_t rows, size_t width, size_t outputs, int32_t experts, const int32_t* offsets,
+                               const void* resultGradients, size_t gradientStride, const void* source, size_t sourceStride,
+                               const void* weights, size_t expertStride, void* sourceGradients, size_t sourceGradientStride,
+                               void* weightGradients, size_t expertGradientStride, void* hipStream);
 
 /* Documents that are evaluated by models of their own: deviceResults[doc * dim + k] = sum over j, in their order, of
  * deviceWeights[doc * perDoc + j] (NULL: 1) times raw value k of evaluator deviceExperts[doc * perDoc + j] (all its trees, as

@@ -274,16 +274,16 @@ def _own_gated(s, cb, code, stream):
     case, x = s["case"], s["source"]
     rows, width, hidden, experts = case["rows"], case["width"], case["hidden"], case["experts"]
     activation, offsets, of_expert = ACTIVATIONS[case["activation"]], _at(s, "offsets"), hidden * width
-    # what the backward pass needs of the forward one: the rows' gate and up values
-    kept = torch.empty(rows, 2 * hidden, dtype=x.dtype, device=DEVICE) if case["backward"] else None
+    # what the backward pass needs of the forward one: the rows' gate and up values, in 32 bits at least
+    kept = torch.empty(rows, 2 * hidden, dtype=torch.promote_types(x.dtype, torch.float32), device=DEVICE) if case["backward"] else None
     cb.gated_rows(code, activation, rows, width, hidden, experts, offsets, x.data_ptr(), width, s["gate"].data_ptr(), s["up"].data_ptr(), of_expert,
                   s["result"].data_ptr(), hidden, 0 if kept is None else kept.data_ptr(), stream)
     out = [s["result"]]
     if kept is not None:
         dgate, dup = torch.empty_like(s["gate"]), torch.empty_like(s["up"])
-        # the gradients of the gate and up values take the place of the values
+        pre = torch.empty(rows, 2 * hidden, dtype=x.dtype, device=DEVICE)  # the gradients of those values
         cb.gated_rows_backward(code, activation, rows, width, hidden, experts, offsets, s["gradients"].data_ptr(), hidden, x.data_ptr(), width,
-                               s["gate"].data_ptr(), s["up"].data_ptr(), of_expert, kept.data_ptr(), kept.data_ptr(),
+                               s["gate"].data_ptr(), s["up"].data_ptr(), of_expert, kept.data_ptr(), pre.data_ptr(),
                                s["source_gradients"].data_ptr(), width, dgate.data_ptr(), dup.data_ptr(), of_expert, stream)
         out += [s["source_gradients"], dgate, dup]
     return out

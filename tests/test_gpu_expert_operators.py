@@ -77,7 +77,8 @@ def product_bound(a, b, kind, extra=0):
 
 # rows, width, outputs, experts, rows behind the last
 SHAPES = [(1, 1, 1, 1, 0), (3, 8, 16, 2, 0), (5, 3, 7, 2, 1), (17, 33, 31, 3, 2), (64, 64, 64, 1, 0), (131, 65, 130, 3, 5), (300, 128, 272, 4, 0),
-          (700, 40, 10, 37, 20), (257, 96, 520, 70, 3), (40, 264, 129, 5, 0), (14, 1024, 96, 16, 2), (150, 24, 2, 2, 0)]
+          (700, 40, 10, 37, 20), (257, 96, 520, 70, 3), (40, 264, 129, 5, 0), (14, 1024, 96, 16, 2), (150, 24, 2, 2, 0),
+          (520, 64, 256, 1, 0), (600, 200, 264, 3, 7), (1100, 56, 328, 2, 0), (260, 136, 8, 1, 0)]
 
 
 def multiply(kind, x, w, offsets, result, rows=None):

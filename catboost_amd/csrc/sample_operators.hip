@@ -1,13 +1,20 @@
 // A class of every row drawn by the softmax of its scores, of the classes that temperature, rank, share and least weight leave.
 //
 // All limits and the draw itself are positions in one order: best score first, of equal ones the lowest class first. A limit is a sum of
-// weights from the front of that order, the draw is the first class whose sum passes uniform * the smallest of those sums. So no
-// row is sorted: a position is found digit by digit, from sums of weights by the leading bits of the scores' keys. Weights are
-// exp((x - best) / temperature) in 64 bits, added as whole numbers: sums do not depend on their order.
+// weights from the front of that order, the draw is the first class whose sum passes uniform * the smallest of those sums. Weights are
+// 2^-t, t = (best - x) / temperature * log2(e), in 64 bits, added as whole numbers: sums do not depend on their order, so a class is the
+// same whichever way it is found. Short rows are sorted, in a thread's registers or a wave's; of long ones only the sums of weights
+// around the positions are needed: by how often each key comes (16 bits), or by t and then by the keys of the part where a
+// position is.
 #include "operator_common.hip.h"
 
 #include <algorithm>
+#include <limits>
 #include <type_traits>
+#ifndef LANES512
+#define LANES512 512
+#define LANES1024 1024
+#endif
 
 namespace cbamd {
 namespace op {
@@ -40,101 +47,63 @@ private:
     }
 };
 
-// The weight of a score beside the row's best one
+constexpr uint32_t kPowers = 64;
+
+// 2^(-i / 64), which a workgroup computes for its weights
+__device__ __forceinline__ void FillPowers(double* powers) {
+    if (threadIdx.x < kPowers) {
+        powers[threadIdx.x] = exp2(static_cast<double>(threadIdx.x) * -0.015625);
+    }
+}
+
+// The weights of a row's scores
 struct TWeigh {
-    double Best, Rate;  // 1 / temperature
-    double Unit;        // 2^shift: how many whole numbers a weight of 1 is
+    double Best;           // the best score
+    double Rate;           // log2(e) / temperature
+    double Unit;           // 2^shift: how many whole numbers a weight of 1 is, at most 2^51
+    const double* Powers;  // in LDS
 
-    __device__ __forceinline__ double Weight(double x) const {
+    // How far under the best one, in powers of two; never less for a smaller score
+    template <typename T>
+    __device__ __forceinline__ double Under(T x) const {
         if (Best == __builtin_inf()) {
-            return x == Best ? 1.0 : 0.0;
+            return static_cast<double>(x) == Best ? 0.0 : 4096.0;
         }
-        // (a difference of the largest scores may pass the largest number, which no temperature is to turn into NaN)
-        return exp(fmax(x - Best, -1.7976931348623157e308) * Rate);
+        double under = Best - static_cast<double>(x);
+        if constexpr (std::is_same_v<T, double>) {
+            // (may pass the largest number, which no temperature is to turn into NaN)
+            under = fmin(under, 1.7976931348623157e308);
+        }
+        return fmin(under * Rate, 4096.0);
     }
+    // 2^-under: the nearest 64th from the table, the rest, under 1/128, by the series of exp up to its fifth power (its sixth is
+    // under 2^-54). About a third of the steps of exp, which is most of what a row of 100000 classes costs.
+    __device__ __forceinline__ double Weight(double under) const {
+        const double steps = rint(under * kPowers);
+        const double y = fma(steps, 0.015625, -under) * 0.69314718055994530942;
+        const int n = static_cast<int>(steps);
+        double e = fma(y, 1.0 / 120, 1.0 / 24);
+        e = fma(e, y, 1.0 / 6);
+        e = fma(e, y, 0.5);
+        e = fma(e, y, 1.0);
+        e = fma(e, y, 1.0);
+        return ldexp(e * Powers[n & (kPowers - 1)], -(n >> 6));
+    }
+    // (what adding 2^52 leaves in the last bits is the nearest whole number)
     __device__ __forceinline__ uint64_t Whole(double weight) const {
-        return static_cast<uint64_t>(weight * Unit + 0.5);
+        return __builtin_bit_cast(uint64_t, fma(weight, Unit, 4503599627370496.0)) & 0xfffffffffffffull;
+    }
+    template <typename T>
+    __device__ __forceinline__ uint64_t WholeOf(T x) const {
+        return Whole(Weight(Under(x)));
     }
 };
 
-// ---------------------------------------------------------------- one workgroup for a row ----
-
-constexpr uint32_t kDigitBits = 11, kDigits = 1u << kDigitBits;
-
-struct TDigitSums {
-    uint64_t Weights[kDigits];
-    uint32_t Counts[kDigits];
-};
-
-// Sums over a workgroup of WAVES waves; every lane gets them
-template <int WAVES>
-__device__ __forceinline__ uint64_t SumOf(uint64_t v, uint64_t* shared) {
-#pragma unroll
-    for (int d = 32; d > 0; d /= 2) {
-        v += __shfl_xor(v, d);
-    }
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) {
-        shared[threadIdx.x >> 6] = v;
-    }
-    __syncthreads();
-    v = 0;
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-        v += shared[w];
-    }
-    return v;
-}
-template <int WAVES, typename TKey>
-__device__ __forceinline__ TKey MostOf(TKey v, uint64_t* shared) {
-#pragma unroll
-    for (int d = 32; d > 0; d /= 2) {
-        const TKey other = __shfl_xor(v, d);
-        v = other > v ? other : v;
-    }
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) {
-        shared[threadIdx.x >> 6] = v;
-    }
-    __syncthreads();
-    v = 0;
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-        const TKey other = static_cast<TKey>(shared[w]);
-        v = other > v ? other : v;
-    }
-    return v;
-}
-
-// f(score, class) for this thread's scores of a row, 16 bytes at a time
-template <typename T, int THREADS, typename F>
-__device__ __forceinline__ void ForRow(const T* row, uint32_t classes, F&& f) {
-    constexpr uint32_t N = 16 / sizeof(T);
-    const uint32_t whole = classes / N;
-    for (uint32_t c = threadIdx.x; c < whole; c += THREADS) {
-        const auto v = TValues<T, N>::Load(row + c * N);
-#pragma unroll
-        for (uint32_t i = 0; i < N; ++i) {
-            f(v.V[i], c * N + i);
-        }
-    }
-    for (uint32_t c = whole * N + threadIdx.x; c < classes; c += THREADS) {
-        f(row[c], c);
-    }
-}
-
-// A position in a row's order: the key there, how many classes and which weights are before those of that key
-template <typename TKey>
-struct TPosition {
-    TKey Key;
-    uint32_t Before, Alike;
-    uint64_t WeightBefore;
-};
-
+// Arguments of a launch, and what they say of a row
 struct TSampleArguments {
-    size_t First;  // row of the launch
+    size_t First, Rows;  // of the launch
     uint32_t Classes;
-    uint32_t Shift;  // whole numbers of a weight of 1: 2^Shift
+    uint32_t Shift;
     size_t Stride;
     CbHipSampling Sampling;
     const float* Uniform;
@@ -142,238 +111,937 @@ struct TSampleArguments {
     void* Weights;
 };
 
+struct TLimits {
+    float Temperature, TopP, Uniform;
+    int32_t TopK;
+    double MinP;
+
+    __device__ __forceinline__ TLimits(const TSampleArguments& p, size_t r)
+        : Temperature(p.Sampling.Temperature != nullptr ? p.Sampling.Temperature[r] : 1.0f)
+        , TopP(p.Sampling.TopP != nullptr ? p.Sampling.TopP[r] : 1.0f)
+        , Uniform(p.Uniform[r])
+        , TopK(p.Sampling.TopK != nullptr ? p.Sampling.TopK[r] : 0)
+    {
+        const float least = p.Sampling.MinP != nullptr ? p.Sampling.MinP[r] : 0.0f;
+        MinP = least > 0 ? (least < 1 ? static_cast<double>(least) : 1.0) : 0.0;
+    }
+    __device__ __forceinline__ bool Greedy() const {
+        return !(Temperature > 0);
+    }
+    __device__ __forceinline__ TWeigh Weigh(double best, uint32_t shift, const double* powers) const {
+        return TWeigh{best, 1.44269504088896340736 / static_cast<double>(Temperature), static_cast<double>(uint64_t(1) << shift), powers};
+    }
+    // The sum that the classes of the share reach first, of `all`
+    __device__ __forceinline__ uint64_t ShareOf(uint64_t all) const {
+        const double share = ceil((TopP > 0 ? static_cast<double>(TopP) : 0.0) * static_cast<double>(all));
+        return share < 1 ? 1 : share < static_cast<double>(all) ? static_cast<uint64_t>(share) : all;
+    }
+    // The sum that the drawn class is the first to reach, of those kept
+    __device__ __forceinline__ uint64_t DrawOf(uint64_t kept) const {
+        const double passed = (Uniform > 0 ? static_cast<double>(Uniform) : 0.0) * static_cast<double>(kept);
+        return (passed < static_cast<double>(kept) && static_cast<uint64_t>(passed) < kept ? static_cast<uint64_t>(passed) : kept - 1) + 1;
+    }
+};
+
+template <typename T>
+__device__ __forceinline__ void Answer(const TSampleArguments& p, size_t r, int32_t index, double weight) {
+    p.Indexes[r] = index;
+    if (p.Weights != nullptr) {
+        static_cast<TAcc<T>*>(p.Weights)[r] = static_cast<TAcc<T>>(weight);
+    }
+}
+
+// ---------------------------------------------------------------- a thread for a row ----
+
+// Rows of exactly C classes, sorted in registers by neighbours that trade places, which keeps equal ones in order
+template <typename T, int C>
+__global__ void __launch_bounds__(256) SampleOfFewKernel(const T* scores, TSampleArguments p) {
+    using A = TAcc<T>;
+    __shared__ double powers[kPowers];
+    FillPowers(powers);
+    __syncthreads();
+    const size_t n = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x;
+    if (n >= p.Rows) {
+        return;
+    }
+    const size_t r = p.First + n;
+    const T* row = scores + r * p.Stride;
+    constexpr A kNone = -std::numeric_limits<A>::infinity();
+    A x[C];
+    int32_t index[C];
+    constexpr int N = std::min<int>(C, 16 / sizeof(T));
+#pragma unroll
+    for (int c = 0; c < C; c += N) {
+        // (a last piece that overlaps the one before it)
+        const int from = c + N <= C ? c : C - N;
+        const auto v = TValues<T, N>::Load(row + from);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const A value = static_cast<A>(v.V[i]);
+            x[from + i] = value == value ? value + A(0) : kNone;  // (one zero of both)
+        }
+    }
+    const TLimits limits(p, r);
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        index[c] = c;
+    }
+#pragma unroll
+    for (int round = 0; round < C; ++round) {
+#pragma unroll
+        for (int c = round & 1; c + 1 < C; c += 2) {
+            const bool trade = x[c + 1] > x[c];
+            const A high = trade ? x[c + 1] : x[c], low = trade ? x[c] : x[c + 1];
+            const int32_t first = trade ? index[c + 1] : index[c], second = trade ? index[c] : index[c + 1];
+            x[c] = high;
+            x[c + 1] = low;
+            index[c] = first;
+            index[c + 1] = second;
+        }
+    }
+    if (x[0] == kNone) {
+        return Answer<T>(p, r, -1, 0);
+    }
+    if (limits.Greedy()) {
+        return Answer<T>(p, r, index[0], 1);
+    }
+    const TWeigh weigh = limits.Weigh(static_cast<double>(x[0]), p.Shift, powers);
+    double weight[C];
+    uint64_t sum[C], all = 0, likely = 0;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        weight[c] = x[c] > kNone ? weigh.Weight(weigh.Under(x[c])) : 0.0;
+        const uint64_t whole = weigh.Whole(weight[c]);
+        all += limits.TopK <= 0 || c < limits.TopK ? whole : 0;
+        likely += weight[c] >= limits.MinP ? whole : 0;
+        sum[c] = (c > 0 ? sum[c > 0 ? c - 1 : 0] : 0) + whole;
+    }
+    uint64_t kept = all < likely ? all : likely;
+    if (limits.TopP < 1) {
+        const uint64_t target = limits.ShareOf(all);
+        uint64_t reached = all;
+#pragma unroll
+        for (int c = C - 1; c >= 0; --c) {
+            reached = sum[c] >= target ? sum[c] : reached;
+        }
+        kept = reached < kept ? reached : kept;
+    }
+    const uint64_t target = limits.DrawOf(kept);
+    int32_t found = index[C - 1];
+    double foundWeight = weight[C - 1];
+#pragma unroll
+    for (int c = C - 2; c >= 0; --c) {
+        const bool there = sum[c] >= target;
+        found = there ? index[c] : found;
+        foundWeight = there ? weight[c] : foundWeight;
+    }
+    Answer<T>(p, r, found, foundWeight * weigh.Unit / static_cast<double>(kept));
+}
+
+// ---------------------------------------------------------------- lanes for a row ----
+
+// A key and its class as one value that orders them, the lowest class first: 32 bits for 16-bit scores, 64 for 32-bit ones
+template <typename T>
+struct TOrdered {
+    using TKey = typename TKeys<T>::TKey;
+    using TWord = std::conditional_t<sizeof(T) == 2, uint32_t, uint64_t>;
+    TWord Word;
+
+    __device__ __forceinline__ static TOrdered Of(TKey key, uint32_t index) {
+        constexpr int kShift = sizeof(T) == 2 ? 16 : 32;
+        return {static_cast<TWord>(key) << kShift | (~index & static_cast<uint32_t>((TWord(1) << kShift) - 1))};
+    }
+    __device__ __forceinline__ TKey Key() const {
+        return static_cast<TKey>(Word >> (sizeof(T) == 2 ? 16 : 32));
+    }
+    __device__ __forceinline__ uint32_t Index() const {
+        return ~static_cast<uint32_t>(Word) & (sizeof(T) == 2 ? 0xffffu : ~0u);
+    }
+    __device__ __forceinline__ bool Before(const TOrdered& other) const {
+        return Word > other.Word;
+    }
+    __device__ __forceinline__ TOrdered Across(int lanes) const {
+        return {static_cast<TWord>(__shfl_xor(Word, lanes))};
+    }
+};
+template <>
+struct TOrdered<double> {
+    uint64_t Word;
+    uint32_t Class;
+
+    __device__ __forceinline__ static TOrdered Of(uint64_t key, uint32_t index) {
+        return {key, index};
+    }
+    __device__ __forceinline__ uint64_t Key() const {
+        return Word;
+    }
+    __device__ __forceinline__ uint32_t Index() const {
+        return Class;
+    }
+    __device__ __forceinline__ bool Before(const TOrdered& other) const {
+        return Word > other.Word || (Word == other.Word && Class < other.Class);
+    }
+    __device__ __forceinline__ TOrdered Across(int lanes) const {
+        return {static_cast<uint64_t>(__shfl_xor(Word, lanes)), static_cast<uint32_t>(__shfl_xor(Class, lanes))};
+    }
+};
+
+// Rows of at most LANES * P classes: place i of the order ends up as value i % P of lane i / P
+template <typename T, int LANES, int P>
+__global__ void __launch_bounds__(256) SampleByLanesKernel(const T* scores, TSampleArguments p) {
+    using TK = TKeys<T>;
+    using TItem = TOrdered<T>;
+    constexpr int kPlaces = LANES * P;
+    __shared__ double powers[kPowers];
+    FillPowers(powers);
+    __syncthreads();
+    const uint32_t lane = threadIdx.x % LANES;
+    const size_t n = static_cast<size_t>(blockIdx.x) * (256 / LANES) + threadIdx.x / LANES;
+    // (rows behind the last one do as it does, so that every lane is there to be read, and store nothing)
+    const size_t r = p.First + (n < p.Rows ? n : p.Rows - 1);
+    const T* row = scores + r * p.Stride;
+    const TLimits limits(p, r);
+    TItem item[P];
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+        const uint32_t c = lane + i * LANES;
+        item[i] = TItem::Of(c < p.Classes ? TK::Of(row[c]) : 0, c);
+    }
+    // runs of `size` places, each the other way round than the next, are merged to ones of twice that
+#pragma unroll
+    for (int size = 2; size <= kPlaces; size *= 2) {
+#pragma unroll
+        for (int step = size / 2; step > 0; step /= 2) {
+            if (step >= P) {
+                const bool low = (lane & (step / P)) == 0, down = (lane * P & size) == 0;
+#pragma unroll
+                for (int i = 0; i < P; ++i) {
+                    const TItem other = item[i].Across(step / P);
+                    item[i] = item[i].Before(other) == (low == down) ? item[i] : other;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < P; ++i) {
+                    if ((i & step) == 0) {
+                        const bool down = ((lane * P + i) & size) == 0;
+                        const TItem a = item[i], b = item[i + step];
+                        const bool trade = a.Before(b) != down;
+                        item[i] = trade ? b : a;
+                        item[i + step] = trade ? a : b;
+                    }
+                }
+            }
+        }
+    }
+    const bool mine = n < p.Rows && lane == 0;
+    const uint32_t base = threadIdx.x & 63 & ~(LANES - 1);  // the row's first lane in its wave
+    const TItem best{item[0]};
+    const auto bestKey = __shfl(best.Key(), base);
+    const uint32_t bestClass = __shfl(best.Index(), base);
+    if (bestKey == 0 || limits.Greedy()) {
+        if (mine) {
+            Answer<T>(p, r, bestKey == 0 ? -1 : static_cast<int32_t>(bestClass), bestKey == 0 ? 0 : 1);
+        }
+    }
+    // (every lane goes on: rows of a wave differ; the values of such a row are not used)
+    TWeigh weigh = limits.Weigh(TK::Value(bestKey), p.Shift, powers);
+    weigh.Rate = limits.Greedy() ? 0 : weigh.Rate;
+    double weight[P];
+    uint64_t sum[P], all = 0, likely = 0, total = 0;
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+        const auto key = item[i].Key();
+        weight[i] = key != 0 ? weigh.Weight(weigh.Under(static_cast<T>(TK::Value(key)))) : 0.0;
+        const uint64_t whole = weigh.Whole(weight[i]);
+        all += limits.TopK <= 0 || lane * P + i < static_cast<uint32_t>(limits.TopK) ? whole : 0;
+        likely += weight[i] >= limits.MinP ? whole : 0;
+        total += whole;
+        sum[i] = total;
+    }
+    uint64_t before = total;
+#pragma unroll
+    for (int d = 1; d < LANES; d *= 2) {
+        const uint64_t other = __shfl_up(before, d, LANES), otherAll = __shfl_xor(all, d), otherLikely = __shfl_xor(likely, d);
+        before += lane >= static_cast<uint32_t>(d) ? other : 0;
+        all += otherAll;
+        likely += otherLikely;
+    }
+    before -= total;
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+        sum[i] += before;
+    }
+    // the value at the place that reaches a sum first
+    const auto at = [&](uint64_t target, auto&& valueOf) {
+        const uint64_t there = __ballot(before < target && sum[P - 1] >= target);
+        auto value = valueOf(P - 1);
+#pragma unroll
+        for (int i = P - 2; i >= 0; --i) {
+            value = sum[i] >= target ? valueOf(i) : value;
+        }
+        const uint64_t ofRow = LANES == 64 ? there : there >> base & ((uint64_t(1) << (LANES & 63)) - 1);
+        return __shfl(value, base + (ofRow != 0 ? __ffsll(static_cast<unsigned long long>(ofRow)) - 1 : 0));
+    };
+    uint64_t kept = all < likely ? all : likely;
+    if (p.Sampling.TopP != nullptr) {
+        const uint64_t reached = at(limits.ShareOf(all), [&](int i) { return sum[i]; });
+        kept = limits.TopP < 1 && reached < kept ? reached : kept;
+    }
+    const uint64_t target = limits.DrawOf(kept);
+    const uint32_t index = at(target, [&](int i) { return item[i].Index(); });
+    const double foundWeight = at(target, [&](int i) { return weight[i]; });
+    if (mine && bestKey != 0 && !limits.Greedy()) {
+        Answer<T>(p, r, static_cast<int32_t>(index), foundWeight * weigh.Unit / static_cast<double>(kept));
+    }
+}
+
+// ---------------------------------------------------------------- a workgroup for a row ----
+
+// Sums by a digit of BITS bits
+template <int BITS>
+struct TDigitSums {
+    uint64_t Weights[1 << BITS];
+    uint32_t Counts[1 << BITS];
+
+    template <int THREADS>
+    __device__ __forceinline__ void Clear() {
+        for (uint32_t d = threadIdx.x; d < 1u << BITS; d += THREADS) {
+            Weights[d] = 0;
+            Counts[d] = 0;
+        }
+    }
+    __device__ __forceinline__ void Add(uint32_t digit, uint64_t weight) {
+        atomicAdd(reinterpret_cast<unsigned long long*>(&Weights[digit]), static_cast<unsigned long long>(weight));
+        atomicAdd(&Counts[digit], 1u);
+    }
+};
+
+// What the waves of a workgroup hand each other
+template <int WAVES>
+struct TShared {
+    uint64_t Sums[WAVES];
+    uint64_t Found[4];
+    uint32_t Counted[WAVES];
+    uint32_t Listed;
+    double Powers[kPowers];
+};
+
+// Sums and maxima over a workgroup; every lane gets them
+template <int WAVES>
+__device__ __forceinline__ uint64_t SumOf(uint64_t v, TShared<WAVES>& shared) {
+#pragma unroll
+    for (int d = 32; d > 0; d /= 2) {
+        v += __shfl_xor(v, d);
+    }
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) {
+        shared.Sums[threadIdx.x >> 6] = v;
+    }
+    __syncthreads();
+    v = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+        v += shared.Sums[w];
+    }
+    return v;
+}
+template <int WAVES, typename TKey>
+__device__ __forceinline__ TKey MostOf(TKey v, TShared<WAVES>& shared) {
+#pragma unroll
+    for (int d = 32; d > 0; d /= 2) {
+        const TKey other = __shfl_xor(v, d);
+        v = other > v ? other : v;
+    }
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) {
+        shared.Sums[threadIdx.x >> 6] = v;
+    }
+    __syncthreads();
+    v = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+        const TKey other = static_cast<TKey>(shared.Sums[w]);
+        v = other > v ? other : v;
+    }
+    return v;
+}
+// The sum over the threads before this one
+template <int WAVES>
+__device__ __forceinline__ uint64_t SumBefore(uint64_t mine, TShared<WAVES>& shared) {
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint64_t sum = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const uint64_t other = __shfl_up(sum, d);
+        sum += lane >= static_cast<uint32_t>(d) ? other : 0;
+    }
+    __syncthreads();
+    if (lane == 63) {
+        shared.Sums[wave] = sum;
+    }
+    __syncthreads();
+    uint64_t before = sum - mine;
+    for (uint32_t w = 0; w < wave; ++w) {
+        before += shared.Sums[w];
+    }
+    return before;
+}
+
+// f(score, class) for this thread's scores of a row, 16 bytes at a time, two of them on their way
+template <typename T, int THREADS, typename F>
+__device__ __forceinline__ void ForRow(const T* row, uint32_t classes, F&& f) {
+    constexpr uint32_t N = 16 / sizeof(T);
+    const uint32_t whole = classes / N;
+    uint32_t c = threadIdx.x;
+    for (; c + THREADS < whole; c += 2 * THREADS) {
+        const auto v = TValues<T, N>::Load(row + c * N), w = TValues<T, N>::Load(row + (c + THREADS) * N);
+#pragma unroll
+        for (uint32_t i = 0; i < N; ++i) {
+            f(v.V[i], c * N + i);
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < N; ++i) {
+            f(w.V[i], (c + THREADS) * N + i);
+        }
+    }
+    if (c < whole) {
+        const auto v = TValues<T, N>::Load(row + c * N);
+#pragma unroll
+        for (uint32_t i = 0; i < N; ++i) {
+            f(v.V[i], c * N + i);
+        }
+    }
+    for (c = whole * N + threadIdx.x; c < classes; c += THREADS) {
+        f(row[c], c);
+    }
+}
+
+// A position in a row's order: the key there, how many classes and which weights are before those of that key, how many have it
+template <typename TKey>
+struct TPosition {
+    TKey Key;
+    uint32_t Before, Alike;
+    uint64_t WeightBefore;
+};
+
+// The position in sums by digits where the count or the weights reach `target`, which they do in one of them; the digit's class counts
+// and weights are added to what `at` has before it
+template <int BITS, int THREADS, typename TKey>
+__device__ __forceinline__ uint32_t ReachDigit(const TDigitSums<BITS>& sums, bool byCount, uint64_t target, TPosition<TKey>& at, TShared<THREADS / 64>& shared) {
+    constexpr uint32_t kMine = (1u << BITS) / THREADS;
+    uint64_t weights = 0, counts = 0;
+    const uint32_t begin = threadIdx.x * kMine;
+#pragma unroll
+    for (uint32_t d = 0; d < kMine; ++d) {
+        weights += sums.Weights[begin + d];
+        counts += sums.Counts[begin + d];
+    }
+    uint64_t weightBefore = SumBefore<THREADS / 64>(weights, shared) + at.WeightBefore;
+    uint64_t countBefore = SumBefore<THREADS / 64>(counts, shared) + at.Before;
+    uint64_t& before = byCount ? countBefore : weightBefore;
+    if (before < target && before + (byCount ? counts : weights) >= target) {
+        uint32_t d = begin;
+        for (; d + 1 < begin + kMine; ++d) {
+            if (before + (byCount ? sums.Counts[d] : sums.Weights[d]) >= target) {
+                break;
+            }
+            weightBefore += sums.Weights[d];
+            countBefore += sums.Counts[d];
+        }
+        shared.Found[0] = d;
+        shared.Found[1] = weightBefore;
+        shared.Found[2] = countBefore;
+        shared.Found[3] = sums.Counts[d];
+    }
+    __syncthreads();
+    at.WeightBefore = shared.Found[1];
+    at.Before = static_cast<uint32_t>(shared.Found[2]);
+    at.Alike = static_cast<uint32_t>(shared.Found[3]);
+    return static_cast<uint32_t>(shared.Found[0]);
+}
+
+// The (nth + 1)-th class with this key
 template <typename T, int THREADS>
+__device__ int32_t ClassOf(const T* row, uint32_t classes, typename TKeys<T>::TKey key, uint32_t nth, TShared<THREADS / 64>& shared) {
+    using TK = TKeys<T>;
+    constexpr uint32_t kWaves = THREADS / 64;
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    // which wave's part of the row has it, then which thread's part of that
+    const uint32_t part = (classes + kWaves - 1) / kWaves;
+    uint32_t begin = wave * part, end = begin + part < classes ? begin + part : classes, n = 0;
+    for (uint32_t c = begin + lane; c < end; c += 64) {
+        n += TK::Of(row[c]) == key;
+    }
+#pragma unroll
+    for (int d = 32; d > 0; d /= 2) {
+        n += __shfl_xor(n, d);
+    }
+    __syncthreads();
+    if (lane == 0) {
+        shared.Counted[wave] = n;
+    }
+    __syncthreads();
+    uint32_t w = 0;
+    while (w + 1 < kWaves && nth >= shared.Counted[w]) {
+        nth -= shared.Counted[w++];
+    }
+    begin = w * part;
+    end = begin + part < classes ? begin + part : classes;
+    const uint32_t each = (part + THREADS - 1) / THREADS;
+    const uint32_t mine = begin + threadIdx.x * each, last = mine + each < end ? mine + each : end;
+    n = 0;
+    for (uint32_t c = mine; c < last; ++c) {
+        n += TK::Of(row[c]) == key;
+    }
+    uint32_t before = static_cast<uint32_t>(SumBefore<kWaves>(n, shared));
+    if (nth >= before && nth < before + n) {
+        for (uint32_t c = mine; c < last; ++c) {
+            if (TK::Of(row[c]) == key && before++ == nth) {
+                shared.Found[0] = c;
+            }
+        }
+    }
+    __syncthreads();
+    return static_cast<int32_t>(shared.Found[0]);
+}
+
+// From sums up to positions: the row's limits, then its class. reach(byCount, target) -> TPosition, where the count or the weights from
+// the front of the order, its own among them, reach `target`; classAt(position, nth) -> class. `all`: every weight's sum, `likely`: of
+// those that MinP leaves, `there`: how many classes take part
+template <typename T, typename TReach, typename TClass>
+__device__ __forceinline__ void DrawFrom(const TSampleArguments& p, size_t r, const TLimits& limits, const TWeigh& weigh, uint64_t all, uint64_t likely,
+                                         uint64_t there, TReach&& reach, TClass&& classAt) {
+    using TK = TKeys<T>;
+    const auto wholeOf = [&](typename TK::TKey key) { return weigh.WholeOf(static_cast<T>(TK::Value(key))); };
+    if (limits.TopK > 0 && static_cast<uint64_t>(limits.TopK) < there) {
+        const auto at = reach(true, static_cast<uint64_t>(limits.TopK));
+        all = at.WeightBefore + (static_cast<uint32_t>(limits.TopK) - at.Before) * wholeOf(at.Key);
+    }
+    uint64_t kept = all < likely ? all : likely;
+    if (limits.TopP < 1) {
+        const uint64_t target = limits.ShareOf(all);
+        const auto at = reach(false, target);
+        const uint64_t whole = wholeOf(at.Key);
+        const uint64_t sum = at.WeightBefore + ((target - at.WeightBefore + whole - 1) / whole) * whole;
+        kept = sum < kept ? sum : kept;
+    }
+    const uint64_t target = limits.DrawOf(kept);
+    const auto at = reach(false, target);
+    const double weight = weigh.Weight(weigh.Under(static_cast<T>(TK::Value(at.Key))));
+    const int32_t index = classAt(at, static_cast<uint32_t>((target - 1 - at.WeightBefore) / weigh.Whole(weight)));
+    if (threadIdx.x == 0) {
+        Answer<T>(p, r, index, weight * weigh.Unit / static_cast<double>(kept));
+    }
+}
+
+// Positions by the digits of how far a key is under the best one, with a pass over the row for each digit but the first: what takes
+// any row, however many of its classes are alike
+template <typename T, int THREADS, int BITS>
+__device__ void DrawByDigits(const T* row, const TSampleArguments& p, size_t r, const TLimits& limits, const TWeigh& weigh, typename TKeys<T>::TKey most,
+                             uint64_t all, uint64_t likely, uint64_t there, TDigitSums<BITS>& sums, TShared<THREADS / 64>& shared) {
+    using TK = TKeys<T>;
+    using TKey = typename TK::TKey;
+    constexpr int kLevels = (TK::kBits + BITS - 1) / BITS;
+    const auto reach = [&](bool byCount, uint64_t target) {
+        TPosition<TKey> at{0, 0, 0, 0};
+        TKey prefix = 0;  // the digits so far
+        for (int level = kLevels - 1; level >= 0; --level) {
+            const uint32_t shift = level * BITS;
+            __syncthreads();
+            sums.template Clear<THREADS>();
+            __syncthreads();
+            ForRow<T, THREADS>(row, p.Classes, [&](T x, uint32_t) {
+                const TKey key = TK::Of(x), under = most - key;
+                if (key != 0 && (level == kLevels - 1 || under >> (shift + BITS) == prefix)) {
+                    sums.Add(static_cast<uint32_t>(under >> shift) & ((1u << BITS) - 1), weigh.WholeOf(x));
+                }
+            });
+            __syncthreads();
+            prefix = prefix << BITS | ReachDigit<BITS, THREADS>(sums, byCount, target, at, shared);
+        }
+        at.Key = most - prefix;
+        return at;
+    };
+    DrawFrom<T>(p, r, limits, weigh, all, likely, there, reach,
+                [&](const TPosition<TKey>& at, uint32_t nth) { return ClassOf<T, THREADS>(row, p.Classes, at.Key, nth, shared); });
+}
+
+// Positions by t first, in steps of 52 / 2^BITS of a power of two. The classes of the step where a position is are listed, their keys
+// told apart digit by digit, from the list.
+template <typename T, int THREADS, int BITS, int LIST>
 __global__ void __launch_bounds__(THREADS) SampleRowKernel(const T* scores, TSampleArguments p) {
     using TK = TKeys<T>;
     using TKey = typename TK::TKey;
-    constexpr int kWaves = THREADS / 64;
-    constexpr uint32_t kMine = kDigits / THREADS;
-    __shared__ TDigitSums first, later;
-    __shared__ uint64_t shared[kWaves];
-    __shared__ uint64_t found[4];
-    __shared__ uint32_t counted[kWaves];
+    constexpr uint32_t kDigits = 1u << BITS;
+    __shared__ TDigitSums<BITS> first, later;
+    __shared__ TShared<THREADS / 64> shared;
+    __shared__ TKey keys[LIST];
+    __shared__ uint32_t listed[LIST];
+
+    const size_t r = p.First + blockIdx.x;
+    const T* row = scores + r * p.Stride;
+    FillPowers(shared.Powers);
+    first.template Clear<THREADS>();
+    TKey most = 0;
+    ForRow<T, THREADS>(row, p.Classes, [&](T x, uint32_t) {
+        const TKey key = TK::Of(x);
+        most = key > most ? key : most;
+    });
+    most = MostOf<THREADS / 64>(most, shared);
+    if (most == 0) {
+        if (threadIdx.x == 0) {
+            Answer<T>(p, r, -1, 0);
+        }
+        return;
+    }
+    const TLimits limits(p, r);
+    if (limits.Greedy()) {
+        const int32_t index = ClassOf<T, THREADS>(row, p.Classes, most, 0, shared);
+        if (threadIdx.x == 0) {
+            Answer<T>(p, r, index, 1);
+        }
+        return;
+    }
+    const TWeigh weigh = limits.Weigh(TK::Value(most), p.Shift, shared.Powers);
+    const auto stepOf = [&](double under) {
+        const uint32_t step = static_cast<uint32_t>(under * (kDigits / 52.0));
+        return step < kDigits ? step : kDigits - 1;
+    };
+    uint64_t all = 0, likely = 0, there = 0;
+    ForRow<T, THREADS>(row, p.Classes, [&](T x, uint32_t) {
+        if (TK::Of(x) != 0) {
+            const double under = weigh.Under(x), weight = weigh.Weight(under);
+            const uint64_t whole = weigh.Whole(weight);
+            ++there;
+            all += whole;
+            likely += weight >= limits.MinP ? whole : 0;
+            first.Add(stepOf(under), whole);
+        }
+    });
+    all = SumOf(all, shared);
+    likely = SumOf(likely, shared);
+    there = SumOf(there, shared);
+
+    // (most classes of a step; more than the list holds: by the keys alone)
+    uint32_t longest = 0;
+    for (uint32_t d = threadIdx.x; d < kDigits; d += THREADS) {
+        longest = first.Counts[d] > longest ? first.Counts[d] : longest;
+    }
+    // the last step has what weighs nothing: no position is there but one by count
+    if (MostOf(longest, shared) > LIST) {
+        return DrawByDigits<T, THREADS, BITS>(row, p, r, limits, weigh, most, all, likely, there, later, shared);
+    }
+    uint32_t listedStep = kDigits;
+    const auto reach = [&](bool byCount, uint64_t target) {
+        TPosition<TKey> at{0, 0, 0, 0};
+        const uint32_t step = ReachDigit<BITS, THREADS>(first, byCount, target, at, shared);
+        __syncthreads();
+        if (step != listedStep) {
+            if (threadIdx.x == 0) {
+                shared.Listed = 0;
+            }
+            __syncthreads();
+            ForRow<T, THREADS>(row, p.Classes, [&](T x, uint32_t c) {
+                const TKey key = TK::Of(x);
+                if (key != 0 && stepOf(weigh.Under(x)) == step) {
+                    const uint32_t place = atomicAdd(&shared.Listed, 1u);
+                    keys[place] = key;
+                    listed[place] = c;
+                }
+            });
+            listedStep = step;
+            __syncthreads();
+        }
+        const uint32_t n = shared.Listed;
+        TKey high = 0, low = 0;  // low: of the complement
+        for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
+            const TKey key = keys[i], other = ~key;
+            high = key > high ? key : high;
+            low = other > low ? other : low;
+        }
+        high = MostOf(high, shared);
+        low = ~MostOf(low, shared);
+        int bits = 0;
+        while (bits < TK::kBits && (high - low) >> bits != 0) {
+            ++bits;
+        }
+        TKey prefix = 0;
+        for (int level = (bits + BITS - 1) / BITS - 1; level >= 0; --level) {
+            const uint32_t shift = level * BITS;
+            __syncthreads();
+            later.template Clear<THREADS>();
+            __syncthreads();
+            for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
+                const TKey under = high - keys[i];
+                if (shift + BITS >= static_cast<uint32_t>(TK::kBits) || under >> (shift + BITS) == prefix) {
+                    later.Add(static_cast<uint32_t>(under >> shift) & (kDigits - 1), weigh.WholeOf(static_cast<T>(TK::Value(keys[i]))));
+                }
+            }
+            __syncthreads();
+            prefix = prefix << BITS | ReachDigit<BITS, THREADS>(later, byCount, target, at, shared);
+        }
+        at.Key = high - prefix;
+        return at;
+    };
+    DrawFrom<T>(p, r, limits, weigh, all, likely, there, reach, [&](const TPosition<TKey>& at, uint32_t nth) {
+        // the last position's list has them all, in no order
+        const uint32_t n = shared.Listed;
+        for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
+            if (keys[i] == at.Key) {
+                uint32_t before = 0;
+                for (uint32_t j = 0; j < n && at.Alike > 1; ++j) {
+                    before += keys[j] == at.Key && listed[j] < listed[i];
+                }
+                if (before == nth) {
+                    shared.Found[0] = listed[i];
+                }
+            }
+        }
+        __syncthreads();
+        return static_cast<int32_t>(shared.Found[0]);
+    });
+}
+
+// 16-bit scores: how often each key comes, counted in 16 bits in LDS, says everything. A weight is computed for each key that there is
+// instead of each class. A key that more than 65535 classes have shows in the counts' sum; such a row is done by digits.
+template <typename T>
+__global__ void __launch_bounds__(1024) SampleCountedKernel(const T* scores, TSampleArguments p) {
+    using TK = TKeys<T>;
+    using TPair = __attribute__((ext_vector_type(2))) uint16_t;
+    using TSignedPair = __attribute__((ext_vector_type(2))) int16_t;
+    constexpr int kThreads = 1024, kWaves = 16;
+    constexpr uint32_t kWords = 32768, kMine = 2 * kWords / kThreads;  // two counts in a word; keys for a thread
+    constexpr uint32_t kInfinity = std::is_same_v<T, _Float16> ? 0x7c00 : 0x7f80;
+    constexpr uint32_t kHighest = 0x8000 | kInfinity, kLowest = 0x7fff ^ kInfinity;  // keys here: of plus and minus infinity
+    __shared__ union {
+        uint32_t Counts[kWords];
+        TDigitSums<11> Sums;
+    } lds;
+    __shared__ TShared<kWaves> shared;
 
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const size_t r = p.First + blockIdx.x;
     const T* row = scores + r * p.Stride;
-    const uint32_t classes = p.Classes;
-
-    TKey most = 0;
-    ForRow<T, THREADS>(row, classes, [&](T x, uint32_t) {
-        const TKey key = TK::Of(x);
-        most = key > most ? key : most;
-    });
-    most = MostOf<kWaves>(most, shared);
-    const auto answer = [&](int32_t index, double weight) {
-        if (threadIdx.x == 0) {
-            p.Indexes[r] = index;
-            if (p.Weights != nullptr) {
-                static_cast<TAcc<T>*>(p.Weights)[r] = static_cast<TAcc<T>>(weight);
+    // A wave's part of the row is contiguous, in pieces of 64 times 16 bytes, four of them on their way. f(keys of a thread's eight classes in pairs, the first one):
+    // keys that grow with the scores, two for the zeros, NaN at both ends
+    const uint32_t pieces = (p.Classes + kWaves * 512 - 1) / (kWaves * 512);
+    const uint32_t begin = wave * pieces * 512 + lane * 8;
+    struct TKeysOfEight {
+        TPair V[4];
+    };
+    const auto keysAt = [&](uint32_t c) {
+        TValues<uint32_t, 4> words;
+        if (c + 8 <= p.Classes) {
+            words = TValues<uint32_t, 4>::Load(row + c);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t none = 0x8000 | kInfinity;
+                const uint32_t low = c + 2 * j < p.Classes ? __builtin_bit_cast(uint16_t, row[c + 2 * j]) : none;
+                const uint32_t high = c + 2 * j + 1 < p.Classes ? __builtin_bit_cast(uint16_t, row[c + 2 * j + 1]) : none;
+                words.V[j] = low | high << 16;
             }
         }
+        return words;
     };
-    if (most == 0) {
-        answer(-1, 0);
+    const auto forPieces = [&](auto&& f) {
+        const auto give = [&](const TValues<uint32_t, 4>& words, uint32_t c) {
+            TKeysOfEight keys;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const TSignedPair sign = __builtin_bit_cast(TSignedPair, words.V[j]) >> TSignedPair{15, 15};
+                keys.V[j] = __builtin_bit_cast(TPair, words.V[j]) ^ (__builtin_bit_cast(TPair, sign) | TPair{0x8000, 0x8000});
+            }
+            f(keys, c);
+        };
+        uint32_t i = 0;
+        for (; i + 4 <= pieces; i += 4) {
+            TValues<uint32_t, 4> words[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                words[j] = keysAt(begin + (i + j) * 512);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                give(words[j], begin + (i + j) * 512);
+            }
+        }
+        for (; i < pieces; ++i) {
+            give(keysAt(begin + i * 512), begin + i * 512);
+        }
+    };
+    FillPowers(shared.Powers);
+#pragma unroll
+    for (uint32_t i = 0; i < kWords / 4 / kThreads; ++i) {
+        reinterpret_cast<uint4*>(lds.Counts)[threadIdx.x + i * kThreads] = uint4{0, 0, 0, 0};
+    }
+    TPair mosts = {0, 0};
+    forPieces([&](const TKeysOfEight& keys, uint32_t) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            mosts = __builtin_elementwise_max(mosts, keys.V[j]);
+        }
+    });
+    uint32_t most = MostOf<kWaves>(static_cast<uint32_t>(mosts[0] > mosts[1] ? mosts[0] : mosts[1]), shared);
+    if (most > kHighest) {
+        // there are NaN over plus infinity (those do not take part: they are over the best key, which counts as far under it)
+        most = 0;
+        forPieces([&](const TKeysOfEight& keys, uint32_t) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t key = keys.V[j / 2][j % 2];
+                most = key <= kHighest && key > most ? key : most;
+            }
+        });
+        most = MostOf<kWaves>(most, shared);
+    }
+    most = most == 0x7fff ? 0x8000 : most;  // minus zero is zero
+    if (most <= kLowest) {
+        if (threadIdx.x == 0) {
+            Answer<T>(p, r, -1, 0);
+        }
         return;
     }
-
-    // the lowest class of the (nth + 1)-th of those with this key
-    const auto classOf = [&](TKey key, uint32_t nth) {
-        // which wave's part of the row has it, then which of the part's 64 * pieces classes
-        const uint32_t part = (classes + kWaves - 1) / kWaves;
-        uint32_t begin = wave * part, end = begin + part < classes ? begin + part : classes, n = 0;
-        for (uint32_t c = begin + lane; c < end; c += 64) {
-            n += TK::Of(row[c]) == key;
-        }
+    const TLimits limits(p, r);
+    const auto sharedKey = [](uint32_t key) { return key - kLowest - (key >> 15); };  // as TKeys has it, with one key for both zeros
+    // the (nth + 1)-th class with this key
+    const auto classOf = [&](uint32_t key, uint32_t nth) {
+        const uint32_t other = key == 0x8000 ? 0x7fff : key;
+        const auto alike = [&](const TKeysOfEight& keys) {
+            uint32_t n = 0;  // a bit for each
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t k = keys.V[j / 2][j % 2];
+                n |= (k == key || k == other ? 1u : 0u) << j;
+            }
+            return n;
+        };
+        uint32_t n = 0;
+        forPieces([&](const TKeysOfEight& keys, uint32_t) { n += __popc(alike(keys)); });
 #pragma unroll
         for (int d = 32; d > 0; d /= 2) {
             n += __shfl_xor(n, d);
         }
         __syncthreads();
         if (lane == 0) {
-            counted[wave] = n;
+            shared.Counted[wave] = n;
         }
         __syncthreads();
-        uint32_t w = 0;
-        while (w + 1 < kWaves && nth >= counted[w]) {
-            nth -= counted[w++];
-        }
-        begin = w * part;
-        end = begin + part < classes ? begin + part : classes;
-        // every thread of the workgroup has some classes in a row of that part
-        const uint32_t each = (part + THREADS - 1) / THREADS;
-        const uint32_t mine = begin + threadIdx.x * each, last = mine + each < end ? mine + each : end;
-        n = 0;
-        for (uint32_t c = mine; c < last; ++c) {
-            n += TK::Of(row[c]) == key;
-        }
-        uint32_t sum = n;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const uint32_t other = __shfl_up(sum, d);
-            sum += lane >= static_cast<uint32_t>(d) ? other : 0;
-        }
-        __syncthreads();
-        if (lane == 63) {
-            counted[wave] = sum;
-        }
-        __syncthreads();
-        uint32_t before = sum - n;
-        for (uint32_t v = 0; v < wave; ++v) {
-            before += counted[v];
+        uint32_t before = 0;
+        for (uint32_t w = 0; w < wave; ++w) {
+            before += shared.Counted[w];
         }
         if (nth >= before && nth < before + n) {
-            for (uint32_t c = mine; c < last; ++c) {
-                if (TK::Of(row[c]) == key && before++ == nth) {
-                    found[0] = c;
+            forPieces([&](const TKeysOfEight& keys, uint32_t c) {
+                const uint32_t mine = alike(keys);
+                if (__ballot(mine != 0) == 0) {
+                    return;
                 }
+                uint32_t sum = __popc(mine);
+#pragma unroll
+                for (int d = 1; d < 64; d *= 2) {
+                    const uint32_t up = __shfl_up(sum, d);
+                    sum += lane >= static_cast<uint32_t>(d) ? up : 0;
+                }
+                uint32_t place = before + sum - __popc(mine);
+                if (nth >= place && nth < before + sum) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        if ((mine >> j & 1) != 0 && place++ == nth) {
+                            shared.Found[0] = c + j;
+                        }
+                    }
+                }
+                before += __shfl(sum, 63);
+            });
+        }
+        __syncthreads();
+        return static_cast<int32_t>(shared.Found[0]);
+    };
+    if (limits.Greedy()) {
+        const int32_t index = classOf(most, 0);
+        if (threadIdx.x == 0) {
+            Answer<T>(p, r, index, 1);
+        }
+        return;
+    }
+    const TWeigh weigh = limits.Weigh(TK::Value(sharedKey(most)), p.Shift, shared.Powers);
+    const uint32_t keys = most - kLowest;  // from the best one down to the last over minus infinity
+    uint32_t mine = 0;
+    forPieces([&](const TKeysOfEight& keysOfEight, uint32_t) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint32_t under = most - keysOfEight.V[j / 2][j % 2];
+            if (under < keys) {
+                ++mine;
+                atomicAdd(&lds.Counts[under >> 1], under & 1 ? 0x10000u : 1u);
+            }
+        }
+    });
+    const uint64_t there = SumOf(mine, shared);
+    const auto countOf = [&](uint32_t under) { return lds.Counts[under >> 1] >> (under & 1) * 16 & 0xffff; };
+    if (threadIdx.x == 0 && most >= 0x8000) {
+        // minus zero's counts become zero's (65536 of both at most show in the sum)
+        const uint32_t zero = most - 0x8000, minus = zero + 1;
+        const uint32_t n = minus < keys ? countOf(minus) : 0;
+        lds.Counts[minus >> 1] -= n << (minus & 1) * 16;
+        lds.Counts[zero >> 1] += n << (zero & 1) * 16;
+    }
+    __syncthreads();
+    // every thread has kMine keys in a row
+    const uint32_t firstKey = threadIdx.x * kMine;
+    const auto weightOf = [&](uint32_t under) { return weigh.Weight(weigh.Under(static_cast<T>(TK::Value(sharedKey(most - under))))); };
+    uint64_t weights = 0, likely = 0, counts = 0;
+    for (uint32_t under = firstKey; under < firstKey + kMine && under < keys; ++under) {
+        const uint32_t n = countOf(under);
+        if (n != 0) {
+            const double weight = weightOf(under);
+            const uint64_t whole = weigh.Whole(weight) * n;
+            weights += whole;
+            likely += weight >= limits.MinP ? whole : 0;
+            counts += n;
+        }
+    }
+    if (SumOf(counts, shared) != there) {
+        weights = likely = 0;
+        ForRow<T, kThreads>(row, p.Classes, [&](T x, uint32_t) {
+            if (TK::Of(x) != 0) {
+                const double weight = weigh.Weight(weigh.Under(x));
+                weights += weigh.Whole(weight);
+                likely += weight >= limits.MinP ? weigh.Whole(weight) : 0;
+            }
+        });
+        weights = SumOf(weights, shared);
+        likely = SumOf(likely, shared);
+        return DrawByDigits<T, kThreads, 11>(row, p, r, limits, weigh, sharedKey(most), weights, likely, there, lds.Sums, shared);
+    }
+    const uint64_t weightBefore = SumBefore<kWaves>(weights, shared), countBefore = SumBefore<kWaves>(counts, shared);
+    const uint64_t all = SumOf(weights, shared);
+    likely = SumOf(likely, shared);
+    const auto reach = [&](bool byCount, uint64_t target) {
+        uint64_t weight = weightBefore, count = countBefore;
+        __syncthreads();
+        if (byCount ? count < target && count + counts >= target : weight < target && weight + weights >= target) {
+            for (uint32_t under = firstKey; under < firstKey + kMine && under < keys; ++under) {
+                const uint32_t n = countOf(under);
+                const uint64_t whole = n != 0 ? weigh.Whole(weightOf(under)) * n : 0;
+                if (byCount ? count + n >= target : weight + whole >= target) {
+                    shared.Found[0] = under;
+                    shared.Found[1] = weight;
+                    shared.Found[2] = count;
+                    shared.Found[3] = n;
+                    break;
+                }
+                weight += whole;
+                count += n;
             }
         }
         __syncthreads();
-        return static_cast<int32_t>(found[0]);
+        return TPosition<typename TK::TKey>{sharedKey(most - static_cast<uint32_t>(shared.Found[0])), static_cast<uint32_t>(shared.Found[2]),
+                                            static_cast<uint32_t>(shared.Found[3]), shared.Found[1]};
     };
-
-    const float temperature = p.Sampling.Temperature != nullptr ? p.Sampling.Temperature[r] : 1.0f;
-    if (!(temperature > 0)) {
-        const int32_t index = classOf(most, 0);
-        answer(index, 1);
-        return;
-    }
-    const TWeigh weigh{TK::Value(most), 1.0 / static_cast<double>(temperature), static_cast<double>(uint64_t(1) << p.Shift)};
-    const float least = p.Sampling.MinP != nullptr ? p.Sampling.MinP[r] : 0.0f;
-    const double minP = least > 0 ? (least < 1 ? least : 1.0) : 0.0;
-
-    // sums by the first digit of how far a key is under the best one, and the limits that need nothing else
-    constexpr int kLevels = (TK::kBits + kDigitBits - 1) / kDigitBits;
-    constexpr uint32_t kTop = (kLevels - 1) * kDigitBits;
-    for (uint32_t d = threadIdx.x; d < kDigits; d += THREADS) {
-        first.Weights[d] = 0;
-        first.Counts[d] = 0;
-    }
-    __syncthreads();
-    uint64_t all = 0, likely = 0, there = 0;
-    ForRow<T, THREADS>(row, classes, [&](T x, uint32_t) {
-        const TKey key = TK::Of(x);
-        if (key != 0) {
-            const double weight = weigh.Weight(static_cast<double>(x));
-            const uint64_t whole = weigh.Whole(weight);
-            ++there;
-            all += whole;
-            likely += weight >= minP ? whole : 0;
-            const uint32_t digit = static_cast<uint32_t>((most - key) >> kTop);
-            atomicAdd(reinterpret_cast<unsigned long long*>(&first.Weights[digit]), static_cast<unsigned long long>(whole));
-            atomicAdd(&first.Counts[digit], 1u);
-        }
-    });
-    all = SumOf<kWaves>(all, shared);
-    likely = SumOf<kWaves>(likely, shared);
-    there = SumOf<kWaves>(there, shared);
-
-    // The position where the count (byCount) or the weights from the front of the order, its own among them, reach `target`, which
-    // they do somewhere
-    const auto reach = [&](bool byCount, uint64_t target) {
-        TPosition<TKey> at{0, 0, 0, 0};
-        TKey prefix = 0;  // the digits so far
-        for (int level = kLevels - 1; level >= 0; --level) {
-            const uint32_t shift = level * kDigitBits;
-            TDigitSums& sums = level == kLevels - 1 ? first : later;
-            if (level < kLevels - 1) {
-                __syncthreads();
-                for (uint32_t d = threadIdx.x; d < kDigits; d += THREADS) {
-                    later.Weights[d] = 0;
-                    later.Counts[d] = 0;
-                }
-                __syncthreads();
-                ForRow<T, THREADS>(row, classes, [&](T x, uint32_t) {
-                    const TKey key = TK::Of(x), under = most - key;
-                    if (key != 0 && under >> (shift + kDigitBits) == prefix) {
-                        const uint32_t digit = static_cast<uint32_t>(under >> shift) & (kDigits - 1);
-                        atomicAdd(reinterpret_cast<unsigned long long*>(&later.Weights[digit]),
-                                  static_cast<unsigned long long>(weigh.Whole(weigh.Weight(static_cast<double>(x)))));
-                        atomicAdd(&later.Counts[digit], 1u);
-                    }
-                });
-            }
-            __syncthreads();
-            // every thread has kMine digits in a row
-            uint64_t mine = 0;
-            const uint32_t begin = threadIdx.x * kMine;
-            for (uint32_t d = begin; d < begin + kMine; ++d) {
-                mine += byCount ? sums.Counts[d] : sums.Weights[d];
-            }
-            uint64_t sum = mine;
-#pragma unroll
-            for (int d = 1; d < 64; d *= 2) {
-                const uint64_t other = __shfl_up(sum, d);
-                sum += lane >= static_cast<uint32_t>(d) ? other : 0;
-            }
-            if (lane == 63) {
-                shared[wave] = sum;
-            }
-            __syncthreads();
-            uint64_t before = (byCount ? at.Before : at.WeightBefore) + sum - mine;
-            for (uint32_t w = 0; w < wave; ++w) {
-                before += shared[w];
-            }
-            if (before < target && before + mine >= target) {
-                uint32_t d = begin;
-                for (; d + 1 < begin + kMine; ++d) {
-                    const uint64_t more = byCount ? sums.Counts[d] : sums.Weights[d];
-                    if (before + more >= target) {
-                        break;
-                    }
-                    before += more;
-                }
-                found[0] = d;
-                found[1] = before;
-            }
-            __syncthreads();
-            const uint32_t digit = static_cast<uint32_t>(found[0]);
-            // the other sum before that digit
-            uint64_t rest = 0;
-            for (uint32_t d = threadIdx.x; d < digit; d += THREADS) {
-                rest += byCount ? sums.Weights[d] : sums.Counts[d];
-            }
-            const uint64_t reached = found[1];
-            rest = SumOf<kWaves>(rest, shared);
-            if (byCount) {
-                at.Before = static_cast<uint32_t>(reached);
-                at.WeightBefore += rest;
-            } else {
-                at.Before += static_cast<uint32_t>(rest);
-                at.WeightBefore = reached;
-            }
-            at.Alike = sums.Counts[digit];
-            prefix = prefix << kDigitBits | digit;
-        }
-        at.Key = most - prefix;
-        return at;
-    };
-    const auto wholeOf = [&](TKey key) { return weigh.Whole(weigh.Weight(TK::Value(key))); };
-
-    // what the limits leave, as sums from the front of the order: the smallest holds
-    const int32_t topK = p.Sampling.TopK != nullptr ? p.Sampling.TopK[r] : 0;
-    if (topK > 0 && static_cast<uint64_t>(topK) < there) {
-        const auto at = reach(true, static_cast<uint64_t>(topK));
-        all = at.WeightBefore + (static_cast<uint32_t>(topK) - at.Before) * wholeOf(at.Key);
-    }
-    uint64_t kept = all < likely ? all : likely;
-    const float topP = p.Sampling.TopP != nullptr ? p.Sampling.TopP[r] : 1.0f;
-    if (topP < 1) {
-        const double share = ceil((topP > 0 ? static_cast<double>(topP) : 0.0) * static_cast<double>(all));
-        const uint64_t target = share < 1 ? 1 : share < static_cast<double>(all) ? static_cast<uint64_t>(share) : all;
-        const auto at = reach(false, target);
-        const uint64_t whole = wholeOf(at.Key);
-        const uint64_t sum = at.WeightBefore + ((target - at.WeightBefore + whole - 1) / whole) * whole;
-        kept = sum < kept ? sum : kept;
-    }
-    const float uniform = p.Uniform[r];
-    const double passed = (uniform > 0 ? static_cast<double>(uniform) : 0.0) * static_cast<double>(kept);
-    const uint64_t draw = passed < static_cast<double>(kept) && static_cast<uint64_t>(passed) < kept ? static_cast<uint64_t>(passed) : kept - 1;
-    const auto at = reach(false, draw + 1);
-    const double weight = weigh.Weight(TK::Value(at.Key));
-    const int32_t index = classOf(at.Key, static_cast<uint32_t>((draw - at.WeightBefore) / weigh.Whole(weight)));
-    answer(index, weight * weigh.Unit / static_cast<double>(kept));
+    DrawFrom<T>(p, r, limits, weigh, all, likely, there, reach,
+                [&](const TPosition<typename TK::TKey>& at, uint32_t nth) { return classOf(at.Key + kLowest + (at.Key >= kInfinity ? 1 : 0), nth); });
 }
 
 }  // namespace op
@@ -383,7 +1051,18 @@ using namespace op;
 namespace {
 
 constexpr size_t kMostClassesToSample = size_t(1) << 24;
-constexpr size_t kMostRowsOfLaunch = size_t(1) << 21;
+constexpr size_t kMostGroupsToSample = size_t(1) << 21;
+
+// f(integral_constant) for the n of 1 to MOST that `n` is
+template <int MOST, typename F>
+void WithNumber(size_t n, F&& f) {
+    if constexpr (MOST > 1) {
+        if (n < MOST) {
+            return WithNumber<MOST - 1>(n, f);
+        }
+    }
+    f(std::integral_constant<int, MOST>());
+}
 
 }  // namespace
 
@@ -407,8 +1086,8 @@ void SampleClasses(int valueType, size_t rows, size_t classes, const void* score
     TSampleArguments p{};
     p.Classes = static_cast<uint32_t>(classes);
     // a row of the best score alone adds up to under 2^63
-    p.Shift = 62;
-    while (p.Shift > 0 && (size_t(1) << (63 - p.Shift)) <= classes) {
+    p.Shift = 51;
+    while ((size_t(1) << (63 - p.Shift)) <= classes) {
         --p.Shift;
     }
     p.Stride = scoreStride;
@@ -416,15 +1095,43 @@ void SampleClasses(int valueType, size_t rows, size_t classes, const void* score
     p.Uniform = uniform;
     p.Indexes = indexes;
     p.Weights = weights;
+    const auto launch = [&](auto kernel, const auto* from, uint32_t threads, size_t rowsOfGroup) {
+        for (p.First = 0; p.First < rows; p.First += kMostGroupsToSample * rowsOfGroup) {
+            p.Rows = std::min(rows - p.First, kMostGroupsToSample * rowsOfGroup);
+            call.Launch(kernel, (p.Rows + rowsOfGroup - 1) / rowsOfGroup, threads, 0, from, p);
+        }
+    };
     WithType(valueType, [&](auto value) {
         using T = decltype(value);
-        for (p.First = 0; p.First < rows; p.First += kMostRowsOfLaunch) {
-            const size_t n = std::min(rows - p.First, kMostRowsOfLaunch);
-            if (classes <= 4096) {
-                call.Launch(SampleRowKernel<T, 256>, n, 256, 0, static_cast<const T*>(scores), p);
-            } else {
-                call.Launch(SampleRowKernel<T, 1024>, n, 1024, 0, static_cast<const T*>(scores), p);
-            }
+        const T* from = static_cast<const T*>(scores);
+        if (classes <= 16) {
+            return WithNumber<16>(classes, [&](auto n) { launch(SampleOfFewKernel<T, decltype(n)::value>, from, 256, 256); });
+        }
+        if (classes <= 32) {
+            return launch(SampleByLanesKernel<T, 32, 1>, from, 256, 8);
+        }
+        if (classes <= 64) {
+            return launch(SampleByLanesKernel<T, 64, 1>, from, 256, 4);
+        }
+        if (classes <= 128) {
+            return launch(SampleByLanesKernel<T, 64, 2>, from, 256, 4);
+        }
+        if (classes <= 256) {
+            return launch(SampleByLanesKernel<T, 64, 4>, from, 256, 4);
+        }
+        if (classes <= LANES512) {
+            return launch(SampleByLanesKernel<T, 64, 8>, from, 256, 4);
+        }
+        if (classes <= LANES1024) {
+            return launch(SampleByLanesKernel<T, 64, 16>, from, 256, 4);
+        }
+        if (classes <= 4096) {
+            return launch(SampleRowKernel<T, 256, 9, 1024>, from, 256, 1);
+        }
+        if constexpr (sizeof(T) == 2) {
+            launch(SampleCountedKernel<T>, from, 1024, 1);
+        } else {
+            launch(SampleRowKernel<T, 1024, 11, sizeof(T) == 8 ? 2048 : 3072>, from, 1024, 1);
         }
     });
 }

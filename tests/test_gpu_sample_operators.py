@@ -158,6 +158,19 @@ def test_ties_among_many(kind, classes):
 
 
 @ALL
+@pytest.mark.parametrize("value", [0.0, 1.5, -1.5])
+def test_a_score_that_most_of_many_classes_have(kind, value):
+    """More classes with one score than 16 bits count, under and over it a few others, zeros of both signs among them."""
+    rng = np.random.default_rng(9)
+    classes, rows = 140001, 8
+    scores = np.full((rows, classes), value)
+    scores[rng.random((rows, classes)) < 0.01] = -0.0
+    scores[rng.random((rows, classes)) < 0.01] = 0.0
+    scores[:, 5:4000:7] = rng.standard_normal((rows, 571)) * 3
+    Draw(kind, scores, rng.random(rows), top_k=[0, 0, 100, 90000, 0, 300, 0, 139000], top_p=[1, 0.8, 1, 0.9, 0.01, 0.5, 0.99, 1], min_p=[0, 0.01, 0, 0, 0, 0, 0.5, 0]).check()
+
+
+@ALL
 @pytest.mark.parametrize("classes", [3, 12, 40, 700, 9000])
 def test_values_at_the_ends(kind, classes):
     """Infinities and NaN, rows without any class, temperatures, numbers and limits outside their ranges."""

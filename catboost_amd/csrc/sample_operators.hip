@@ -47,7 +47,7 @@ private:
     }
 };
 
-constexpr uint32_t kPowers = 64;
+constexpr uint32_t kPowers = 64;  // (shifts by 6 below)
 
 // 2^(-i / 64), which a workgroup computes for its weights
 __device__ __forceinline__ void FillPowers(double* powers) {
@@ -57,37 +57,50 @@ __device__ __forceinline__ void FillPowers(double* powers) {
 }
 
 // The weights of a row's scores
+template <bool TABLE>
 struct TWeigh {
     double Best;           // the best score
     double Rate;           // log2(e) / temperature
     double Unit;           // 2^shift: how many whole numbers a weight of 1 is, at most 2^51
-    const double* Powers;  // in LDS
+    const double* Powers;  // in LDS, of TABLE
 
-    // How far under the best one, in powers of two; never less for a smaller score
+    // How far under the best one, in powers of two; never less for a smaller score. All of plus infinity are alike, and the others
+    // too far under it (a difference that is no number counts as 4096).
     template <typename T>
     __device__ __forceinline__ double Under(T x) const {
-        if (Best == __builtin_inf()) {
-            return static_cast<double>(x) == Best ? 0.0 : 4096.0;
-        }
         double under = Best - static_cast<double>(x);
         if constexpr (std::is_same_v<T, double>) {
             // (may pass the largest number, which no temperature is to turn into NaN)
-            under = fmin(under, 1.7976931348623157e308);
+            under = Best < __builtin_inf() ? fmin(under, 1.7976931348623157e308) : under;
         }
-        return fmin(under * Rate, 4096.0);
+        under = fmin(under * Rate, 4096.0);
+        return static_cast<double>(x) == Best ? 0.0 : under;
     }
-    // 2^-under: the nearest 64th from the table, the rest, under 1/128, by the series of exp up to its fifth power (its sixth is
-    // under 2^-54). About a third of the steps of exp, which is most of what a row of 100000 classes costs.
+    // 2^-under. With the table the rest beside the nearest 64th is under 1/128 and the series of exp ends with its fifth power (the
+    // sixth is under 2^-54): a third of the steps of exp, which is most of what a row of 100000 classes costs. Where a workgroup has
+    // few weights to compute the rest beside the nearest whole number is up to 1/2, and the series has 13.
     __device__ __forceinline__ double Weight(double under) const {
-        const double steps = rint(under * kPowers);
-        const double y = fma(steps, 0.015625, -under) * 0.69314718055994530942;
-        const int n = static_cast<int>(steps);
-        double e = fma(y, 1.0 / 120, 1.0 / 24);
-        e = fma(e, y, 1.0 / 6);
-        e = fma(e, y, 0.5);
-        e = fma(e, y, 1.0);
-        e = fma(e, y, 1.0);
-        return ldexp(e * Powers[n & (kPowers - 1)], -(n >> 6));
+        if constexpr (TABLE) {
+            const double steps = rint(under * kPowers);
+            const double y = fma(steps, 1.0 / kPowers, -under) * 0.69314718055994530942;
+            const int n = static_cast<int>(steps);
+            double e = fma(y, 1.0 / 120, 1.0 / 24);
+            e = fma(e, y, 1.0 / 6);
+            e = fma(e, y, 0.5);
+            e = fma(e, y, 1.0);
+            e = fma(e, y, 1.0);
+            return ldexp(e * Powers[n & (kPowers - 1)], -(n >> 6));
+        } else {
+            const double steps = rint(under);
+            const double y = (steps - under) * 0.69314718055994530942;
+            double e = 1.0 / 6227020800.0;
+            constexpr double kTerms[] = {1.0 / 479001600, 1.0 / 39916800, 1.0 / 3628800, 1.0 / 362880, 1.0 / 40320, 1.0 / 5040, 1.0 / 720, 1.0 / 120, 1.0 / 24, 1.0 / 6, 0.5, 1.0, 1.0};
+#pragma unroll
+            for (const double term : kTerms) {
+                e = fma(e, y, term);
+            }
+            return ldexp(e, -static_cast<int>(steps));
+        }
     }
     // (what adding 2^52 leaves in the last bits is the nearest whole number)
     __device__ __forceinline__ uint64_t Whole(double weight) const {
@@ -128,8 +141,9 @@ struct TLimits {
     __device__ __forceinline__ bool Greedy() const {
         return !(Temperature > 0);
     }
-    __device__ __forceinline__ TWeigh Weigh(double best, uint32_t shift, const double* powers) const {
-        return TWeigh{best, 1.44269504088896340736 / static_cast<double>(Temperature), static_cast<double>(uint64_t(1) << shift), powers};
+    template <bool TABLE>
+    __device__ __forceinline__ TWeigh<TABLE> Weigh(double best, uint32_t shift, const double* powers) const {
+        return {best, 1.44269504088896340736 / static_cast<double>(Temperature), static_cast<double>(uint64_t(1) << shift), powers};
     }
     // The sum that the classes of the share reach first, of `all`
     __device__ __forceinline__ uint64_t ShareOf(uint64_t all) const {
@@ -189,14 +203,18 @@ __global__ void __launch_bounds__(256) SampleOfFewKernel(const T* scores, TSampl
 #pragma unroll
     for (int round = 0; round < C; ++round) {
 #pragma unroll
-        for (int c = round & 1; c + 1 < C; c += 2) {
-            const bool trade = x[c + 1] > x[c];
-            const A high = trade ? x[c + 1] : x[c], low = trade ? x[c] : x[c + 1];
-            const int32_t first = trade ? index[c + 1] : index[c], second = trade ? index[c] : index[c + 1];
-            x[c] = high;
-            x[c + 1] = low;
-            index[c] = first;
-            index[c + 1] = second;
+        for (int c = 0; c + 1 < C; ++c) {
+            if ((c & 1) != (round & 1)) {
+                continue;
+            }
+            // (values of their own: a choice between elements would be one between addresses, and the rows would leave their registers)
+            const A a = x[c], b = x[c + 1];
+            const int32_t i = index[c], j = index[c + 1];
+            const bool trade = b > a;
+            x[c] = trade ? b : a;
+            x[c + 1] = trade ? a : b;
+            index[c] = trade ? j : i;
+            index[c + 1] = trade ? i : j;
         }
     }
     if (x[0] == kNone) {
@@ -205,35 +223,39 @@ __global__ void __launch_bounds__(256) SampleOfFewKernel(const T* scores, TSampl
     if (limits.Greedy()) {
         return Answer<T>(p, r, index[0], 1);
     }
-    const TWeigh weigh = limits.Weigh(static_cast<double>(x[0]), p.Shift, powers);
+    const auto weigh = limits.Weigh<true>(static_cast<double>(x[0]), p.Shift, powers);
     double weight[C];
     uint64_t sum[C], all = 0, likely = 0;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-        weight[c] = x[c] > kNone ? weigh.Weight(weigh.Under(x[c])) : 0.0;
+        const double w = weigh.Weight(weigh.Under(x[c]));
+        weight[c] = x[c] > kNone ? w : 0.0;
         const uint64_t whole = weigh.Whole(weight[c]);
         all += limits.TopK <= 0 || c < limits.TopK ? whole : 0;
         likely += weight[c] >= limits.MinP ? whole : 0;
         sum[c] = (c > 0 ? sum[c > 0 ? c - 1 : 0] : 0) + whole;
     }
     uint64_t kept = all < likely ? all : likely;
-    if (limits.TopP < 1) {
+    if (p.Sampling.TopP != nullptr) {
         const uint64_t target = limits.ShareOf(all);
         uint64_t reached = all;
 #pragma unroll
         for (int c = C - 1; c >= 0; --c) {
-            reached = sum[c] >= target ? sum[c] : reached;
+            const uint64_t here = sum[c];
+            reached = here >= target ? here : reached;
         }
-        kept = reached < kept ? reached : kept;
+        kept = limits.TopP < 1 && reached < kept ? reached : kept;
     }
     const uint64_t target = limits.DrawOf(kept);
     int32_t found = index[C - 1];
     double foundWeight = weight[C - 1];
 #pragma unroll
     for (int c = C - 2; c >= 0; --c) {
+        const int32_t here = index[c];
+        const double hereWeight = weight[c];
         const bool there = sum[c] >= target;
-        found = there ? index[c] : found;
-        foundWeight = there ? weight[c] : foundWeight;
+        found = there ? here : found;
+        foundWeight = there ? hereWeight : foundWeight;
     }
     Answer<T>(p, r, found, foundWeight * weigh.Unit / static_cast<double>(kept));
 }
@@ -260,6 +282,9 @@ struct TOrdered {
     __device__ __forceinline__ bool Before(const TOrdered& other) const {
         return Word > other.Word;
     }
+    __device__ __forceinline__ static TOrdered Choose(bool first, const TOrdered& a, const TOrdered& b) {
+        return {first ? a.Word : b.Word};
+    }
     __device__ __forceinline__ TOrdered Across(int lanes) const {
         return {static_cast<TWord>(__shfl_xor(Word, lanes))};
     }
@@ -279,7 +304,11 @@ struct TOrdered<double> {
         return Class;
     }
     __device__ __forceinline__ bool Before(const TOrdered& other) const {
-        return Word > other.Word || (Word == other.Word && Class < other.Class);
+        return (Word > other.Word) | ((Word == other.Word) & (Class < other.Class));
+    }
+    // (member by member: a choice between structs went by way of memory, ten times as slow)
+    __device__ __forceinline__ static TOrdered Choose(bool first, const TOrdered& a, const TOrdered& b) {
+        return {first ? a.Word : b.Word, first ? a.Class : b.Class};
     }
     __device__ __forceinline__ TOrdered Across(int lanes) const {
         return {static_cast<uint64_t>(__shfl_xor(Word, lanes)), static_cast<uint32_t>(__shfl_xor(Class, lanes))};
@@ -292,9 +321,6 @@ __global__ void __launch_bounds__(256) SampleByLanesKernel(const T* scores, TSam
     using TK = TKeys<T>;
     using TItem = TOrdered<T>;
     constexpr int kPlaces = LANES * P;
-    __shared__ double powers[kPowers];
-    FillPowers(powers);
-    __syncthreads();
     const uint32_t lane = threadIdx.x % LANES;
     const size_t n = static_cast<size_t>(blockIdx.x) * (256 / LANES) + threadIdx.x / LANES;
     // (rows behind the last one do as it does, so that every lane is there to be read, and store nothing)
@@ -317,7 +343,7 @@ __global__ void __launch_bounds__(256) SampleByLanesKernel(const T* scores, TSam
 #pragma unroll
                 for (int i = 0; i < P; ++i) {
                     const TItem other = item[i].Across(step / P);
-                    item[i] = item[i].Before(other) == (low == down) ? item[i] : other;
+                    item[i] = TItem::Choose(item[i].Before(other) == (low == down), item[i], other);
                 }
             } else {
 #pragma unroll
@@ -326,8 +352,8 @@ __global__ void __launch_bounds__(256) SampleByLanesKernel(const T* scores, TSam
                         const bool down = ((lane * P + i) & size) == 0;
                         const TItem a = item[i], b = item[i + step];
                         const bool trade = a.Before(b) != down;
-                        item[i] = trade ? b : a;
-                        item[i + step] = trade ? a : b;
+                        item[i] = TItem::Choose(trade, b, a);
+                        item[i + step] = TItem::Choose(trade, a, b);
                     }
                 }
             }
@@ -344,14 +370,15 @@ __global__ void __launch_bounds__(256) SampleByLanesKernel(const T* scores, TSam
         }
     }
     // (every lane goes on: rows of a wave differ; the values of such a row are not used)
-    TWeigh weigh = limits.Weigh(TK::Value(bestKey), p.Shift, powers);
+    auto weigh = limits.Weigh<false>(TK::Value(bestKey), p.Shift, nullptr);
     weigh.Rate = limits.Greedy() ? 0 : weigh.Rate;
     double weight[P];
     uint64_t sum[P], all = 0, likely = 0, total = 0;
 #pragma unroll
     for (int i = 0; i < P; ++i) {
         const auto key = item[i].Key();
-        weight[i] = key != 0 ? weigh.Weight(weigh.Under(static_cast<T>(TK::Value(key)))) : 0.0;
+        const double w = weigh.Weight(weigh.Under(static_cast<T>(TK::Value(key))));
+        weight[i] = key != 0 ? w : 0.0;
         const uint64_t whole = weigh.Whole(weight[i]);
         all += limits.TopK <= 0 || lane * P + i < static_cast<uint32_t>(limits.TopK) ? whole : 0;
         likely += weight[i] >= limits.MinP ? whole : 0;
@@ -609,7 +636,7 @@ __device__ int32_t ClassOf(const T* row, uint32_t classes, typename TKeys<T>::TK
 // the front of the order, its own among them, reach `target`; classAt(position, nth) -> class. `all`: every weight's sum, `likely`: of
 // those that MinP leaves, `there`: how many classes take part
 template <typename T, typename TReach, typename TClass>
-__device__ __forceinline__ void DrawFrom(const TSampleArguments& p, size_t r, const TLimits& limits, const TWeigh& weigh, uint64_t all, uint64_t likely,
+__device__ __forceinline__ void DrawFrom(const TSampleArguments& p, size_t r, const TLimits& limits, const TWeigh<true>& weigh, uint64_t all, uint64_t likely,
                                          uint64_t there, TReach&& reach, TClass&& classAt) {
     using TK = TKeys<T>;
     const auto wholeOf = [&](typename TK::TKey key) { return weigh.WholeOf(static_cast<T>(TK::Value(key))); };
@@ -637,7 +664,7 @@ __device__ __forceinline__ void DrawFrom(const TSampleArguments& p, size_t r, co
 // Positions by the digits of how far a key is under the best one, with a pass over the row for each digit but the first: what takes
 // any row, however many of its classes are alike
 template <typename T, int THREADS, int BITS>
-__device__ void DrawByDigits(const T* row, const TSampleArguments& p, size_t r, const TLimits& limits, const TWeigh& weigh, typename TKeys<T>::TKey most,
+__device__ void DrawByDigits(const T* row, const TSampleArguments& p, size_t r, const TLimits& limits, const TWeigh<true>& weigh, typename TKeys<T>::TKey most,
                              uint64_t all, uint64_t likely, uint64_t there, TDigitSums<BITS>& sums, TShared<THREADS / 64>& shared) {
     using TK = TKeys<T>;
     using TKey = typename TK::TKey;
@@ -702,7 +729,7 @@ __global__ void __launch_bounds__(THREADS) SampleRowKernel(const T* scores, TSam
         }
         return;
     }
-    const TWeigh weigh = limits.Weigh(TK::Value(most), p.Shift, shared.Powers);
+    const auto weigh = limits.Weigh<true>(TK::Value(most), p.Shift, shared.Powers);
     const auto stepOf = [&](double under) {
         const uint32_t step = static_cast<uint32_t>(under * (kDigits / 52.0));
         return step < kDigits ? step : kDigits - 1;
@@ -965,7 +992,7 @@ __global__ void __launch_bounds__(1024) SampleCountedKernel(const T* scores, TSa
         }
         return;
     }
-    const TWeigh weigh = limits.Weigh(TK::Value(sharedKey(most)), p.Shift, shared.Powers);
+    const auto weigh = limits.Weigh<true>(TK::Value(sharedKey(most)), p.Shift, shared.Powers);
     const uint32_t keys = most - kLowest;  // from the best one down to the last over minus infinity
     uint32_t mine = 0;
     forPieces([&](const TKeysOfEight& keysOfEight, uint32_t) {

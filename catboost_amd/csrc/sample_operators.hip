@@ -11,10 +11,6 @@
 #include <algorithm>
 #include <limits>
 #include <type_traits>
-#ifndef LANES512
-#define LANES512 512
-#define LANES1024 1024
-#endif
 
 namespace cbamd {
 namespace op {
@@ -693,13 +689,36 @@ __device__ void DrawByDigits(const T* row, const TSampleArguments& p, size_t r, 
                 [&](const TPosition<TKey>& at, uint32_t nth) { return ClassOf<T, THREADS>(row, p.Classes, at.Key, nth, shared); });
 }
 
-// Positions by t first, in steps of 52 / 2^BITS of a power of two. The classes of the step where a position is are listed, their keys
-// told apart digit by digit, from the list.
+// The same from nothing but the best key
+template <typename T, int THREADS, int BITS>
+__device__ void DrawAny(const T* row, const TSampleArguments& p, size_t r, const TLimits& limits, const TWeigh<true>& weigh, typename TKeys<T>::TKey most,
+                        TDigitSums<BITS>& sums, TShared<THREADS / 64>& shared) {
+    uint64_t all = 0, likely = 0, there = 0;
+    ForRow<T, THREADS>(row, p.Classes, [&](T x, uint32_t) {
+        if (TKeys<T>::Of(x) != 0) {
+            const double weight = weigh.Weight(weigh.Under(x));
+            ++there;
+            all += weigh.Whole(weight);
+            likely += weight >= limits.MinP ? weigh.Whole(weight) : 0;
+        }
+    });
+    all = SumOf(all, shared);
+    likely = SumOf(likely, shared);
+    there = SumOf(there, shared);
+    DrawByDigits<T, THREADS, BITS>(row, p, r, limits, weigh, most, all, likely, there, sums, shared);
+}
+
+// Positions by t first, in steps of 56 / 2^BITS of a power of two. The classes of the step where a position is are listed, their keys
+// told apart digit by digit, from the list. Weights, most of the work, are computed for classes up to the step of rank TopK. Scores are
+// compared as they are, with bounds a little wider than a step's, before anything is computed for them.
 template <typename T, int THREADS, int BITS, int LIST>
 __global__ void __launch_bounds__(THREADS) SampleRowKernel(const T* scores, TSampleArguments p) {
     using TK = TKeys<T>;
     using TKey = typename TK::TKey;
+    using A = TAcc<T>;
     constexpr uint32_t kDigits = 1u << BITS;
+    constexpr double kStep = 56.0 / kDigits;
+    constexpr A kNone = -std::numeric_limits<A>::infinity();
     __shared__ TDigitSums<BITS> first, later;
     __shared__ TShared<THREADS / 64> shared;
     __shared__ TKey keys[LIST];
@@ -709,12 +728,9 @@ __global__ void __launch_bounds__(THREADS) SampleRowKernel(const T* scores, TSam
     const T* row = scores + r * p.Stride;
     FillPowers(shared.Powers);
     first.template Clear<THREADS>();
-    TKey most = 0;
-    ForRow<T, THREADS>(row, p.Classes, [&](T x, uint32_t) {
-        const TKey key = TK::Of(x);
-        most = key > most ? key : most;
-    });
-    most = MostOf<THREADS / 64>(most, shared);
+    A best = kNone;
+    ForRow<T, THREADS>(row, p.Classes, [&](T x, uint32_t) { best = fmax(best, static_cast<A>(x)); });  // (NaN is passed over)
+    const TKey most = MostOf(TK::Of(static_cast<T>(best)), shared);
     if (most == 0) {
         if (threadIdx.x == 0) {
             Answer<T>(p, r, -1, 0);
@@ -730,33 +746,78 @@ __global__ void __launch_bounds__(THREADS) SampleRowKernel(const T* scores, TSam
         return;
     }
     const auto weigh = limits.Weigh<true>(TK::Value(most), p.Shift, shared.Powers);
+    if (weigh.Best == __builtin_inf()) {
+        return DrawAny<T, THREADS, BITS>(row, p, r, limits, weigh, most, later, shared);
+    }
+    // as Under, for a finite best score
+    const auto underOf = [&](A x) {
+        double under = weigh.Best - static_cast<double>(x);
+        if constexpr (std::is_same_v<T, double>) {
+            under = fmin(under, 1.7976931348623157e308);
+        }
+        return fmin(under * weigh.Rate, 4096.0);
+    };
     const auto stepOf = [&](double under) {
-        const uint32_t step = static_cast<uint32_t>(under * (kDigits / 52.0));
+        const uint32_t step = static_cast<uint32_t>(under * (1 / kStep));
         return step < kDigits ? step : kDigits - 1;
     };
-    uint64_t all = 0, likely = 0, there = 0;
+    // A bound of the scores that are `under` or less; and more, on the side of `away`
+    const auto boundOf = [&](double under, double away) {
+        const double apart = under / weigh.Rate, bound = weigh.Best - apart;
+        return static_cast<A>(bound + away * 1e-6 * (fabs(bound) + fabs(apart) + 1e-30));
+    };
+    // the last step of the classes that count: what is in the very last one weighs nothing
+    uint32_t lastStep = kDigits - 1;
+    uint64_t there = 0;
+    if (limits.TopK > 0) {
+        ForRow<T, THREADS>(row, p.Classes, [&](T x, uint32_t) {
+            if (static_cast<A>(x) > kNone) {
+                atomicAdd(&first.Counts[stepOf(underOf(static_cast<A>(x)))], 1u);
+            }
+        });
+        __syncthreads();
+        for (uint32_t d = threadIdx.x; d < kDigits; d += THREADS) {
+            there += first.Counts[d];
+        }
+        there = SumOf(there, shared);
+        if (static_cast<uint64_t>(limits.TopK) < there) {
+            TPosition<TKey> at{0, 0, 0, 0};
+            lastStep = ReachDigit<BITS, THREADS>(first, true, static_cast<uint64_t>(limits.TopK), at, shared);
+        }
+        there = lastStep < kDigits - 1 ? there : 0;  // no class that weighs anything is left out by its rank
+        __syncthreads();
+        first.template Clear<THREADS>();
+        __syncthreads();
+    }
+    const A lowest = lastStep < kDigits - 1 ? boundOf((lastStep + 1) * kStep, -1) : kNone;
+    uint64_t likely = 0;
+    const bool atLeast = limits.MinP > 0;
     ForRow<T, THREADS>(row, p.Classes, [&](T x, uint32_t) {
-        if (TK::Of(x) != 0) {
-            const double under = weigh.Under(x), weight = weigh.Weight(under);
+        const A score = static_cast<A>(x);
+        if (score >= lowest && score > kNone) {
+            const double under = underOf(score), weight = weigh.Weight(under);
+            const uint32_t step = stepOf(under);
             const uint64_t whole = weigh.Whole(weight);
-            ++there;
-            all += whole;
-            likely += weight >= limits.MinP ? whole : 0;
-            first.Add(stepOf(under), whole);
+            if (step <= lastStep) {
+                first.Add(step, whole);
+                if (atLeast) {
+                    likely += weight >= limits.MinP ? whole : 0;
+                }
+            }
         }
     });
-    all = SumOf(all, shared);
-    likely = SumOf(likely, shared);
-    there = SumOf(there, shared);
-
-    // (most classes of a step; more than the list holds: by the keys alone)
+    __syncthreads();
+    uint64_t all = 0;
     uint32_t longest = 0;
     for (uint32_t d = threadIdx.x; d < kDigits; d += THREADS) {
-        longest = first.Counts[d] > longest ? first.Counts[d] : longest;
+        all += first.Weights[d];
+        longest = first.Counts[d] > longest && d < kDigits - 1 ? first.Counts[d] : longest;
     }
-    // the last step has what weighs nothing: no position is there but one by count
+    all = SumOf(all, shared);
+    likely = atLeast ? SumOf(likely, shared) : all;
+    // (a step of more classes than the list holds: by the keys alone)
     if (MostOf(longest, shared) > LIST) {
-        return DrawByDigits<T, THREADS, BITS>(row, p, r, limits, weigh, most, all, likely, there, later, shared);
+        return DrawAny<T, THREADS, BITS>(row, p, r, limits, weigh, most, later, shared);
     }
     uint32_t listedStep = kDigits;
     const auto reach = [&](bool byCount, uint64_t target) {
@@ -768,11 +829,12 @@ __global__ void __launch_bounds__(THREADS) SampleRowKernel(const T* scores, TSam
                 shared.Listed = 0;
             }
             __syncthreads();
+            const A low = boundOf((step + 1) * kStep, -1), high = step > 0 ? boundOf(step * kStep, 1) : static_cast<A>(weigh.Best);
             ForRow<T, THREADS>(row, p.Classes, [&](T x, uint32_t c) {
-                const TKey key = TK::Of(x);
-                if (key != 0 && stepOf(weigh.Under(x)) == step) {
+                const A score = static_cast<A>(x);
+                if (score >= low && score <= high && score > kNone && stepOf(underOf(score)) == step) {
                     const uint32_t place = atomicAdd(&shared.Listed, 1u);
-                    keys[place] = key;
+                    keys[place] = TK::Of(x);
                     listed[place] = c;
                 }
             });
@@ -837,7 +899,7 @@ __global__ void __launch_bounds__(1024) SampleCountedKernel(const T* scores, TSa
     using TPair = __attribute__((ext_vector_type(2))) uint16_t;
     using TSignedPair = __attribute__((ext_vector_type(2))) int16_t;
     constexpr int kThreads = 1024, kWaves = 16;
-    constexpr uint32_t kWords = 32768, kMine = 2 * kWords / kThreads;  // two counts in a word; keys for a thread
+    constexpr uint32_t kWords = 32768;  // two counts in each
     constexpr uint32_t kInfinity = std::is_same_v<T, _Float16> ? 0x7c00 : 0x7f80;
     constexpr uint32_t kHighest = 0x8000 | kInfinity, kLowest = 0x7fff ^ kInfinity;  // keys here: of plus and minus infinity
     __shared__ union {
@@ -845,6 +907,7 @@ __global__ void __launch_bounds__(1024) SampleCountedKernel(const T* scores, TSa
         TDigitSums<11> Sums;
     } lds;
     __shared__ TShared<kWaves> shared;
+    __shared__ TDigitSums<8> segments;
 
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const size_t r = p.First + blockIdx.x;
@@ -1015,57 +1078,100 @@ __global__ void __launch_bounds__(1024) SampleCountedKernel(const T* scores, TSa
         lds.Counts[zero >> 1] += n << (zero & 1) * 16;
     }
     __syncthreads();
-    // every thread has kMine keys in a row
-    const uint32_t firstKey = threadIdx.x * kMine;
+    // Sums of 256 keys in a row, four for a lane; a wave has every sixteenth of them, since the keys that there are lie together
     const auto weightOf = [&](uint32_t under) { return weigh.Weight(weigh.Under(static_cast<T>(TK::Value(sharedKey(most - under))))); };
-    uint64_t weights = 0, likely = 0, counts = 0;
-    for (uint32_t under = firstKey; under < firstKey + kMine && under < keys; ++under) {
-        const uint32_t n = countOf(under);
-        if (n != 0) {
-            const double weight = weightOf(under);
-            const uint64_t whole = weigh.Whole(weight) * n;
-            weights += whole;
-            likely += weight >= limits.MinP ? whole : 0;
-            counts += n;
+    struct TOfLane {
+        uint64_t Weights[4];
+        uint32_t Counts[4];
+    };
+    const auto keysOf = [&](uint32_t segment, uint64_t* atLeast) {
+        const uint2 words = reinterpret_cast<const uint2*>(lds.Counts)[segment * 64 + lane];
+        TOfLane v = {{0, 0, 0, 0}, {words.x & 0xffff, words.x >> 16, words.y & 0xffff, words.y >> 16}};
+        if (__ballot((words.x | words.y) != 0) != 0) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const double weight = weightOf(segment * 256 + lane * 4 + j);
+                v.Weights[j] = v.Counts[j] != 0 ? weigh.Whole(weight) * v.Counts[j] : 0;
+                if (atLeast != nullptr) {
+                    *atLeast += weight >= limits.MinP ? v.Weights[j] : 0;
+                }
+            }
+        }
+        return v;
+    };
+    uint64_t likely = 0, all = 0, counts = 0;
+    for (uint32_t segment = wave; segment < 256; segment += kWaves) {
+        const TOfLane v = keysOf(segment, &likely);
+        uint64_t weight = (v.Weights[0] + v.Weights[1]) + (v.Weights[2] + v.Weights[3]);
+        uint32_t count = (v.Counts[0] + v.Counts[1]) + (v.Counts[2] + v.Counts[3]);
+        if (__ballot(count != 0) != 0) {
+#pragma unroll
+            for (int d = 32; d > 0; d /= 2) {
+                weight += __shfl_xor(weight, d);
+                count += __shfl_xor(count, d);
+            }
+        }
+        if (lane == 0) {
+            segments.Weights[segment] = weight;
+            segments.Counts[segment] = count;
+            all += weight;
+            counts += count;
         }
     }
     if (SumOf(counts, shared) != there) {
-        weights = likely = 0;
-        ForRow<T, kThreads>(row, p.Classes, [&](T x, uint32_t) {
-            if (TK::Of(x) != 0) {
-                const double weight = weigh.Weight(weigh.Under(x));
-                weights += weigh.Whole(weight);
-                likely += weight >= limits.MinP ? weigh.Whole(weight) : 0;
-            }
-        });
-        weights = SumOf(weights, shared);
-        likely = SumOf(likely, shared);
-        return DrawByDigits<T, kThreads, 11>(row, p, r, limits, weigh, sharedKey(most), weights, likely, there, lds.Sums, shared);
+        return DrawAny<T, kThreads, 11>(row, p, r, limits, weigh, sharedKey(most), lds.Sums, shared);
     }
-    const uint64_t weightBefore = SumBefore<kWaves>(weights, shared), countBefore = SumBefore<kWaves>(counts, shared);
-    const uint64_t all = SumOf(weights, shared);
+    all = SumOf(all, shared);
     likely = SumOf(likely, shared);
+    // every wave for itself: the segment, then the key in it
     const auto reach = [&](bool byCount, uint64_t target) {
-        uint64_t weight = weightBefore, count = countBefore;
-        __syncthreads();
-        if (byCount ? count < target && count + counts >= target : weight < target && weight + weights >= target) {
-            for (uint32_t under = firstKey; under < firstKey + kMine && under < keys; ++under) {
-                const uint32_t n = countOf(under);
-                const uint64_t whole = n != 0 ? weigh.Whole(weightOf(under)) * n : 0;
-                if (byCount ? count + n >= target : weight + whole >= target) {
-                    shared.Found[0] = under;
-                    shared.Found[1] = weight;
-                    shared.Found[2] = count;
-                    shared.Found[3] = n;
-                    break;
-                }
-                weight += whole;
-                count += n;
+        uint64_t weight = 0;
+        uint32_t count = 0;
+        const auto place = [&](const TOfLane& v) {
+            uint64_t weights = (v.Weights[0] + v.Weights[1]) + (v.Weights[2] + v.Weights[3]);
+            uint32_t counted = (v.Counts[0] + v.Counts[1]) + (v.Counts[2] + v.Counts[3]);
+            const uint64_t mine = weights;
+            const uint32_t mineCounted = counted;
+#pragma unroll
+            for (int d = 1; d < 64; d *= 2) {
+                const uint64_t other = __shfl_up(weights, d);
+                const uint32_t otherCounted = __shfl_up(counted, d);
+                weights += lane >= static_cast<uint32_t>(d) ? other : 0;
+                counted += lane >= static_cast<uint32_t>(d) ? otherCounted : 0;
             }
+            weights += weight;
+            counted += count;
+            const uint64_t reached = __ballot(byCount ? counted >= target : weights >= target);
+            const int from = __ffsll(static_cast<unsigned long long>(reached)) - 1;
+            weight = weights - mine;
+            count = counted - mineCounted;
+            uint32_t place = lane * 4, of = v.Counts[3];
+#pragma unroll
+            for (int j = 0; j < 3; ++j) {
+                const uint64_t w = v.Weights[j];
+                const uint32_t c = v.Counts[j];
+                const bool past = place == lane * 4 + j && (byCount ? count + c < target : weight + w < target);
+                of = place == lane * 4 + j && !past ? c : of;
+                weight += past ? w : 0;
+                count += past ? c : 0;
+                place += past ? 1 : 0;
+            }
+            weight = __shfl(weight, from);
+            count = __shfl(count, from);
+            struct TFound {
+                uint32_t Place, Counts;
+            };
+            return TFound{static_cast<uint32_t>(__shfl(place, from)), static_cast<uint32_t>(__shfl(of, from))};
+        };
+        TOfLane v;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            v.Weights[j] = segments.Weights[lane * 4 + j];
+            v.Counts[j] = segments.Counts[lane * 4 + j];
         }
-        __syncthreads();
-        return TPosition<typename TK::TKey>{sharedKey(most - static_cast<uint32_t>(shared.Found[0])), static_cast<uint32_t>(shared.Found[2]),
-                                            static_cast<uint32_t>(shared.Found[3]), shared.Found[1]};
+        const uint32_t segment = place(v).Place;
+        const auto found = place(keysOf(segment, nullptr));
+        return TPosition<typename TK::TKey>{sharedKey(most - (segment * 256 + found.Place)), count, found.Counts, weight};
     };
     DrawFrom<T>(p, r, limits, weigh, all, likely, there, reach,
                 [&](const TPosition<typename TK::TKey>& at, uint32_t nth) { return classOf(at.Key + kLowest + (at.Key >= kInfinity ? 1 : 0), nth); });
@@ -1146,11 +1252,13 @@ void SampleClasses(int valueType, size_t rows, size_t classes, const void* score
         if (classes <= 256) {
             return launch(SampleByLanesKernel<T, 64, 4>, from, 256, 4);
         }
-        if (classes <= LANES512) {
+        if (classes <= 512) {
             return launch(SampleByLanesKernel<T, 64, 8>, from, 256, 4);
         }
-        if (classes <= LANES1024) {
-            return launch(SampleByLanesKernel<T, 64, 16>, from, 256, 4);
+        if constexpr (sizeof(T) < 8) {
+            if (classes <= 1024) {
+                return launch(SampleByLanesKernel<T, 64, 16>, from, 256, 4);
+            }
         }
         if (classes <= 4096) {
             return launch(SampleRowKernel<T, 256, 9, 1024>, from, 256, 1);

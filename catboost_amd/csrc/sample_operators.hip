@@ -449,15 +449,56 @@ struct TShared {
     double Powers[kPowers];
 };
 
+// The sum over the lanes up to this one. Steps are moves within the vector unit (rows of 16 lanes, then from the last lane of a row to the
+// next rows), a tenth of the time of trips through LDS.
+template <int CONTROL, int ROWS, typename V>
+__device__ __forceinline__ V MovedOver(V v) {
+    if constexpr (sizeof(V) == 8) {
+        const uint32_t low = __builtin_amdgcn_update_dpp(0u, static_cast<uint32_t>(v), CONTROL, ROWS, 0xf, false);
+        const uint32_t high = __builtin_amdgcn_update_dpp(0u, static_cast<uint32_t>(v >> 32), CONTROL, ROWS, 0xf, false);
+        return static_cast<V>(high) << 32 | low;
+    } else {
+        return __builtin_amdgcn_update_dpp(0u, v, CONTROL, ROWS, 0xf, false);
+    }
+}
+template <typename V>
+__device__ __forceinline__ V SumUpTo(V v) {
+    v += MovedOver<0x111, 0xf>(v);  // 1, 2, 4, 8 lanes on in a row
+    v += MovedOver<0x112, 0xf>(v);
+    v += MovedOver<0x114, 0xf>(v);
+    v += MovedOver<0x118, 0xf>(v);
+    v += MovedOver<0x142, 0xa>(v);  // lane 15 of rows 0 and 2 to rows 1 and 3
+    v += MovedOver<0x143, 0xc>(v);  // lane 31 to rows 2 and 3
+    return v;
+}
+template <typename V>
+__device__ __forceinline__ V OfLane(V v, int lane) {
+    if constexpr (sizeof(V) == 8) {
+        const uint32_t low = __builtin_amdgcn_readlane(static_cast<uint32_t>(v), lane), high = __builtin_amdgcn_readlane(static_cast<uint32_t>(v >> 32), lane);
+        return static_cast<V>(high) << 32 | low;
+    } else {
+        return __builtin_amdgcn_readlane(v, lane);
+    }
+}
+// The largest of the wave's
+template <typename V>
+__device__ __forceinline__ V MostOfWave(V v) {
+    const auto larger = [&](V other) { v = other > v ? other : v; };
+    larger(MovedOver<0x111, 0xf>(v));
+    larger(MovedOver<0x112, 0xf>(v));
+    larger(MovedOver<0x114, 0xf>(v));
+    larger(MovedOver<0x118, 0xf>(v));
+    larger(MovedOver<0x142, 0xa>(v));
+    larger(MovedOver<0x143, 0xc>(v));
+    return OfLane(v, 63);
+}
+
 // Sums and maxima over a workgroup; every lane gets them
 template <int WAVES>
 __device__ __forceinline__ uint64_t SumOf(uint64_t v, TShared<WAVES>& shared) {
-#pragma unroll
-    for (int d = 32; d > 0; d /= 2) {
-        v += __shfl_xor(v, d);
-    }
+    v = SumUpTo(v);
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) {
+    if ((threadIdx.x & 63) == 63) {
         shared.Sums[threadIdx.x >> 6] = v;
     }
     __syncthreads();
@@ -470,11 +511,7 @@ __device__ __forceinline__ uint64_t SumOf(uint64_t v, TShared<WAVES>& shared) {
 }
 template <int WAVES, typename TKey>
 __device__ __forceinline__ TKey MostOf(TKey v, TShared<WAVES>& shared) {
-#pragma unroll
-    for (int d = 32; d > 0; d /= 2) {
-        const TKey other = __shfl_xor(v, d);
-        v = other > v ? other : v;
-    }
+    v = MostOfWave(v);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) {
         shared.Sums[threadIdx.x >> 6] = v;
@@ -488,53 +525,50 @@ __device__ __forceinline__ TKey MostOf(TKey v, TShared<WAVES>& shared) {
     }
     return v;
 }
-// The sum over the threads before this one
+// The sums over the threads before this one
 template <int WAVES>
-__device__ __forceinline__ uint64_t SumBefore(uint64_t mine, TShared<WAVES>& shared) {
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    uint64_t sum = mine;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const uint64_t other = __shfl_up(sum, d);
-        sum += lane >= static_cast<uint32_t>(d) ? other : 0;
-    }
+__device__ __forceinline__ void SumBefore(uint64_t& weights, uint32_t& counts, TShared<WAVES>& shared) {
+    const uint32_t wave = threadIdx.x >> 6;
+    const uint64_t sum = SumUpTo(weights);
+    const uint32_t counted = SumUpTo(counts);
     __syncthreads();
-    if (lane == 63) {
+    if ((threadIdx.x & 63) == 63) {
         shared.Sums[wave] = sum;
+        shared.Counted[wave] = counted;
     }
     __syncthreads();
-    uint64_t before = sum - mine;
-    for (uint32_t w = 0; w < wave; ++w) {
-        before += shared.Sums[w];
+    weights = sum - weights;
+    counts = counted - counts;
+#pragma unroll
+    for (uint32_t w = 0; w < WAVES; ++w) {
+        weights += w < wave ? shared.Sums[w] : 0;
+        counts += w < wave ? shared.Counted[w] : 0;
     }
-    return before;
 }
 
-// f(score, class) for this thread's scores of a row, 16 bytes at a time, two of them on their way
+// f(score, class) for this thread's scores of a row, 16 bytes at a time, four of them on their way
 template <typename T, int THREADS, typename F>
 __device__ __forceinline__ void ForRow(const T* row, uint32_t classes, F&& f) {
     constexpr uint32_t N = 16 / sizeof(T);
     const uint32_t whole = classes / N;
-    uint32_t c = threadIdx.x;
-    for (; c + THREADS < whole; c += 2 * THREADS) {
-        const auto v = TValues<T, N>::Load(row + c * N), w = TValues<T, N>::Load(row + (c + THREADS) * N);
+    for (uint32_t c = threadIdx.x; c < whole; c += 4 * THREADS) {
+        TValues<T, N> v[4];
 #pragma unroll
-        for (uint32_t i = 0; i < N; ++i) {
-            f(v.V[i], c * N + i);
+        for (int j = 0; j < 4; ++j) {
+            // (behind the end the last ones again, so that no load waits in a branch)
+            v[j] = TValues<T, N>::Load(row + (c + j * THREADS < whole ? c + j * THREADS : whole - 1) * N);
         }
 #pragma unroll
-        for (uint32_t i = 0; i < N; ++i) {
-            f(w.V[i], (c + THREADS) * N + i);
-        }
-    }
-    if (c < whole) {
-        const auto v = TValues<T, N>::Load(row + c * N);
+        for (int j = 0; j < 4; ++j) {
+            if (c + j * THREADS < whole) {
 #pragma unroll
-        for (uint32_t i = 0; i < N; ++i) {
-            f(v.V[i], c * N + i);
+                for (uint32_t i = 0; i < N; ++i) {
+                    f(v[j].V[i], (c + j * THREADS) * N + i);
+                }
+            }
         }
     }
-    for (c = whole * N + threadIdx.x; c < classes; c += THREADS) {
+    for (uint32_t c = whole * N + threadIdx.x; c < classes; c += THREADS) {
         f(row[c], c);
     }
 }
@@ -552,20 +586,24 @@ struct TPosition {
 template <int BITS, int THREADS, typename TKey>
 __device__ __forceinline__ uint32_t ReachDigit(const TDigitSums<BITS>& sums, bool byCount, uint64_t target, TPosition<TKey>& at, TShared<THREADS / 64>& shared) {
     constexpr uint32_t kMine = (1u << BITS) / THREADS;
-    uint64_t weights = 0, counts = 0;
+    uint64_t weights = 0;
+    uint32_t counts = 0;
     const uint32_t begin = threadIdx.x * kMine;
 #pragma unroll
     for (uint32_t d = 0; d < kMine; ++d) {
         weights += sums.Weights[begin + d];
         counts += sums.Counts[begin + d];
     }
-    uint64_t weightBefore = SumBefore<THREADS / 64>(weights, shared) + at.WeightBefore;
-    uint64_t countBefore = SumBefore<THREADS / 64>(counts, shared) + at.Before;
-    uint64_t& before = byCount ? countBefore : weightBefore;
-    if (before < target && before + (byCount ? counts : weights) >= target) {
+    uint64_t weightBefore = weights;
+    uint32_t countBefore = counts;
+    SumBefore(weightBefore, countBefore, shared);
+    weightBefore += at.WeightBefore;
+    countBefore += at.Before;
+    const auto reached = [&](uint64_t weight, uint32_t count) { return byCount ? countBefore + uint64_t(count) >= target : weightBefore + weight >= target; };
+    if (!reached(0, 0) && reached(weights, counts)) {
         uint32_t d = begin;
         for (; d + 1 < begin + kMine; ++d) {
-            if (before + (byCount ? sums.Counts[d] : sums.Weights[d]) >= target) {
+            if (reached(sums.Weights[d], sums.Counts[d])) {
                 break;
             }
             weightBefore += sums.Weights[d];
@@ -595,12 +633,9 @@ __device__ int32_t ClassOf(const T* row, uint32_t classes, typename TKeys<T>::TK
     for (uint32_t c = begin + lane; c < end; c += 64) {
         n += TK::Of(row[c]) == key;
     }
-#pragma unroll
-    for (int d = 32; d > 0; d /= 2) {
-        n += __shfl_xor(n, d);
-    }
+    n = SumUpTo(n);
     __syncthreads();
-    if (lane == 0) {
+    if (lane == 63) {
         shared.Counted[wave] = n;
     }
     __syncthreads();
@@ -616,7 +651,9 @@ __device__ int32_t ClassOf(const T* row, uint32_t classes, typename TKeys<T>::TK
     for (uint32_t c = mine; c < last; ++c) {
         n += TK::Of(row[c]) == key;
     }
-    uint32_t before = static_cast<uint32_t>(SumBefore<kWaves>(n, shared));
+    uint64_t none = 0;
+    uint32_t before = n;
+    SumBefore(none, before, shared);
     if (nth >= before && nth < before + n) {
         for (uint32_t c = mine; c < last; ++c) {
             if (TK::Of(row[c]) == key && before++ == nth) {
@@ -786,8 +823,6 @@ __global__ void __launch_bounds__(THREADS) SampleRowKernel(const T* scores, TSam
         }
         there = lastStep < kDigits - 1 ? there : 0;  // no class that weighs anything is left out by its rank
         __syncthreads();
-        first.template Clear<THREADS>();
-        __syncthreads();
     }
     const A lowest = lastStep < kDigits - 1 ? boundOf((lastStep + 1) * kStep, -1) : kNone;
     uint64_t likely = 0;
@@ -799,7 +834,7 @@ __global__ void __launch_bounds__(THREADS) SampleRowKernel(const T* scores, TSam
             const uint32_t step = stepOf(under);
             const uint64_t whole = weigh.Whole(weight);
             if (step <= lastStep) {
-                first.Add(step, whole);
+                atomicAdd(reinterpret_cast<unsigned long long*>(&first.Weights[step]), static_cast<unsigned long long>(whole));
                 if (atLeast) {
                     likely += weight >= limits.MinP ? whole : 0;
                 }
@@ -808,33 +843,34 @@ __global__ void __launch_bounds__(THREADS) SampleRowKernel(const T* scores, TSam
     });
     __syncthreads();
     uint64_t all = 0;
-    uint32_t longest = 0;
     for (uint32_t d = threadIdx.x; d < kDigits; d += THREADS) {
         all += first.Weights[d];
-        longest = first.Counts[d] > longest && d < kDigits - 1 ? first.Counts[d] : longest;
     }
     all = SumOf(all, shared);
     likely = atLeast ? SumOf(likely, shared) : all;
-    // (a step of more classes than the list holds: by the keys alone)
-    if (MostOf(longest, shared) > LIST) {
-        return DrawAny<T, THREADS, BITS>(row, p, r, limits, weigh, most, later, shared);
-    }
     uint32_t listedStep = kDigits;
     const auto reach = [&](bool byCount, uint64_t target) {
         TPosition<TKey> at{0, 0, 0, 0};
         const uint32_t step = ReachDigit<BITS, THREADS>(first, byCount, target, at, shared);
+        const A low = boundOf((step + 1) * kStep, -1), high = step > 0 ? boundOf(step * kStep, 1) : static_cast<A>(weigh.Best);
+        const auto forStep = [&](auto&& f) {
+            ForRow<T, THREADS>(row, p.Classes, [&](T x, uint32_t c) {
+                const A score = static_cast<A>(x);
+                if (score >= low && score <= high && score > kNone && stepOf(underOf(score)) == step) {
+                    f(TK::Of(x), c);
+                }
+            });
+        };
         __syncthreads();
         if (step != listedStep) {
             if (threadIdx.x == 0) {
                 shared.Listed = 0;
             }
             __syncthreads();
-            const A low = boundOf((step + 1) * kStep, -1), high = step > 0 ? boundOf(step * kStep, 1) : static_cast<A>(weigh.Best);
-            ForRow<T, THREADS>(row, p.Classes, [&](T x, uint32_t c) {
-                const A score = static_cast<A>(x);
-                if (score >= low && score <= high && score > kNone && stepOf(underOf(score)) == step) {
-                    const uint32_t place = atomicAdd(&shared.Listed, 1u);
-                    keys[place] = TK::Of(x);
+            forStep([&](TKey key, uint32_t c) {
+                const uint32_t place = atomicAdd(&shared.Listed, 1u);
+                if (place < LIST) {
+                    keys[place] = key;
                     listed[place] = c;
                 }
             });
@@ -842,39 +878,54 @@ __global__ void __launch_bounds__(THREADS) SampleRowKernel(const T* scores, TSam
             __syncthreads();
         }
         const uint32_t n = shared.Listed;
-        TKey high = 0, low = 0;  // low: of the complement
-        for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
-            const TKey key = keys[i], other = ~key;
-            high = key > high ? key : high;
-            low = other > low ? other : low;
-        }
-        high = MostOf(high, shared);
-        low = ~MostOf(low, shared);
+        const auto forKeys = [&](auto&& f) {
+            if (n <= LIST) {
+                for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
+                    f(keys[i]);
+                }
+            } else {
+                // a step of more classes than the list holds
+                forStep([&](TKey key, uint32_t) { f(key); });
+            }
+        };
+        TKey most = 0, least = 0;  // least: of the complement
+        forKeys([&](TKey key) {
+            const TKey other = ~key;
+            most = key > most ? key : most;
+            least = other > least ? other : least;
+        });
+        most = MostOf(most, shared);
+        least = ~MostOf(least, shared);
         int bits = 0;
-        while (bits < TK::kBits && (high - low) >> bits != 0) {
+        while (bits < TK::kBits && (most - least) >> bits != 0) {
             ++bits;
         }
         TKey prefix = 0;
+        at.Alike = n;
         for (int level = (bits + BITS - 1) / BITS - 1; level >= 0; --level) {
             const uint32_t shift = level * BITS;
             __syncthreads();
             later.template Clear<THREADS>();
             __syncthreads();
-            for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
-                const TKey under = high - keys[i];
+            forKeys([&](TKey key) {
+                const TKey under = most - key;
                 if (shift + BITS >= static_cast<uint32_t>(TK::kBits) || under >> (shift + BITS) == prefix) {
-                    later.Add(static_cast<uint32_t>(under >> shift) & (kDigits - 1), weigh.WholeOf(static_cast<T>(TK::Value(keys[i]))));
+                    later.Add(static_cast<uint32_t>(under >> shift) & (kDigits - 1), weigh.WholeOf(static_cast<T>(TK::Value(key))));
                 }
-            }
+            });
             __syncthreads();
             prefix = prefix << BITS | ReachDigit<BITS, THREADS>(later, byCount, target, at, shared);
         }
-        at.Key = high - prefix;
+        at.Key = most - prefix;
         return at;
     };
     DrawFrom<T>(p, r, limits, weigh, all, likely, there, reach, [&](const TPosition<TKey>& at, uint32_t nth) {
-        // the last position's list has them all, in no order
         const uint32_t n = shared.Listed;
+        if (n > LIST) {
+            return ClassOf<T, THREADS>(row, p.Classes, at.Key, nth, shared);
+        }
+        // the last position's list has them all, in no order
+        __syncthreads();
         for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
             if (keys[i] == at.Key) {
                 uint32_t before = 0;
@@ -912,8 +963,8 @@ __global__ void __launch_bounds__(1024) SampleCountedKernel(const T* scores, TSa
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const size_t r = p.First + blockIdx.x;
     const T* row = scores + r * p.Stride;
-    // A wave's part of the row is contiguous, in pieces of 64 times 16 bytes, four of them on their way. f(keys of a thread's eight classes in pairs, the first one):
-    // keys that grow with the scores, two for the zeros, NaN at both ends
+    // A wave's part of the row is contiguous, in pieces of 64 times 16 bytes, eight of them on their way. f(keys of a thread's eight classes
+    // in pairs, the first one, the piece): keys that grow with the scores, two for the zeros, NaN at both ends
     const uint32_t pieces = (p.Classes + kWaves * 512 - 1) / (kWaves * 512);
     const uint32_t begin = wave * pieces * 512 + lane * 8;
     struct TKeysOfEight {
@@ -934,30 +985,35 @@ __global__ void __launch_bounds__(1024) SampleCountedKernel(const T* scores, TSa
         }
         return words;
     };
-    const auto forPieces = [&](auto&& f) {
-        const auto give = [&](const TValues<uint32_t, 4>& words, uint32_t c) {
-            TKeysOfEight keys;
+    const auto give = [&](const TValues<uint32_t, 4>& words, uint32_t piece, auto&& f) {
+        TKeysOfEight keys;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const TSignedPair sign = __builtin_bit_cast(TSignedPair, words.V[j]) >> TSignedPair{15, 15};
-                keys.V[j] = __builtin_bit_cast(TPair, words.V[j]) ^ (__builtin_bit_cast(TPair, sign) | TPair{0x8000, 0x8000});
-            }
-            f(keys, c);
-        };
-        uint32_t i = 0;
-        for (; i + 4 <= pieces; i += 4) {
-            TValues<uint32_t, 4> words[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                words[j] = keysAt(begin + (i + j) * 512);
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                give(words[j], begin + (i + j) * 512);
-            }
+        for (int j = 0; j < 4; ++j) {
+            const TSignedPair sign = __builtin_bit_cast(TSignedPair, words.V[j]) >> TSignedPair{15, 15};
+            keys.V[j] = __builtin_bit_cast(TPair, words.V[j]) ^ (__builtin_bit_cast(TPair, sign) | TPair{0x8000, 0x8000});
         }
-        for (; i < pieces; ++i) {
-            give(keysAt(begin + i * 512), begin + i * 512);
+        f(keys, begin + piece * 512, piece);
+    };
+    const auto forPieces = [&](auto&& f) {
+        for (uint32_t i = 0; i < pieces; i += 8) {
+            TValues<uint32_t, 4> words[8];
+            // (the last pieces again behind the end; a wave's whole pieces without the row's end need no look at each class)
+            if (begin - lane * 8 + (i + 8 < pieces ? i + 8 : pieces) * 512 <= p.Classes) {
+#pragma unroll
+                for (uint32_t j = 0; j < 8; ++j) {
+                    words[j] = TValues<uint32_t, 4>::Load(row + begin + (i + j < pieces ? i + j : pieces - 1) * 512);
+                }
+#pragma unroll
+                for (uint32_t j = 0; j < 8; ++j) {
+                    if (i + j < pieces) {
+                        give(words[j], i + j, f);
+                    }
+                }
+            } else {
+                for (uint32_t j = i; j < i + 8 && j < pieces; ++j) {
+                    give(keysAt(begin + j * 512), j, f);
+                }
+            }
         }
     };
     FillPowers(shared.Powers);
@@ -966,7 +1022,7 @@ __global__ void __launch_bounds__(1024) SampleCountedKernel(const T* scores, TSa
         reinterpret_cast<uint4*>(lds.Counts)[threadIdx.x + i * kThreads] = uint4{0, 0, 0, 0};
     }
     TPair mosts = {0, 0};
-    forPieces([&](const TKeysOfEight& keys, uint32_t) {
+    forPieces([&](const TKeysOfEight& keys, uint32_t, uint32_t) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             mosts = __builtin_elementwise_max(mosts, keys.V[j]);
@@ -976,7 +1032,7 @@ __global__ void __launch_bounds__(1024) SampleCountedKernel(const T* scores, TSa
     if (most > kHighest) {
         // there are NaN over plus infinity (those do not take part: they are over the best key, which counts as far under it)
         most = 0;
-        forPieces([&](const TKeysOfEight& keys, uint32_t) {
+        forPieces([&](const TKeysOfEight& keys, uint32_t, uint32_t) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const uint32_t key = keys.V[j / 2][j % 2];
@@ -1006,44 +1062,54 @@ __global__ void __launch_bounds__(1024) SampleCountedKernel(const T* scores, TSa
             }
             return n;
         };
-        uint32_t n = 0;
-        forPieces([&](const TKeysOfEight& keys, uint32_t) { n += __popc(alike(keys)); });
-#pragma unroll
-        for (int d = 32; d > 0; d /= 2) {
-            n += __shfl_xor(n, d);
+        // how many of them the pieces have, 256 parts of the row that hold some in a row each: of each part first, then in its pieces
+        const uint32_t each = (pieces + 15) / 16;  // pieces of a part
+        __syncthreads();
+        if (threadIdx.x < 256) {
+            segments.Counts[threadIdx.x] = 0;
         }
         __syncthreads();
-        if (lane == 0) {
-            shared.Counted[wave] = n;
-        }
+        forPieces([&](const TKeysOfEight& keys, uint32_t, uint32_t piece) {
+            const uint32_t n = __popc(alike(keys));
+            if (n != 0) {
+                atomicAdd(&segments.Counts[wave * 16 + piece / each], n);
+            }
+        });
         __syncthreads();
-        uint32_t before = 0;
-        for (uint32_t w = 0; w < wave; ++w) {
-            before += shared.Counted[w];
+        uint32_t counts[4], sum = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            counts[j] = segments.Counts[lane * 4 + j];
+            sum += counts[j];
         }
-        if (nth >= before && nth < before + n) {
-            forPieces([&](const TKeysOfEight& keys, uint32_t c) {
-                const uint32_t mine = alike(keys);
-                if (__ballot(mine != 0) == 0) {
-                    return;
-                }
-                uint32_t sum = __popc(mine);
+        uint32_t before = SumUpTo(sum) - sum, part = lane * 4;
+        const int from = __ffsll(static_cast<unsigned long long>(__ballot(nth < before + sum))) - 1;
 #pragma unroll
-                for (int d = 1; d < 64; d *= 2) {
-                    const uint32_t up = __shfl_up(sum, d);
-                    sum += lane >= static_cast<uint32_t>(d) ? up : 0;
-                }
-                uint32_t place = before + sum - __popc(mine);
-                if (nth >= place && nth < before + sum) {
+        for (uint32_t j = 0; j < 3; ++j) {
+            const uint32_t n = counts[j];
+            const bool past = part == lane * 4 + j && nth >= before + n;
+            before += past ? n : 0;
+            part += past ? 1 : 0;
+        }
+        before = OfLane(before, from);
+        part = OfLane(part, from);
+        if (part / 16 == wave) {
+            for (uint32_t piece = part % 16 * each; piece < (part % 16 + 1) * each && piece < pieces; ++piece) {
+                give(keysAt(begin + piece * 512), piece, [&](const TKeysOfEight& keys, uint32_t c, uint32_t) {
+                    const uint32_t mine = alike(keys);
+                    const uint32_t upTo = before + SumUpTo(static_cast<uint32_t>(__popc(mine)));
+                    uint32_t place = upTo - __popc(mine);
+                    if (nth >= place && nth < upTo) {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        if ((mine >> j & 1) != 0 && place++ == nth) {
-                            shared.Found[0] = c + j;
+                        for (int j = 0; j < 8; ++j) {
+                            if ((mine >> j & 1) != 0 && place++ == nth) {
+                                shared.Found[0] = c + j;
+                            }
                         }
                     }
-                }
-                before += __shfl(sum, 63);
-            });
+                    before = OfLane(upTo, 63);
+                });
+            }
         }
         __syncthreads();
         return static_cast<int32_t>(shared.Found[0]);
@@ -1058,7 +1124,7 @@ __global__ void __launch_bounds__(1024) SampleCountedKernel(const T* scores, TSa
     const auto weigh = limits.Weigh<true>(TK::Value(sharedKey(most)), p.Shift, shared.Powers);
     const uint32_t keys = most - kLowest;  // from the best one down to the last over minus infinity
     uint32_t mine = 0;
-    forPieces([&](const TKeysOfEight& keysOfEight, uint32_t) {
+    forPieces([&](const TKeysOfEight& keysOfEight, uint32_t, uint32_t) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const uint32_t under = most - keysOfEight.V[j / 2][j % 2];
@@ -1105,13 +1171,10 @@ __global__ void __launch_bounds__(1024) SampleCountedKernel(const T* scores, TSa
         uint64_t weight = (v.Weights[0] + v.Weights[1]) + (v.Weights[2] + v.Weights[3]);
         uint32_t count = (v.Counts[0] + v.Counts[1]) + (v.Counts[2] + v.Counts[3]);
         if (__ballot(count != 0) != 0) {
-#pragma unroll
-            for (int d = 32; d > 0; d /= 2) {
-                weight += __shfl_xor(weight, d);
-                count += __shfl_xor(count, d);
-            }
+            weight = SumUpTo(weight);
+            count = SumUpTo(count);
         }
-        if (lane == 0) {
+        if (lane == 63) {
             segments.Weights[segment] = weight;
             segments.Counts[segment] = count;
             all += weight;
@@ -1132,13 +1195,8 @@ __global__ void __launch_bounds__(1024) SampleCountedKernel(const T* scores, TSa
             uint32_t counted = (v.Counts[0] + v.Counts[1]) + (v.Counts[2] + v.Counts[3]);
             const uint64_t mine = weights;
             const uint32_t mineCounted = counted;
-#pragma unroll
-            for (int d = 1; d < 64; d *= 2) {
-                const uint64_t other = __shfl_up(weights, d);
-                const uint32_t otherCounted = __shfl_up(counted, d);
-                weights += lane >= static_cast<uint32_t>(d) ? other : 0;
-                counted += lane >= static_cast<uint32_t>(d) ? otherCounted : 0;
-            }
+            weights = SumUpTo(weights);
+            counted = SumUpTo(counted);
             weights += weight;
             counted += count;
             const uint64_t reached = __ballot(byCount ? counted >= target : weights >= target);
@@ -1156,12 +1214,12 @@ __global__ void __launch_bounds__(1024) SampleCountedKernel(const T* scores, TSa
                 count += past ? c : 0;
                 place += past ? 1 : 0;
             }
-            weight = __shfl(weight, from);
-            count = __shfl(count, from);
+            weight = OfLane(weight, from);
+            count = OfLane(count, from);
             struct TFound {
                 uint32_t Place, Counts;
             };
-            return TFound{static_cast<uint32_t>(__shfl(place, from)), static_cast<uint32_t>(__shfl(of, from))};
+            return TFound{OfLane(place, from), OfLane(of, from)};
         };
         TOfLane v;
 #pragma unroll

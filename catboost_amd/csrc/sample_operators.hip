@@ -573,6 +573,15 @@ __device__ __forceinline__ void ForRow(const T* row, uint32_t classes, F&& f) {
     }
 }
 
+// The same one after the other, for what is rarely done: it takes few registers from the rest of a kernel
+template <typename T, int THREADS, typename F>
+__device__ __forceinline__ void ForRowSlowly(const T* row, uint32_t classes, F&& f) {
+#pragma unroll 1
+    for (uint32_t c = threadIdx.x; c < classes; c += THREADS) {
+        f(row[c], c);
+    }
+}
+
 // A position in a row's order: the key there, how many classes and which weights are before those of that key, how many have it
 template <typename TKey>
 struct TPosition {
@@ -710,7 +719,7 @@ __device__ void DrawByDigits(const T* row, const TSampleArguments& p, size_t r, 
             __syncthreads();
             sums.template Clear<THREADS>();
             __syncthreads();
-            ForRow<T, THREADS>(row, p.Classes, [&](T x, uint32_t) {
+            ForRowSlowly<T, THREADS>(row, p.Classes, [&](T x, uint32_t) {
                 const TKey key = TK::Of(x), under = most - key;
                 if (key != 0 && (level == kLevels - 1 || under >> (shift + BITS) == prefix)) {
                     sums.Add(static_cast<uint32_t>(under >> shift) & ((1u << BITS) - 1), weigh.WholeOf(x));
@@ -731,7 +740,7 @@ template <typename T, int THREADS, int BITS>
 __device__ void DrawAny(const T* row, const TSampleArguments& p, size_t r, const TLimits& limits, const TWeigh<true>& weigh, typename TKeys<T>::TKey most,
                         TDigitSums<BITS>& sums, TShared<THREADS / 64>& shared) {
     uint64_t all = 0, likely = 0, there = 0;
-    ForRow<T, THREADS>(row, p.Classes, [&](T x, uint32_t) {
+    ForRowSlowly<T, THREADS>(row, p.Classes, [&](T x, uint32_t) {
         if (TKeys<T>::Of(x) != 0) {
             const double weight = weigh.Weight(weigh.Under(x));
             ++there;
@@ -943,7 +952,8 @@ __global__ void __launch_bounds__(THREADS) SampleRowKernel(const T* scores, TSam
 }
 
 // 16-bit scores: how often each key comes, counted in 16 bits in LDS, says everything. A weight is computed for each key that there is
-// instead of each class. A key that more than 65535 classes have shows in the counts' sum; such a row is done by digits.
+// instead of each class, and only up to the one of rank TopK. A key that more than 65535 classes have shows in the counts' sum; such a row
+// is done by digits.
 template <typename T>
 __global__ void __launch_bounds__(1024) SampleCountedKernel(const T* scores, TSampleArguments p) {
     using TK = TKeys<T>;
@@ -963,66 +973,72 @@ __global__ void __launch_bounds__(1024) SampleCountedKernel(const T* scores, TSa
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const size_t r = p.First + blockIdx.x;
     const T* row = scores + r * p.Stride;
-    // A wave's part of the row is contiguous, in pieces of 64 times 16 bytes, eight of them on their way. f(keys of a thread's eight classes
-    // in pairs, the first one, the piece): keys that grow with the scores, two for the zeros, NaN at both ends
+    // A wave's part of the row's whole 16 bytes is contiguous, in pieces of 64 times as many; up to seven classes behind them are the first
+    // threads' own. Keys grow with the scores, the zeros have one, NaN are at both ends.
+    const uint32_t whole = p.Classes & ~7u;
     const uint32_t pieces = (p.Classes + kWaves * 512 - 1) / (kWaves * 512);
     const uint32_t begin = wave * pieces * 512 + lane * 8;
     struct TKeysOfEight {
         TPair V[4];
     };
-    const auto keysAt = [&](uint32_t c) {
-        TValues<uint32_t, 4> words;
-        if (c + 8 <= p.Classes) {
-            words = TValues<uint32_t, 4>::Load(row + c);
-        } else {
+    const auto keysAt = [&](uint32_t piece) {
+        const uint32_t c = begin + piece * 512;
+        TValues<uint32_t, 4> words = TValues<uint32_t, 4>::Load(row + (c < whole ? c : 0));
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t none = 0x8000 | kInfinity;
-                const uint32_t low = c + 2 * j < p.Classes ? __builtin_bit_cast(uint16_t, row[c + 2 * j]) : none;
-                const uint32_t high = c + 2 * j + 1 < p.Classes ? __builtin_bit_cast(uint16_t, row[c + 2 * j + 1]) : none;
-                words.V[j] = low | high << 16;
-            }
+        for (int j = 0; j < 4; ++j) {
+            words.V[j] = c < whole ? words.V[j] : 0x10001u * (0x8000 | kInfinity);
         }
         return words;
     };
-    const auto give = [&](const TValues<uint32_t, 4>& words, uint32_t piece, auto&& f) {
+    const auto keysOfWords = [](const TValues<uint32_t, 4>& words) {
         TKeysOfEight keys;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const TSignedPair sign = __builtin_bit_cast(TSignedPair, words.V[j]) >> TSignedPair{15, 15};
-            keys.V[j] = __builtin_bit_cast(TPair, words.V[j]) ^ (__builtin_bit_cast(TPair, sign) | TPair{0x8000, 0x8000});
+            const TPair key = __builtin_bit_cast(TPair, words.V[j]) ^ (__builtin_bit_cast(TPair, sign) | TPair{0x8000, 0x8000});
+            // minus zero's, 0x7fff, becomes zero's
+            keys.V[j] = key + (TPair{1, 1} - __builtin_elementwise_min(key ^ TPair{0x7fff, 0x7fff}, TPair{1, 1}));
         }
-        f(keys, begin + piece * 512, piece);
+        return keys;
+    };
+    // f(keys of a thread's eight classes of a piece in pairs, the piece)
+    constexpr uint32_t kAtOnce = 8;
+    TKeysOfEight held[kAtOnce];
+    const auto load = [&](uint32_t first) {
+        TValues<uint32_t, 4> words[kAtOnce];
+#pragma unroll
+        for (uint32_t j = 0; j < kAtOnce; ++j) {
+            // (the last piece again behind the end: no load waits in a branch)
+            words[j] = keysAt(first + j < pieces ? first + j : pieces - 1);
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < kAtOnce; ++j) {
+            held[j] = keysOfWords(words[j]);
+        }
     };
     const auto forPieces = [&](auto&& f) {
-        for (uint32_t i = 0; i < pieces; i += 8) {
-            TValues<uint32_t, 4> words[8];
-            // (the last pieces again behind the end; a wave's whole pieces without the row's end need no look at each class)
-            if (begin - lane * 8 + (i + 8 < pieces ? i + 8 : pieces) * 512 <= p.Classes) {
+        for (uint32_t first = 0; first < pieces; first += kAtOnce) {
+            load(first);
 #pragma unroll
-                for (uint32_t j = 0; j < 8; ++j) {
-                    words[j] = TValues<uint32_t, 4>::Load(row + begin + (i + j < pieces ? i + j : pieces - 1) * 512);
-                }
-#pragma unroll
-                for (uint32_t j = 0; j < 8; ++j) {
-                    if (i + j < pieces) {
-                        give(words[j], i + j, f);
-                    }
-                }
-            } else {
-                for (uint32_t j = i; j < i + 8 && j < pieces; ++j) {
-                    give(keysAt(begin + j * 512), j, f);
+            for (uint32_t j = 0; j < kAtOnce; ++j) {
+                if (first + j < pieces) {
+                    f(held[j], first + j);
                 }
             }
         }
     };
+    uint32_t ownKey = kLowest;
+    if (whole + threadIdx.x < p.Classes) {
+        const TValues<uint32_t, 4> word = {{__builtin_bit_cast(uint16_t, row[whole + threadIdx.x]), 0, 0, 0}};
+        ownKey = keysOfWords(word).V[0][0];
+    }
     FillPowers(shared.Powers);
 #pragma unroll
     for (uint32_t i = 0; i < kWords / 4 / kThreads; ++i) {
         reinterpret_cast<uint4*>(lds.Counts)[threadIdx.x + i * kThreads] = uint4{0, 0, 0, 0};
     }
-    TPair mosts = {0, 0};
-    forPieces([&](const TKeysOfEight& keys, uint32_t, uint32_t) {
+    TPair mosts = {static_cast<uint16_t>(ownKey), 0};
+    forPieces([&](const TKeysOfEight& keys, uint32_t) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             mosts = __builtin_elementwise_max(mosts, keys.V[j]);
@@ -1031,8 +1047,8 @@ __global__ void __launch_bounds__(1024) SampleCountedKernel(const T* scores, TSa
     uint32_t most = MostOf<kWaves>(static_cast<uint32_t>(mosts[0] > mosts[1] ? mosts[0] : mosts[1]), shared);
     if (most > kHighest) {
         // there are NaN over plus infinity (those do not take part: they are over the best key, which counts as far under it)
-        most = 0;
-        forPieces([&](const TKeysOfEight& keys, uint32_t, uint32_t) {
+        most = ownKey <= kHighest ? ownKey : 0;
+        forPieces([&](const TKeysOfEight& keys, uint32_t) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const uint32_t key = keys.V[j / 2][j % 2];
@@ -1041,7 +1057,6 @@ __global__ void __launch_bounds__(1024) SampleCountedKernel(const T* scores, TSa
         });
         most = MostOf<kWaves>(most, shared);
     }
-    most = most == 0x7fff ? 0x8000 : most;  // minus zero is zero
     if (most <= kLowest) {
         if (threadIdx.x == 0) {
             Answer<T>(p, r, -1, 0);
@@ -1052,16 +1067,9 @@ __global__ void __launch_bounds__(1024) SampleCountedKernel(const T* scores, TSa
     const auto sharedKey = [](uint32_t key) { return key - kLowest - (key >> 15); };  // as TKeys has it, with one key for both zeros
     // the (nth + 1)-th class with this key
     const auto classOf = [&](uint32_t key, uint32_t nth) {
-        const uint32_t other = key == 0x8000 ? 0x7fff : key;
-        const auto alike = [&](const TKeysOfEight& keys) {
-            uint32_t n = 0;  // a bit for each
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const uint32_t k = keys.V[j / 2][j % 2];
-                n |= (k == key || k == other ? 1u : 0u) << j;
-            }
-            return n;
-        };
+        const TPair wanted = {static_cast<uint16_t>(key), static_cast<uint16_t>(key)};
+        // 1 where a key is another one
+        const auto other = [&](TPair keys) { return __builtin_elementwise_min(keys ^ wanted, TPair{1, 1}); };
         // how many of them the pieces have, 256 parts of the row that hold some in a row each: of each part first, then in its pieces
         const uint32_t each = (pieces + 15) / 16;  // pieces of a part
         __syncthreads();
@@ -1069,8 +1077,9 @@ __global__ void __launch_bounds__(1024) SampleCountedKernel(const T* scores, TSa
             segments.Counts[threadIdx.x] = 0;
         }
         __syncthreads();
-        forPieces([&](const TKeysOfEight& keys, uint32_t, uint32_t piece) {
-            const uint32_t n = __popc(alike(keys));
+        forPieces([&](const TKeysOfEight& keys, uint32_t piece) {
+            const TPair others = (other(keys.V[0]) + other(keys.V[1])) + (other(keys.V[2]) + other(keys.V[3]));
+            const uint32_t n = 8 - others[0] - others[1];
             if (n != 0) {
                 atomicAdd(&segments.Counts[wave * 16 + piece / each], n);
             }
@@ -1084,6 +1093,7 @@ __global__ void __launch_bounds__(1024) SampleCountedKernel(const T* scores, TSa
         }
         uint32_t before = SumUpTo(sum) - sum, part = lane * 4;
         const int from = __ffsll(static_cast<unsigned long long>(__ballot(nth < before + sum))) - 1;
+        const uint32_t inPieces = OfLane(before + sum, 63);
 #pragma unroll
         for (uint32_t j = 0; j < 3; ++j) {
             const uint32_t n = counts[j];
@@ -1091,24 +1101,33 @@ __global__ void __launch_bounds__(1024) SampleCountedKernel(const T* scores, TSa
             before += past ? n : 0;
             part += past ? 1 : 0;
         }
-        before = OfLane(before, from);
-        part = OfLane(part, from);
-        if (part / 16 == wave) {
+        before = OfLane(before, from < 0 ? 0 : from);
+        part = OfLane(part, from < 0 ? 0 : from);
+        if (from < 0) {
+            // behind the whole 16 bytes
+            const uint64_t own = __ballot(ownKey == key);
+            if (wave == 0 && ownKey == key && inPieces + __popcll(own & ((uint64_t(1) << lane) - 1)) == nth) {
+                shared.Found[0] = whole + lane;
+            }
+        } else if (part / 16 == wave) {
             for (uint32_t piece = part % 16 * each; piece < (part % 16 + 1) * each && piece < pieces; ++piece) {
-                give(keysAt(begin + piece * 512), piece, [&](const TKeysOfEight& keys, uint32_t c, uint32_t) {
-                    const uint32_t mine = alike(keys);
-                    const uint32_t upTo = before + SumUpTo(static_cast<uint32_t>(__popc(mine)));
-                    uint32_t place = upTo - __popc(mine);
-                    if (nth >= place && nth < upTo) {
+                const TKeysOfEight keys = keysOfWords(keysAt(piece));
+                uint32_t mine = 0;
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            if ((mine >> j & 1) != 0 && place++ == nth) {
-                                shared.Found[0] = c + j;
-                            }
+                for (int j = 0; j < 8; ++j) {
+                    mine += keys.V[j / 2][j % 2] == key;
+                }
+                const uint32_t upTo = before + SumUpTo(mine);
+                uint32_t place = upTo - mine;
+                if (nth >= place && nth < upTo) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        if (keys.V[j / 2][j % 2] == key && place++ == nth) {
+                            shared.Found[0] = begin + piece * 512 + j;
                         }
                     }
-                    before = OfLane(upTo, 63);
-                });
+                }
+                before = OfLane(upTo, 63);
             }
         }
         __syncthreads();
@@ -1124,25 +1143,27 @@ __global__ void __launch_bounds__(1024) SampleCountedKernel(const T* scores, TSa
     const auto weigh = limits.Weigh<true>(TK::Value(sharedKey(most)), p.Shift, shared.Powers);
     const uint32_t keys = most - kLowest;  // from the best one down to the last over minus infinity
     uint32_t mine = 0;
-    forPieces([&](const TKeysOfEight& keysOfEight, uint32_t, uint32_t) {
+    if (most - ownKey < keys) {
+        ++mine;
+        atomicAdd(&lds.Counts[(most - ownKey) >> 1], 1u << ((most - ownKey) << 4 & 31));
+    }
+    const TPair best = {static_cast<uint16_t>(most), static_cast<uint16_t>(most)};
+    forPieces([&](const TKeysOfEight& keysOfEight, uint32_t) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const uint32_t under = most - keysOfEight.V[j / 2][j % 2];
-            if (under < keys) {
-                ++mine;
-                atomicAdd(&lds.Counts[under >> 1], under & 1 ? 0x10000u : 1u);
+        for (int j = 0; j < 4; ++j) {
+            // (keys over the best one, of NaN, come out at `most` at least)
+            const TPair pair = best - keysOfEight.V[j];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const uint32_t under = pair[k];
+                if (under < keys) {
+                    ++mine;
+                    atomicAdd(&lds.Counts[under >> 1], 1u << (under << 4 & 31));
+                }
             }
         }
     });
     const uint64_t there = SumOf(mine, shared);
-    const auto countOf = [&](uint32_t under) { return lds.Counts[under >> 1] >> (under & 1) * 16 & 0xffff; };
-    if (threadIdx.x == 0 && most >= 0x8000) {
-        // minus zero's counts become zero's (65536 of both at most show in the sum)
-        const uint32_t zero = most - 0x8000, minus = zero + 1;
-        const uint32_t n = minus < keys ? countOf(minus) : 0;
-        lds.Counts[minus >> 1] -= n << (minus & 1) * 16;
-        lds.Counts[zero >> 1] += n << (zero & 1) * 16;
-    }
     __syncthreads();
     // Sums of 256 keys in a row, four for a lane; a wave has every sixteenth of them, since the keys that there are lie together
     const auto weightOf = [&](uint32_t under) { return weigh.Weight(weigh.Under(static_cast<T>(TK::Value(sharedKey(most - under))))); };
@@ -1165,24 +1186,41 @@ __global__ void __launch_bounds__(1024) SampleCountedKernel(const T* scores, TSa
         }
         return v;
     };
-    uint64_t likely = 0, all = 0, counts = 0;
+    uint64_t counts = 0;
     for (uint32_t segment = wave; segment < 256; segment += kWaves) {
-        const TOfLane v = keysOf(segment, &likely);
-        uint64_t weight = (v.Weights[0] + v.Weights[1]) + (v.Weights[2] + v.Weights[3]);
-        uint32_t count = (v.Counts[0] + v.Counts[1]) + (v.Counts[2] + v.Counts[3]);
-        if (__ballot(count != 0) != 0) {
-            weight = SumUpTo(weight);
-            count = SumUpTo(count);
-        }
+        const uint2 words = reinterpret_cast<const uint2*>(lds.Counts)[segment * 64 + lane];
+        const uint32_t count = (words.x & 0xffff) + (words.x >> 16) + (words.y & 0xffff) + (words.y >> 16);
+        const uint32_t sum = SumUpTo(count);
+        counts += count;
         if (lane == 63) {
-            segments.Weights[segment] = weight;
-            segments.Counts[segment] = count;
-            all += weight;
-            counts += count;
+            segments.Counts[segment] = sum;
+            segments.Weights[segment] = 0;
         }
     }
     if (SumOf(counts, shared) != there) {
         return DrawAny<T, kThreads, 11>(row, p, r, limits, weigh, sharedKey(most), lds.Sums, shared);
+    }
+    // the last segment whose weights are asked for
+    uint32_t lastSegment = 255;
+    if (limits.TopK > 0 && static_cast<uint64_t>(limits.TopK) < there) {
+        uint32_t sum = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            sum += segments.Counts[lane * 4 + j];
+        }
+        const uint64_t reached = __ballot(SumUpTo(sum) >= static_cast<uint32_t>(limits.TopK));
+        lastSegment = (__ffsll(static_cast<unsigned long long>(reached)) - 1) * 4 + 3;
+    }
+    uint64_t likely = 0, all = 0;
+    for (uint32_t segment = wave; segment <= lastSegment; segment += kWaves) {
+        if (segments.Counts[segment] != 0) {
+            const TOfLane v = keysOf(segment, &likely);
+            const uint64_t weight = SumUpTo((v.Weights[0] + v.Weights[1]) + (v.Weights[2] + v.Weights[3]));
+            if (lane == 63) {
+                segments.Weights[segment] = weight;
+                all += weight;
+            }
+        }
     }
     all = SumOf(all, shared);
     likely = SumOf(likely, shared);

@@ -503,6 +503,12 @@ __device__ __forceinline__ void CopyToLds(const void* from, char* to) {
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (__attribute__((address_space(3))) void*)to, 16, 0, 0);
 }
 
+// What every wave copied so far is in LDS for all
+__device__ __forceinline__ void CopiesAreThere() {
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): copies count as loads
+    __syncthreads();
+}
+
 // One operand of a tile of 64 k, as TOperand, but copied straight to LDS: lines without gaps, in which pieces of 16 bytes trade
 // places, so that the lanes which read at a time meet different banks.
 template <typename T, int SIZE, bool LINE_IS_K, int THREADS>
@@ -689,7 +695,7 @@ __global__ void __launch_bounds__(WM* WN* WK * 64) LargeProductKernel(const TPro
         copy(group, myEven);
     }
     for (uint32_t step = group; step - group < allSteps; step += 2 * WK) {
-        __syncthreads();  // the step's copies are there, what the ones to come overwrite has been read
+        CopiesAreThere();  // of this step; and what those to come overwrite has been read
         if (step + WK < allSteps) {
             copy(step + WK, myOdd);
         }
@@ -697,7 +703,7 @@ __global__ void __launch_bounds__(WM* WN* WK * 64) LargeProductKernel(const TPro
             multiply(myEven);
         }
         if (step - group + WK < allSteps) {
-            __syncthreads();
+            CopiesAreThere();
             if (step + 2 * WK < allSteps) {
                 copy(step + 2 * WK, myEven);
             }
@@ -918,7 +924,7 @@ __global__ void __launch_bounds__(256) StreamProductKernel(const TProduct<T> p) 
 
 // ---------------------------------------------------------------- launches ----
 
-constexpr uint64_t kMostGroups = uint64_t(1) << 22;  // of a launch
+constexpr uint64_t kMostGroups = uint64_t(1) << 21;  // of a launch, of up to 1024 threads
 
 template <int FORM, int PROJECTIONS, typename T, int TM, int TN>
 void SetTiles(TProduct<T>& p) {
@@ -978,6 +984,12 @@ bool TakesCopies(const TProduct<T>& p) {
 template <int FORM, int PROJECTIONS, typename T>
 void MultiplyBy(const TCallDevice& call, const TProduct<T>& p) {
     const uint32_t used = std::max(1u, std::min(p.Segments.Experts, p.Segments.Rows)), each = p.Segments.Rows / used;
+    // tiles of `size` that there are about
+    const auto tiles = [&](uint64_t size) {
+        const auto parts = [&](uint64_t n) { return (n + size - 1) / size; };
+        const uint64_t of = parts(p.N) * PROJECTIONS;
+        return FORM == kWeights ? p.Segments.Experts * parts(p.M) * of : FORM == kRows ? used * parts(each) * of : used * parts(each) * parts(p.N);
+    };
     if constexpr (FORM == kRows) {
         // weights that are read for 16 rows (14 x 4096 to 1024 of 64 experts 24 and 44; 30 and 60 by tiles; one row to 131000 outputs 186, 201)
         if (each <= 16) {
@@ -986,12 +998,6 @@ void MultiplyBy(const TCallDevice& call, const TProduct<T>& p) {
     }
     if constexpr (sizeof(T) == 2) {
         if (TakesCopies<FORM, PROJECTIONS>(p)) {
-            // tiles of `size` that there are about
-            const auto tiles = [&](uint64_t size) {
-                const auto parts = [&](uint64_t n) { return (n + size - 1) / size; };
-                const uint64_t of = parts(p.N) * PROJECTIONS;
-                return FORM == kWeights ? p.Segments.Experts * parts(p.M) * of : FORM == kRows ? used * parts(each) * of : used * parts(each) * parts(p.N);
-            };
             if constexpr (FORM == kWeights) {
                 // (2048 x 4096 weights of one expert's 1024 rows, 256 tiles, 46 and 50; 2048 x 2048 of 2048 rows, 64 tiles, 68 and 39)
                 if (tiles(256) >= 256) {
@@ -1038,9 +1044,11 @@ void MultiplyBy(const TCallDevice& call, const TProduct<T>& p) {
             }
         }
     }
-    if constexpr (sizeof(T) == 8) {
-        LaunchProduct<FORM, PROJECTIONS, T, 64, 64, 2, 2, 64>(call, p);
-    } else {
+    // (32 bits, 5003 x 1001 to 699 of 5 experts, 240 tiles: 100 and 152; 4096 x 4096 to 4096, 1024 tiles: 1315 and 1177)
+    if (sizeof(T) == 8 || tiles(128) <= 384) {
+        return LaunchProduct<FORM, PROJECTIONS, T, 64, 64, 2, 2, 64>(call, p);
+    }
+    if constexpr (sizeof(T) < 8) {
         LaunchProduct<FORM, PROJECTIONS, T, 128, 128, 2, 2, 64>(call, p);
     }
 }

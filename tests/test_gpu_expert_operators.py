@@ -349,3 +349,232 @@ def test_infinities_stay_in_their_rows(kind):
     bad = ~torch.isfinite(dx)
     assert not bad[first].any() and bad[second, 0].all() and bad.sum() == second.stop - second.start
     assert torch.isfinite(dw).all()
+
+
+def far(rows, width, stride, kind, fill):
+    """Rows of random values `stride` apart, in memory that is not touched between them."""
+    whole = torch.empty((rows - 1) * stride + width, dtype=TYPES[kind], device="cuda")
+    t = whole.as_strided((rows, width), (stride, 1))
+    t.copy_(fill)
+    return t
+
+
+@pytest.mark.parametrize("stride", [(1 << 22) - 8, (1 << 22) + 3], ids=["copied", "loaded"])
+def test_offsets_past_32_bits(stride):
+    """1100 rows that far apart: the last ones are 2^32 values and more behind the first."""
+    kind, rows, width, outputs, experts = cb.BFLOAT16, 1100, 72, 64, 3
+    rng = np.random.default_rng(2)
+    routes = Rows(rng, rows, experts, 3, 0)
+    x = far(rows, width, stride, kind, torch.from_numpy(rng.standard_normal((rows, width))))
+    d = far(rows, outputs, stride, kind, torch.from_numpy(rng.standard_normal((rows, outputs))))
+    w = weights_of(rng, kind, experts, outputs, width)
+    y, dx = far(rows, outputs, stride, kind, torch.full((rows, outputs), SENTINEL)), far(rows, width, stride, kind, torch.full((rows, width), SENTINEL))
+    dw = torch.full_like(w, SENTINEL)
+    multiply(kind, x, w, routes.offsets.data_ptr(), y)
+    cb.multiply_rows_backward(kind, rows, width, outputs, experts, routes.offsets.data_ptr(), d.data_ptr(), stride, x.data_ptr(), stride, w.data_ptr(),
+                              w.stride(0), dx.data_ptr(), stride, dw.data_ptr(), dw.stride(0), torch.cuda.current_stream().cuda_stream)
+    X, W, D, Y, DX, DW = (exactly(t) for t in (x, w, d, y, dx, dw))
+    for e in range(experts):
+        part = routes.of(e)
+        within(Y[part], X[part] @ W[e].T, product_bound(X[part], W[e], kind), kind)
+        within(DX[part], D[part] @ W[e], product_bound(D[part], W[e].T, kind), kind)
+        within(DW[e], D[part].T @ X[part], product_bound(D[part].T, X[part].T, kind), kind)
+    assert np.all(Y[routes.bounds[-1]:] == SENTINEL) and np.all(DX[routes.bounds[-1]:] == SENTINEL)
+
+
+@pytest.mark.parametrize("kind", [cb.FLOAT32, cb.BFLOAT16], ids=NAMES.get)
+def test_experts_far_apart(kind):
+    """Weights whose experts are 2^31 values apart."""
+    rng = np.random.default_rng(4)
+    rows, width, outputs, apart = 300, 64, 72, 1 << 31
+    routes = Rows(rng, rows, 3, 0, 0)
+    values = torch.from_numpy(rng.standard_normal((3, outputs, width))).to(TYPES[kind])
+    w, dw = (torch.empty(2 * apart + outputs * width, dtype=TYPES[kind], device="cuda").as_strided((3, outputs, width), (apart, width, 1)) for _ in range(2))
+    w.copy_(values)
+    x, d = padded(rng.standard_normal((rows, width)), kind), padded(rng.standard_normal((rows, outputs)), kind)
+    y = torch.zeros(rows, outputs, dtype=TYPES[kind], device="cuda")
+    multiply(kind, x, w, routes.offsets.data_ptr(), y)
+    cb.multiply_rows_backward(kind, rows, width, outputs, 3, routes.offsets.data_ptr(), d.data_ptr(), outputs, x.data_ptr(), width, w.data_ptr(), apart, 0, 0,
+                              dw.data_ptr(), apart, torch.cuda.current_stream().cuda_stream)
+    X, W, D, Y, DW = (exactly(t) for t in (x, w, d, y, dw))
+    for e in range(3):
+        part = routes.of(e)
+        within(Y[part], X[part] @ W[e].T, product_bound(X[part], W[e], kind), kind)
+        within(DW[e], D[part].T @ X[part], product_bound(D[part].T, X[part].T, kind), kind)
+
+
+# rows, width, outputs, experts: each of the kernels for many rows or few tiles
+LARGER = [(3000, 136, 512, 2), (4200, 256, 2048, 4), (600, 520, 264, 3), (40, 2080, 512, 4), (14, 1000, 2056, 6), (33, 300, 5000, 2), (2500, 64, 16, 3), (9000, 72, 72, 1)]
+
+
+@pytest.mark.parametrize("kind", [cb.FLOAT32, cb.FLOAT16, cb.BFLOAT16], ids=NAMES.get)
+@pytest.mark.parametrize("shape", LARGER, ids=str)
+def test_larger_sizes(kind, shape):
+    rows, width, hidden, experts = shape
+    rng = np.random.default_rng(rows)
+    routes = Rows(rng, rows, experts, 0, 0)
+    x, d = padded(rng.standard_normal((rows, width)), kind), padded(rng.standard_normal((rows, hidden)), kind)
+    gate, up = (weights_of(rng, kind, experts, hidden, width).mul_(width ** -0.5) for _ in range(2))
+    h, y = torch.zeros(rows, hidden, dtype=TYPES[kind], device="cuda"), torch.zeros(rows, hidden, dtype=TYPES[kind], device="cuda")
+    kept, pre = torch.zeros(rows, 2 * hidden, dtype=torch.float32, device="cuda"), torch.zeros(rows, 2 * hidden, dtype=TYPES[kind], device="cuda")
+    dx, dgate, dup = torch.zeros_like(x), torch.zeros_like(gate), torch.zeros_like(up)
+    offsets = routes.offsets.data_ptr()
+    multiply(kind, x, gate, offsets, y)
+    gated(kind, cb.RELU, x, gate, up, offsets, h, kept)
+    gated_backward(kind, cb.RELU, d, x, gate, up, offsets, kept, pre, dx, dgate, dup)
+    X, G, U, H, Y, K, P, DX, DG, DU = (exactly(t) for t in (x, gate, up, h, y, kept, pre, dx, dgate, dup))
+    for e in range(experts):
+        part = routes.of(e)
+        g, v = X[part] @ G[e].T, X[part] @ U[e].T
+        g_off, v_off = product_bound(X[part], G[e], kind), product_bound(X[part], U[e], kind)
+        within(Y[part], g, g_off, kind)
+        within(K[part, :hidden], g, g_off, cb.FLOAT32)
+        within(K[part, hidden:], v, v_off, cb.FLOAT32)
+        a = np.maximum(g, 0)
+        within(H[part], a * v, g_off * (np.abs(v) + v_off) + a * v_off + 2 * u(kind) * np.abs(a * v), kind)
+        dg, du = P[part, :hidden], P[part, hidden:]
+        both = np.concatenate([dg, du], 1)
+        within(DX[part], dg @ G[e] + du @ U[e], product_bound(both, np.concatenate([G[e], U[e]]).T, kind, 64), kind)
+        within(DG[e], dg.T @ X[part], product_bound(dg.T, X[part].T, kind), kind)
+        within(DU[e], du.T @ X[part], product_bound(du.T, X[part].T, kind), kind)
+
+
+class Block:
+    """A step of a routed block, from rows to drawn classes and back to the gradients of what its experts learn."""
+
+    def __init__(self, rows=300, width=128, hidden=192, experts=8, per_row=2, classes=5000, kind=cb.BFLOAT16):
+        g = torch.Generator(device="cuda").manual_seed(5)
+        t = TYPES[kind]
+        self.sizes = rows, width, hidden, experts, per_row, classes, kind
+
+        def randn(*shape):
+            return torch.randn(*shape, generator=g, device="cuda")
+
+        self.x, self.router = randn(rows, width).to(t), (randn(1, experts, width) * 0.2).to(t)
+        self.gate, self.up = ((randn(experts, hidden, width) * width ** -0.5).to(t) for _ in range(2))
+        self.down, self.head = (randn(experts, width, hidden) * hidden ** -0.5).to(t), (randn(1, classes, width) * 0.3).to(t)
+        self.uniform, self.dout = torch.rand(rows, generator=g, device="cuda"), randn(rows, width).to(t)
+        slots = rows * per_row
+        empty = lambda *shape, dtype=t: torch.zeros(*shape, dtype=dtype, device="cuda")  # noqa: E731
+        self.gates, self.ids, self.weights = empty(rows, experts), empty(rows, per_row, dtype=torch.int32), empty(rows, per_row, dtype=torch.float32)
+        self.places, self.offsets = empty(slots, dtype=torch.int32), empty(experts + 1, dtype=torch.int32)
+        self.work = empty(cb.sort_by_expert_bytes(slots, experts), dtype=torch.uint8)
+        self.sorted, self.h, self.y = empty(slots, width), empty(slots, hidden), empty(slots, width)
+        self.kept, self.pre = empty(slots, 2 * hidden, dtype=torch.float32), empty(slots, 2 * hidden)
+        self.out, self.scores, self.classes, self.shares = empty(rows, width), empty(rows, classes), empty(rows, dtype=torch.int32), empty(rows, dtype=torch.float32)
+        self.dy, self.dh, self.dsorted, self.dx = empty(slots, width), empty(slots, hidden), empty(slots, width), empty(rows, width)
+        self.ddown, self.dgate, self.dup, self.dweights = (torch.zeros_like(v) for v in (self.down, self.gate, self.up, self.weights))
+
+    def __call__(self):
+        rows, width, hidden, experts, per_row, classes, kind = self.sizes
+        s, slots, p = torch.cuda.current_stream().cuda_stream, rows * per_row, lambda t: t.data_ptr()  # noqa: E731
+        cb.multiply_rows(kind, rows, width, experts, 1, 0, p(self.x), width, p(self.router), 0, p(self.gates), experts, s)
+        cb.select_top(kind, rows, experts, p(self.gates), experts, per_row, True, p(self.ids), p(self.weights), s)
+        cb.sort_by_expert(slots, experts, p(self.ids), p(self.places), p(self.offsets), p(self.work), self.work.numel(), s)
+        cb.dispatch_rows(kind, rows, width, per_row, p(self.x), width, p(self.places), p(self.sorted), slots, width, s)
+        cb.gated_rows(kind, cb.SILU, slots, width, hidden, experts, p(self.offsets), p(self.sorted), width, p(self.gate), p(self.up), hidden * width, p(self.h),
+                      hidden, p(self.kept), s)
+        cb.multiply_rows(kind, slots, hidden, width, experts, p(self.offsets), p(self.h), hidden, p(self.down), hidden * width, p(self.y), width, s)
+        cb.combine_rows(kind, rows, width, per_row, p(self.y), slots, width, p(self.places), p(self.weights), p(self.out), width, s)
+        cb.multiply_rows(kind, rows, width, classes, 1, 0, p(self.out), width, p(self.head), 0, p(self.scores), classes, s)
+        cb.sample_classes(kind, rows, classes, p(self.scores), classes, cb.sampling(), p(self.uniform), p(self.classes), p(self.shares), 0, 0, s)
+        # and back
+        cb.combine_rows_backward(kind, rows, width, per_row, p(self.dout), width, p(self.y), slots, width, p(self.places), p(self.weights), p(self.dy), width,
+                                 p(self.dweights), s)
+        cb.multiply_rows_backward(kind, slots, hidden, width, experts, p(self.offsets), p(self.dy), width, p(self.h), hidden, p(self.down), hidden * width,
+                                  p(self.dh), hidden, p(self.ddown), hidden * width, s)
+        cb.gated_rows_backward(kind, cb.SILU, slots, width, hidden, experts, p(self.offsets), p(self.dh), hidden, p(self.sorted), width, p(self.gate), p(self.up),
+                               hidden * width, p(self.kept), p(self.pre), p(self.dsorted), width, p(self.dgate), p(self.dup), hidden * width, s)
+        cb.combine_rows(kind, rows, width, per_row, p(self.dsorted), slots, width, p(self.places), 0, p(self.dx), width, s)
+
+    def results(self):
+        return [self.out, self.scores, self.classes, self.shares, self.dx, self.dgate, self.dup, self.ddown, self.dweights]
+
+
+def test_a_block_forward_and_back():
+    """All of them as they are used together, against one expression in 64 bits and its derivatives."""
+    b = Block()
+    b()
+    rows, width, hidden, experts, per_row, classes, kind = b.sizes
+    x = b.x.double().requires_grad_()
+    gate, up, down, weights = (t.double().requires_grad_() for t in (b.gate, b.up, b.down, b.weights))
+    out = torch.zeros(rows, width, dtype=torch.float64, device="cuda")
+    for k in range(per_row):
+        for e in range(experts):
+            at = torch.nonzero(b.ids[:, k] == e)[:, 0]
+            h = torch.nn.functional.silu(x[at] @ gate[e].T) * (x[at] @ up[e].T)
+            out = out.index_add(0, at, (h @ down[e].T) * weights[at, k, None])
+    gradients = torch.autograd.grad(out, [x, gate, up, down, weights], b.dout.double())
+    # In the norm, every rounding to bf16 on the way adds at most half a step, 2^-8, of what it rounds: rows have 3 (h, y, the sum), gradients of
+    # rows 5 (dy, dh, the values' gradients, their product, the sum) and of weights up to 4
+    for got, want, roundings in [(b.out, out, 3), (b.dx, gradients[0], 5), (b.dgate, gradients[1], 4), (b.dup, gradients[2], 4), (b.ddown, gradients[3], 3),
+                                 (b.dweights, gradients[4], 2)]:
+        assert (got.double() - want).norm() <= roundings * 2.0 ** -8 * want.norm()
+    scores = b.out.double() @ b.head[0].double().T
+    assert (b.scores.double() - scores).abs().max() <= 2.0 ** -8 * scores.abs().max() * 1.01
+    p = torch.softmax(b.scores.double(), 1)
+    drawn = torch.gather(p, 1, b.classes[:, None].long())[:, 0]
+    assert torch.allclose(b.shares.double(), drawn, rtol=1e-6, atol=0)
+    best_first = torch.sort(b.scores.double(), dim=1, descending=True, stable=True).indices
+    sums = torch.cumsum(torch.gather(p, 1, best_first), 1)
+    rank = (best_first == b.classes[:, None]).long().argmax(1)
+    upto = torch.gather(sums, 1, rank[:, None])[:, 0]
+    assert torch.all(upto > b.uniform.double() - 1e-9) and torch.all(upto - drawn <= b.uniform.double() + 1e-9)
+
+
+def test_a_block_in_a_graph():
+    """Captured, and replayed on other values with other work between, it gives what the eager calls give."""
+    b = Block(rows=130)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        b()
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            b()
+    for step in range(3):
+        b.x.mul_(-0.9)
+        b.uniform.copy_(torch.rand(130, device="cuda"))
+        b()
+        expected = [t.clone() for t in b.results()]
+        for t in b.results():
+            t.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, e) for a, e in zip(b.results(), expected))
+
+
+def test_two_blocks_on_streams_of_their_own():
+    blocks, streams = [Block(rows=200), Block(rows=400)], [torch.cuda.Stream() for _ in range(2)]
+    expected = []
+    for b in blocks:
+        b()
+        torch.cuda.synchronize()
+        expected.append([t.clone() for t in b.results()])
+        for t in b.results():
+            t.zero_()
+    torch.cuda.synchronize()
+    for b, s in zip(blocks * 3, streams * 3):
+        with torch.cuda.stream(s):
+            b()
+    torch.cuda.synchronize()
+    for b, e in zip(blocks, expected):
+        assert all(torch.equal(x, y) for x, y in zip(b.results(), e))
+
+
+def test_more_experts_than_a_wave_has_lanes():
+    rng = np.random.default_rng(8)
+    kind, rows, width, outputs, experts = cb.BFLOAT16, 5000, 32, 24, 1024
+    routes = Rows(rng, rows, experts, 9, 0.5)
+    x, w = padded(rng.standard_normal((rows, width)), kind), weights_of(rng, kind, experts, outputs, width)
+    y = torch.full((rows, outputs), SENTINEL, dtype=torch.bfloat16, device="cuda")
+    multiply(kind, x, w, routes.offsets.data_ptr(), y)
+    X, W, Y = exactly(x), exactly(w), exactly(y)
+    of = np.searchsorted(routes.bounds[1:], np.arange(rows - 9), side="right")
+    expected, bound = np.zeros((rows - 9, outputs)), np.zeros((rows - 9, outputs))
+    for r, e in enumerate(of):
+        expected[r], bound[r] = W[e] @ X[r], (width + 1) * 2.0 ** -24 * 1.01 * (np.abs(W[e]) @ np.abs(X[r]))
+    within(Y[:rows - 9], expected, bound, kind)
+    assert np.all(Y[rows - 9:] == SENTINEL)

@@ -244,3 +244,63 @@ def test_replays(kind, classes):
         torch.cuda.synchronize()
         assert torch.equal(d.indexes, expected[0]) and torch.equal(d.weights, expected[1])
         d.check()
+
+
+@pytest.mark.parametrize("kind", [cb.FLOAT32, cb.BFLOAT16], ids=NAMES.get)
+@pytest.mark.parametrize("classes", [10, 100, 2000, 20000])
+def test_rows_past_32_bits(kind, classes):
+    """Rows that begin more than 2^32 bytes, and 2^31 values, behind the first."""
+    rows, stride = 3, (1 << 31) + 1
+    rng = np.random.default_rng(classes)
+    d = Draw(kind, scores_of(rng, rows, classes, kind), rng.random(rows), top_p=[0.9] * rows)
+    expected = d.indexes.clone()
+    wide = torch.empty((rows - 1) * stride + classes, dtype=TYPES[kind], device="cuda").as_strided((rows, classes), (stride, 1))
+    wide.copy_(d.scores)
+    d.scores = wide
+    d.indexes.fill_(-7)
+    d()
+    assert torch.equal(d.indexes, expected)
+
+
+@ALL
+@pytest.mark.parametrize("classes", [16, 33, 512, 3000, 33333])
+def test_rows_at_any_address(kind, classes):
+    """Rows that begin anywhere, next to others of NaN."""
+    rng = np.random.default_rng(1)
+    d = Draw(kind, scores_of(rng, 5, classes, kind), rng.random(5), top_k=[0, 9, 0, 200, 0], top_p=[1, 1, 0.5, 0.9, 0.2])
+    expected = d.indexes.clone(), d.weights.clone()
+    values = d.scores.clone()
+    for shift in (1, 2, 3, 5):
+        flat = torch.full((shift + 5 * (classes + 1) + 8,), float("nan"), dtype=TYPES[kind], device="cuda")
+        d.scores = flat[shift:shift + 5 * (classes + 1)].view(5, classes + 1)[:, :classes]
+        d.scores.copy_(values)
+        d()
+        assert torch.equal(d.indexes, expected[0]) and torch.equal(d.weights, expected[1])
+
+
+def test_two_threads_at_once():
+    """Calls from two threads on streams of their own do not disturb each other."""
+    import threading
+
+    rng = np.random.default_rng(6)
+    draws = [Draw(cb.BFLOAT16, scores_of(rng, 20, 30000, 0), rng.random(20)), Draw(cb.FLOAT32, scores_of(rng, 20, 9000, 0), rng.random(20))]
+    expected = [d.indexes.clone() for d in draws]
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(d, e):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(20):
+                d.indexes.fill_(-1)
+                d()
+                s.synchronize()
+                if not torch.equal(d.indexes, e):
+                    failed.append(d.kind)
+
+    threads = [threading.Thread(target=work, args=a) for a in zip(draws, expected)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed

@@ -509,19 +509,19 @@ __device__ __forceinline__ void CopiesAreThere() {
     __syncthreads();
 }
 
-// One operand of a tile of 64 k, as TOperand, but copied straight to LDS: lines without gaps, in which pieces of 16 bytes trade
+// One operand of a tile of K (32 or 64) k, as TOperand, but copied straight to LDS: lines without gaps, in which pieces of 16 bytes trade
 // places, so that the lanes which read at a time meet different banks.
-template <typename T, int SIZE, bool LINE_IS_K, int THREADS>
+template <typename T, int SIZE, int K, bool LINE_IS_K, int THREADS>
 struct TCopied {
-    static constexpr uint32_t kK = 64;
+    static constexpr uint32_t kK = K;
     static constexpr uint32_t kLineChunks = (LINE_IS_K ? kK : SIZE) / 8;
     static constexpr uint32_t kBytes = SIZE * kK * 2;
     static constexpr int kChunks = kBytes / 16 / THREADS;
-    static_assert(kBytes % (16 * THREADS) == 0 && kLineChunks >= 8, "whole waves copy whole lines");
+    static_assert(kBytes % (16 * THREADS) == 0 && (LINE_IS_K || kLineChunks >= 8), "whole waves copy whole lines");
 
     // what a piece's place in its line is crossed with
     __device__ __forceinline__ static uint32_t Cross(uint32_t line) {
-        return LINE_IS_K ? line & 7 : ((line & 3) | (line >> 1 & 4)) << 1 & (kLineChunks - 1);
+        return LINE_IS_K ? (K == 64 ? line & 7 : line >> 1 & 3) : ((line & 3) | (line >> 1 & 4)) << 1 & (kLineChunks - 1);
     }
     // The line, and the piece of it, that goes to this thread's i-th place
     __device__ __forceinline__ static uint32_t Line(uint32_t thread, int i) {
@@ -536,7 +536,7 @@ struct TCopied {
     __device__ __forceinline__ static uint4 Get(const char* lds, uint32_t row, uint32_t part, uint32_t lane) {
         if constexpr (LINE_IS_K) {
             const uint32_t line = row + (lane & 15);
-            return *reinterpret_cast<const uint4*>(lds + line * 128 + ((part * 4 + (lane >> 4)) ^ (lane & 7)) * 16);
+            return *reinterpret_cast<const uint4*>(lds + line * (K * 2) + ((part * 4 + (lane >> 4)) ^ Cross(lane)) * 16);  // (rows begin at multiples of 16)
         } else {
             struct TParts {
                 TShort4 V[2];
@@ -552,13 +552,13 @@ struct TCopied {
 };
 
 // WK: groups of WM * WN waves that share the steps of k in turns, where there are few tiles for many of those
-template <typename T, int TM, int TN, int WM, int WN, int WK, int FORM, int PROJECTIONS>
+template <typename T, int TM, int TN, int WM, int WN, int WK, int K, int FORM, int PROJECTIONS>
 __global__ void __launch_bounds__(WM* WN* WK * 64) LargeProductKernel(const TProduct<T> p) {
     constexpr int kThreads = WM * WN * 64;  // of a group
     constexpr bool kGated = FORM == kRows && PROJECTIONS == 2;
-    using TA = TCopied<T, TM, FORM != kWeights, kThreads>;
-    using TB = TCopied<T, TN, FORM == kRows, kThreads>;
-    constexpr uint32_t kStepK = 64;
+    using TA = TCopied<T, TM, K, FORM != kWeights, kThreads>;
+    using TB = TCopied<T, TN, K, FORM == kRows, kThreads>;
+    constexpr uint32_t kStepK = K;
     constexpr int kColumns = kGated ? TN / 2 : TN;
     constexpr uint32_t kStage = TA::kBytes + TB::kBytes;
     __shared__ __attribute__((aligned(16))) char even[WK * kStage];
@@ -659,7 +659,7 @@ __global__ void __launch_bounds__(WM* WN* WK * 64) LargeProductKernel(const TPro
             return;
         }
 #pragma unroll
-        for (int part = 0; part < 2; ++part) {
+        for (int part = 0; part < K / 32; ++part) {
             uint4 a[kTilesM], b[kTilesN];
 #pragma unroll
             for (int j = 0; j < kTilesN; ++j) {
@@ -677,7 +677,7 @@ __global__ void __launch_bounds__(WM* WN* WK * 64) LargeProductKernel(const TPro
                 }
             }
         }
-        if constexpr (FORM == kRows) {
+        if constexpr (FORM == kRows && kTilesM == 8 && kTilesN == 4) {
             // the first part's twelve fragments, then one of the second part's after every other product (without it the compiler waits for
             // each two fragments: 8192 rows 8192 to 4096 421 us, 405 with it; the other forms' fragments are two reads each, and it costs them)
             __builtin_amdgcn_sched_group_barrier(0x100, 12, 0);
@@ -737,42 +737,48 @@ __global__ void __launch_bounds__(WM* WN* WK * 64) LargeProductKernel(const TPro
 
     // The tile goes to memory by way of LDS, so that lanes in a row store a row's pieces of 16 bytes: from the products' own layout, 32
     // bytes of 16 rows at a time, stores came to 1.3 TB/s
-    constexpr uint32_t kHalf = TM / 2;
-    static_assert(kHalf * kColumns * (kGated ? 4 : 2) <= kStage, "half of the rows fit in each part of LDS");
+    // (all rows at a time, or those of the waves of the same columns one after the other, where LDS does not hold more)
+    constexpr int kRounds = TM / 2 * kColumns * (kGated ? 4 : 2) <= kStage ? 1 : WM;
+    constexpr uint32_t kRoundRows = TM / kRounds, kHalf = kRoundRows / 2;
+    static_assert(kHalf * kColumns * (kGated ? 4 : 2) <= kStage, "half of a round's rows fit in each part of LDS");
     const auto store = [&](auto type, auto&& valueOf, auto* to, uint64_t stride, uint32_t rows, uint32_t columns) {
         using TTo = decltype(type);
         constexpr uint32_t kValues = 16 / sizeof(TTo), kPieces = kColumns / kValues;
         const auto at = [&](uint32_t row, uint32_t piece) {
             return (row < kHalf ? even : odd) + ((row & (kHalf - 1)) * kPieces + (piece ^ (row & 15 & (kPieces - 1)))) * 16;
         };
-        __syncthreads();
 #pragma unroll
-        for (int i = 0; i < kTilesM; ++i) {
-            if (group > 0) {
-                break;
-            }
+        for (int round = 0; round < kRounds; ++round) {
+            __syncthreads();
+            if (group == 0 && (kRounds == 1 || waveM == round * kRoundRows)) {
 #pragma unroll
-            for (int j = 0; j < kTilesN; j += kGated ? 2 : 1) {
-                TValues<TTo, 4> v;
+                for (int i = 0; i < kTilesM; ++i) {
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    v.V[r] = static_cast<TTo>(valueOf(i, j, r));
+                    for (int j = 0; j < kTilesN; j += kGated ? 2 : 1) {
+                        TValues<TTo, 4> v;
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            v.V[r] = static_cast<TTo>(valueOf(i, j, r));
+                        }
+                        const uint32_t n = (kGated ? (waveN + j * 16) / 2 : waveN + j * 16) + 4 * (lane >> 4);
+                        using TWords = std::conditional_t<sizeof(TTo) == 2, uint2, uint4>;
+                        *reinterpret_cast<TWords*>(at(waveM - round * kRoundRows + i * 16 + (lane & 15), n / kValues) + n % kValues * sizeof(TTo)) =
+                            __builtin_bit_cast(TWords, v);
+                    }
                 }
-                const uint32_t n = (kGated ? (waveN + j * 16) / 2 : waveN + j * 16) + 4 * (lane >> 4);
-                using TWords = std::conditional_t<sizeof(TTo) == 2, uint2, uint4>;
-                *reinterpret_cast<TWords*>(at(waveM + i * 16 + (lane & 15), n / kValues) + n % kValues * sizeof(TTo)) = __builtin_bit_cast(TWords, v);
             }
-        }
-        __syncthreads();
+            __syncthreads();
 #pragma unroll
-        for (uint32_t i = 0; i < (TM * kPieces + WK * kThreads - 1) / (WK * kThreads); ++i) {
-            const uint32_t row = (threadIdx.x + i * WK * kThreads) / kPieces, piece = (threadIdx.x + i * WK * kThreads) % kPieces;
-            if (row >= TM) {
-                break;
-            }
-            const auto v = __builtin_bit_cast(TValues<TTo, kValues>, *reinterpret_cast<const uint4*>(at(row, piece)));
-            if (row < rows && piece * kValues < columns) {
-                StoreUpTo(v, to + row * stride + piece * kValues, columns - piece * kValues);
+            for (uint32_t i = 0; i < (kRoundRows * kPieces + WK * kThreads - 1) / (WK * kThreads); ++i) {
+                const uint32_t row = (threadIdx.x + i * WK * kThreads) / kPieces, piece = (threadIdx.x + i * WK * kThreads) % kPieces;
+                if (row >= kRoundRows) {
+                    break;
+                }
+                const auto v = __builtin_bit_cast(TValues<TTo, kValues>, *reinterpret_cast<const uint4*>(at(row, piece)));
+                const uint32_t m = round * kRoundRows + row;
+                if (m < rows && piece * kValues < columns) {
+                    StoreUpTo(v, to + m * stride + piece * kValues, columns - piece * kValues);
+                }
             }
         }
     };
@@ -952,11 +958,11 @@ void LaunchProduct(const TCallDevice& call, TProduct<T> p) {
     }
 }
 
-template <int FORM, int PROJECTIONS, typename T, int TM, int TN, int WM, int WN, int WK>
+template <int FORM, int PROJECTIONS, typename T, int TM, int TN, int WM, int WN, int WK, int K = 64>
 void LaunchLarge(const TCallDevice& call, TProduct<T> p) {
     SetTiles<FORM, PROJECTIONS, T, TM, TN>(p);
     for (p.First = 0; p.First < p.Tiles; p.First += kMostGroups) {
-        call.Launch(LargeProductKernel<T, TM, TN, WM, WN, WK, FORM, PROJECTIONS>, std::min(kMostGroups, p.Tiles - p.First), WM * WN * WK * 64, 0, p);
+        call.Launch(LargeProductKernel<T, TM, TN, WM, WN, WK, K, FORM, PROJECTIONS>, std::min(kMostGroups, p.Tiles - p.First), WM * WN * WK * 64, 0, p);
     }
 }
 
@@ -999,9 +1005,10 @@ void MultiplyBy(const TCallDevice& call, const TProduct<T>& p) {
     if constexpr (sizeof(T) == 2) {
         if (TakesCopies<FORM, PROJECTIONS>(p)) {
             if constexpr (FORM == kWeights) {
-                // (2048 x 4096 weights of one expert's 1024 rows, 256 tiles, 46 and 50; 2048 x 2048 of 2048 rows, 64 tiles, 68 and 39)
+                // (1024 x 4096 weights of 64 experts with 1000 rows each 759, 859 by the tiles below; of 64 rows each 224 and 233; 2048 x 2048 of 2048
+                // rows, 64 tiles of 256, 69 and 39)
                 if (tiles(256) >= 256) {
-                    return LaunchLarge<FORM, PROJECTIONS, T, 256, 256, 2, 4, 1>(call, p);
+                    return LaunchLarge<FORM, PROJECTIONS, T, 128, 256, 2, 4, 1, 32>(call, p);
                 }
                 // few tiles with many rows to add over (512 x 512 of 65536 rows 347, 964 without sharing; 1024 x 1024 of 4096 rows 26 and 66; 256 tiles of
                 // 2048 rows 56 and 39)
@@ -1023,10 +1030,16 @@ void MultiplyBy(const TCallDevice& call, const TProduct<T>& p) {
                         return LaunchLarge<FORM, PROJECTIONS, T, 64, 128, 1, 4, 1>(call, p);
                     }
                 }
-                // (65536 x 4096 to 1024 of 64 experts 609 and 1338, 661 and 1458 by the tiles below; 16384 rows of 64 experts 264, 243; 65536 x 1024 to
-                // 1024 of one expert gated 392 and 344)
-                if (each >= 512 && tiles(256) >= 1024 && (FORM != kRows || PROJECTIONS == 1 || p.K >= 2048)) {
-                    return LaunchLarge<FORM, PROJECTIONS, T, 256, 256, 2, 4, 1>(call, p);
+                if constexpr (FORM == kRows) {
+                    // (64000 x 4096 to 1024 of 64 experts 601 and 1285, 661 and 1420 by the tiles below; 16384 rows of 64 experts 236, 229; 65536 x 1024 to
+                    // 1024 of one expert gated 371 and 329)
+                    if (each >= 512 && tiles(256) >= 1024 && (PROJECTIONS == 1 || p.K >= 2048)) {
+                        return LaunchLarge<FORM, PROJECTIONS, T, 256, 256, 2, 4, 1>(call, p);
+                    }
+                } else if (tiles(128) >= 512) {
+                    // (inputs' gradients of 64000 x 4096 by 1024 of 64 experts 773, 912 by the tiles below, 879 by tiles of 256; of 30000 x 1024 by 256 of 128
+                    // experts 52, 56 and 61)
+                    return LaunchLarge<FORM, PROJECTIONS, T, 128, 256, 2, 4, 1, 32>(call, p);
                 }
             }
             // two workgroups of a compute unit, one of which loads or stores while the other one multiplies

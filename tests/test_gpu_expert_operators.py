@@ -404,7 +404,8 @@ def test_experts_far_apart(kind):
 
 
 # rows, width, outputs, experts: each of the kernels for many rows or few tiles
-LARGER = [(3000, 136, 512, 2), (4200, 256, 2048, 4), (600, 520, 264, 3), (40, 2080, 512, 4), (14, 1000, 2056, 6), (33, 300, 5000, 2), (2500, 64, 16, 3), (9000, 72, 72, 1)]
+LARGER = [(3000, 136, 512, 2), (4200, 256, 2048, 4), (600, 520, 264, 3), (40, 2080, 512, 4), (14, 1000, 2056, 6), (33, 300, 5000, 2), (2500, 64, 16, 3), (9000, 72, 72, 1),
+          (9000, 1032, 64, 2), (300, 1032, 1096, 16)]
 
 
 @pytest.mark.parametrize("kind", [cb.FLOAT32, cb.FLOAT16, cb.BFLOAT16], ids=NAMES.get)

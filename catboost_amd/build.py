@@ -16,7 +16,8 @@ LIB_PATH = os.path.join(LIB_DIR, "libcatboostmodel.so")
 
 HOST_SOURCES = ["model.cpp", "cbm_format.cpp", "json_model.cpp", "model_builder.cpp", "exchange_plan.cpp", "cat_hash.cpp", "fast_exp.cpp", "routed_evaluation.cpp", "c_api.cpp"]
 HIP_SOURCES = ["hip_evaluator.hip", "score_operators.hip", "sample_operators.hip", "row_operators.hip", "expert_operators.hip",
-               "expert_products_f64.hip", "expert_products_f32.hip", "expert_products_f16.hip", "expert_products_bf16.hip"]
+               "expert_products_f64.hip", "expert_products_f32.hip", "expert_products_f16.hip", "expert_products_bf16.hip",
+               "expert_gradients_f16.hip", "expert_gradients_bf16.hip"]
 
 COMMON = ["-O3", "-std=c++17", "-fPIC", "-Wall", "-Wextra", "-Wno-unused-parameter", "-ffp-contract=off"]
 # packed fp32 VALU forms are kept off for every device function of this library

@@ -38,7 +38,7 @@ __global__ void __launch_bounds__(256) GateGradientsKernel(TSegments segments, u
     StoreUpTo(du, preGradients + gate + hidden, left);
 }
 
-// (compiled by expert_products_*.hip)
+// (compiled by expert_products_*.hip and expert_gradients_*.hip)
 #define PRODUCTS_OF(T)                                                                        \
     extern template void MultiplyBy<kRows, 1, T>(const TCallDevice&, const TProduct<T>&);    \
     extern template void MultiplyBy<kRows, 2, T>(const TCallDevice&, const TProduct<T>&);    \

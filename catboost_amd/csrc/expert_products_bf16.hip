@@ -6,10 +6,6 @@ namespace op {
 
 template void MultiplyBy<kRows, 1, __bf16>(const TCallDevice&, const TProduct<__bf16>&);
 template void MultiplyBy<kRows, 2, __bf16>(const TCallDevice&, const TProduct<__bf16>&);
-template void MultiplyBy<kInputs, 1, __bf16>(const TCallDevice&, const TProduct<__bf16>&);
-template void MultiplyBy<kInputs, 2, __bf16>(const TCallDevice&, const TProduct<__bf16>&);
-template void MultiplyBy<kWeights, 1, __bf16>(const TCallDevice&, const TProduct<__bf16>&);
-template void MultiplyBy<kWeights, 2, __bf16>(const TCallDevice&, const TProduct<__bf16>&);
 
 }  // namespace op
 }  // namespace cbamd

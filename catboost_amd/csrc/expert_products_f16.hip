@@ -6,10 +6,6 @@ namespace op {
 
 template void MultiplyBy<kRows, 1, _Float16>(const TCallDevice&, const TProduct<_Float16>&);
 template void MultiplyBy<kRows, 2, _Float16>(const TCallDevice&, const TProduct<_Float16>&);
-template void MultiplyBy<kInputs, 1, _Float16>(const TCallDevice&, const TProduct<_Float16>&);
-template void MultiplyBy<kInputs, 2, _Float16>(const TCallDevice&, const TProduct<_Float16>&);
-template void MultiplyBy<kWeights, 1, _Float16>(const TCallDevice&, const TProduct<_Float16>&);
-template void MultiplyBy<kWeights, 2, _Float16>(const TCallDevice&, const TProduct<_Float16>&);
 
 }  // namespace op
 }  // namespace cbamd

@@ -1362,7 +1362,10 @@ void SampleClasses(int valueType, size_t rows, size_t classes, const void* score
         if constexpr (sizeof(T) == 2) {
             launch(SampleCountedKernel<T>, from, 1024, 1);
         } else {
-            launch(SampleRowKernel<T, 1024, 11, sizeof(T) == 8 ? 2048 : 3072>, from, 1024, 1);
+            // two workgroups for a compute unit where rows are more than those (384 x 100003 f32 161 us, 174 with 1024 threads each; 2000 x 10000 95, 162;
+            // 32 x 100003 80 and 64)
+            constexpr int kList = sizeof(T) == 8 ? 2048 : 3072;
+            rows > 256 ? launch(SampleRowKernel<T, 512, 11, kList>, from, 512, 1) : launch(SampleRowKernel<T, 1024, 11, kList>, from, 1024, 1);
         }
     });
 }

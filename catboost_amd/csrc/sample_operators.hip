@@ -258,6 +258,70 @@ __global__ void __launch_bounds__(256) SampleOfFewKernel(const T* scores, TSampl
 
 // ---------------------------------------------------------------- lanes for a row ----
 
+// The sum over the lanes up to this one. Steps are moves within the vector unit (rows of 16 lanes, then from the last lane of a row to the
+// next rows), a tenth of the time of trips through LDS.
+template <int CONTROL, int ROWS, typename V>
+__device__ __forceinline__ V MovedOver(V v) {
+    if constexpr (sizeof(V) == 8) {
+        const uint32_t low = __builtin_amdgcn_update_dpp(0u, static_cast<uint32_t>(v), CONTROL, ROWS, 0xf, false);
+        const uint32_t high = __builtin_amdgcn_update_dpp(0u, static_cast<uint32_t>(v >> 32), CONTROL, ROWS, 0xf, false);
+        return static_cast<V>(high) << 32 | low;
+    } else {
+        return __builtin_amdgcn_update_dpp(0u, v, CONTROL, ROWS, 0xf, false);
+    }
+}
+template <typename V>
+__device__ __forceinline__ V SumUpTo(V v) {
+    v += MovedOver<0x111, 0xf>(v);  // 1, 2, 4, 8 lanes on in a row
+    v += MovedOver<0x112, 0xf>(v);
+    v += MovedOver<0x114, 0xf>(v);
+    v += MovedOver<0x118, 0xf>(v);
+    v += MovedOver<0x142, 0xa>(v);  // lane 15 of rows 0 and 2 to rows 1 and 3
+    v += MovedOver<0x143, 0xc>(v);  // lane 31 to rows 2 and 3
+    return v;
+}
+template <typename V>
+__device__ __forceinline__ V OfLane(V v, int lane) {
+    if constexpr (sizeof(V) == 8) {
+        const uint32_t low = __builtin_amdgcn_readlane(static_cast<uint32_t>(v), lane), high = __builtin_amdgcn_readlane(static_cast<uint32_t>(v >> 32), lane);
+        return static_cast<V>(high) << 32 | low;
+    } else {
+        return __builtin_amdgcn_readlane(v, lane);
+    }
+}
+// The largest of the wave's
+template <typename V>
+__device__ __forceinline__ V MostOfWave(V v) {
+    const auto larger = [&](V other) { v = other > v ? other : v; };
+    larger(MovedOver<0x111, 0xf>(v));
+    larger(MovedOver<0x112, 0xf>(v));
+    larger(MovedOver<0x114, 0xf>(v));
+    larger(MovedOver<0x118, 0xf>(v));
+    larger(MovedOver<0x142, 0xa>(v));
+    larger(MovedOver<0x143, 0xc>(v));
+    return OfLane(v, 63);
+}
+
+// The value of the lane that differs in this bit: moves within the vector unit where rows of 16 lanes have both (trips through LDS take
+// half as long again for a whole sort: 250000 x 64 f64 310 us, 202)
+template <int LANES, typename V>
+__device__ __forceinline__ V AcrossLanes(V v) {
+    if constexpr (sizeof(V) == 8) {
+        return static_cast<V>(AcrossLanes<LANES>(static_cast<uint32_t>(v >> 32))) << 32 | AcrossLanes<LANES>(static_cast<uint32_t>(v));
+    } else if constexpr (LANES == 1) {
+        return __builtin_amdgcn_update_dpp(0u, v, 0xb1, 0xf, 0xf, true);
+    } else if constexpr (LANES == 2) {
+        return __builtin_amdgcn_update_dpp(0u, v, 0x4e, 0xf, 0xf, true);
+    } else if constexpr (LANES == 4) {
+        // (eight lanes the other way round, then each four of them)
+        return __builtin_amdgcn_update_dpp(0u, __builtin_amdgcn_update_dpp(0u, v, 0x141, 0xf, 0xf, true), 0x1b, 0xf, 0xf, true);
+    } else if constexpr (LANES == 8) {
+        return __builtin_amdgcn_update_dpp(0u, v, 0x128, 0xf, 0xf, true);
+    } else {
+        return __shfl_xor(v, LANES);
+    }
+}
+
 // A key and its class as one value that orders them, the lowest class first: 32 bits for 16-bit scores, 64 for 32-bit ones
 template <typename T>
 struct TOrdered {
@@ -281,8 +345,9 @@ struct TOrdered {
     __device__ __forceinline__ static TOrdered Choose(bool first, const TOrdered& a, const TOrdered& b) {
         return {first ? a.Word : b.Word};
     }
-    __device__ __forceinline__ TOrdered Across(int lanes) const {
-        return {static_cast<TWord>(__shfl_xor(Word, lanes))};
+    template <int LANES>
+    __device__ __forceinline__ TOrdered Across() const {
+        return {AcrossLanes<LANES>(Word)};
     }
 };
 template <>
@@ -306,17 +371,47 @@ struct TOrdered<double> {
     __device__ __forceinline__ static TOrdered Choose(bool first, const TOrdered& a, const TOrdered& b) {
         return {first ? a.Word : b.Word, first ? a.Class : b.Class};
     }
-    __device__ __forceinline__ TOrdered Across(int lanes) const {
-        return {static_cast<uint64_t>(__shfl_xor(Word, lanes)), static_cast<uint32_t>(__shfl_xor(Class, lanes))};
+    template <int LANES>
+    __device__ __forceinline__ TOrdered Across() const {
+        return {AcrossLanes<LANES>(Word), AcrossLanes<LANES>(Class)};
     }
 };
+
+// Places lane * P + i in order: runs of SIZE places, each the other way round than the next, are merged to ones of twice that, by
+// trades between places STEP apart
+template <int LANES, int P, int SIZE, int STEP, typename TItem>
+__device__ __forceinline__ void Merge(TItem (&item)[P], uint32_t lane) {
+    if constexpr (STEP >= P) {
+        const bool low = (lane & (STEP / P)) == 0, down = (lane * P & SIZE) == 0;
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            const TItem other = item[i].template Across<STEP / P>();
+            item[i] = TItem::Choose(item[i].Before(other) == (low == down), item[i], other);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            if ((i & STEP) == 0) {
+                const bool down = ((lane * P + i) & SIZE) == 0;
+                const TItem a = item[i], b = item[i + STEP];
+                const bool trade = a.Before(b) != down;
+                item[i] = TItem::Choose(trade, b, a);
+                item[i + STEP] = TItem::Choose(trade, a, b);
+            }
+        }
+    }
+    if constexpr (STEP > 1) {
+        Merge<LANES, P, SIZE, STEP / 2>(item, lane);
+    } else if constexpr (SIZE < LANES * P) {
+        Merge<LANES, P, SIZE * 2, SIZE>(item, lane);
+    }
+}
 
 // Rows of at most LANES * P classes: place i of the order ends up as value i % P of lane i / P
 template <typename T, int LANES, int P>
 __global__ void __launch_bounds__(256) SampleByLanesKernel(const T* scores, TSampleArguments p) {
     using TK = TKeys<T>;
     using TItem = TOrdered<T>;
-    constexpr int kPlaces = LANES * P;
     const uint32_t lane = threadIdx.x % LANES;
     const size_t n = static_cast<size_t>(blockIdx.x) * (256 / LANES) + threadIdx.x / LANES;
     // (rows behind the last one do as it does, so that every lane is there to be read, and store nothing)
@@ -329,32 +424,7 @@ __global__ void __launch_bounds__(256) SampleByLanesKernel(const T* scores, TSam
         const uint32_t c = lane + i * LANES;
         item[i] = TItem::Of(c < p.Classes ? TK::Of(row[c]) : 0, c);
     }
-    // runs of `size` places, each the other way round than the next, are merged to ones of twice that
-#pragma unroll
-    for (int size = 2; size <= kPlaces; size *= 2) {
-#pragma unroll
-        for (int step = size / 2; step > 0; step /= 2) {
-            if (step >= P) {
-                const bool low = (lane & (step / P)) == 0, down = (lane * P & size) == 0;
-#pragma unroll
-                for (int i = 0; i < P; ++i) {
-                    const TItem other = item[i].Across(step / P);
-                    item[i] = TItem::Choose(item[i].Before(other) == (low == down), item[i], other);
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < P; ++i) {
-                    if ((i & step) == 0) {
-                        const bool down = ((lane * P + i) & size) == 0;
-                        const TItem a = item[i], b = item[i + step];
-                        const bool trade = a.Before(b) != down;
-                        item[i] = TItem::Choose(trade, b, a);
-                        item[i + step] = TItem::Choose(trade, a, b);
-                    }
-                }
-            }
-        }
-    }
+    Merge<LANES, P, 2, 1>(item, lane);
     const bool mine = n < p.Rows && lane == 0;
     const uint32_t base = threadIdx.x & 63 & ~(LANES - 1);  // the row's first lane in its wave
     const TItem best{item[0]};
@@ -382,12 +452,19 @@ __global__ void __launch_bounds__(256) SampleByLanesKernel(const T* scores, TSam
         sum[i] = total;
     }
     uint64_t before = total;
+    if constexpr (LANES == 64) {
+        before = SumUpTo(total);
+        all = limits.TopK > 0 ? OfLane(SumUpTo(all), 63) : OfLane(before, 63);
+        likely = OfLane(SumUpTo(likely), 63);
+    } else {
 #pragma unroll
-    for (int d = 1; d < LANES; d *= 2) {
-        const uint64_t other = __shfl_up(before, d, LANES), otherAll = __shfl_xor(all, d), otherLikely = __shfl_xor(likely, d);
-        before += lane >= static_cast<uint32_t>(d) ? other : 0;
-        all += otherAll;
-        likely += otherLikely;
+        for (int d = 1; d < LANES; d *= 2) {
+            const uint64_t other = __shfl_up(before, d, LANES);
+            const uint64_t otherAll = __shfl_xor(all, d), otherLikely = __shfl_xor(likely, d);
+            before += lane >= static_cast<uint32_t>(d) ? other : 0;
+            all += otherAll;
+            likely += otherLikely;
+        }
     }
     before -= total;
 #pragma unroll
@@ -448,50 +525,6 @@ struct TShared {
     uint32_t Listed;
     double Powers[kPowers];
 };
-
-// The sum over the lanes up to this one. Steps are moves within the vector unit (rows of 16 lanes, then from the last lane of a row to the
-// next rows), a tenth of the time of trips through LDS.
-template <int CONTROL, int ROWS, typename V>
-__device__ __forceinline__ V MovedOver(V v) {
-    if constexpr (sizeof(V) == 8) {
-        const uint32_t low = __builtin_amdgcn_update_dpp(0u, static_cast<uint32_t>(v), CONTROL, ROWS, 0xf, false);
-        const uint32_t high = __builtin_amdgcn_update_dpp(0u, static_cast<uint32_t>(v >> 32), CONTROL, ROWS, 0xf, false);
-        return static_cast<V>(high) << 32 | low;
-    } else {
-        return __builtin_amdgcn_update_dpp(0u, v, CONTROL, ROWS, 0xf, false);
-    }
-}
-template <typename V>
-__device__ __forceinline__ V SumUpTo(V v) {
-    v += MovedOver<0x111, 0xf>(v);  // 1, 2, 4, 8 lanes on in a row
-    v += MovedOver<0x112, 0xf>(v);
-    v += MovedOver<0x114, 0xf>(v);
-    v += MovedOver<0x118, 0xf>(v);
-    v += MovedOver<0x142, 0xa>(v);  // lane 15 of rows 0 and 2 to rows 1 and 3
-    v += MovedOver<0x143, 0xc>(v);  // lane 31 to rows 2 and 3
-    return v;
-}
-template <typename V>
-__device__ __forceinline__ V OfLane(V v, int lane) {
-    if constexpr (sizeof(V) == 8) {
-        const uint32_t low = __builtin_amdgcn_readlane(static_cast<uint32_t>(v), lane), high = __builtin_amdgcn_readlane(static_cast<uint32_t>(v >> 32), lane);
-        return static_cast<V>(high) << 32 | low;
-    } else {
-        return __builtin_amdgcn_readlane(v, lane);
-    }
-}
-// The largest of the wave's
-template <typename V>
-__device__ __forceinline__ V MostOfWave(V v) {
-    const auto larger = [&](V other) { v = other > v ? other : v; };
-    larger(MovedOver<0x111, 0xf>(v));
-    larger(MovedOver<0x112, 0xf>(v));
-    larger(MovedOver<0x114, 0xf>(v));
-    larger(MovedOver<0x118, 0xf>(v));
-    larger(MovedOver<0x142, 0xa>(v));
-    larger(MovedOver<0x143, 0xc>(v));
-    return OfLane(v, 63);
-}
 
 // Sums and maxima over a workgroup; every lane gets them
 template <int WAVES>
@@ -1364,7 +1397,7 @@ void SampleClasses(int valueType, size_t rows, size_t classes, const void* score
         } else {
             // two workgroups for a compute unit where rows are more than those (384 x 100003 f32 161 us, 174 with 1024 threads each; 2000 x 10000 95, 162;
             // 32 x 100003 80 and 64)
-            constexpr int kList = sizeof(T) == 8 ? 2048 : 3072;
+            constexpr int kList = 2048;
             rows > 256 ? launch(SampleRowKernel<T, 512, 11, kList>, from, 512, 1) : launch(SampleRowKernel<T, 1024, 11, kList>, from, 1024, 1);
         }
     });

@@ -215,14 +215,14 @@ struct TOperand {
         }
         return line;
     }
-    __device__ __forceinline__ static bool Mine(int i) {
-        return kWhole || threadIdx.x + i * THREADS < kLines * kLineChunks;
+    __device__ __forceinline__ static bool Mine(uint32_t thread, int i) {
+        return kWhole || thread + i * THREADS < kLines * kLineChunks;
     }
-    __device__ __forceinline__ static void Put(char* lds, const TChunk* held) {
+    __device__ __forceinline__ static void Put(char* lds, uint32_t thread, const TChunk* held) {
 #pragma unroll
         for (int i = 0; i < kChunks; ++i) {
-            const uint32_t c = threadIdx.x + i * THREADS;
-            if (Mine(i)) {
+            const uint32_t c = thread + i * THREADS;
+            if (Mine(thread, i)) {
                 *reinterpret_cast<uint4*>(lds + Place(c / kLineChunks) * kLineBytes + c % kLineChunks * 16) = __builtin_bit_cast(uint4, held[i]);
             }
         }
@@ -372,9 +372,10 @@ __device__ __forceinline__ void StoreProduct(const TProduct<T>& p, const TTileOf
     }
 }
 
-template <typename T, int TM, int TN, int WM, int WN, int KBYTES, int FORM, int PROJECTIONS>
-__global__ void __launch_bounds__(WM* WN * 64) ProductKernel(const TProduct<T> p) {
-    constexpr int kThreads = WM * WN * 64;
+// WK: groups of WM * WN waves that share the steps of k in turns, where there are few tiles for many of those
+template <typename T, int TM, int TN, int WM, int WN, int WK, int KBYTES, int FORM, int PROJECTIONS>
+__global__ void __launch_bounds__(WM* WN* WK * 64) ProductKernel(const TProduct<T> p) {
+    constexpr int kThreads = WM * WN * 64;  // of a group
     constexpr bool kGated = FORM == kRows && PROJECTIONS == 2;
     using TA = TOperand<T, TM, KBYTES, FORM != kWeights, kThreads>;
     using TB = TOperand<T, TN, KBYTES, FORM == kRows, kThreads>;
@@ -383,7 +384,9 @@ __global__ void __launch_bounds__(WM* WN * 64) ProductKernel(const TProduct<T> p
     constexpr int kColumns = kGated ? TN / 2 : TN;  // outputs of a tile
     extern __shared__ __attribute__((aligned(16))) char lds[];
 
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t group = WK == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / kThreads);
+    const uint32_t thread = WK == 1 ? threadIdx.x : threadIdx.x % kThreads;
+    const uint32_t lane = threadIdx.x & 63, wave = thread >> 6;
     const TTileOfProduct t(p, TM, kColumns, FORM, PROJECTIONS);
     if (!t.There) {
         return;
@@ -407,8 +410,8 @@ __global__ void __launch_bounds__(WM* WN * 64) ProductKernel(const TProduct<T> p
         constexpr bool kFitsA = FORM != kWeights;  // rows behind the last are read as the last one, and not stored
 #pragma unroll
         for (int i = 0; i < TA::kChunks; ++i) {
-            const uint32_t c = threadIdx.x + i * kThreads;
-            if (!TA::Mine(i)) {
+            const uint32_t c = thread + i * kThreads;
+            if (!TA::Mine(thread, i)) {
                 continue;
             }
             const uint32_t line = c / TA::kLineChunks, at = c % TA::kLineChunks * kValues;
@@ -425,8 +428,8 @@ __global__ void __launch_bounds__(WM* WN * 64) ProductKernel(const TProduct<T> p
         }
 #pragma unroll
         for (int i = 0; i < TB::kChunks; ++i) {
-            const uint32_t c = threadIdx.x + i * kThreads;
-            if (!TB::Mine(i)) {
+            const uint32_t c = thread + i * kThreads;
+            if (!TB::Mine(thread, i)) {
                 continue;
             }
             const uint32_t line = c / TB::kLineChunks, at = c % TB::kLineChunks * kValues;
@@ -450,16 +453,21 @@ __global__ void __launch_bounds__(WM* WN * 64) ProductKernel(const TProduct<T> p
     const uint32_t waveM = wave % WM * (TM / WM), waveN = wave / WM * (TN / WN);
     TOut out[kTilesM][kTilesN] = {};
     constexpr int kStage = TA::kBytes + TB::kBytes;
-    if (allSteps > 0) {
-        load(0);
-        TA::Put(lds, heldA);
-        TB::Put(lds + TA::kBytes, heldB);
+    char* const mine = lds + group * 2 * kStage;
+    if (group < allSteps) {
+        load(group);
+        TA::Put(mine, thread, heldA);
+        TB::Put(mine + TA::kBytes, thread, heldB);
     }
-    for (uint32_t step = 0; step < allSteps; ++step) {
+    for (uint32_t turn = 0; turn * WK < allSteps; ++turn) {
         __syncthreads();
-        const char* now = lds + (step & 1) * kStage;
-        if (step + 1 < allSteps) {
-            load(step + 1);
+        const uint32_t step = turn * WK + group;
+        const char* now = mine + (turn & 1) * kStage;
+        if (step + WK < allSteps) {
+            load(step + WK);
+        }
+        if (WK > 1 && step >= allSteps) {
+            continue;
         }
 #pragma unroll
         for (int part = 0; part < KBYTES / 64; ++part) {
@@ -480,10 +488,33 @@ __global__ void __launch_bounds__(WM* WN * 64) ProductKernel(const TProduct<T> p
                 }
             }
         }
-        if (step + 1 < allSteps) {
-            char* next = lds + ((step + 1) & 1) * kStage;
-            TA::Put(next, heldA);
-            TB::Put(next + TA::kBytes, heldB);
+        if (step + WK < allSteps) {
+            char* next = mine + ((turn + 1) & 1) * kStage;
+            TA::Put(next, thread, heldA);
+            TB::Put(next + TA::kBytes, thread, heldB);
+        }
+    }
+    if constexpr (WK > 1) {
+        // the groups' sums, added in their order, by way of the same memory
+        constexpr uint32_t kSums = kTilesM * kTilesN * kThreads * sizeof(TOut);
+        static_assert((WK - 1) * kSums <= WK * 2 * kStage, "what the other groups hand over fits");
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kTilesM * kTilesN; ++i) {
+            if (group > 0) {
+                *reinterpret_cast<TOut*>(lds + (group - 1) * kSums + (i * kThreads + thread) * sizeof(TOut)) = out[i / kTilesN][i % kTilesN];
+            }
+        }
+        __syncthreads();
+        if (group > 0) {
+            return;
+        }
+#pragma unroll
+        for (int g = 0; g < WK - 1; ++g) {
+#pragma unroll
+            for (int i = 0; i < kTilesM * kTilesN; ++i) {
+                out[i / kTilesN][i % kTilesN] += *reinterpret_cast<const TOut*>(lds + g * kSums + (i * kThreads + thread) * sizeof(TOut));
+            }
         }
     }
 
@@ -946,15 +977,16 @@ void SetTiles(TProduct<T>& p) {
     }
 }
 
-template <int FORM, int PROJECTIONS, typename T, int TM, int TN, int WM, int WN, int KBYTES>
+template <int FORM, int PROJECTIONS, typename T, int TM, int TN, int WM, int WN, int WK>
 void LaunchProduct(const TCallDevice& call, TProduct<T> p) {
     constexpr int kThreads = WM * WN * 64;
-    constexpr size_t lds = 2 * (TOperand<T, TM, KBYTES, FORM != kWeights, kThreads>::kBytes + TOperand<T, TN, KBYTES, FORM == kRows, kThreads>::kBytes);
+    constexpr int KBYTES = WK > 1 && sizeof(T) > 2 ? 128 : 64;  // (as many as LDS holds, where a step is a wait for memory)
+    constexpr size_t lds = WK * 2 * (TOperand<T, TM, KBYTES, FORM != kWeights, kThreads>::kBytes + TOperand<T, TN, KBYTES, FORM == kRows, kThreads>::kBytes);
     SetTiles<FORM, PROJECTIONS, T, TM, TN>(p);
-    const auto kernel = ProductKernel<T, TM, TN, WM, WN, KBYTES, FORM, PROJECTIONS>;
+    const auto kernel = ProductKernel<T, TM, TN, WM, WN, WK, KBYTES, FORM, PROJECTIONS>;
     call.AllowLds(reinterpret_cast<const void*>(kernel), lds);
     for (p.First = 0; p.First < p.Tiles; p.First += kMostGroups) {
-        call.Launch(kernel, std::min(kMostGroups, p.Tiles - p.First), kThreads, lds, p);
+        call.Launch(kernel, std::min(kMostGroups, p.Tiles - p.First), WK * kThreads, lds, p);
     }
 }
 
@@ -1058,11 +1090,18 @@ void MultiplyBy(const TCallDevice& call, const TProduct<T>& p) {
         }
     }
     // (32 bits, 5003 x 1001 to 699 of 5 experts, 240 tiles: 100 and 152; 4096 x 4096 to 4096, 1024 tiles: 1315 and 1177)
+    if constexpr (FORM == kWeights) {
+        // few tiles with many rows to add over (32 bits, 1024 x 1024 of 60000 rows 2591 without sharing; 1024 x 1024 of 4096 rows 146; 512 x 512 of 2000
+        // rows 73; with it 1313, 105, 49 and less)
+        if (tiles(64) <= 512) {
+            return LaunchProduct<FORM, PROJECTIONS, T, 64, 64, 2, 2, 4>(call, p);
+        }
+    }
     if (sizeof(T) == 8 || tiles(128) <= 384) {
-        return LaunchProduct<FORM, PROJECTIONS, T, 64, 64, 2, 2, 64>(call, p);
+        return LaunchProduct<FORM, PROJECTIONS, T, 64, 64, 2, 2, 1>(call, p);
     }
     if constexpr (sizeof(T) < 8) {
-        LaunchProduct<FORM, PROJECTIONS, T, 128, 128, 2, 2, 64>(call, p);
+        LaunchProduct<FORM, PROJECTIONS, T, 128, 128, 2, 2, 1>(call, p);
     }
 }
 

@@ -1366,6 +1366,7 @@ void SampleClasses(int valueType, size_t rows, size_t classes, const void* score
     WithType(valueType, [&](auto value) {
         using T = decltype(value);
         const T* from = static_cast<const T*>(scores);
+        // (2M x 10 f64 58 us, 1M x 16 f32 58; 250000 x 64 f64 206; 16000 x 1000 f64 238, 258 with a workgroup each, 100 rows of it 30 and 26)
         if (classes <= 16) {
             return WithNumber<16>(classes, [&](auto n) { launch(SampleOfFewKernel<T, decltype(n)::value>, from, 256, 256); });
         }
@@ -1384,15 +1385,14 @@ void SampleClasses(int valueType, size_t rows, size_t classes, const void* score
         if (classes <= 512) {
             return launch(SampleByLanesKernel<T, 64, 8>, from, 256, 4);
         }
-        if constexpr (sizeof(T) < 8) {
-            if (classes <= 1024) {
-                return launch(SampleByLanesKernel<T, 64, 16>, from, 256, 4);
-            }
+        if (classes <= 1024) {
+            return launch(SampleByLanesKernel<T, 64, 16>, from, 256, 4);
         }
         if (classes <= 4096) {
             return launch(SampleRowKernel<T, 256, 9, 1024>, from, 256, 1);
         }
         if constexpr (sizeof(T) == 2) {
+            // (64 x 131000 bf16 46 us, 359 with weights of each class)
             launch(SampleCountedKernel<T>, from, 1024, 1);
         } else {
             // two workgroups for a compute unit where rows are more than those (384 x 100003 f32 161 us, 174 with 1024 threads each; 2000 x 10000 95, 162;

@@ -1092,7 +1092,7 @@ void MultiplyBy(const TCallDevice& call, const TProduct<T>& p) {
     // (32 bits, 5003 x 1001 to 699 of 5 experts, 240 tiles: 100 and 152; 4096 x 4096 to 4096, 1024 tiles: 1315 and 1177)
     if constexpr (FORM == kWeights) {
         // few tiles with many rows to add over (32 bits, 1024 x 1024 of 60000 rows 2591 without sharing; 1024 x 1024 of 4096 rows 146; 512 x 512 of 2000
-        // rows 73; with it 1313, 105, 49 and less)
+        // rows 73; with it 1288, 101 and 47)
         if (tiles(64) <= 512) {
             return LaunchProduct<FORM, PROJECTIONS, T, 64, 64, 2, 2, 4>(call, p);
         }

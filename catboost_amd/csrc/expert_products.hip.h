@@ -396,7 +396,7 @@ __global__ void __launch_bounds__(WM* WN* WK * 64) ProductKernel(const TProduct<
     const uint32_t steps = (partK + kStepK - 1) / kStepK;
     const uint32_t allSteps = FORM == kInputs ? steps * PROJECTIONS : steps;
 
-    // f(i, line, chunk of the line) for the chunks of 16 bytes that this thread loads
+    // the chunks of 16 bytes that this thread loads for a step
     typename TA::TChunk heldA[TA::kChunks];
     typename TB::TChunk heldB[TB::kChunks];
     const auto load = [&](uint32_t step) {
@@ -526,8 +526,6 @@ __global__ void __launch_bounds__(WM* WN* WK * 64) ProductKernel(const TProduct<
 // Bytes that stand for what lies behind the last k of a product
 __device__ __attribute__((aligned(16))) const uint32_t gZeros[4] = {};
 
-using TLdsBytes = __attribute__((address_space(3))) char;
-using TGlobalBytes = const __attribute__((address_space(1))) char;
 
 // 16 bytes of each lane from its address to LDS, 1 KB in a row for the wave, without a trip through registers
 __device__ __forceinline__ void CopyToLds(const void* from, char* to) {

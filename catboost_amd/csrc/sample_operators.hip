@@ -57,7 +57,7 @@ template <bool TABLE>
 struct TWeigh {
     double Best;           // the best score
     double Rate;           // log2(e) / temperature
-    double Unit;           // 2^shift: how many whole numbers a weight of 1 is, at most 2^51
+    double Unit;           // 2^shift: how many whole numbers a weight of 1 is, at most 2^51 (what Whole takes)
     const double* Powers;  // in LDS, of TABLE
 
     // How far under the best one, in powers of two; never less for a smaller score. All of plus infinity are alike, and the others
@@ -108,11 +108,22 @@ struct TWeigh {
     }
 };
 
+constexpr uint32_t kMostBits = 51;  // of a weight (see Whole)
+
 // Arguments of a launch, and what they say of a row
 struct TSampleArguments {
     size_t First, Rows;  // of the launch
     uint32_t Classes;
     uint32_t Shift;
+
+    // Whole numbers of 2^-Shift leave room for a row of nothing but best scores. What they round away, half of one for each class at most, is
+    // under 2^-28 of the sum up to 2^18 classes and in any flat row. Of other rows the weights are added a second time (1M f32 classes
+    // 678 us for eight rows, 429 without), in as many more bits as the sum leaves: with the roundings of both it stays under 2^63. Before,
+    // draws of 4M classes passed over 2^-20 of a row.
+    __device__ __forceinline__ uint32_t MoreBits(uint64_t all) const {
+        const uint32_t room = all >> 27 >= Classes ? 0 : __clzll(static_cast<long long>(all + Classes));
+        return room < 2 ? 0 : room - 2 < kMostBits - Shift ? room - 2 : kMostBits - Shift;
+    }
     size_t Stride;
     CbHipSampling Sampling;
     const float* Uniform;
@@ -770,20 +781,27 @@ __device__ void DrawByDigits(const T* row, const TSampleArguments& p, size_t r, 
 
 // The same from nothing but the best key
 template <typename T, int THREADS, int BITS>
-__device__ void DrawAny(const T* row, const TSampleArguments& p, size_t r, const TLimits& limits, const TWeigh<true>& weigh, typename TKeys<T>::TKey most,
+__device__ void DrawAny(const T* row, const TSampleArguments& p, size_t r, const TLimits& limits, TWeigh<true> weigh, typename TKeys<T>::TKey most,
                         TDigitSums<BITS>& sums, TShared<THREADS / 64>& shared) {
-    uint64_t all = 0, likely = 0, there = 0;
-    ForRowSlowly<T, THREADS>(row, p.Classes, [&](T x, uint32_t) {
-        if (TKeys<T>::Of(x) != 0) {
-            const double weight = weigh.Weight(weigh.Under(x));
-            ++there;
-            all += weigh.Whole(weight);
-            likely += weight >= limits.MinP ? weigh.Whole(weight) : 0;
+    uint64_t all, likely, there;
+    for (uint32_t more = 0;;) {
+        all = likely = there = 0;
+        ForRowSlowly<T, THREADS>(row, p.Classes, [&](T x, uint32_t) {
+            if (TKeys<T>::Of(x) != 0) {
+                const double weight = weigh.Weight(weigh.Under(x));
+                ++there;
+                all += weigh.Whole(weight);
+                likely += weight >= limits.MinP ? weigh.Whole(weight) : 0;
+            }
+        });
+        all = SumOf(all, shared);
+        likely = SumOf(likely, shared);
+        there = SumOf(there, shared);
+        if (more != 0 || (more = p.MoreBits(all)) == 0) {
+            break;
         }
-    });
-    all = SumOf(all, shared);
-    likely = SumOf(likely, shared);
-    there = SumOf(there, shared);
+        weigh.Unit = ldexp(weigh.Unit, static_cast<int>(more));
+    }
     DrawByDigits<T, THREADS, BITS>(row, p, r, limits, weigh, most, all, likely, there, sums, shared);
 }
 
@@ -824,7 +842,7 @@ __global__ void __launch_bounds__(THREADS) SampleRowKernel(const T* scores, TSam
         }
         return;
     }
-    const auto weigh = limits.Weigh<true>(TK::Value(most), p.Shift, shared.Powers);
+    auto weigh = limits.Weigh<true>(TK::Value(most), p.Shift, shared.Powers);
     if (weigh.Best == __builtin_inf()) {
         return DrawAny<T, THREADS, BITS>(row, p, r, limits, weigh, most, later, shared);
     }
@@ -867,29 +885,39 @@ __global__ void __launch_bounds__(THREADS) SampleRowKernel(const T* scores, TSam
         __syncthreads();
     }
     const A lowest = lastStep < kDigits - 1 ? boundOf((lastStep + 1) * kStep, -1) : kNone;
-    uint64_t likely = 0;
+    uint64_t all, likely;
     const bool atLeast = limits.MinP > 0;
-    ForRow<T, THREADS>(row, p.Classes, [&](T x, uint32_t) {
-        const A score = static_cast<A>(x);
-        if (score >= lowest && score > kNone) {
-            const double under = underOf(score), weight = weigh.Weight(under);
-            const uint32_t step = stepOf(under);
-            const uint64_t whole = weigh.Whole(weight);
-            if (step <= lastStep) {
-                atomicAdd(reinterpret_cast<unsigned long long*>(&first.Weights[step]), static_cast<unsigned long long>(whole));
-                if (atLeast) {
-                    likely += weight >= limits.MinP ? whole : 0;
+    for (uint32_t more = 0;;) {
+        all = likely = 0;
+        ForRow<T, THREADS>(row, p.Classes, [&](T x, uint32_t) {
+            const A score = static_cast<A>(x);
+            if (score >= lowest && score > kNone) {
+                const double under = underOf(score), weight = weigh.Weight(under);
+                const uint32_t step = stepOf(under);
+                const uint64_t whole = weigh.Whole(weight);
+                if (step <= lastStep) {
+                    atomicAdd(reinterpret_cast<unsigned long long*>(&first.Weights[step]), static_cast<unsigned long long>(whole));
+                    if (atLeast) {
+                        likely += weight >= limits.MinP ? whole : 0;
+                    }
                 }
             }
+        });
+        __syncthreads();
+        for (uint32_t d = threadIdx.x; d < kDigits; d += THREADS) {
+            all += first.Weights[d];
         }
-    });
-    __syncthreads();
-    uint64_t all = 0;
-    for (uint32_t d = threadIdx.x; d < kDigits; d += THREADS) {
-        all += first.Weights[d];
+        all = SumOf(all, shared);
+        likely = atLeast ? SumOf(likely, shared) : all;
+        if (more != 0 || (more = p.MoreBits(all)) == 0) {
+            break;
+        }
+        weigh.Unit = ldexp(weigh.Unit, static_cast<int>(more));
+        for (uint32_t d = threadIdx.x; d < kDigits; d += THREADS) {
+            first.Weights[d] = 0;
+        }
+        __syncthreads();
     }
-    all = SumOf(all, shared);
-    likely = atLeast ? SumOf(likely, shared) : all;
     uint32_t listedStep = kDigits;
     const auto reach = [&](bool byCount, uint64_t target) {
         TPosition<TKey> at{0, 0, 0, 0};
@@ -1173,7 +1201,7 @@ __global__ void __launch_bounds__(1024) SampleCountedKernel(const T* scores, TSa
         }
         return;
     }
-    const auto weigh = limits.Weigh<true>(TK::Value(sharedKey(most)), p.Shift, shared.Powers);
+    auto weigh = limits.Weigh<true>(TK::Value(sharedKey(most)), p.Shift, shared.Powers);
     const uint32_t keys = most - kLowest;  // from the best one down to the last over minus infinity
     uint32_t mine = 0;
     if (most - ownKey < keys) {
@@ -1244,19 +1272,26 @@ __global__ void __launch_bounds__(1024) SampleCountedKernel(const T* scores, TSa
         const uint64_t reached = __ballot(SumUpTo(sum) >= static_cast<uint32_t>(limits.TopK));
         lastSegment = (__ffsll(static_cast<unsigned long long>(reached)) - 1) * 4 + 3;
     }
-    uint64_t likely = 0, all = 0;
-    for (uint32_t segment = wave; segment <= lastSegment; segment += kWaves) {
-        if (segments.Counts[segment] != 0) {
-            const TOfLane v = keysOf(segment, &likely);
-            const uint64_t weight = SumUpTo((v.Weights[0] + v.Weights[1]) + (v.Weights[2] + v.Weights[3]));
-            if (lane == 63) {
-                segments.Weights[segment] = weight;
-                all += weight;
+    uint64_t likely, all;
+    for (uint32_t more = 0;;) {
+        likely = all = 0;
+        for (uint32_t segment = wave; segment <= lastSegment; segment += kWaves) {
+            if (segments.Counts[segment] != 0) {
+                const TOfLane v = keysOf(segment, &likely);
+                const uint64_t weight = SumUpTo((v.Weights[0] + v.Weights[1]) + (v.Weights[2] + v.Weights[3]));
+                if (lane == 63) {
+                    segments.Weights[segment] = weight;
+                    all += weight;
+                }
             }
         }
+        all = SumOf(all, shared);
+        likely = SumOf(likely, shared);
+        if (more != 0 || (more = p.MoreBits(all)) == 0) {
+            break;
+        }
+        weigh.Unit = ldexp(weigh.Unit, static_cast<int>(more));
     }
-    all = SumOf(all, shared);
-    likely = SumOf(likely, shared);
     // every wave for itself: the segment, then the key in it
     const auto reach = [&](bool byCount, uint64_t target) {
         uint64_t weight = 0;
@@ -1348,7 +1383,7 @@ void SampleClasses(int valueType, size_t rows, size_t classes, const void* score
     TSampleArguments p{};
     p.Classes = static_cast<uint32_t>(classes);
     // a row of the best score alone adds up to under 2^63
-    p.Shift = 51;
+    p.Shift = kMostBits;
     while ((size_t(1) << (63 - p.Shift)) <= classes) {
         --p.Shift;
     }

@@ -294,8 +294,9 @@ size_t CbHipSampleClassesBytes(int valueType, size_t rows, size_t classes);
  * lowest), the first whose weights, its own among them, add up to more than uniform[r] (in [0, 1), what is outside counts as the
  * nearest) of their sum. weights[r] (float, double for CBHIP_FLOAT64; NULL: not wanted) = its weight among them. Minus infinity
  * and NaN never take part; a row that has nothing else gets -1 and weight 0. Classes of plus infinity share the whole
- * weight. At most 2^24 classes. Weights are computed in 64 bits for every type and added as whole numbers of 2^-45 of the best
- * one's (131072 classes; a bit less for each doubling), so that the order of additions changes nothing. */
+ * weight. At most 2^24 classes. Weights are computed in 64 bits for every type and added as whole numbers, so that the order of
+ * additions changes nothing: of 2^-45 of the best one's and less up to 262143 classes, of as much as keeps what all of them are rounded
+ * by under 2^-28 of the row's sum for more. */
 bool CbHipSampleClasses(int valueType, size_t rows, size_t classes, const void* scores, size_t scoreStride, const CbHipSampling* sampling,
                         const float* uniform, int32_t* indexes, void* weights, void* workspace, size_t workspaceBytes, void* hipStream);
 

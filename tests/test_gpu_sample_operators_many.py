@@ -95,3 +95,51 @@ def test_many_classes_of_all_weights(kind):
     indexes, weights = draw(kind, scores, uniform, temperature, **limits)
     for r in range(rows):
         check(Row(scores[r], temperature[r]), indexes[r], weights[r], uniform[r], **{k: v[r] for k, v in limits.items()})
+
+
+# ---- more long rows than compute units
+
+def chunked(kind, scores, uniform, limits, step):
+    """The same rows, some at a time."""
+    got = [draw(kind, scores[b:b + step], uniform[b:b + step], **{k: v[b:b + step] for k, v in limits.items()}) for b in range(0, scores.shape[0], step)]
+    return np.concatenate([g[0] for g in got]), np.concatenate([g[1] for g in got])
+
+
+@ALL
+@pytest.mark.parametrize("rows,classes", [(257, 9001), (300, 4097), (1000, 6000)])
+def test_many_long_rows(kind, rows, classes):
+    """Every limit, masked classes, rows of infinities, of NaN, of nothing, of equals and of the best class alone, at any address."""
+    rng = np.random.default_rng(classes)
+    x = rng.standard_normal((rows, classes)) * rng.uniform(0.1, 5, (rows, 1))
+    x[rng.random((rows, classes)) < 0.2] = -np.inf
+    x[rng.random((rows, classes)) < 0.001] = np.nan
+    x[5::40] = np.round(x[5::40])  # more equals than are listed
+    x[6::40] = 1.5
+    x[7::40] = -np.inf
+    x[8::40] = np.nan
+    x[9::40, 7::50] = np.inf
+    x[10::40] = np.where(np.isfinite(x[10::40]), x[10::40] * 1e-4, x[10::40])  # all in the first step
+    wide = torch.full((rows, classes + 3), float("nan"), dtype=TYPES[kind], device="cuda")
+    scores = wide[:, :classes]
+    scores.copy_(torch.from_numpy(x))
+    uniform = rng.random(rows).astype(np.float32)
+    limits = dict(temperature=np.where(rng.random(rows) < 0.1, 0, rng.uniform(0.3, 2, rows)).astype(np.float32),
+                  top_k=np.where(rng.random(rows) < 0.5, 0, rng.integers(1, classes, rows)).astype(np.int32),
+                  top_p=np.where(rng.random(rows) < 0.5, 1, rng.random(rows)).astype(np.float32),
+                  min_p=np.where(rng.random(rows) < 0.7, 0, 10.0 ** -rng.uniform(0, 5, rows)).astype(np.float32))
+    indexes, weights = draw(kind, scores, uniform, **limits)
+    for step in (rows, 256, 100):
+        again = chunked(kind, scores, uniform, limits, step)
+        assert np.array_equal(indexes, again[0]) and np.array_equal(weights, again[1])
+    for r in range(rows):
+        row = scores[r].to(torch.float64)
+        row = torch.where(torch.isnan(row), -float("inf"), row)
+        best, at = row.max().item(), int(row.argmax())
+        if best == -np.inf:
+            assert indexes[r] == -1 and weights[r] == 0
+        elif not limits["temperature"][r] > 0:
+            assert row[indexes[r]] == best and indexes[r] == int(torch.nonzero(row == best)[0, 0]) and weights[r] == 1, at
+        elif best == np.inf:
+            assert row[indexes[r]] == np.inf
+        else:
+            check(Row(row, limits["temperature"][r]), indexes[r], weights[r], uniform[r], **{k: v[r] for k, v in limits.items() if k != "temperature"})

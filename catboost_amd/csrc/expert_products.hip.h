@@ -1015,7 +1015,8 @@ bool TakesCopies(const TProduct<T>& p) {
            (FORM == kWeights ? p.OtherStride : FORM == kInputs ? p.N : p.K) < kMostStride;
 }
 
-// Which kernel. The host does not see the offsets: `each` is what an expert has on average. Times are of bf16, in microseconds, x W^T of
+// Which kernel. The host does not see the offsets: `each` is what an expert has on average (2048 x 4096 to 1024 of 128 experts 249 evenly; 178
+// where four have all, by tiles of 16 rows that read their weights again and again. 16384 of 64 experts 246 and 162). Times are of bf16, in microseconds, x W^T of
 // rows x inputs to outputs (and the same gated) unless said otherwise.
 template <int FORM, int PROJECTIONS, typename T>
 void MultiplyBy(const TCallDevice& call, const TProduct<T>& p) {

@@ -1430,8 +1430,8 @@ void SampleClasses(int valueType, size_t rows, size_t classes, const void* score
             // (64 x 131000 bf16 46 us, 359 with weights of each class)
             launch(SampleCountedKernel<T>, from, 1024, 1);
         } else {
-            // two workgroups for a compute unit where rows are more than those (384 x 100003 f32 161 us, 174 with 1024 threads each; 2000 x 10000 95, 162;
-            // 32 x 100003 80 and 64)
+            // two workgroups for a compute unit where rows are more than those (with a share of 0.95, 384 x 100003 f32 151 us, 164 with 1024 threads each;
+            // 2000 x 10000 107 and 182; 257 x 100003 126 and 131; 256 x 100003 112 and 89, 32 x 100003 92 and 72)
             constexpr int kList = 2048;
             rows > 256 ? launch(SampleRowKernel<T, 512, 11, kList>, from, 512, 1) : launch(SampleRowKernel<T, 1024, 11, kList>, from, 1024, 1);
         }

@@ -287,7 +287,8 @@ typedef struct CbHipSampling {
     const float* MinP;
 } CbHipSampling;
 
-/* Bytes of workspace (at a multiple of 8) that CbHipSampleClasses needs; 0 where it needs none. */
+/* Bytes of workspace (at a multiple of 8) that CbHipSampleClasses needs; 0 where it needs none, as for every size at present: a workspace
+ * that is given all the same is not looked at. */
 size_t CbHipSampleClassesBytes(int valueType, size_t rows, size_t classes);
 
 /* indexes[r] = a class of row r, drawn with the softmax weights of the classes that take part: best first (of equal ones the
@@ -351,8 +352,8 @@ bool CbHipGatedRows(int valueType, int activation, size_t rows, size_t width, si
                     const void* source, size_t sourceStride, const void* gateWeights, const void* upWeights, size_t expertStride,
                     void* result, size_t resultStride, void* kept, void* hipStream);
 
-/* Its gradients, from what it kept: preGradients of the gate and up values, laid out as `kept` but in the value type (32-bit and
- * 64-bit ones may be `kept` itself); from those sourceGradients (NULL: not wanted; `gateWeights` and `upWeights` are not read then), and
+/* Its gradients, from what it kept: preGradients of the gate and up values, laid out as `kept` but rounded to the value type (32-bit and
+ * 64-bit ones may be `kept` itself; a 16-bit one past the type's largest value is infinite); from those, as rounded, sourceGradients (NULL: not wanted; `gateWeights` and `upWeights` are not read then), and
  * gateGradients and upGradients (both or neither; `source` is not read then), which are written for experts without rows, and
  * without rows at all, too. */
 bool CbHipGatedRowsBackward(int valueType, int activation, size_t rows, size_t width, size_t hidden, int32_t experts,
